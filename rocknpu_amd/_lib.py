@@ -1,5 +1,5 @@
 """ctypes binding of librocknpu_capi.so (include/rocknpu.h, rocknpu_ggml.h,
-rocknpu_hip.h, rocknpu_sidecar.h, rocknpu_route.h).
+rocknpu_hip.h, rocknpu_kv.h, rocknpu_sidecar.h, rocknpu_route.h).
 
 The library is loaded from this package directory only. A missing library is
 an error, never a fallback: every compute path in this package goes through
@@ -17,6 +17,7 @@ _u32 = ctypes.c_uint32
 _vp = ctypes.c_void_p
 _ctx = ctypes.c_void_p
 _i = ctypes.c_int
+_i64 = ctypes.c_int64
 
 # (name, restype, argtypes) for every exported symbol the headers declare.
 SIGNATURES = {
@@ -85,6 +86,12 @@ SIGNATURES = {
     "rocknpu_hip_gemv_tiled_preferred": (_i, [_u32, _sz, _sz]),
     "rocknpu_hip_gemv_take_stall": (_i, []),
     "rocknpu_hip_gemv_test_stall": (_i, [_i]),
+    # rocknpu_kv.h — 8-bit key/value cache and attention
+    "rocknpu_hip_kv_append": (_i, [_vp, _u32, _vp, _i64, _i64, _vp, _i64, _i64, _sz, _vp, _vp, _sz, _vp]),
+    "rocknpu_hip_kv_read": (_i, [_vp, _vp, _vp, _sz, _u32, _vp, _vp, _vp]),
+    "rocknpu_hip_kv_attention": (_i, [_vp, _vp, _vp, _sz, _vp]),
+    "rocknpu_hip_kv_attention_workspace": (_i, [_vp, _vp, _i, _vp]),
+    "rocknpu_hip_kv_evict": (_i, [_vp, _vp]),
 }
 
 

@@ -1,0 +1,71 @@
+// What the kernels of the 8-bit key/value cache share: a block's byte layout,
+// a step's lengths as the device reads them, and element conversions.
+//
+// A page (include/rocknpu_kv.h) holds 32 tokens of one kv head, keys then
+// values. The orders are those in which a wave's lanes feed the matrix
+// instructions: for v_mfma_f32_16x16x32_f16 lane l = 16 q + r supplies 8
+// contraction values of row r. Keys are the first operand of the scores
+// (row = token, contraction = dims): lane (r, q) loads the 16 bytes of dims
+// 64 c + 16 q .. + 15 of token r, two instructions' worth. Values are the first
+// operand of the output (row = dim, contraction = tokens): the scores leave
+// their instruction with lane (., q) holding tokens 4 q + 0..3 of each 16-token
+// tile, so a lane's 8 contraction values are those tokens of both tiles, and 16
+// bytes serve dims d and d + 16.
+#pragma once
+
+#include "common.h"
+#include "rocknpu_kv.h"
+
+namespace rk {
+
+constexpr int kKvBlock = 32;
+constexpr float kKvScaleFloor = 0x1p-100f;
+constexpr int kKvMaxWeightRows = 256;
+constexpr int kKvEvictMaxBlocks = 16384;
+
+// Byte of key dim d of token t within a page's keys, and of value dim d within
+// its values.
+__host__ __device__ constexpr int kv_key_at(int t, int d) { return (d / 64 * kKvBlock + t) * 64 + d % 64; }
+__host__ __device__ constexpr int kv_value_at(int t, int d) {
+    return ((d / 32 * 16 + d % 16) * 4 + t / 4 % 4) * 16 + (d / 16 % 2) * 8 + t / 16 * 4 + t % 4;
+}
+
+template <int TYPE>
+struct KvType;
+template <>
+struct KvType<ROCKNPU_KV_F32> {
+    using T = float;
+    static __device__ __forceinline__ float to_f32(T x) { return x; }
+    static __device__ __forceinline__ T from_f32(float x) { return x; }
+};
+template <>
+struct KvType<ROCKNPU_KV_F16> {
+    using T = _Float16;
+    static __device__ __forceinline__ float to_f32(T x) { return static_cast<float>(x); }
+    static __device__ __forceinline__ T from_f32(float x) { return static_cast<T>(x); }
+};
+template <>
+struct KvType<ROCKNPU_KV_BF16> {
+    using T = __bf16;
+    static __device__ __forceinline__ float to_f32(T x) { return static_cast<float>(x); }
+    static __device__ __forceinline__ T from_f32(float x) { return static_cast<T>(x); }
+};
+
+// A sequence's part of a step: `past` tokens before it, rows row0 .. row0 + n - 1.
+// Whatever past and cu hold, the rows lie inside the step's tensors.
+struct KvSpan {
+    int past, row0, n;
+};
+__device__ __forceinline__ KvSpan kv_span(const int32_t* past, const int32_t* cu, int b, int rows, int max_new) {
+    KvSpan s;
+    s.past = min(max(past[b], 0), 0x3fffffff);
+    s.row0 = min(max(cu[b], 0), rows);
+    const int end = min(max(cu[b + 1], s.row0), rows);
+    s.n = min(end - s.row0, max_new);
+    return s;
+}
+
+// Whether a cache description is one that the kernels can take. kv_cache.hip.
+bool kv_cache_ok(const rocknpu_kv_cache* c);
+
+}  // namespace rk

@@ -1,0 +1,246 @@
+"""The 8-bit key/value cache and the attention that reads it
+(include/rocknpu_kv.h) on device tensors.
+
+A `Cache` is a set of pages, each one block of 32 tokens of one kv head in int8
+with an f32 scale for its keys and one for its values, and the table that names
+every sequence's pages. A step of a model's layer is
+
+    kv.append(cache, k, v, past, cu, max_new)          # the step's new rows
+    out = kv.attention(cache, q, past, cu, max_new)    # its queries over all rows
+
+with past [batch] the tokens that each sequence had before the step and
+cu [batch + 1] the row offsets of its new ones, both int32 on the device and
+shared by all layers. Calls enqueue on the current torch stream and return
+immediately; they read no lengths on the host, so a step can be captured in a
+HIP graph.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib, hip
+from .hip import LaunchError
+
+BLOCK = 32
+HEAD_DIMS = (64, 128, 192, 256)
+MAX_WEIGHT_ROWS = 256
+MAX_EVICT_BLOCKS = 16384
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+_vp = ctypes.c_void_p
+_i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
+
+
+class _CacheStruct(ctypes.Structure):
+    """rocknpu_kv_cache (include/rocknpu_kv.h)."""
+
+    _fields_ = [("pages", _vp), ("scales", _vp), ("table", _vp), ("starts", _vp), ("dropped", _vp), ("weights", _vp),
+                ("n_pages", _i64), ("batch", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("max_blocks", _i32)]
+
+
+class _AttentionStruct(ctypes.Structure):
+    """rocknpu_kv_attention_args (include/rocknpu_kv.h)."""
+
+    _fields_ = [("q", _vp), ("out", _vp), ("past", _vp), ("cu", _vp), ("prefix", _vp), ("slopes", _vp),
+                ("weights_out", _vp), ("q_row", _i64), ("q_head", _i64), ("out_row", _i64), ("out_head", _i64),
+                ("rows", _i64), ("max_new", _i64), ("max_tokens", _i64), ("type", ctypes.c_uint32), ("heads", _i32),
+                ("causal", _i32), ("window", _i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
+
+
+class _EvictStruct(ctypes.Structure):
+    """rocknpu_kv_evict_args (include/rocknpu_kv.h)."""
+
+    _fields_ = [("table", _vp), ("starts", _vp), ("weights", _vp), ("tokens", _vp), ("dropped", _vp),
+                ("table_out", _vp), ("starts_out", _vp), ("weights_out", _vp), ("dropped_out", _vp), ("batch", _i32),
+                ("kv_heads", _i32), ("max_blocks", _i32), ("budget", _i32), ("sinks", _i32), ("recent", _i32)]
+
+
+def _is(t, shape, dtype, what, device=None):
+    """`t` is a contiguous tensor of that shape and type, on that device."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what} has to be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the cache on {device}")
+    return t
+
+
+def _rows(t, heads, head_dim, what, device):
+    """`t` is [rows, heads, head_dim] of a known type with a contiguous last dimension: its strides."""
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{what} is {t.dtype}: float32, float16 or bfloat16 is wanted")
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != head_dim:
+        raise ValueError(f"{what} has to be [rows, {'heads' if heads is None else heads}, {head_dim}], not {tuple(t.shape)}")
+    row, head, one = t.stride()
+    if one != 1 and t.numel():
+        raise ValueError(f"{what} has to be contiguous in its last dimension")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the cache on {device}")
+    return row, head
+
+
+class Cache:
+    """One layer's pages and tables (rocknpu_kv_cache): `pages` int8 or uint8
+    [n_pages, 64 * head_dim], `scales` f32 [n_pages, 2], `table` and `starts`
+    int32 [batch, kv_heads, max_blocks], `dropped` int32 [batch], `weights` f32
+    [batch, kv_heads, max_blocks] or None. The tensors are used in place and
+    kept alive by the object."""
+
+    def __init__(self, pages, scales, table, starts, dropped, weights=None, *, head_dim: int):
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim {head_dim} is not one of {HEAD_DIMS}")
+        if table.dim() != 3 or 0 in table.shape:
+            raise ValueError("table has to be [batch, kv_heads, max_blocks]")
+        if pages.dtype not in (torch.int8, torch.uint8):
+            raise ValueError("pages have to be int8 or uint8")
+        at = table.device
+        n = pages.shape[0]
+        if n == 0:
+            raise ValueError("a cache needs at least one page")
+        self.pages = _is(pages, (n, 2 * BLOCK * head_dim), pages.dtype, "pages", at)
+        self.scales = _is(scales, (n, 2), torch.float32, "scales", at)
+        self.table = _is(table, table.shape, torch.int32, "table", at)
+        self.starts = _is(starts, table.shape, torch.int32, "starts", at)
+        self.dropped = _is(dropped, table.shape[:1], torch.int32, "dropped", at)
+        self.weights = None if weights is None else _is(weights, table.shape, torch.float32, "weights", at)
+        self.batch, self.kv_heads, self.max_blocks = table.shape
+        self.head_dim, self.device = head_dim, at
+        self._struct = _CacheStruct(
+            pages.data_ptr(), scales.data_ptr(), table.data_ptr(), starts.data_ptr(), dropped.data_ptr(),
+            None if weights is None else weights.data_ptr(), n, self.batch, self.kv_heads, head_dim, self.max_blocks)
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, head_dim: int, max_blocks: int, device="cuda", weights: bool = True):
+        """A cache with max_blocks pages of its own for every sequence and head."""
+        n = batch * kv_heads * max_blocks
+        table = torch.arange(n, dtype=torch.int32, device=device).view(batch, kv_heads, max_blocks)
+        return cls(torch.zeros((n, 2 * BLOCK * head_dim), dtype=torch.int8, device=device),
+                   torch.full((n, 2), 2.0 ** -100, device=device), table, torch.zeros_like(table),
+                   torch.zeros(batch, dtype=torch.int32, device=device),
+                   torch.zeros(table.shape, device=device) if weights else None, head_dim=head_dim)
+
+    def lengths(self, t, what):
+        return ctypes.c_void_p(_is(t, (self.batch,), torch.int32, what, self.device).data_ptr())
+
+    def offsets(self, t):
+        return ctypes.c_void_p(_is(t, (self.batch + 1,), torch.int32, "cu", self.device).data_ptr())
+
+
+def append(cache: Cache, k: torch.Tensor, v: torch.Tensor, past: torch.Tensor, cu: torch.Tensor, max_new: int) -> None:
+    """Quantises rows k and v [rows, kv_heads, head_dim] (f32, f16 or bf16; any
+    row and head strides) into the blocks of their sequences. max_new bounds
+    the rows of any one sequence. A partly filled block's scale only grows, and
+    its older codes are rounded anew when it does; a value that is not finite
+    makes its block NaN."""
+    k_row, k_head = _rows(k, cache.kv_heads, cache.head_dim, "k", cache.device)
+    v_row, v_head = _rows(v, cache.kv_heads, cache.head_dim, "v", cache.device)
+    if k.dtype != v.dtype or k.shape != v.shape:
+        raise ValueError("k and v differ in type or shape")
+    hip._check(_lib.load().rocknpu_hip_kv_append(
+        cache._ref, _TYPES[k.dtype], k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, k.shape[0],
+        cache.lengths(past, "past"), cache.offsets(cu), max_new, hip._stream()), "kv_append")
+
+
+def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dtype: torch.dtype = torch.float32):
+    """(keys, values), each [batch, count, kv_heads, head_dim]: what the cache
+    stands for at positions first[b] .. first[b] + count - 1, zero at or past
+    tokens[b] and in evicted blocks."""
+    if dtype not in _TYPES:
+        raise ValueError(f"{dtype}: float32, float16 or bfloat16 is wanted")
+    k, v = (torch.empty((cache.batch, count, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+            for _ in range(2))
+    hip._check(_lib.load().rocknpu_hip_kv_read(
+        cache._ref, cache.lengths(first, "first"), cache.lengths(tokens, "tokens"), count, _TYPES[dtype],
+        k.data_ptr(), v.data_ptr(), hip._stream()), "kv_read")
+    return k, v
+
+
+# Workspaces of the attention, one per (device, stream); a call needs nothing
+# of what an earlier one left there. A replaced one is kept for the graphs that
+# hold its address, as the K-split workspaces are.
+_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
+    ws = hip._stream_workspace(_workspaces, device, nbytes, 1 << 20)
+    if ws is None:
+        raise LaunchError("attention under graph capture needs this stream's workspace: make one eager call of the "
+                          "same shape on the capturing stream first")
+    return ws
+
+
+def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tensor, max_new: int, *,
+              max_tokens: int = 0, scale: float | None = None, causal: bool = True, window: int = 0,
+              prefix: torch.Tensor | None = None, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+              weights_out: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of query rows q [rows, heads, head_dim] over the cache, whose
+    last rows are theirs (append them first). out has q's shape and type.
+
+    scale defaults to 1 / sqrt(head_dim). A row at position p sees the keys at
+    positions s <= p, with `window` only those with s > p - window, and with
+    `prefix` (int32 [batch]) all with s < prefix as well; causal=False sees all.
+    `softcap` caps scores by softcap * tanh(x / softcap), `slopes` (f32 [heads])
+    adds slopes * (s - p). A row that sees nothing is 0. `weights_out` takes
+    cache.weights plus what each block got of this step's attention (it may be
+    cache.weights; at most 256 rows times heads per kv head). max_tokens, the
+    most tokens a sequence is expected to hold, sizes the work split only;
+    without it the table's width does."""
+    row, head = _rows(q, None, cache.head_dim, "q", cache.device)
+    rows, heads = q.shape[:2]
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"{heads} query heads over {cache.kv_heads} kv heads")
+    if out is None:
+        out = torch.empty((rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise ValueError("out has to have q's type and shape")
+    o_row, o_head = _rows(out, heads, cache.head_dim, "out", cache.device)
+    args = _AttentionStruct(
+        q.data_ptr(), out.data_ptr(), cache.lengths(past, "past"), cache.offsets(cu),
+        None if prefix is None else cache.lengths(prefix, "prefix"),
+        None if slopes is None else _is(slopes, (heads,), torch.float32, "slopes", cache.device).data_ptr(),
+        None if weights_out is None else _is(weights_out, cache.table.shape, torch.float32, "weights_out",
+                                             cache.device).data_ptr(),
+        row, head, o_row, o_head, rows, max_new, max_tokens, _TYPES[q.dtype], heads, int(causal), window,
+        1.0 / math.sqrt(cache.head_dim) if scale is None else scale, softcap)
+    lib = _lib.load()
+    ref = ctypes.addressof(args)
+    need = ctypes.c_size_t()
+    hip._check(lib.rocknpu_hip_kv_attention_workspace(cache._ref, ref, 0, ctypes.byref(need)), "kv_attention")
+    ws, nbytes = None, 0
+    if need.value:
+        ws = workspace_for(cache.device, need.value) if workspace is None else workspace
+        nbytes = ws.numel() * ws.element_size()
+    hip._check(lib.rocknpu_hip_kv_attention(cache._ref, ref, hip._ptr(ws), nbytes, hip._stream()), "kv_attention")
+    return out
+
+
+def evict(table: torch.Tensor, starts: torch.Tensor, weights: torch.Tensor, tokens: torch.Tensor, dropped: torch.Tensor,
+          budget: int, *, sinks: int = 0, recent: int = 1, out=None):
+    """Cuts every sequence's blocks to `budget` by accumulated weight, per kv
+    head: the first `sinks`, the last `recent` and the heaviest others stay
+    (equal weights: the lowest place). Returns new (table, starts, weights,
+    dropped), or fills `out`; each row holds the kept entries in order, then the
+    evicted, whose pages the sequence's next blocks take, then the rest. out[:3]
+    may be the inputs themselves, out[3] must not be `dropped`."""
+    if table.dim() != 3 or 0 in table.shape:
+        raise ValueError("table has to be [batch, kv_heads, max_blocks]")
+    at = table.device
+    batch, kv_heads, max_blocks = table.shape
+    kinds = ((table, torch.int32, "table"), (starts, torch.int32, "starts"), (weights, torch.float32, "weights"))
+    if out is None:
+        out = (torch.empty_like(table), torch.empty_like(starts), torch.empty_like(weights), torch.empty_like(dropped))
+    for (t, dtype, what), o in zip(kinds, out):
+        _is(t, table.shape, dtype, what, at)
+        _is(o, table.shape, dtype, what + "_out", at)
+    for t, what in ((tokens, "tokens"), (dropped, "dropped"), (out[3], "dropped_out")):
+        _is(t, (batch,), torch.int32, what, at)
+    args = _EvictStruct(table.data_ptr(), starts.data_ptr(), weights.data_ptr(), tokens.data_ptr(), dropped.data_ptr(),
+                        *[t.data_ptr() for t in out], batch, kv_heads, max_blocks, budget, sinks, recent)
+    hip._check(_lib.load().rocknpu_hip_kv_evict(ctypes.addressof(args), hip._stream()), "kv_evict")
+    return out

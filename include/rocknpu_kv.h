@@ -115,9 +115,10 @@ typedef struct rocknpu_kv_attention_args {
  * window (window), or if s < prefix[b]; without causal it sees all keys (window
  * and prefix must then be absent). out = sum(exp(x) v) / sum(exp(x)) over what it
  * sees, and 0 where it sees nothing. Scores, the running maximum and sum and the
- * products' sums are f32; q and the weights enter the matrix instructions as
- * f16 for f16 and bf16 calls and as pairs of f16 (22 bits) for f32 calls, the
- * codes exactly.
+ * products' sums are f32. The codes enter the matrix instructions exactly, q as
+ * f16 for f16 and bf16 calls and as a pair of f16 (22 bits) for f32 calls (each
+ * row scaled by a power of two first), the weights with 11 bits or more for f16
+ * and bf16 calls and with 24 for f32 calls, over f32's range.
  * With weights_out, also weights_out = cache->weights + the weight that each
  * block got from all rows and the kv head's heads (entries past the blocks in
  * use are copied); at most 256 rows times heads per kv head.

@@ -21,6 +21,7 @@ namespace rk {
 constexpr int kKvBlock = 32;
 constexpr float kKvScaleFloor = 0x1p-100f;
 constexpr int kKvMaxWeightRows = 256;
+constexpr int kKvMaxBatch = 4095;  // times 16 row tiles fits a grid dimension
 constexpr int kKvEvictMaxBlocks = 16384;
 
 // Byte of key dim d of token t within a page's keys, and of value dim d within

@@ -1,0 +1,195 @@
+// What the attention kernels over the 8-bit key/value cache share: a launch's
+// description, the range of blocks that rows see, and code conversions.
+//
+// Softmax over blocks with scales of their own. With keys kc * sk and values
+// vc * sv in a block (kc, vc whole numbers), and everything in powers of two,
+//   o = sum 2^y vc / sum 2^y / sv,   y = x log2(e) + log2(sv) - M
+// for any M: folding a block's value scale into the exponent leaves the codes
+// as they are (exact in f16 and bf16), takes one add per block and row, and one
+// product per block and row for the denominator. M is the row's running maximum
+// of x log2(e) + log2(sv).
+#pragma once
+
+#include "kv.h"
+
+namespace rk {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kKvTileRows = 16;  // rows of a tile of the streaming kernel
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+struct KvAttend {
+    rocknpu_kv_cache c;
+    rocknpu_kv_attention_args a;
+    int group;       // heads per kv head
+    int row_tiles;   // tiles of rows that a sequence and kv head may have
+    int splits;      // workgroups that share a tile's blocks
+    int chunk;       // blocks per split, at least
+    bool vec_q, vec_out;
+    // workspace, one entry per (sequence, kv head, row tile, split): sums of the output [rows][head_dim], maxima and
+    // sums [rows][2]; one per (sequence, kv head, block, row): its weight's sum and the maximum it refers to
+    float* part_out;
+    float* part_state;
+    float* block_sums;
+};
+
+// A page's scale, NaN where there is none or it is not finite.
+__device__ __forceinline__ float kv_scale(float s, bool ok) {
+    return ok && fabsf(s) <= 3.402823466e38f ? s : __builtin_nanf("");
+}
+
+// How many of a row's n ascending starts are below `value`: 64 probes a round,
+// the same answer in every lane.
+__device__ __forceinline__ int starts_below(const int32_t* starts, int n, int value) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, size = n;  // the count lies in [lo, lo + size]
+    while (size > 0) {
+        const int step = (size + 63) / 64;
+        const int at = lane * step;
+        const bool below = at < size && starts[lo + at] < value;
+        const int c = __popcll(__ballot(below));
+        if (c == 0) return lo;
+        // entry (c - 1) step is below, entry c step (if any) is not
+        lo += (c - 1) * step + 1;
+        size = min(step - 1, size - (c - 1) * step - 1);
+    }
+    return lo;
+}
+
+// The blocks that rows at positions q0 .. q1 see: entries [0, first) and
+// [from, to) of the table's row.
+struct KvRange {
+    int first, from, to;
+    __device__ __forceinline__ int count() const { return first + to - from; }
+    __device__ __forceinline__ int entry(int i) const { return i < first ? i : i - first + from; }
+};
+__device__ __forceinline__ KvRange kv_range(const rocknpu_kv_attention_args& a, const int32_t* starts, int held, int gone,
+                                            int q0, int q1, int prefix) {
+    KvRange r{0, 0, max(held, 0)};
+    if (!a.causal || held <= 0) return r;
+    // newest blocks begin behind the rows
+    const int last = max(q1, prefix - 1);
+    r.to = min(held, max(last / kKvBlock + 1 - gone, 0));
+    if (gone && last / kKvBlock + 1 - gone < held) r.to = starts_below(starts, held, last + 1);
+    if (a.window == 0) return r;
+    const int lowest = q0 - a.window + 1;  // first position that a row's window holds
+    if (lowest <= 0) return r;
+    const int from_start = lowest / kKvBlock * kKvBlock;
+    r.from = min(gone ? starts_below(starts, held, from_start) : from_start / kKvBlock, r.to);
+    if (prefix > 0) r.first = min(gone ? starts_below(starts, held, prefix) : (prefix + kKvBlock - 1) / kKvBlock, r.from);
+    return r;
+}
+
+// Whether a row at qpos sees the key at kpos.
+__device__ __forceinline__ bool kv_seen(const rocknpu_kv_attention_args& a, int kpos, int qpos, int prefix, int total) {
+    const bool seen = !a.causal || (kpos <= qpos && (a.window == 0 || kpos > qpos - a.window)) || kpos < prefix;
+    return seen && kpos < total;
+}
+
+// Whether every row at q0 .. q1 sees all of the block that begins at `start`.
+__device__ __forceinline__ bool kv_all_seen(const rocknpu_kv_attention_args& a, int start, int q0, int q1, int prefix, int total) {
+    const bool seen = !a.causal || (start + kKvBlock - 1 <= q0 && (a.window == 0 || start > q1 - a.window)) ||
+                      start + kKvBlock <= prefix;
+    return seen && start + kKvBlock <= total;
+}
+
+// Eight signed bytes as f16, exactly: byte + 128 lands in the low mantissa bits
+// of 1024 (f16 0x6400 + u is 1024 + u), and 1152 comes off again.
+__device__ __forceinline__ half8 codes_to_half(uint32_t lo, uint32_t hi) {
+    union {
+        uint32_t u[4];
+        half2v h[4];
+        half8 v;
+    } r;
+    lo ^= 0x80808080u;
+    hi ^= 0x80808080u;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u);
+    const half2v off = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.h[i] = r.h[i] - off;
+    return r.v;
+}
+
+// Eight signed bytes as bf16, exactly (|code| <= 127 fits its 8 bits): the high
+// halves of their f32.
+__device__ __forceinline__ bhalf8 codes_to_bhalf(uint32_t lo, uint32_t hi) {
+    union {
+        uint32_t u[4];
+        bhalf8 v;
+    } r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? lo : hi;
+        const float a = static_cast<float>(static_cast<int8_t>(w >> (i % 2 * 16)));
+        const float b = static_cast<float>(static_cast<int8_t>(w >> (i % 2 * 16 + 8)));
+        r.u[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+    return r.v;
+}
+
+// Non-negative x as the sum of PARTS bf16 (8 bits each, cut off; the last one's
+// rest is dropped), eight at a time: 16 bits in two, f32's 24 in three, over
+// f32's whole range.
+template <int PARTS>
+__device__ __forceinline__ void split_bhalf(const float (&x)[8], bhalf8 (&part)[PARTS]) {
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        union {
+            uint32_t u[4];
+            bhalf8 v;
+        } r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r.u[i] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * i + 1]), __float_as_uint(rest[2 * i]), 0x07060302u);
+        part[p] = r.v;
+        if (p + 1 < PARTS) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xffff0000u);
+        }
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Eight consecutive elements of a row as f32.
+template <int TYPE>
+__device__ __forceinline__ void load8(const typename KvType<TYPE>::T* p, bool vec, float (&x)[8]) {
+    using K = KvType<TYPE>;
+    if (vec) {
+        constexpr int kPer = 16 / sizeof(typename K::T);
+        struct alignas(16) Quad {
+            typename K::T e[kPer];
+        };
+#pragma unroll
+        for (int i = 0; i < 8 / kPer; ++i) {
+            const Quad v = reinterpret_cast<const Quad*>(p)[i];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) x[i * kPer + j] = K::to_f32(v.e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = K::to_f32(p[i]);
+    }
+}
+
+// The power of two that brings a row of magnitude `top` to 2^13 .. 2^14, where
+// f16 holds it with room on both sides (1 for an empty or not finite row).
+__device__ __forceinline__ float row_power(float top) {
+    const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+    if (e == -127 || e == 128) return 1.0f;
+    return __uint_as_float(static_cast<uint32_t>(127 + min(max(13 - e, -114), 120)) << 23);
+}
+
+int launch_kv_stream(const KvAttend& p, hipStream_t stream);   // kv_stream.hip
+
+}  // namespace rk

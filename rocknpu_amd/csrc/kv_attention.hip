@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <climits>
 
-#include "kv.h"
+#include "kv_attend.h"
 
 namespace rk {
 namespace {
@@ -10,14 +10,7 @@ namespace {
 struct AttentionParams {
     rocknpu_kv_cache c;
     rocknpu_kv_attention_args a;
-    float* state;  // [rows][heads][2]: running maximum and sum, for the block weights
 };
-
-// A page's scale, NaN where there is none or it is not finite.
-__device__ __forceinline__ float kv_scale(const rocknpu_kv_cache& c, int64_t page, int which, bool ok) {
-    const float s = ok ? c.scales[2 * page + which] : 0.0f;
-    return ok && fabsf(s) <= 3.402823466e38f ? s : __builtin_nanf("");
-}
 
 // The score of one key after scale, cap, bias and mask.
 __device__ __forceinline__ float masked_score(const rocknpu_kv_attention_args& a, float dot, int head, int kpos, int qpos,
@@ -58,7 +51,7 @@ __global__ __launch_bounds__(64) void kv_attention_kernel(AttentionParams p) {
         const int64_t pg = ok ? page : 0;
         const int8_t* keys = reinterpret_cast<const int8_t*>(c.pages) + pg * (2 * kKvBlock * D);
         const int8_t* values = keys + kKvBlock * D;
-        const float sk = kv_scale(c, pg, 0, ok), sv = kv_scale(c, pg, 1, ok);
+        const float sk = kv_scale(c.scales[2 * pg], ok), sv = kv_scale(c.scales[2 * pg + 1], ok);
         float dot = 0.0f;
         for (int e = 0; e < D / 2; ++e) {
             const int d = half * (D / 2) + e;
@@ -89,67 +82,12 @@ __global__ __launch_bounds__(64) void kv_attention_kernel(AttentionParams p) {
     T* out = static_cast<T*>(a.out) + (s.row0 + i) * a.out_row + head * a.out_head;
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) out[lane + 64 * e] = K::from_f32(sum == 0.0f ? 0.0f : o[e] / sum);
-    if (p.state && lane == 0) {
-        float* st = p.state + 2 * (static_cast<int64_t>(s.row0 + i) * a.heads + head);
-        st[0] = top;
-        st[1] = sum;
-    }
-}
-
-// One wave per block of a sequence and kv head: the scores of its rows again,
-// with their final maximum and sum.
-template <int TYPE, int D>
-__global__ __launch_bounds__(64) void kv_weights_kernel(AttentionParams p) {
-    using K = KvType<TYPE>;
-    using T = typename K::T;
-    __shared__ float q[D];
-    const rocknpu_kv_cache& c = p.c;
-    const rocknpu_kv_attention_args& a = p.a;
-    const int lane = threadIdx.x, b = blockIdx.z, h = blockIdx.y, at = blockIdx.x;
-    const KvSpan s = kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new));
-    const int total = s.past + s.n, group = a.heads / c.kv_heads;
-    const int held = min((total + kKvBlock - 1) / kKvBlock - max(c.dropped[b], 0), c.max_blocks);
-    const int prefix = a.prefix ? a.prefix[b] : 0;
-    const int64_t entry = (static_cast<int64_t>(b) * c.kv_heads + h) * c.max_blocks + at;
-    float got = 0.0f;
-    if (at < held) {
-        const int page = c.table[entry];
-        const bool ok = page >= 0 && page < c.n_pages;
-        const int64_t pg = ok ? page : 0;
-        const int8_t* keys = reinterpret_cast<const int8_t*>(c.pages) + pg * (2 * kKvBlock * D);
-        const float sk = kv_scale(c, pg, 0, ok);
-        const int t = lane & 31, half = lane >> 5;
-        for (int r = 0; r < s.n * group; ++r) {
-            const int i = r / group, head = h * group + r % group;
-            const T* qr = static_cast<const T*>(a.q) + (s.row0 + i) * a.q_row + head * a.q_head;
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < D / 64; ++e) q[lane + 64 * e] = K::to_f32(qr[lane + 64 * e]);
-            __syncthreads();
-            float dot = 0.0f;
-            for (int e = 0; e < D / 2; ++e) {
-                const int d = half * (D / 2) + e;
-                dot += q[d] * static_cast<float>(keys[kv_key_at(t, d)]);
-            }
-            dot += __shfl_xor(dot, 32, 64);
-            const float x = masked_score(a, dot * sk, head, c.starts[entry] + t, s.past + i, total, prefix);
-            const float* st = p.state + 2 * (static_cast<int64_t>(s.row0 + i) * a.heads + head);
-            float l = half || x == -__builtin_inff() ? 0.0f : expf(x - st[0]) / st[1];
-#pragma unroll
-            for (int g = 32; g >= 1; g >>= 1) l += __shfl_xor(l, g, 64);
-            got += l;
-        }
-    }
-    if (lane == 0) a.weights_out[entry] = c.weights[entry] + got;
 }
 
 template <int TYPE, int D>
 int launch(const AttentionParams& p, hipStream_t stream) {
     const rocknpu_kv_attention_args& a = p.a;
-    if (a.rows > 0 && a.max_new > 0)
-        kv_attention_kernel<TYPE, D><<<dim3(static_cast<unsigned>(a.max_new), a.heads, p.c.batch), 64, 0, stream>>>(p);
-    if (a.weights_out)
-        kv_weights_kernel<TYPE, D><<<dim3(p.c.max_blocks, p.c.kv_heads, p.c.batch), 64, 0, stream>>>(p);
+    kv_attention_kernel<TYPE, D><<<dim3(static_cast<unsigned>(a.max_new), a.heads, p.c.batch), 64, 0, stream>>>(p);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
@@ -181,8 +119,46 @@ bool attention_ok(const rocknpu_kv_cache* c, const rocknpu_kv_attention_args* a)
     return true;
 }
 
-size_t attention_bytes(const rocknpu_kv_attention_args& a) {
-    return a.weights_out ? (static_cast<size_t>(a.rows) * a.heads * 8 + 255) / 256 * 256 : 0;
+size_t padded(size_t n) { return (n + 255) / 256 * 256; }
+
+// Rows of a kv head up to which the cache is streamed through 16-row tiles.
+constexpr int64_t kStreamRows = 32;
+// Blocks of a split, at least: two for each of a workgroup's waves.
+constexpr int64_t kMinChunk = 8;
+
+struct Plan {
+    KvAttend p;
+    bool stream;
+    size_t out_bytes, state_bytes, sums_bytes;
+    size_t bytes() const { return out_bytes + state_bytes + sums_bytes; }
+};
+
+Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus) {
+    Plan r{};
+    KvAttend& p = r.p;
+    p.c = c;
+    p.a = a;
+    p.group = a.heads / c.kv_heads;
+    const int64_t per = a.type == ROCKNPU_KV_F32 ? 4 : 8;
+    p.vec_q = aligned(a.q, 16) && a.q_row % per == 0 && a.q_head % per == 0;
+    p.vec_out = aligned(a.out, 16) && a.out_row % per == 0 && a.out_head % per == 0;
+    const int64_t rows = std::max<int64_t>(a.max_new, 1) * p.group;
+    r.stream = rows <= kStreamRows || a.weights_out;
+    if (!r.stream) return r;
+    p.row_tiles = static_cast<int>((rows + kKvTileRows - 1) / kKvTileRows);
+    const int64_t units = static_cast<int64_t>(c.batch) * c.kv_heads * p.row_tiles;
+    int64_t blocks = a.max_tokens > 0 ? (a.max_tokens + kKvBlock - 1) / kKvBlock : c.max_blocks;
+    if (a.window > 0) blocks = std::min<int64_t>(blocks, (static_cast<int64_t>(a.window) + a.max_new) / kKvBlock + 2);
+    blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, c.max_blocks));
+    const int64_t want = std::max<int64_t>(1, 4 * cus / units);
+    p.splits = static_cast<int>(std::min<int64_t>(want, (blocks + kMinChunk - 1) / kMinChunk));
+    p.chunk = static_cast<int>((blocks + p.splits - 1) / p.splits);
+    const size_t slots = static_cast<size_t>(units) * p.splits * kKvTileRows;
+    if (p.splits > 1) r.out_bytes = padded(slots * c.head_dim * 4);
+    if (p.splits > 1 || a.weights_out) r.state_bytes = padded(slots * 8);
+    if (a.weights_out)
+        r.sums_bytes = padded(static_cast<size_t>(c.batch) * c.kv_heads * c.max_blocks * p.row_tiles * kKvTileRows * 8);
+    return r;
 }
 
 }  // namespace
@@ -192,8 +168,7 @@ extern "C" int rocknpu_hip_kv_attention_workspace(const rocknpu_kv_cache* cache,
                                                   int cus, size_t* bytes) {
     using namespace rk;
     if (!bytes || !attention_ok(cache, args)) return kStatusInvalid;
-    (void)cus;
-    *bytes = attention_bytes(*args);
+    *bytes = plan(*cache, *args, cus > 0 ? cus : device_cu_count()).bytes();
     return kStatusOk;
 }
 
@@ -201,11 +176,19 @@ extern "C" int rocknpu_hip_kv_attention(const rocknpu_kv_cache* cache, const roc
                                         void* workspace, size_t workspace_bytes, void* stream) {
     using namespace rk;
     if (!attention_ok(cache, args)) return kStatusInvalid;
-    const size_t need = attention_bytes(*args);
+    Plan r = plan(*cache, *args, device_cu_count());
+    const size_t need = r.bytes();
     if (need > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < need)) return kStatusInvalid;
     if ((args->rows == 0 || args->max_new == 0) && !args->weights_out) return kStatusOk;
-    AttentionParams p{*cache, *args, need ? static_cast<float*>(workspace) : nullptr};
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (r.stream) {
+        uint8_t* at = static_cast<uint8_t*>(workspace);
+        if (r.out_bytes) r.p.part_out = reinterpret_cast<float*>(at);
+        if (r.state_bytes) r.p.part_state = reinterpret_cast<float*>(at + r.out_bytes);
+        if (r.sums_bytes) r.p.block_sums = reinterpret_cast<float*>(at + r.out_bytes + r.state_bytes);
+        return launch_kv_stream(r.p, s);
+    }
+    AttentionParams p{*cache, *args};
     switch (args->type) {
         case ROCKNPU_KV_F32: return launch_dim<ROCKNPU_KV_F32>(p, s);
         case ROCKNPU_KV_F16: return launch_dim<ROCKNPU_KV_F16>(p, s);

@@ -394,7 +394,7 @@ int status() { return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 bool kv_cache_ok(const rocknpu_kv_cache* c) {
     if (!c || !c->pages || !c->scales || !c->table || !c->starts || !c->dropped) return false;
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 192 && c->head_dim != 256) return false;
-    if (c->n_pages < 1 || c->n_pages > INT_MAX || c->batch < 1 || c->batch > 65535 || c->kv_heads < 1 ||
+    if (c->n_pages < 1 || c->n_pages > INT_MAX || c->batch < 1 || c->batch > kKvMaxBatch || c->kv_heads < 1 ||
         c->kv_heads > 65535 || c->max_blocks < 1 || c->max_blocks > INT_MAX / kKvBlock)
         return false;
     return aligned(c->pages, 16) && aligned(c->scales, 8) && aligned(c->table, 4) && aligned(c->starts, 4) &&

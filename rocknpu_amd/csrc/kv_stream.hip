@@ -1,0 +1,387 @@
+// Attention of few rows over a long cache: the cache streams through the matrix
+// units once for up to 16 rows (a kv head's heads times the step's tokens).
+//
+// A workgroup of four waves takes one split of a (sequence, kv head, tile of 16
+// rows); a wave takes every fourth block. Blocks come from memory straight into
+// the operand registers (whole 1 KiB runs per load, the next block's loads in
+// flight behind the current one's work), so LDS is used only to join the waves.
+// Scores: keys (16 tokens x 32 dims) times the rows' queries; they leave in the
+// layout in which the next product takes weights: values (16 dims x 32 tokens)
+// times weights. Bound by the cache's bytes.
+#include "kv_attend.h"
+
+namespace rk {
+namespace {
+
+constexpr int kWaves = 4;
+
+template <int D>
+struct BlockRegs {
+    uint4 k[2][D / 64];  // token tile, 64 dims
+    uint4 v[D / 32];
+};
+
+template <int D>
+__device__ __forceinline__ void load_block(const uint8_t* pages, int64_t page, int lane, BlockRegs<D>& r) {
+    const uint8_t* keys = pages + page * (2 * kKvBlock * D) + lane % 16 * 64 + lane / 16 * 16;
+    const uint8_t* values = pages + page * (2 * kKvBlock * D) + kKvBlock * D + lane % 16 * 64 + lane / 16 * 16;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) r.k[t][c] = *reinterpret_cast<const uint4*>(keys + (c * 32 + t * 16) * 64);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) r.v[c] = *reinterpret_cast<const uint4*>(values + c * 1024);
+}
+
+__device__ __forceinline__ float max_over_quads(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float sum_over_quads(float x) {
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+
+// Queries enter as f16, those of f32 calls as hi + lo; weights as two bf16, those
+// of f32 calls as three, which keeps f32's range: an output dim whose greatest
+// weights meet zero codes is as exact as any other.
+template <int TYPE, int D>
+__global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
+    using K = KvType<TYPE>;
+    using T = typename K::T;
+    constexpr bool PAIR = TYPE == ROCKNPU_KV_F32;
+    constexpr int kParts = PAIR ? 2 : 1, kWeightParts = PAIR ? 3 : 2;
+    const rocknpu_kv_cache& c = p.c;
+    const rocknpu_kv_attention_args& a = p.a;
+    __shared__ float state[kWaves][kKvTileRows][2];
+    __shared__ alignas(16) float sums[kWaves][kKvTileRows][D + 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane % 16, quad = lane / 16;
+    const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z / p.row_tiles, tile = blockIdx.z % p.row_tiles;
+    const KvSpan s = kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new));
+    const int rows = s.n * p.group, r0 = tile * kKvTileRows;
+    if (r0 >= rows) return;
+    const int total = s.past + s.n, gone = max(c.dropped[b], 0);
+    const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
+    const int prefix = a.prefix ? a.prefix[b] : 0;
+    const int64_t entry_row = (static_cast<int64_t>(b) * c.kv_heads + h) * c.max_blocks;
+    const int q0 = s.past + r0 / p.group, q1 = s.past + (min(r0 + kKvTileRows, rows) - 1) / p.group;
+    const KvRange range = kv_range(a, c.starts + entry_row, held, gone, q0, q1, prefix);
+    const int count = range.count();
+    const int chunk = max(p.chunk, (count + p.splits - 1) / p.splits);
+    const int begin = split * chunk, end = min(begin + chunk, count);
+    const int64_t slot = ((static_cast<int64_t>(b) * c.kv_heads + h) * p.row_tiles + tile) * p.splits + split;
+    if (begin >= end && p.splits > 1) {
+        if (tid < kKvTileRows) {
+            p.part_state[(slot * kKvTileRows + tid) * 2] = -__builtin_inff();
+            p.part_state[(slot * kKvTileRows + tid) * 2 + 1] = 0.0f;
+        }
+        return;
+    }
+
+    // this lane's row: column n of the products
+    const int row = min(r0 + n, rows - 1), head = h * p.group + row % p.group;
+    const int qpos = s.past + row / p.group;
+    half8 q[kParts][D / 32];
+    float unit;  // score per unit of (query as held) . (key codes), without the key scale
+    {
+        const T* src = static_cast<const T*>(a.q) + (s.row0 + row / p.group) * a.q_row + head * a.q_head;
+        float x[D / 32][8], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            load8<TYPE>(src + i / 2 * 64 + quad * 16 + i % 2 * 8, p.vec_q, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+        }
+        const float power = row_power(max_over_quads(top));
+        unit = a.scale / power;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = x[i][e] * power;
+                q[0][i][e] = static_cast<_Float16>(v);
+                if constexpr (PAIR) q[1][i][e] = static_cast<_Float16>(v - static_cast<float>(q[0][i][e]));
+            }
+    }
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+
+    float top = -__builtin_inff(), sum = 0.0f;
+    float4v o[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i] = float4v{0, 0, 0, 0};
+
+    for (int base = begin; base < end; base += 64 * kWaves) {
+        // lane l looks up the wave's l-th block
+        const int mine = base + lane * kWaves + wave;
+        int my_page = 0, my_start = 0;
+        float my_sk = 0.0f, my_sv = 0.0f;
+        if (mine < end) {
+            const int at = range.entry(mine);
+            const int page = c.table[entry_row + at];
+            const bool ok = page >= 0 && page < c.n_pages;
+            my_page = ok ? page : 0;
+            my_start = c.starts[entry_row + at];
+            const float2 sc = reinterpret_cast<const float2*>(c.scales)[my_page];
+            my_sk = kv_scale(sc.x, ok);
+            my_sv = kv_scale(sc.y, ok);
+        }
+        const int here = (min(end - base, 64 * kWaves) - wave + kWaves - 1) / kWaves;  // the wave's blocks
+        BlockRegs<D> next;
+        if (here > 0) load_block<D>(c.pages, __builtin_amdgcn_readlane(my_page, 0), lane, next);
+        for (int k = 0; k < here; ++k) {
+            const BlockRegs<D> cur = next;
+            if (k + 1 < here) load_block<D>(c.pages, __builtin_amdgcn_readlane(my_page, k + 1), lane, next);
+            const int start = __builtin_amdgcn_readlane(my_start, k);
+            const float sk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_sk), k));
+            const float sv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_sv), k));
+            float4v x[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                x[t] = float4v{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const uint4 raw = cur.k[t][i / 2];
+                    const half8 key = i % 2 ? codes_to_half(raw.z, raw.w) : codes_to_half(raw.x, raw.y);
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part)
+                        x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[part][i], x[t], 0, 0, 0);
+                }
+            }
+            // scores in powers of two: x[t][i] is token 16 t + 4 quad + i
+            const bool plain = a.softcap == 0.0f && !a.slopes;
+            float factor = unit * sk * kLog2e;
+            if (!plain) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float y = x[t][i] * (unit * sk);
+                        if (a.softcap != 0.0f) y = a.softcap * tanhf(y / a.softcap);
+                        if (a.slopes) y += slope * static_cast<float>(start + t * 16 + quad * 4 + i - qpos);
+                        x[t][i] = y;
+                    }
+                factor = kLog2e;
+            }
+            const float lift = __log2f(sv);
+            float most = -__builtin_inff();
+            const bool folded = !kv_all_seen(a, start, q0, q1, prefix, total);
+            if (!folded) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = fmaxf(most, __builtin_fmaf(x[t][i], factor, lift));
+            } else {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool seen = kv_seen(a, start + t * 16 + quad * 4 + i, qpos, prefix, total);
+                        // a masked score is -inf whatever its factor: NaN and the sign of `factor` included
+                        x[t][i] = seen ? __builtin_fmaf(x[t][i], factor, lift) : -__builtin_inff();
+                        most = fmaxf(most, x[t][i]);
+                    }
+                factor = 1.0f;
+            }
+            most = max_over_quads(most);
+            const float now = fmaxf(top, most);
+            const float ref = now == -__builtin_inff() ? 0.0f : now;
+            if (__any(now != top)) {
+                const float keep = exp2_fast(top - ref);
+                sum *= keep;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[i] *= keep;
+                top = now;
+            }
+            const float shift = (folded ? 0.0f : lift) - ref;
+            float e[8], got = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    e[t * 4 + i] = exp2_fast(__builtin_fmaf(x[t][i], factor, shift));
+                    got += e[t * 4 + i];
+                }
+            bhalf8 w[kWeightParts];
+            split_bhalf(e, w);
+            got = got == 0.0f ? 0.0f : got / sv;
+            sum += got;
+            if (p.block_sums) {
+                const float all = sum_over_quads(got);
+                if (quad == 0 && r0 + n < rows) {
+                    const int64_t at = (entry_row + range.entry(base + k * kWaves + wave)) * (p.row_tiles * kKvTileRows) + r0 + n;
+                    reinterpret_cast<float2*>(p.block_sums)[at] = make_float2(all, ref);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const uint4 raw = cur.v[i / 2];
+                const bhalf8 value = i % 2 ? codes_to_bhalf(raw.z, raw.w) : codes_to_bhalf(raw.x, raw.y);
+#pragma unroll
+                for (int part = 0; part < kWeightParts; ++part)
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, w[part], o[i], 0, 0, 0);
+            }
+        }
+    }
+
+    // join the waves
+    sum = sum_over_quads(sum);
+    if (quad == 0) {
+        state[wave][n][0] = top;
+        state[wave][n][1] = sum;
+    }
+    __syncthreads();
+    float most = state[0][n][0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, state[w][n][0]);
+    const float ref = most == -__builtin_inff() ? 0.0f : most;
+    const float keep = exp2_fast(top - ref);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+        *reinterpret_cast<float4v*>(&sums[wave][n][i * 16 + quad * 4]) = o[i] * keep;
+    __syncthreads();
+    for (int i = tid; i < kKvTileRows * D / 4; i += 64 * kWaves) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        if (r0 + r >= rows) break;
+        float4v acc = *reinterpret_cast<float4v*>(&sums[0][r][d]);
+        float m = state[0][r][0], l = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            acc += *reinterpret_cast<float4v*>(&sums[w][r][d]);
+            m = fmaxf(m, state[w][r][0]);
+        }
+        const float at = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) l += state[w][r][1] * exp2_fast(state[w][r][0] - at);
+        if (p.splits > 1 || p.block_sums) {
+            if (d == 0) {
+                p.part_state[(slot * kKvTileRows + r) * 2] = m;
+                p.part_state[(slot * kKvTileRows + r) * 2 + 1] = l;
+            }
+        }
+        if (p.splits > 1) {
+            *reinterpret_cast<float4v*>(p.part_out + (slot * kKvTileRows + r) * D + d) = acc;
+        } else {
+            const int rr = r0 + r, hd = h * p.group + rr % p.group;
+            T* out = static_cast<T*>(a.out) + (s.row0 + rr / p.group) * a.out_row + hd * a.out_head + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = K::from_f32(l == 0.0f ? 0.0f : acc[e] / l);
+        }
+    }
+}
+
+// Joins the splits: the first workgroups a wave per row, the others (with block
+// weights) a thread per block.
+template <int TYPE, int D>
+__global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_blocks) {
+    using K = KvType<TYPE>;
+    using T = typename K::T;
+    const rocknpu_kv_cache& c = p.c;
+    const rocknpu_kv_attention_args& a = p.a;
+    __shared__ float final_state[kKvMaxWeightRows][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.y, b = blockIdx.z;
+    const KvSpan s = kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new));
+    const int rows = s.n * p.group;
+    const int64_t seq = static_cast<int64_t>(b) * c.kv_heads + h;
+    // maximum and sum of a row over its splits
+    const auto join = [&](int r, float& most, float& total) {
+        const float* st = p.part_state + ((seq * p.row_tiles + r / kKvTileRows) * p.splits * kKvTileRows + r % kKvTileRows) * 2;
+        most = -__builtin_inff();
+        for (int i = lane; i < p.splits; i += 64) most = fmaxf(most, st[static_cast<int64_t>(i) * kKvTileRows * 2]);
+        most = wave_max(most);
+        const float ref = most == -__builtin_inff() ? 0.0f : most;
+        total = 0.0f;
+        for (int i = lane; i < p.splits; i += 64) {
+            const float* at = st + static_cast<int64_t>(i) * kKvTileRows * 2;
+            total += at[1] * exp2_fast(at[0] - ref);
+        }
+#pragma unroll
+        for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
+        most = ref;
+    };
+    if (static_cast<int>(blockIdx.x) < row_blocks) {
+        const int r = blockIdx.x * 4 + wave;
+        if (r >= rows) return;
+        float ref, l;
+        join(r, ref, l);
+        float acc[D / 64] = {};
+        const int64_t slot0 = (seq * p.row_tiles + r / kKvTileRows) * p.splits;
+        for (int i = 0; i < p.splits; ++i) {
+            const int64_t at = (slot0 + i) * kKvTileRows + r % kKvTileRows;
+            const float m = p.part_state[at * 2];
+            if (m == -__builtin_inff() && p.part_state[at * 2 + 1] == 0.0f) continue;  // a split without blocks wrote no sums
+            const float keep = exp2_fast(m - ref);
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) acc[e] += keep * p.part_out[at * D + e * 64 + lane];
+        }
+        const int hd = h * p.group + r % p.group;
+        T* out = static_cast<T*>(a.out) + (s.row0 + r / p.group) * a.out_row + hd * a.out_head;
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) out[e * 64 + lane] = K::from_f32(l == 0.0f ? 0.0f : acc[e] / l);
+        return;
+    }
+    for (int r = wave; r < rows; r += 4) {
+        float ref, l;
+        join(r, ref, l);
+        if (lane == 0) {
+            final_state[r][0] = ref;
+            final_state[r][1] = l;
+        }
+    }
+    __syncthreads();
+    const int at = (blockIdx.x - row_blocks) * 256 + tid;
+    if (at >= c.max_blocks) return;
+    const int64_t entry = seq * c.max_blocks + at;
+    float got = 0.0f;
+    const int total = s.past + s.n, gone = max(c.dropped[b], 0);
+    if (at < min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks)) {
+        const int start = c.starts[entry], prefix = a.prefix ? a.prefix[b] : 0;
+        for (int tile = 0; tile * kKvTileRows < rows; ++tile) {
+            const int r0 = tile * kKvTileRows, r1 = min(r0 + kKvTileRows, rows);
+            // the blocks that kv_range gave the tile
+            const int q0 = s.past + r0 / p.group, q1 = s.past + (r1 - 1) / p.group;
+            if (a.causal && start >= prefix &&
+                (start > q1 || (a.window != 0 && start + kKvBlock <= q0 - a.window + 1)))
+                continue;
+            const float2* sums = reinterpret_cast<const float2*>(p.block_sums) + entry * (p.row_tiles * kKvTileRows);
+            for (int r = r0; r < r1; ++r) {
+                const float2 x = sums[r];
+                if (x.x != 0.0f) got += x.x * exp2_fast(x.y - final_state[r][0]) / final_state[r][1];
+            }
+        }
+    }
+    a.weights_out[entry] = c.weights[entry] + got;
+}
+
+template <int TYPE, int D>
+int launch(const KvAttend& p, hipStream_t stream) {
+    const unsigned heads = p.c.kv_heads, batch = p.c.batch;
+    if (p.a.rows > 0 && p.a.max_new > 0)
+        kv_stream_kernel<TYPE, D><<<dim3(p.splits, heads, batch * p.row_tiles), 64 * kWaves, 0, stream>>>(p);
+    const int row_blocks = p.splits > 1 ? (p.row_tiles * kKvTileRows + 3) / 4 : 0;
+    const int weight_blocks = p.a.weights_out ? (p.c.max_blocks + 255) / 256 : 0;
+    if (row_blocks + weight_blocks > 0)
+        kv_join_kernel<TYPE, D><<<dim3(row_blocks + weight_blocks, heads, batch), 256, 0, stream>>>(p, row_blocks);
+    return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
+}
+
+template <int TYPE>
+int launch_dim(const KvAttend& p, hipStream_t stream) {
+    switch (p.c.head_dim) {
+        case 64: return launch<TYPE, 64>(p, stream);
+        case 128: return launch<TYPE, 128>(p, stream);
+        case 192: return launch<TYPE, 192>(p, stream);
+        default: return launch<TYPE, 256>(p, stream);
+    }
+}
+
+}  // namespace
+
+int launch_kv_stream(const KvAttend& p, hipStream_t stream) {
+    switch (p.a.type) {
+        case ROCKNPU_KV_F32: return launch_dim<ROCKNPU_KV_F32>(p, stream);
+        case ROCKNPU_KV_F16: return launch_dim<ROCKNPU_KV_F16>(p, stream);
+        default: return launch_dim<ROCKNPU_KV_BF16>(p, stream);
+    }
+}
+
+}  // namespace rk

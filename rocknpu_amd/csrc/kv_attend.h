@@ -15,6 +15,7 @@
 namespace rk {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kKvMaxSplits = 256;  // workgroups that share a tile's blocks, at most
 constexpr int kKvTileRows = 16;  // rows of a tile of the streaming kernel
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -27,11 +28,12 @@ struct KvAttend {
     rocknpu_kv_attention_args a;
     int group;       // heads per kv head
     int row_tiles;   // tiles of rows that a sequence and kv head may have
-    int splits;      // workgroups that share a tile's blocks
-    int chunk;       // blocks per split, at least
+    int share;       // workgroups that the sequences share, per kv head and row tile; 0: one each
+    int slots;       // workgroups in all per kv head and row tile: share + batch, or batch
+    int min_chunk;   // blocks per workgroup, at least
     bool vec_q, vec_out;
-    // workspace, one entry per (sequence, kv head, row tile, split): sums of the output [rows][head_dim], maxima and
-    // sums [rows][2]; one per (sequence, kv head, block, row): its weight's sum and the maximum it refers to
+    // workspace, one entry per (kv head, row tile, slot): sums of the output [rows][head_dim], maxima and sums
+    // [rows][2]; one per (sequence, kv head, block, row): its weight's sum and the maximum it refers to
     float* part_out;
     float* part_state;
     float* block_sums;
@@ -82,6 +84,62 @@ __device__ __forceinline__ KvRange kv_range(const rocknpu_kv_attention_args& a, 
     r.from = min(gone ? starts_below(starts, held, from_start) : from_start / kKvBlock, r.to);
     if (prefix > 0) r.first = min(gone ? starts_below(starts, held, prefix) : (prefix + kKvBlock - 1) / kKvBlock, r.from);
     return r;
+}
+
+// Which sequence a slot works on, and which of the sequence's `splits` parts it
+// takes (seq < 0: none). Every sequence with rows gets one slot for each `chunk`
+// blocks that its rows may see, where chunk is such that all of them come to
+// about p.share slots: a batch of unequal lengths loads the GPU evenly. All
+// slots of a launch, and the join behind them, work out the same division.
+struct KvSlot {
+    int seq, split, splits, first;
+};
+__device__ __forceinline__ int kv_blocks_estimate(const KvAttend& p, int b) {
+    const KvSpan s = kv_span(p.a.past, p.a.cu, b, static_cast<int>(p.a.rows), static_cast<int>(p.a.max_new));
+    if (s.n == 0) return 0;
+    int blocks = min((s.past + s.n + kKvBlock - 1) / kKvBlock - max(p.c.dropped[b], 0), p.c.max_blocks);
+    if (p.a.window > 0) {
+        const int prefix = p.a.prefix ? min(max(p.a.prefix[b], 0), 0x3fffffff) : 0;
+        blocks = min(blocks, min(p.a.window, 0x3fffffff) / kKvBlock + (s.n + prefix) / kKvBlock + 3);
+    }
+    return max(blocks, 1);
+}
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+    return x;
+}
+// `want`: the slot asked for, or -1 - b for sequence b's first slot.
+__device__ __forceinline__ KvSlot kv_slot(const KvAttend& p, int want) {
+    const int lane = threadIdx.x & 63, batch = p.c.batch;
+    if (p.share == 0) {
+        const int b = want < 0 ? -1 - want : want;
+        return KvSlot{b, 0, 1, b};
+    }
+    int all = 0;
+    for (int base = 0; base < batch; base += 64) all += base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
+    all = wave_sum(all);
+    const int chunk = max(p.min_chunk, (all + p.share - 1) / p.share);
+    int before = 0;
+    for (int base = 0; base < batch; base += 64) {
+        const int blocks = base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
+        const int splits = min((blocks + chunk - 1) / chunk, kKvMaxSplits);
+        int upto = splits;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += y;
+        }
+        upto += before;
+        const uint64_t hit = want < 0 ? __ballot(base + lane == -1 - want) : __ballot(want < upto);
+        if (hit) {
+            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            const int end = __shfl(upto, l, 64), n = __shfl(splits, l, 64);
+            return KvSlot{base + l, want < 0 ? 0 : want - (end - n), n, end - n};
+        }
+        before = __shfl(upto, 63, 64);
+    }
+    return KvSlot{-1, 0, 0, 0};
 }
 
 // Whether a row at qpos sees the key at kpos.

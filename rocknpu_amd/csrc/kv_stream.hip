@@ -14,6 +14,7 @@ namespace rk {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kMaxSplits = kKvMaxSplits;
 
 template <int D>
 struct BlockRegs {
@@ -56,7 +57,10 @@ __global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
     __shared__ float state[kWaves][kKvTileRows][2];
     __shared__ alignas(16) float sums[kWaves][kKvTileRows][D + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane % 16, quad = lane / 16;
-    const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z / p.row_tiles, tile = blockIdx.z % p.row_tiles;
+    const int h = blockIdx.y, tile = blockIdx.z;
+    const KvSlot mine = kv_slot(p, blockIdx.x);
+    const int b = mine.seq;
+    if (b < 0) return;
     const KvSpan s = kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new));
     const int rows = s.n * p.group, r0 = tile * kKvTileRows;
     if (r0 >= rows) return;
@@ -67,10 +71,10 @@ __global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
     const int q0 = s.past + r0 / p.group, q1 = s.past + (min(r0 + kKvTileRows, rows) - 1) / p.group;
     const KvRange range = kv_range(a, c.starts + entry_row, held, gone, q0, q1, prefix);
     const int count = range.count();
-    const int chunk = max(p.chunk, (count + p.splits - 1) / p.splits);
-    const int begin = split * chunk, end = min(begin + chunk, count);
-    const int64_t slot = ((static_cast<int64_t>(b) * c.kv_heads + h) * p.row_tiles + tile) * p.splits + split;
-    if (begin >= end && p.splits > 1) {
+    const int chunk = (count + mine.splits - 1) / mine.splits;
+    const int begin = mine.split * chunk, end = min(begin + chunk, count);
+    const int64_t slot = (static_cast<int64_t>(h) * p.row_tiles + tile) * p.slots + blockIdx.x;
+    if (begin >= end && mine.splits > 1) {
         if (tid < kKvTileRows) {
             p.part_state[(slot * kKvTileRows + tid) * 2] = -__builtin_inff();
             p.part_state[(slot * kKvTileRows + tid) * 2 + 1] = 0.0f;
@@ -112,11 +116,11 @@ __global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
 
     for (int base = begin; base < end; base += 64 * kWaves) {
         // lane l looks up the wave's l-th block
-        const int mine = base + lane * kWaves + wave;
+        const int nth = base + lane * kWaves + wave;
         int my_page = 0, my_start = 0;
         float my_sk = 0.0f, my_sv = 0.0f;
-        if (mine < end) {
-            const int at = range.entry(mine);
+        if (nth < end) {
+            const int at = range.entry(nth);
             const int page = c.table[entry_row + at];
             const bool ok = page >= 0 && page < c.n_pages;
             my_page = ok ? page : 0;
@@ -252,13 +256,13 @@ __global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
         const float at = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) l += state[w][r][1] * exp2_fast(state[w][r][0] - at);
-        if (p.splits > 1 || p.block_sums) {
+        if (mine.splits > 1 || p.block_sums) {
             if (d == 0) {
                 p.part_state[(slot * kKvTileRows + r) * 2] = m;
                 p.part_state[(slot * kKvTileRows + r) * 2 + 1] = l;
             }
         }
-        if (p.splits > 1) {
+        if (mine.splits > 1) {
             *reinterpret_cast<float4v*>(p.part_out + (slot * kKvTileRows + r) * D + d) = acc;
         } else {
             const int rr = r0 + r, hd = h * p.group + rr % p.group;
@@ -269,66 +273,93 @@ __global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
     }
 }
 
-// Joins the splits: the first workgroups a wave per row, the others (with block
-// weights) a thread per block.
+// Joins the splits of a tile's rows: the first workgroups take a row each, its
+// splits' sums read side by side (all of a row's loads are in flight together),
+// the others (with block weights) a block per thread.
 template <int TYPE, int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_blocks) {
+__global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups) {
     using K = KvType<TYPE>;
     using T = typename K::T;
+    constexpr int kPer = D / 4;                 // threads that read a split's row
+    constexpr int kBeside = 256 / kPer;         // splits read side by side
     const rocknpu_kv_cache& c = p.c;
     const rocknpu_kv_attention_args& a = p.a;
     __shared__ float final_state[kKvMaxWeightRows][2];
+    __shared__ float keep[kMaxSplits];
+    __shared__ alignas(16) float part[kBeside][D];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.y, b = blockIdx.z;
     const KvSpan s = kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new));
     const int rows = s.n * p.group;
     const int64_t seq = static_cast<int64_t>(b) * c.kv_heads + h;
-    // maximum and sum of a row over its splits
-    const auto join = [&](int r, float& most, float& total) {
-        const float* st = p.part_state + ((seq * p.row_tiles + r / kKvTileRows) * p.splits * kKvTileRows + r % kKvTileRows) * 2;
-        most = -__builtin_inff();
-        for (int i = lane; i < p.splits; i += 64) most = fmaxf(most, st[static_cast<int64_t>(i) * kKvTileRows * 2]);
-        most = wave_max(most);
-        const float ref = most == -__builtin_inff() ? 0.0f : most;
-        total = 0.0f;
-        for (int i = lane; i < p.splits; i += 64) {
-            const float* at = st + static_cast<int64_t>(i) * kKvTileRows * 2;
-            total += at[1] * exp2_fast(at[0] - ref);
-        }
-#pragma unroll
-        for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
-        most = ref;
+    if (static_cast<int>(blockIdx.x) < row_groups && static_cast<int>(blockIdx.x) >= rows) return;
+    const KvSlot slot = kv_slot(p, -1 - b);
+    const auto slot_of = [&](int r) { return (static_cast<int64_t>(h) * p.row_tiles + r / kKvTileRows) * p.slots + slot.first; };
+    const auto state_of = [&](int r) {
+        return reinterpret_cast<const float2*>(p.part_state) + slot_of(r) * kKvTileRows + r % kKvTileRows;
     };
-    if (static_cast<int>(blockIdx.x) < row_blocks) {
-        const int r = blockIdx.x * 4 + wave;
-        if (r >= rows) return;
-        float ref, l;
-        join(r, ref, l);
-        float acc[D / 64] = {};
-        const int64_t slot0 = (seq * p.row_tiles + r / kKvTileRows) * p.splits;
-        for (int i = 0; i < p.splits; ++i) {
-            const int64_t at = (slot0 + i) * kKvTileRows + r % kKvTileRows;
-            const float m = p.part_state[at * 2];
-            if (m == -__builtin_inff() && p.part_state[at * 2 + 1] == 0.0f) continue;  // a split without blocks wrote no sums
-            const float keep = exp2_fast(m - ref);
+    if (static_cast<int>(blockIdx.x) < row_groups) {
+        const int r = blockIdx.x;
+        if (slot.splits <= 1) return;  // its only workgroup wrote the row
+        if (wave == 0) {
+            const float2* st = state_of(r);
+            float most = -__builtin_inff(), total = 0.0f;
+            float2 mine[kMaxSplits / 64];
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e) acc[e] += keep * p.part_out[at * D + e * 64 + lane];
+            for (int k = 0; k < kMaxSplits / 64; ++k) {
+                const int i = k * 64 + lane;
+                mine[k] = i < slot.splits ? st[i * kKvTileRows] : make_float2(-__builtin_inff(), 0.0f);
+                most = fmaxf(most, mine[k].x);
+            }
+            most = wave_max(most);
+            const float ref = most == -__builtin_inff() ? 0.0f : most;
+#pragma unroll
+            for (int k = 0; k < kMaxSplits / 64; ++k) total += mine[k].y * exp2_fast(mine[k].x - ref);
+#pragma unroll
+            for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
+            // a split without blocks wrote no sums: its factor is 0 and its sums are not read
+#pragma unroll
+            for (int k = 0; k < kMaxSplits / 64; ++k)
+                if (k * 64 + lane < slot.splits)
+                    keep[k * 64 + lane] = mine[k].y == 0.0f ? 0.0f : exp2_fast(mine[k].x - ref) / total;
         }
-        const int hd = h * p.group + r % p.group;
-        T* out = static_cast<T*>(a.out) + (s.row0 + r / p.group) * a.out_row + hd * a.out_head;
+        __syncthreads();
+        const int d = tid % kPer * 4, beside = tid / kPer;
+        float4v acc = {0, 0, 0, 0};
+        if (beside < kBeside) {
+            const float* from = p.part_out + (slot_of(r) * kKvTileRows + r % kKvTileRows) * D + d;
+#pragma unroll 4
+            for (int i = beside; i < slot.splits; i += kBeside) {
+                const float f = keep[i];
+                if (f != 0.0f) acc += f * *reinterpret_cast<const float4v*>(from + static_cast<int64_t>(i) * kKvTileRows * D);
+            }
+            *reinterpret_cast<float4v*>(&part[beside][d]) = acc;
+        }
+        __syncthreads();
+        if (tid < D) {
+            float x = 0.0f;
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) out[e * 64 + lane] = K::from_f32(l == 0.0f ? 0.0f : acc[e] / l);
+            for (int i = 0; i < kBeside; ++i) x += part[i][tid];
+            const int hd = h * p.group + r % p.group;
+            static_cast<T*>(a.out)[(s.row0 + r / p.group) * a.out_row + hd * a.out_head + tid] = K::from_f32(x);
+        }
         return;
     }
     for (int r = wave; r < rows; r += 4) {
-        float ref, l;
-        join(r, ref, l);
+        const float2* st = state_of(r);
+        float most = -__builtin_inff(), total = 0.0f;
+        for (int i = lane; i < slot.splits; i += 64) most = fmaxf(most, st[i * kKvTileRows].x);
+        most = wave_max(most);
+        const float ref = most == -__builtin_inff() ? 0.0f : most;
+        for (int i = lane; i < slot.splits; i += 64) total += st[i * kKvTileRows].y * exp2_fast(st[i * kKvTileRows].x - ref);
+#pragma unroll
+        for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
         if (lane == 0) {
             final_state[r][0] = ref;
-            final_state[r][1] = l;
+            final_state[r][1] = total;
         }
     }
     __syncthreads();
-    const int at = (blockIdx.x - row_blocks) * 256 + tid;
+    const int at = (blockIdx.x - row_groups) * 256 + tid;
     if (at >= c.max_blocks) return;
     const int64_t entry = seq * c.max_blocks + at;
     float got = 0.0f;
@@ -356,11 +387,11 @@ template <int TYPE, int D>
 int launch(const KvAttend& p, hipStream_t stream) {
     const unsigned heads = p.c.kv_heads, batch = p.c.batch;
     if (p.a.rows > 0 && p.a.max_new > 0)
-        kv_stream_kernel<TYPE, D><<<dim3(p.splits, heads, batch * p.row_tiles), 64 * kWaves, 0, stream>>>(p);
-    const int row_blocks = p.splits > 1 ? (p.row_tiles * kKvTileRows + 3) / 4 : 0;
-    const int weight_blocks = p.a.weights_out ? (p.c.max_blocks + 255) / 256 : 0;
-    if (row_blocks + weight_blocks > 0)
-        kv_join_kernel<TYPE, D><<<dim3(row_blocks + weight_blocks, heads, batch), 256, 0, stream>>>(p, row_blocks);
+        kv_stream_kernel<TYPE, D><<<dim3(p.slots, heads, p.row_tiles), 64 * kWaves, 0, stream>>>(p);
+    const int row_groups = p.part_out ? static_cast<int>(p.a.max_new) * p.group : 0;
+    const int weight_groups = p.a.weights_out ? (p.c.max_blocks + 255) / 256 : 0;
+    if (row_groups + weight_groups > 0)
+        kv_join_kernel<TYPE, D><<<dim3(row_groups + weight_groups, heads, batch), 256, 0, stream>>>(p, row_groups);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 

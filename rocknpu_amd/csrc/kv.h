@@ -66,6 +66,10 @@ __device__ __forceinline__ KvSpan kv_span(const int32_t* past, const int32_t* cu
     return s;
 }
 
+// A value that is the same in every lane, into a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ KvSpan uniform(KvSpan s) { return KvSpan{uniform(s.past), uniform(s.row0), uniform(s.n)}; }
+
 // Whether a cache description is one that the kernels can take. kv_cache.hip.
 bool kv_cache_ok(const rocknpu_kv_cache* c);
 

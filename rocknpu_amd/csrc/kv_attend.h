@@ -28,6 +28,7 @@ struct KvAttend {
     rocknpu_kv_attention_args a;
     int group;       // heads per kv head
     int row_tiles;   // tiles of rows that a sequence and kv head may have
+    int tile_rows;
     int share;       // workgroups that the sequences share, per kv head and row tile; 0: one each
     int slots;       // workgroups in all per kv head and row tile: share + batch, or batch
     int min_chunk;   // blocks per workgroup, at least
@@ -77,12 +78,14 @@ __device__ __forceinline__ KvRange kv_range(const rocknpu_kv_attention_args& a, 
     const int last = max(q1, prefix - 1);
     r.to = min(held, max(last / kKvBlock + 1 - gone, 0));
     if (gone && last / kKvBlock + 1 - gone < held) r.to = starts_below(starts, held, last + 1);
+    r.to = uniform(r.to);
     if (a.window == 0) return r;
     const int lowest = q0 - a.window + 1;  // first position that a row's window holds
     if (lowest <= 0) return r;
     const int from_start = lowest / kKvBlock * kKvBlock;
     r.from = min(gone ? starts_below(starts, held, from_start) : from_start / kKvBlock, r.to);
-    if (prefix > 0) r.first = min(gone ? starts_below(starts, held, prefix) : (prefix + kKvBlock - 1) / kKvBlock, r.from);
+    r.from = uniform(r.from);
+    if (prefix > 0) r.first = uniform(min(gone ? starts_below(starts, held, prefix) : (prefix + kKvBlock - 1) / kKvBlock, r.from));
     return r;
 }
 
@@ -118,7 +121,7 @@ __device__ __forceinline__ KvSlot kv_slot(const KvAttend& p, int want) {
     }
     int all = 0;
     for (int base = 0; base < batch; base += 64) all += base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
-    all = wave_sum(all);
+    all = uniform(wave_sum(all));
     const int chunk = max(p.min_chunk, (all + p.share - 1) / p.share);
     int before = 0;
     for (int base = 0; base < batch; base += 64) {
@@ -131,13 +134,13 @@ __device__ __forceinline__ KvSlot kv_slot(const KvAttend& p, int want) {
             if (lane >= o) upto += y;
         }
         upto += before;
-        const uint64_t hit = want < 0 ? __ballot(base + lane == -1 - want) : __ballot(want < upto);
+        const unsigned long long hit = want < 0 ? __ballot(base + lane == -1 - want) : __ballot(want < upto);
         if (hit) {
-            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-            const int end = __shfl(upto, l, 64), n = __shfl(splits, l, 64);
+            const int l = uniform(__ffsll(hit) - 1);
+            const int end = __builtin_amdgcn_readlane(upto, l), n = __builtin_amdgcn_readlane(splits, l);
             return KvSlot{base + l, want < 0 ? 0 : want - (end - n), n, end - n};
         }
-        before = __shfl(upto, 63, 64);
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
     return KvSlot{-1, 0, 0, 0};
 }
@@ -248,6 +251,11 @@ __device__ __forceinline__ float row_power(float top) {
     return __uint_as_float(static_cast<uint32_t>(127 + min(max(13 - e, -114), 120)) << 23);
 }
 
-int launch_kv_stream(const KvAttend& p, hipStream_t stream);   // kv_stream.hip
+// kv_stream.hip: tiles of kKvTileRows rows; kv_prompt.hip: of kv_prompt_tile rows.
+int launch_kv_stream(const KvAttend& p, hipStream_t stream);
+int kv_prompt_tile(int head_dim);
+int launch_kv_prompt(const KvAttend& p, hipStream_t stream);
+// Joins the parts that either left, and the block weights. kv_stream.hip.
+int launch_kv_join(const KvAttend& p, hipStream_t stream);
 
 }  // namespace rk

@@ -61,12 +61,12 @@ __global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
     const KvSlot mine = kv_slot(p, blockIdx.x);
     const int b = mine.seq;
     if (b < 0) return;
-    const KvSpan s = kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new));
+    const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
     const int rows = s.n * p.group, r0 = tile * kKvTileRows;
     if (r0 >= rows) return;
-    const int total = s.past + s.n, gone = max(c.dropped[b], 0);
+    const int total = s.past + s.n, gone = uniform(max(c.dropped[b], 0));
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
-    const int prefix = a.prefix ? a.prefix[b] : 0;
+    const int prefix = a.prefix ? uniform(a.prefix[b]) : 0;
     const int64_t entry_row = (static_cast<int64_t>(b) * c.kv_heads + h) * c.max_blocks;
     const int q0 = s.past + r0 / p.group, q1 = s.past + (min(r0 + kKvTileRows, rows) - 1) / p.group;
     const KvRange range = kv_range(a, c.starts + entry_row, held, gone, q0, q1, prefix);
@@ -288,14 +288,14 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     __shared__ float keep[kMaxSplits];
     __shared__ alignas(16) float part[kBeside][D];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.y, b = blockIdx.z;
-    const KvSpan s = kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new));
+    const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
     const int rows = s.n * p.group;
     const int64_t seq = static_cast<int64_t>(b) * c.kv_heads + h;
     if (static_cast<int>(blockIdx.x) < row_groups && static_cast<int>(blockIdx.x) >= rows) return;
     const KvSlot slot = kv_slot(p, -1 - b);
-    const auto slot_of = [&](int r) { return (static_cast<int64_t>(h) * p.row_tiles + r / kKvTileRows) * p.slots + slot.first; };
+    const auto slot_of = [&](int r) { return (static_cast<int64_t>(h) * p.row_tiles + r / p.tile_rows) * p.slots + slot.first; };
     const auto state_of = [&](int r) {
-        return reinterpret_cast<const float2*>(p.part_state) + slot_of(r) * kKvTileRows + r % kKvTileRows;
+        return reinterpret_cast<const float2*>(p.part_state) + slot_of(r) * p.tile_rows + r % p.tile_rows;
     };
     if (static_cast<int>(blockIdx.x) < row_groups) {
         const int r = blockIdx.x;
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 64; ++k) {
                 const int i = k * 64 + lane;
-                mine[k] = i < slot.splits ? st[i * kKvTileRows] : make_float2(-__builtin_inff(), 0.0f);
+                mine[k] = i < slot.splits ? st[i * p.tile_rows] : make_float2(-__builtin_inff(), 0.0f);
                 most = fmaxf(most, mine[k].x);
             }
             most = wave_max(most);
@@ -326,11 +326,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
         const int d = tid % kPer * 4, beside = tid / kPer;
         float4v acc = {0, 0, 0, 0};
         if (beside < kBeside) {
-            const float* from = p.part_out + (slot_of(r) * kKvTileRows + r % kKvTileRows) * D + d;
+            const float* from = p.part_out + (slot_of(r) * p.tile_rows + r % p.tile_rows) * D + d;
 #pragma unroll 4
             for (int i = beside; i < slot.splits; i += kBeside) {
                 const float f = keep[i];
-                if (f != 0.0f) acc += f * *reinterpret_cast<const float4v*>(from + static_cast<int64_t>(i) * kKvTileRows * D);
+                if (f != 0.0f) acc += f * *reinterpret_cast<const float4v*>(from + static_cast<int64_t>(i) * p.tile_rows * D);
             }
             *reinterpret_cast<float4v*>(&part[beside][d]) = acc;
         }
@@ -347,10 +347,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     for (int r = wave; r < rows; r += 4) {
         const float2* st = state_of(r);
         float most = -__builtin_inff(), total = 0.0f;
-        for (int i = lane; i < slot.splits; i += 64) most = fmaxf(most, st[i * kKvTileRows].x);
+        for (int i = lane; i < slot.splits; i += 64) most = fmaxf(most, st[i * p.tile_rows].x);
         most = wave_max(most);
         const float ref = most == -__builtin_inff() ? 0.0f : most;
-        for (int i = lane; i < slot.splits; i += 64) total += st[i * kKvTileRows].y * exp2_fast(st[i * kKvTileRows].x - ref);
+        for (int i = lane; i < slot.splits; i += 64) total += st[i * p.tile_rows].y * exp2_fast(st[i * p.tile_rows].x - ref);
 #pragma unroll
         for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
         if (lane == 0) {
@@ -363,17 +363,17 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     if (at >= c.max_blocks) return;
     const int64_t entry = seq * c.max_blocks + at;
     float got = 0.0f;
-    const int total = s.past + s.n, gone = max(c.dropped[b], 0);
+    const int total = s.past + s.n, gone = uniform(max(c.dropped[b], 0));
     if (at < min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks)) {
-        const int start = c.starts[entry], prefix = a.prefix ? a.prefix[b] : 0;
-        for (int tile = 0; tile * kKvTileRows < rows; ++tile) {
-            const int r0 = tile * kKvTileRows, r1 = min(r0 + kKvTileRows, rows);
+        const int start = c.starts[entry], prefix = a.prefix ? uniform(a.prefix[b]) : 0;
+        for (int tile = 0; tile * p.tile_rows < rows; ++tile) {
+            const int r0 = tile * p.tile_rows, r1 = min(r0 + p.tile_rows, rows);
             // the blocks that kv_range gave the tile
             const int q0 = s.past + r0 / p.group, q1 = s.past + (r1 - 1) / p.group;
             if (a.causal && start >= prefix &&
                 (start > q1 || (a.window != 0 && start + kKvBlock <= q0 - a.window + 1)))
                 continue;
-            const float2* sums = reinterpret_cast<const float2*>(p.block_sums) + entry * (p.row_tiles * kKvTileRows);
+            const float2* sums = reinterpret_cast<const float2*>(p.block_sums) + entry * (p.row_tiles * p.tile_rows);
             for (int r = r0; r < r1; ++r) {
                 const float2 x = sums[r];
                 if (x.x != 0.0f) got += x.x * exp2_fast(x.y - final_state[r][0]) / final_state[r][1];
@@ -385,34 +385,42 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
 
 template <int TYPE, int D>
 int launch(const KvAttend& p, hipStream_t stream) {
-    const unsigned heads = p.c.kv_heads, batch = p.c.batch;
     if (p.a.rows > 0 && p.a.max_new > 0)
-        kv_stream_kernel<TYPE, D><<<dim3(p.slots, heads, p.row_tiles), 64 * kWaves, 0, stream>>>(p);
-    const int row_groups = p.part_out ? static_cast<int>(p.a.max_new) * p.group : 0;
-    const int weight_groups = p.a.weights_out ? (p.c.max_blocks + 255) / 256 : 0;
-    if (row_groups + weight_groups > 0)
-        kv_join_kernel<TYPE, D><<<dim3(row_groups + weight_groups, heads, batch), 256, 0, stream>>>(p, row_groups);
+        kv_stream_kernel<TYPE, D><<<dim3(p.slots, p.c.kv_heads, p.row_tiles), 64 * kWaves, 0, stream>>>(p);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
-template <int TYPE>
+template <int TYPE, int D>
+int launch_join(const KvAttend& p, hipStream_t stream) {
+    const int row_groups = p.part_out ? static_cast<int>(p.a.max_new) * p.group : 0;
+    const int weight_groups = p.a.weights_out ? (p.c.max_blocks + 255) / 256 : 0;
+    if (row_groups + weight_groups > 0)
+        kv_join_kernel<TYPE, D><<<dim3(row_groups + weight_groups, p.c.kv_heads, p.c.batch), 256, 0, stream>>>(p, row_groups);
+    return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
+}
+
+template <int TYPE, bool JOIN>
 int launch_dim(const KvAttend& p, hipStream_t stream) {
     switch (p.c.head_dim) {
-        case 64: return launch<TYPE, 64>(p, stream);
-        case 128: return launch<TYPE, 128>(p, stream);
-        case 192: return launch<TYPE, 192>(p, stream);
-        default: return launch<TYPE, 256>(p, stream);
+        case 64: return JOIN ? launch_join<TYPE, 64>(p, stream) : launch<TYPE, 64>(p, stream);
+        case 128: return JOIN ? launch_join<TYPE, 128>(p, stream) : launch<TYPE, 128>(p, stream);
+        case 192: return JOIN ? launch_join<TYPE, 192>(p, stream) : launch<TYPE, 192>(p, stream);
+        default: return JOIN ? launch_join<TYPE, 256>(p, stream) : launch<TYPE, 256>(p, stream);
+    }
+}
+
+template <bool JOIN>
+int launch_type(const KvAttend& p, hipStream_t stream) {
+    switch (p.a.type) {
+        case ROCKNPU_KV_F32: return launch_dim<ROCKNPU_KV_F32, JOIN>(p, stream);
+        case ROCKNPU_KV_F16: return launch_dim<ROCKNPU_KV_F16, JOIN>(p, stream);
+        default: return launch_dim<ROCKNPU_KV_BF16, JOIN>(p, stream);
     }
 }
 
 }  // namespace
 
-int launch_kv_stream(const KvAttend& p, hipStream_t stream) {
-    switch (p.a.type) {
-        case ROCKNPU_KV_F32: return launch_dim<ROCKNPU_KV_F32>(p, stream);
-        case ROCKNPU_KV_F16: return launch_dim<ROCKNPU_KV_F16>(p, stream);
-        default: return launch_dim<ROCKNPU_KV_BF16>(p, stream);
-    }
-}
+int launch_kv_stream(const KvAttend& p, hipStream_t stream) { return launch_type<false>(p, stream); }
+int launch_kv_join(const KvAttend& p, hipStream_t stream) { return launch_type<true>(p, stream); }
 
 }  // namespace rk

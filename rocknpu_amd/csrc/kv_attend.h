@@ -253,7 +253,7 @@ __device__ __forceinline__ float row_power(float top) {
 
 // kv_stream.hip: tiles of kKvTileRows rows; kv_prompt.hip: of kv_prompt_tile rows.
 int launch_kv_stream(const KvAttend& p, hipStream_t stream);
-int kv_prompt_tile(int head_dim);
+int kv_prompt_tile();
 int launch_kv_prompt(const KvAttend& p, hipStream_t stream);
 // Joins the parts that either left, and the block weights. kv_stream.hip.
 int launch_kv_join(const KvAttend& p, hipStream_t stream);

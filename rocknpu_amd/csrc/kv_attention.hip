@@ -53,7 +53,7 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.vec_out = aligned(a.out, 16) && a.out_row % per == 0 && a.out_head % per == 0;
     const int64_t rows = std::max<int64_t>(a.max_new, 1) * p.group;
     r.stream = rows <= kStreamRows || a.weights_out;
-    p.tile_rows = r.stream ? kKvTileRows : kv_prompt_tile(c.head_dim);
+    p.tile_rows = r.stream ? kKvTileRows : kv_prompt_tile();
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     int64_t blocks = a.max_tokens > 0 ? (a.max_tokens + kKvBlock - 1) / kKvBlock : c.max_blocks;
     if (a.window > 0) blocks = std::min<int64_t>(blocks, (static_cast<int64_t>(a.window) + a.max_new) / kKvBlock + 2);

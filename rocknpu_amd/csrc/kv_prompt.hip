@@ -1,19 +1,22 @@
 // Attention of many rows over the cache: prompts, and pieces of them.
 //
-// A workgroup takes a tile of rows of one sequence and kv head (the step's
-// tokens times the kv head's heads, so that keys and values serve all of them),
-// 32 rows a wave. Two blocks at a time pass through LDS: the codes are converted
-// once per workgroup, into the order in which v_mfma_f32_32x32x16 takes them,
-// while the blocks before are worked on and those behind are on their way from
-// memory. Scores: keys (32 tokens x 16 dims) times queries; a lane ends up with
-// 16 tokens of one row, so maximum and sum are per lane but for one exchange,
-// and the weights are the second operand of the next product, values (32 dims x
-// 16 tokens) times weights, as they stand.
+// A workgroup of four waves takes a tile of rows of one sequence and kv head
+// (the step's tokens times the kv head's heads, so that keys and values serve
+// all of them), 32 rows a wave. Blocks pass through LDS one by one: a block's
+// codes are converted once per workgroup, into the order in which
+// v_mfma_f32_32x32x16 takes them. Scores: keys (32 tokens x 16 dims) times
+// queries; a lane ends up with 16 tokens of one row, so maximum and sum are per
+// lane but for one exchange, and the weights are the second operand of the next
+// product, values (32 dims x 16 tokens) times weights, as they stand.
 //
-// Per block and wave D/16 + D/16 matrix instructions of 32 cycles, and for each
-// of a lane's 16 scores a fused multiply-add, an exponential (16 cycles), half a
-// maximum, conversion and sum each: matrix and vector units are both near their
-// rate with 128 dims, the vector unit is what bounds 64 dims.
+// Per block a wave has D/8 products of 32 cycles; for each of a lane's 16 scores
+// a fused multiply-add, an exponential (16 cycles), half a maximum, conversion
+// and sum; and its share of the conversion. Both units stay busy because a wave
+// takes block j's exponentials between the products of block j + 1's scores and
+// the conversion of block j + 2 between the products of block j's values, and
+// because the CU's two workgroups are not in step.
+#include <type_traits>
+
 #include "kv_attend.h"
 
 namespace rk {
@@ -26,23 +29,21 @@ typedef float float2v __attribute__((ext_vector_type(2)));
 // maximum only when that grows by more than kSlack: rescaling the output costs
 // as much as a block's exponentials. 2^(kBias + kSlack) stays below f16's 65504.
 constexpr float kBias = 9.0f, kSlack = 6.0f;
+// the reference of a row that has seen nothing yet: 2^-inf over it is 0, and so is 2^it over any other
+constexpr float kNothing = -1e30f;
 // bytes of a 512-byte run of operands in LDS, padded so that the writers' 8
 // lanes a cycle meet 8 different 16-byte columns
 constexpr int kKeyRun = 528, kValueRun = 544;
 
-template <int D>
-constexpr int prompt_waves() { return D <= 128 ? 8 : 4; }
+// operands are read from LDS this many products before they are used
+constexpr int kAhead = 4;
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kTile = 32 * kWaves;
 
+// This thread's 16-byte pieces of a block.
 template <int D>
-struct StageRegs {
-    static constexpr int kPieces = 2 * 2 * kKvBlock * D / 16;  // 16-byte pieces of two blocks
-    static constexpr int kEach = (kPieces + 64 * prompt_waves<D>() - 1) / (64 * prompt_waves<D>());
+struct BlockPieces {
+    static constexpr int kAll = 2 * kKvBlock * D / 16, kEach = kAll / kThreads;
     uint4 raw[kEach];
-};
-
-struct StageMeta {
-    int page[2], start[2];
-    float sk[2], sv[2];
 };
 
 template <int D>
@@ -50,47 +51,77 @@ constexpr int key_bytes() { return D / 8 * kKeyRun; }
 template <int D>
 constexpr int block_bytes_lds() { return key_bytes<D>() + D / 8 * kValueRun; }
 
-// Fetches this thread's pieces of the two blocks.
 template <int D>
-__device__ __forceinline__ void fetch(const uint8_t* pages, const StageMeta& m, StageRegs<D>& r) {
-    constexpr int kThreads = 64 * prompt_waves<D>(), kPer = 2 * kKvBlock * D / 16;
+__device__ __forceinline__ void fetch(const uint8_t* pages, int page, BlockPieces<D>& r) {
+    const uint8_t* from = pages + static_cast<int64_t>(page) * (64 * D);
 #pragma unroll
-    for (int i = 0; i < StageRegs<D>::kEach; ++i) {
-        const int at = threadIdx.x + i * kThreads, blk = at / kPer;
-        r.raw[i] = *reinterpret_cast<const uint4*>(pages + static_cast<int64_t>(blk ? m.page[1] : m.page[0]) * (64 * D) +
-                                                   at % kPer * 16);
-    }
+    for (int i = 0; i < BlockPieces<D>::kEach; ++i)
+        r.raw[i] = *reinterpret_cast<const uint4*>(from + (threadIdx.x + i * kThreads) * 16);
 }
 
-// Converts them into LDS. Values become bf16 for f32 calls, else f16.
-template <int D, bool PAIR>
-__device__ __forceinline__ void place(const StageRegs<D>& r, uint8_t* lds) {
-    constexpr int kThreads = 64 * prompt_waves<D>(), kPer = 2 * kKvBlock * D / 16;
+// The pieces are not used before this.
+template <int D>
+__device__ __forceinline__ void hold(BlockPieces<D>& r) {
 #pragma unroll
-    for (int i = 0; i < StageRegs<D>::kEach; ++i) {
-        const int at = threadIdx.x + i * kThreads, blk = at / kPer, piece = at % kPer;
-        uint8_t* to = lds + blk * block_bytes_lds<D>();
-        const uint4 w = r.raw[i];
-        if (piece < kPer / 2) {  // keys: token, 16 dims
-            const int step = piece / 128 * 4 + piece % 4, t = piece / 4 % 32;
-            uint8_t* p = to + step * 2 * kKeyRun + t * 16;
+    for (int i = 0; i < BlockPieces<D>::kEach; ++i)
+        asm volatile("" : "+v"(r.raw[i].x), "+v"(r.raw[i].y), "+v"(r.raw[i].z), "+v"(r.raw[i].w));
+}
+
+// Eight signed bytes as f16 plus 1152.
+__device__ __forceinline__ half8 codes_to_half_raised(uint32_t lo, uint32_t hi) {
+    union {
+        uint32_t u[4];
+        half8 v;
+    } r;
+    lo ^= 0x80808080u;
+    hi ^= 0x80808080u;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u);
+    return r.v;
+}
+
+// Converts piece i into LDS. Values become bf16 for f32 calls, else f16. Keys of
+// f16 and bf16 calls stay raised by 1152 (their scores come down by 1152 times
+// the row's sum, which rounds a score by about 2^-24 of that: less than those
+// calls' weights are rounded by); f32 calls take them exactly.
+template <int D, bool PAIR>
+__device__ __forceinline__ void place(const BlockPieces<D>& r, int i, int wave, uint8_t* to) {
+    const int piece = threadIdx.x + i * kThreads;
+    const uint4 w = r.raw[i];
+    constexpr int kKeys = BlockPieces<D>::kAll / 2;
+    // whole waves take keys or values, and where a round of the workgroup does, that is known here
+    if ((i + 1) * kThreads <= kKeys || (i * kThreads < kKeys && wave * 64 + i * kThreads < kKeys)) {  // keys: token, 16 dims
+        uint8_t* p = to + (piece / 128 * 4 + piece % 4) * 2 * kKeyRun + piece / 4 % 32 * 16;
+        *reinterpret_cast<half8*>(p) = PAIR ? codes_to_half(w.x, w.y) : codes_to_half_raised(w.x, w.y);
+        *reinterpret_cast<half8*>(p + kKeyRun) = PAIR ? codes_to_half(w.z, w.w) : codes_to_half_raised(w.z, w.w);
+    } else {  // values: dims d and d + 16, 8 tokens
+        const int v = piece - kKeys;
+        uint8_t* p = to + key_bytes<D>() + (v / 64 * 4 + v % 4) * kValueRun + v / 4 % 16 * 16;
+        if constexpr (PAIR) {
+            *reinterpret_cast<bhalf8*>(p) = codes_to_bhalf(w.x, w.y);
+            *reinterpret_cast<bhalf8*>(p + 256) = codes_to_bhalf(w.z, w.w);
+        } else {
             *reinterpret_cast<half8*>(p) = codes_to_half(w.x, w.y);
-            *reinterpret_cast<half8*>(p + kKeyRun) = codes_to_half(w.z, w.w);
-        } else {  // values: dims d and d + 16, 8 tokens
-            const int v = piece - kPer / 2;
-            uint8_t* p = to + key_bytes<D>() + (v / 64 * 4 + v % 4) * kValueRun + v / 4 % 16 * 16;
-            if constexpr (PAIR) {
-                *reinterpret_cast<bhalf8*>(p) = codes_to_bhalf(w.x, w.y);
-                *reinterpret_cast<bhalf8*>(p + 256) = codes_to_bhalf(w.z, w.w);
-            } else {
-                *reinterpret_cast<half8*>(p) = codes_to_half(w.x, w.y);
-                *reinterpret_cast<half8*>(p + 256) = codes_to_half(w.z, w.w);
-            }
+            *reinterpret_cast<half8*>(p + 256) = codes_to_half(w.z, w.w);
         }
     }
 }
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// A barrier for what passes through LDS: loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// The larger of a row's two lanes' values.
+__device__ __forceinline__ float max_of_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float x) { return x + __shfl_xor(x, 32, 64); }
 
 __device__ __forceinline__ float tanh_fast(float x) {
     // 1 - 2 / (1 + e^2x): its error is of 1, not of small results
@@ -98,14 +129,15 @@ __device__ __forceinline__ float tanh_fast(float x) {
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(64 * prompt_waves<D>()) void kv_prompt_kernel(KvAttend p, int tiles) {
+__global__ __launch_bounds__(kThreads, (D <= (TYPE == ROCKNPU_KV_F32 ? 64 : 128) ? 2 : 1)) void kv_prompt_kernel(KvAttend p, int tiles) {
     using K = KvType<TYPE>;
     using T = typename K::T;
     constexpr bool PAIR = TYPE == ROCKNPU_KV_F32;
-    constexpr int kParts = PAIR ? 2 : 1, kWaves = prompt_waves<D>(), kTile = 32 * kWaves;
+    constexpr int kParts = PAIR ? 2 : 1;
+    constexpr int kSteps = D / 16;  // products of 16 dims of keys, and of values by 32 dims and 16 tokens
     const rocknpu_kv_cache& c = p.c;
     const rocknpu_kv_attention_args& a = p.a;
-    __shared__ alignas(16) uint8_t lds[2][2 * block_bytes_lds<D>()];
+    __shared__ alignas(16) uint8_t lds[3][block_bytes_lds<D>()];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the tiles with the most blocks first, a tile's kv heads side by side (one each per XCD where they are 8)
@@ -128,273 +160,326 @@ __global__ __launch_bounds__(64 * prompt_waves<D>()) void kv_prompt_kernel(KvAtt
     const int begin = mine.split * chunk, end = min(begin + chunk, count);
     const int64_t slot = (static_cast<int64_t>(h) * p.row_tiles + tile) * p.slots + slot_at;
     if (begin >= end && mine.splits > 1) {
-        if (tid < kTile) {
-            p.part_state[(slot * kTile + tid) * 2] = -__builtin_inff();
-            p.part_state[(slot * kTile + tid) * 2 + 1] = 0.0f;
-        }
+        if (tid < kTile) reinterpret_cast<float2*>(p.part_state)[slot * kTile + tid] = make_float2(-__builtin_inff(), 0.0f);
         return;
     }
 
+    // The wave's rows are w0 + n. A row sees [low, low + span] and what lies before `pre`; `full` and `some`: what every
+    // row and some row of the wave sees.
     const int w0 = r0 + wave * 32;
-    const bool active = w0 < rows;
-    const int row = min(w0 + n, rows - 1), head = h * p.group + row % p.group, qpos = s.past + row / p.group;
+    const bool active = w0 < rows, windowed = a.window != 0, plain = a.softcap == 0.0f && !a.slopes;
     const int q0 = s.past + min(w0, rows - 1) / p.group, q1 = s.past + (min(w0 + 32, rows) - 1) / p.group;
-    half8 q[kParts][D / 16];
-    float unit;
+    const int pre = min(prefix, total), newest = total - 1;
+    const int full_low = windowed ? max(q1 - a.window + 1, 0) : 0, full_high = a.causal ? min(q0, newest) : newest;
+    const int some_low = windowed ? max(q0 - a.window + 1, 0) : 0, some_high = a.causal ? min(q1, newest) : newest;
+    const int row = min(w0 + n, rows - 1), head = h * p.group + row % p.group, qpos = s.past + row / p.group;
+    const int low = windowed ? max(qpos - a.window + 1, 0) : 0;
+    const unsigned span = static_cast<unsigned>((a.causal ? min(qpos, newest) : newest) - low);
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    // Block j of the workgroup's part: its bytes are loaded in iteration j - 4 (a trip to memory takes longer than an
+    // iteration) and go to LDS in iteration j - 2. Page numbers, positions and scales are looked up 64 blocks at a time, a
+    // block per lane, half a batch ahead. (Looked up block by block they were what an iteration waited for: 4096 tokens,
+    // 32/8 heads of 128, bf16: 197 us instead of TIME.)
+    struct Batch {
+        int page, start;
+        float sk, sv;
+    };
+    struct Meta {
+        int start;
+        float sk, sv;
+    };
+    const int32_t* table = c.table + entry_row;
+    const int32_t* starts = c.starts + entry_row;
+    const int blocks = end - begin;
+    Batch batch{}, batch_1{};  // of blocks base .. base + 63, and of the next 64
+    int base = 0;
+    const auto look_up = [&](int first, Batch& r) {
+        if (first + lane < blocks) {
+            const int at = range.entry(begin + first + lane);
+            r.page = table[at];
+            r.start = starts[at];
+        }
+    };
+    const auto look_up_scales = [&](int first, Batch& r) {
+        const bool ok = r.page >= 0 && r.page < c.n_pages;
+        r.page = ok ? r.page : 0;
+        if (first + lane < blocks) {
+            const float2 x = reinterpret_cast<const float2*>(c.scales)[r.page];
+            r.sk = kv_scale(x.x, ok);
+            r.sv = kv_scale(x.y, ok);
+        }
+    };
+    // a field of block j, for base <= j < base + 128; past the end what it is does not matter, but it is a page that exists
+    const auto of_block = [&](int j, int here, int there) {
+        return j - base < 64 ? __builtin_amdgcn_readlane(here, j - base) : __builtin_amdgcn_readlane(there, j - base - 64);
+    };
+    const auto meta_of = [&](int j) {
+        return Meta{of_block(j, batch.start, batch_1.start),
+                    __uint_as_float(of_block(j, __float_as_uint(batch.sk), __float_as_uint(batch_1.sk))),
+                    __uint_as_float(of_block(j, __float_as_uint(batch.sv), __float_as_uint(batch_1.sv)))};
+    };
+    const auto fetch_block = [&](int j, BlockPieces<D>& r) { fetch<D>(c.pages, of_block(j, batch.page, batch_1.page), r); };
+
+    BlockPieces<D> even, odd;
+    look_up(0, batch);
+    half8 q[kParts][kSteps];
+    float unit, lower = 0.0f;  // of a product: its weight in the score; what it is too large by
     {
         const T* src = static_cast<const T*>(a.q) + (s.row0 + row / p.group) * a.q_row + head * a.q_head + half * 8;
-        float top = 0.0f;
+        float x[kSteps][8], top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            float x[8];
-            load8<TYPE>(src + i * 16, p.vec_q, x);
+        for (int i = 0; i < kSteps; ++i) load8<TYPE>(src + i * 16, p.vec_q, x[i]);
+        // the first blocks' bytes, whose pages are known by now, come while the queries are worked on
+        look_up_scales(0, batch);
+        fetch_block(0, even);
+        fetch_block(1, odd);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-        }
-        const float power = row_power(fmaxf(top, other_half(top)));
-        unit = a.scale / power;
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            float x[8];
-            load8<TYPE>(src + i * 16, p.vec_q, x);
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+        const float power = row_power(max_of_halves(top));
+        // the queries take the scale's sign, so that scores rise with their products
+        unit = fabsf(a.scale) / power;
+        const float signed_power = a.scale < 0.0f ? -power : power;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = x[e] * power;
+                const float v = x[i][e] * signed_power;
                 q[0][i][e] = static_cast<_Float16>(v);
-                if constexpr (PAIR) q[1][i][e] = static_cast<_Float16>(v - static_cast<float>(q[0][i][e]));
+                if constexpr (PAIR)
+                    q[1][i][e] = static_cast<_Float16>(v - static_cast<float>(q[0][i][e]));
+                else
+                    lower += static_cast<float>(q[0][i][e]);
             }
-        }
+        if constexpr (!PAIR) lower = 1152.0f * sum_of_halves(lower);
     }
-    const float slope = a.slopes ? a.slopes[head] : 0.0f;
-    const bool plain = a.softcap == 0.0f && !a.slopes;
 
     float16v o[D / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = float16v{};
-    float ref = -__builtin_inff(), sum = 0.0f;
+    for (int d = 0; d < D / 32; ++d) o[d] = float16v{};
+    float ref = kNothing, sum = 0.0f;
 
-    // a stage's two blocks: the second may lie past the end, and is then masked whole (its data is the first's)
-    const auto look_up = [&](int stage, StageMeta& m) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int at = range.entry(min(begin + 2 * stage + i, end - 1));
-            m.page[i] = __builtin_amdgcn_readfirstlane(c.table[entry_row + at]);
-            m.start[i] = __builtin_amdgcn_readfirstlane(c.starts[entry_row + at]);
-        }
+    using Value = typename std::conditional<PAIR, bhalf8, half8>::type;
+    // operand k of the scores' products (16 dims), and of the values': all tiles of 32 dims with 16 of the tokens, then with
+    // the others
+    const auto read_key = [&](const uint8_t* at, int k) {
+        return *reinterpret_cast<const half8*>(at + half * kKeyRun + n * 16 + k * 2 * kKeyRun);
     };
-    const auto look_up_scales = [&](int stage, StageMeta& m) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const bool ok = m.page[i] >= 0 && m.page[i] < c.n_pages;
-            m.page[i] = ok ? m.page[i] : 0;
-            const float2 sc = reinterpret_cast<const float2*>(c.scales)[m.page[i]];
-            m.sk[i] = kv_scale(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sc.x))), ok);
-            m.sv[i] = kv_scale(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sc.y))), ok);
-            if (begin + 2 * stage + i >= end) m.start[i] = 0x7fffff00;
-        }
+    const auto read_value = [&](const uint8_t* at, int k) {
+        return *reinterpret_cast<const Value*>(at + key_bytes<D>() + half * kValueRun + n * 16 +
+                                               (k % (kSteps / 2) * 2 + k / (kSteps / 2)) * 2 * kValueRun);
     };
-    const int stages = (end - begin + 1) / 2;
-    StageMeta m0{}, m1{}, m2{};  // stages s, s + 1, s + 2
-    StageRegs<D> regs;
-    if (stages > 0) {
-        look_up(0, m0);
-        look_up(1, m1);
-        look_up_scales(0, m0);
-        fetch<D>(c.pages, m0, regs);
-        look_up_scales(1, m1);
-        place<D, PAIR>(regs, lds[0]);
-        fetch<D>(c.pages, m1, regs);
-        look_up(2, m2);
-    }
-    __syncthreads();
-    for (int st = 0; st < stages; ++st) {
-        const uint8_t* now = lds[st & 1];
-        if (st + 1 < stages) place<D, PAIR>(regs, lds[(st + 1) & 1]);
-        look_up_scales(st + 2, m2);
-        if (st + 2 < stages) fetch<D>(c.pages, m2, regs);
-        StageMeta m3{};
-        look_up(st + 3, m3);
+    // x[r]: token 8 (r / 4) + 4 half + r % 4 of the block, row n
+    const auto product = [&](const half8& key, int k, float16v& x) {
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, q[part][k], x, 0, 0, 0);
+    };
 
-        // blocks that no row of the wave sees
-        bool any[2];
+    Meta meta{}, meta_1{};  // of blocks j, j + 1
+    int now = 0;            // block j is in lds[now], block j + 1 in the next buffer
+    // Iteration j: x holds block j's products, x_1 takes block j + 1's; `two` holds block j + 2 and takes block j + 4.
+    const auto iterate = [&](int j, float16v& x, float16v& x_1, BlockPieces<D>& two) {
+        const int then = now == 2 ? 0 : now + 1, later = then == 2 ? 0 : then + 1;
+        const uint8_t* at = lds[now];
+        const uint8_t* at_1 = lds[then];
+        const float sk = meta.sk, sv = meta.sv;
+        const bool before = meta.start + kKvBlock <= pre;
+        const bool any = active && ((meta.start <= some_high && meta.start + kKvBlock > some_low) || meta.start < pre);
+        x_1 = float16v{};
+        if (__builtin_expect(any, 1)) {
+            // scores to exponents over the row's reference, which follows the maximum
+            const float lift = __log2f(sv);
+            float factor = unit * sk * kLog2e, off = __builtin_fmaf(-lower, factor, lift), most;
+            if (__builtin_expect(plain && (before || (meta.start >= full_low && meta.start + kKvBlock - 1 <= full_high)), 1)) {
+                most = x[0];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            any[i] = active && m0.start[i] < total && (!a.causal || m0.start[i] <= q1 || m0.start[i] < prefix) &&
-                     (a.window == 0 || m0.start[i] + kKvBlock > q0 - a.window + 1 || m0.start[i] < prefix);
-        if (any[0] || any[1]) {
-            float16v x[2];
-            float most = -__builtin_inff(), factor[2], shift[2];
+                for (int r = 1; r < 16; ++r) most = fmaxf(most, x[r]);
+                most = __builtin_fmaf(most, factor, off);
+            } else {
+                most = kNothing;
+                const float to_score = plain ? factor : unit * sk;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                x[i] = float16v{};
-                const uint8_t* keys = now + i * block_bytes_lds<D>() + half * kKeyRun + n * 16;
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const half8 key = *reinterpret_cast<const half8*>(keys + k * 2 * kKeyRun);
-#pragma unroll
-                    for (int part = 0; part < kParts; ++part)
-                        x[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, q[part][k], x[i], 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                // x[i][r]: token 8 (r / 4) + 4 half + r % 4
-                const float lift = __log2f(m0.sv[i]);
-                factor[i] = unit * m0.sk[i] * kLog2e;
-                shift[i] = lift;
-                if (plain && kv_all_seen(a, m0.start[i], q0, q1, prefix, total)) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) most = fmaxf(most, __builtin_fmaf(x[i][r], factor[i], lift));
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int kpos = m0.start[i] + r / 4 * 8 + half * 4 + r % 4;
-                        float y;
-                        if (plain) {
-                            y = __builtin_fmaf(x[i][r], factor[i], lift);
-                        } else {
-                            y = x[i][r] * (unit * m0.sk[i]);
-                            if (a.softcap != 0.0f)
-                                y = a.softcap * (PAIR ? tanhf(y / a.softcap) : tanh_fast(y / a.softcap));
-                            if (a.slopes) y += slope * static_cast<float>(kpos - qpos);
-                            y = __builtin_fmaf(y, kLog2e, lift);
-                        }
-                        x[i][r] = kv_seen(a, kpos, qpos, prefix, total) ? y : -__builtin_inff();
-                        most = fmaxf(most, x[i][r]);
+                for (int r = 0; r < 16; ++r) {
+                    const int kpos = meta.start + r / 4 * 8 + half * 4 + r % 4;
+                    float y = (x[r] - lower) * to_score;
+                    if (!plain) {
+                        if (a.softcap != 0.0f) y = a.softcap * (PAIR ? tanhf(y / a.softcap) : tanh_fast(y / a.softcap));
+                        if (a.slopes) y += slope * static_cast<float>(kpos - qpos);
+                        y *= kLog2e;
                     }
-                    factor[i] = 1.0f;
-                    shift[i] = 0.0f;
+                    x[r] = static_cast<unsigned>(kpos - low) <= span || kpos < pre ? y + lift : -__builtin_inff();
+                    most = fmaxf(most, x[r]);
                 }
+                factor = 1.0f;
+                off = 0.0f;
             }
-            most = fmaxf(most, other_half(most));
-            if (__any(most > ref + kSlack || (ref == -__builtin_inff() && most != ref))) {
+            most = max_of_halves(most);
+            if (__builtin_expect(__any(most > ref + kSlack), 0)) {
                 const float to = fmaxf(ref, most);
-                const float keep = ref == to ? 1.0f : exp2_fast(ref - to);
+                const float keep = exp2_fast(ref - to);
                 ref = to;
                 sum *= keep;
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) o[i] *= keep;
+                for (int d = 0; d < D / 32; ++d) o[d] *= keep;
             }
-            const float base = (PAIR ? 0.0f : kBias) - (ref == -__builtin_inff() ? 0.0f : ref);
+            off += (PAIR ? 0.0f : kBias) - ref;
+
+            // the next block's scores, and between them this one's weights
+            half8 w[2], key[kSteps];
+            Value value[kSteps];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float off = shift[i] + base;
-                float e[16], got = 0.0f;
+            for (int k = 0; k < kAhead; ++k) key[k] = read_key(at_1, k);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) e[r] = exp2_fast(__builtin_fmaf(x[i][r], factor[i], off));
-                const uint8_t* values = now + i * block_bytes_lds<D>() + key_bytes<D>() + half * kValueRun + n * 16;
+            for (int k = 0; k < kSteps; ++k) {
+                if (k + kAhead < kSteps)
+                    key[k + kAhead] = read_key(at_1, k + kAhead);
+                else
+                    value[k + kAhead - kSteps] = read_value(at, k + kAhead - kSteps);
+                product(key[k], k, x_1);
+#pragma unroll
+                for (int e = 16 * k / kSteps; e < 16 * (k + 1) / kSteps; ++e) x[e] = exp2_fast(__builtin_fmaf(x[e], factor, off));
+            }
+            bhalf8 ww[2][3];
+            float got = 0.0f;
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
                 if constexpr (PAIR) {
+                    float part[8];
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        float ee[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            ee[j] = e[j / 4 * 8 + m * 4 + j % 4];
-                            got += ee[j];
-                        }
-                        bhalf8 w[3];
-                        split_bhalf(ee, w);
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d) {
-                            const bhalf8 value = *reinterpret_cast<const bhalf8*>(values + (d * 4 + m * 2) * kValueRun);
-#pragma unroll
-                            for (int part = 0; part < 3; ++part)
-                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value, w[part], o[d], 0, 0, 0);
-                        }
+                    for (int i = 0; i < 8; ++i) {
+                        part[i] = x[i / 4 * 8 + h2 * 4 + i % 4];
+                        got += part[i];
                     }
+                    split_bhalf(part, ww[h2]);
                 } else {
                     union {
                         half2v h[4];
                         half8 v;
-                    } w[2];
-                    half2v least = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+                    } u;
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = j / 2 * 8 + m * 4 + j % 2 * 2;
-                            w[m].h[j] = __builtin_convertvector(float2v{e[r], e[r + 1]}, half2v);
-                            got = __builtin_amdgcn_fdot2(w[m].h[j], half2v{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)},
-                                                         got, false);
-                            least = __builtin_elementwise_min(least, w[m].h[j]);
-                        }
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d) {
-                            const half8 value = *reinterpret_cast<const half8*>(values + (d * 4 + m * 2) * kValueRun);
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value, w[m].v, o[d], 0, 0, 0);
-                        }
-                    // Weights that f16 holds with fewer than its 11 bits (below 2^-14) go in once more, 2^28 times as
-                    // large, and so on down f32's range, less what went in: an output dim whose greatest weights meet
-                    // zero codes is as exact as any other. Rare but for rows of extreme scores.
-                    const float small = fminf(static_cast<float>(least[0]), static_cast<float>(least[1]));
-                    if (__any(small < 0x1p-14f)) {
-                        float rest[16];
-                        bool more = false;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            rest[r] = e[r] - static_cast<float>(w[r / 4 % 2].h[r / 8 * 2 + r % 4 / 2][r % 2]);
-                            rest[r] = e[r] < 0x1p-14f ? rest[r] : 0.0f;
-                            more |= rest[r] != 0.0f;
-                        }
-                        float up = 1.0f;
-                        while (__any(more)) {
-                            up *= 0x1p28f;
-                            more = false;
-#pragma unroll
-                            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const int r = j / 4 * 8 + m * 4 + j % 4;
-                                    const _Float16 x16 = static_cast<_Float16>(rest[r] * up);
-                                    w[m].v[j] = x16;
-                                    const float left = rest[r] - static_cast<float>(x16) * (1.0f / up);
-                                    rest[r] = fabsf(rest[r] * up) < 0x1p-14f ? left : 0.0f;
-                                    more |= rest[r] != 0.0f && up < 0x1p100f;
-                                }
-#pragma unroll
-                            for (int d = 0; d < D / 32; ++d) {
-                                float16v part = {};
-#pragma unroll
-                                for (int m = 0; m < 2; ++m) {
-                                    const half8 value = *reinterpret_cast<const half8*>(values + (d * 4 + m * 2) * kValueRun);
-                                    part = __builtin_amdgcn_mfma_f32_32x32x16_f16(value, w[m].v, part, 0, 0, 0);
-                                }
-                                o[d] += part * (1.0f / up);
-                            }
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = i / 2 * 8 + h2 * 4 + i % 2 * 2;
+                        u.h[i] = __builtin_convertvector(float2v{x[r], x[r + 1]}, half2v);
+                        got = __builtin_amdgcn_fdot2(u.h[i], half2v{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, got,
+                                                     false);
                     }
+                    w[h2] = u.v;
                 }
-                sum += got == 0.0f ? 0.0f : got / m0.sv[i];
             }
+            sum += got == 0.0f ? 0.0f : got * __builtin_amdgcn_rcpf(sv);
+            // Values times weights, and between them the later block's conversion. Its bytes are first touched here: moved
+            // up, the conversion would wait for them at the iteration's start.
+            __builtin_amdgcn_sched_barrier(0);
+            hold<D>(two);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const int h2 = k / (kSteps / 2), d = k % (kSteps / 2);
+                if (k + kAhead < kSteps) value[k + kAhead] = read_value(at, k + kAhead);
+                if constexpr (PAIR) {
+#pragma unroll
+                    for (int part = 0; part < 3; ++part)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value[k], ww[h2][part], o[d], 0, 0, 0);
+                } else {
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value[k], w[h2], o[d], 0, 0, 0);
+                }
+                if (k % (kSteps / BlockPieces<D>::kEach) == 0)
+                    place<D, PAIR>(two, k / (kSteps / BlockPieces<D>::kEach), wave, lds[later]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) product(read_key(at_1, k), k, x_1);
+            hold<D>(two);
+#pragma unroll
+            for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(two, i, wave, lds[later]);
         }
-        m0 = m1;
-        m1 = m2;
-        m2 = m3;
-        __syncthreads();
+        meta = meta_1;
+        meta_1 = meta_of(j + 2);
+        fetch_block(j + 4, two);
+        if (j + 1 - base == 32) look_up(base + 64, batch_1);
+        if (j + 1 - base == 48) look_up_scales(base + 64, batch_1);
+        if (j + 1 - base == 64) {
+            batch = batch_1;
+            base += 64;
+        }
+        now = then;
+        lds_barrier();
+    };
+
+    float16v x = {}, x_1;
+    if (blocks > 0) {
+        // blocks 0 and 1 into LDS, blocks 2 and 3 on their way
+        meta = meta_of(0);
+        meta_1 = meta_of(1);
+#pragma unroll
+        for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(even, i, wave, lds[0]);
+        fetch_block(2, even);
+#pragma unroll
+        for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(odd, i, wave, lds[1]);
+        fetch_block(3, odd);
+    }
+    lds_barrier();
+    if (blocks > 0) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) product(read_key(lds[0], k), k, x);
+    }
+    for (int j = 0; j < blocks; j += 2) {
+        iterate(j, x, x_1, even);
+        if (j + 1 < blocks) iterate(j + 1, x_1, x, odd);
     }
 
     if (!active) return;
-    sum += other_half(sum);
+    sum = sum_of_halves(sum);
     const int r = w0 + n;
-    if (r >= rows) return;
     // o[d][i]: dim 32 d + 8 (i / 4) + 4 half + i % 4 of row r
     if (mine.splits > 1) {
-        if (half == 0) {
-            p.part_state[(slot * kTile + r - r0) * 2] = ref;
-            p.part_state[(slot * kTile + r - r0) * 2 + 1] = sum;
-        }
+        if (r >= rows) return;
+        if (half == 0) reinterpret_cast<float2*>(p.part_state)[slot * kTile + r - r0] = make_float2(ref, sum);
         float* to = p.part_out + (slot * kTile + r - r0) * D + half * 4;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float4v*>(to + d * 32 + i * 8) = float4v{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]};
+                *reinterpret_cast<float4v*>(to + d * 32 + i * 8) =
+                    float4v{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]};
         return;
     }
     const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* out = static_cast<T*>(a.out) + (s.row0 + row / p.group) * a.out_row + head * a.out_head + half * 4;
+    T* out = static_cast<T*>(a.out);
+    if (!PAIR && p.vec_out) {
+        // through LDS, so that whole rows are stored, 16 bytes a lane
+        constexpr int kRow = D + 8;  // elements, padded
+        T* rows_lds = reinterpret_cast<T*>(&lds[0][0]) + wave * 32 * kRow;
+        static_assert(PAIR || kWaves * 32 * kRow * 2 <= 3 * block_bytes_lds<D>());
+        struct alignas(8) Four {
+            T e[4];
+        };
+        struct alignas(16) Eight {
+            T e[16 / sizeof(T)];
+        };
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                Four v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v.e[e] = K::from_f32(sum == 0.0f ? 0.0f : o[d][i * 4 + e] * over);
+                *reinterpret_cast<Four*>(rows_lds + n * kRow + d * 32 + i * 8 + half * 4) = v;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+#pragma unroll
+        for (int i = 0; i < 32 * D / 8 / 64; ++i) {
+            const int at = i * 64 + lane, m = at / (D / 8), d = at % (D / 8) * 8, rr = w0 + m;
+            if (rr < rows)
+                *reinterpret_cast<Eight*>(out + (s.row0 + rr / p.group) * a.out_row + (h * p.group + rr % p.group) * a.out_head + d) =
+                    *reinterpret_cast<Eight*>(rows_lds + m * kRow + d);
+        }
+        return;
+    }
+    if (r >= rows) return;
+    out += (s.row0 + row / p.group) * a.out_row + head * a.out_head + half * 4;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -403,12 +488,12 @@ __global__ __launch_bounds__(64 * prompt_waves<D>()) void kv_prompt_kernel(KvAtt
                 T e[4];
             } v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v.e[j] = K::from_f32(sum == 0.0f ? 0.0f : o[d][i * 4 + j] * over);
+            for (int e = 0; e < 4; ++e) v.e[e] = K::from_f32(sum == 0.0f ? 0.0f : o[d][i * 4 + e] * over);
             if (p.vec_out) {
                 *reinterpret_cast<Four*>(out + d * 32 + i * 8) = v;
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) out[d * 32 + i * 8 + j] = v.e[j];
+                for (int e = 0; e < 4; ++e) out[d * 32 + i * 8 + e] = v.e[e];
             }
         }
 }
@@ -417,7 +502,7 @@ template <int TYPE, int D>
 int launch(const KvAttend& p, hipStream_t stream) {
     const int64_t grid = static_cast<int64_t>(p.row_tiles) * p.slots * p.c.kv_heads;
     if (grid > 0x7fffffff) return kStatusInvalid;
-    kv_prompt_kernel<TYPE, D><<<static_cast<unsigned>(grid), 64 * prompt_waves<D>(), 0, stream>>>(p, p.row_tiles);
+    kv_prompt_kernel<TYPE, D><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, p.row_tiles);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
@@ -433,7 +518,7 @@ int launch_dim(const KvAttend& p, hipStream_t stream) {
 
 }  // namespace
 
-int kv_prompt_tile(int head_dim) { return head_dim <= 128 ? 256 : 128; }
+int kv_prompt_tile() { return kTile; }
 
 int launch_kv_prompt(const KvAttend& p, hipStream_t stream) {
     switch (p.a.type) {

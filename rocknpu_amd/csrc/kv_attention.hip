@@ -28,8 +28,15 @@ bool attention_ok(const rocknpu_kv_cache* c, const rocknpu_kv_attention_args* a)
 
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 
-// Rows of a kv head up to which the cache is streamed through 16-row tiles.
+// The streaming kernel reads the cache once per 16 rows, the prompt kernel once
+// per 128, with several times the work for a block. Streaming serves calls of at
+// most 32 rows a kv head; and short contexts in launches that leave the prompt
+// kernel too few tiles, up to kShortBlocks blocks and four 16-row tiles a CU
+// (32/8 heads of 128, bf16, one sequence, 512 rows over 512 and 912 tokens: 38
+// and 42 us, prompt kernel 44 and 49; over 2512: 87 and 63; 64 rows over 16000:
+// 106 and 55. f32: 30, 45, 98 and 115 against 51, 55, 83 and 75).
 constexpr int64_t kStreamRows = 32;
+constexpr int64_t kShortBlocks = 32;
 // Blocks of a split, at least: two for each of a workgroup's waves.
 constexpr int kMinChunk = 8;
 // Sequences up to which their blocks are shared out over the workgroups.
@@ -52,21 +59,23 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.vec_q = aligned(a.q, 16) && a.q_row % per == 0 && a.q_head % per == 0;
     p.vec_out = aligned(a.out, 16) && a.out_row % per == 0 && a.out_head % per == 0;
     const int64_t rows = std::max<int64_t>(a.max_new, 1) * p.group;
-    r.stream = rows <= kStreamRows || a.weights_out;
-    p.tile_rows = r.stream ? kKvTileRows : kv_prompt_tile();
-    p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     int64_t blocks = a.max_tokens > 0 ? (a.max_tokens + kKvBlock - 1) / kKvBlock : c.max_blocks;
     if (a.window > 0) blocks = std::min<int64_t>(blocks, (static_cast<int64_t>(a.window) + a.max_new) / kKvBlock + 2);
     blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, c.max_blocks));
+    const int64_t tiles = (rows + kKvTileRows - 1) / kKvTileRows * c.batch * c.kv_heads;
+    r.stream = rows <= kStreamRows || a.weights_out || (blocks <= kShortBlocks && tiles <= 4 * cus);
+    p.tile_rows = r.stream ? kKvTileRows : kv_prompt_tile();
+    p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.min_chunk = kMinChunk;
     // One round of the workgroups that the GPU holds at once: a second round pays every workgroup's start (lookups, the
     // queries, the first blocks' latency) again. Sharing rounds each sequence up, by half a workgroup on average. 32
     // ragged sequences of 500-4100 tokens, 8 kv heads of 128: 40.4 us; three quarters and one and a half rounds 48.7
-    // and 47.3; a fixed four parts a sequence 51.4.
-    const int64_t resident = (!r.stream ? 1 : c.head_dim <= 64 ? 3 : c.head_dim <= 128 ? 2 : 1) * cus;
+    // and 47.3; a fixed four parts a sequence 51.4. The prompt kernel shares blocks out where that gives every sequence
+    // and tile at least four parts: below, joining costs what it saves.
+    const int64_t resident = (c.head_dim <= 64 && r.stream ? 3 : c.head_dim <= 128 ? 2 : 1) * cus;
     const int64_t share = std::max<int64_t>(resident / (c.kv_heads * p.row_tiles) - c.batch / 2, 1);
     const bool shared = blocks > p.min_chunk && c.batch <= kMaxShared && rows > 0;
-    p.share = shared && share > 1 ? static_cast<int>(std::min<int64_t>(share, c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk))) : 0;
+    p.share = shared && share >= (r.stream ? 2 : 4) ? static_cast<int>(std::min<int64_t>(share, c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk))) : 0;
     p.slots = p.share + c.batch;
     const size_t slots = static_cast<size_t>(p.slots) * c.kv_heads * p.row_tiles * p.tile_rows;
     if (p.share) r.out_bytes = padded(slots * c.head_dim * 4);

@@ -35,8 +35,6 @@ constexpr float kNothing = -1e30f;
 // lanes a cycle meet 8 different 16-byte columns
 constexpr int kKeyRun = 528, kValueRun = 544;
 
-// operands are read from LDS this many products before they are used
-constexpr int kAhead = 4;
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kTile = 32 * kWaves;
 
 // This thread's 16-byte pieces of a block.
@@ -129,11 +127,12 @@ __device__ __forceinline__ float tanh_fast(float x) {
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(kThreads, (D <= (TYPE == ROCKNPU_KV_F32 ? 64 : 128) ? 2 : 1)) void kv_prompt_kernel(KvAttend p, int tiles) {
+__global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel(KvAttend p, int tiles) {
     using K = KvType<TYPE>;
     using T = typename K::T;
     constexpr bool PAIR = TYPE == ROCKNPU_KV_F32;
     constexpr int kParts = PAIR ? 2 : 1;
+    constexpr int kAhead = PAIR ? 2 : 4;  // operands are read from LDS this many steps before they are used
     constexpr int kSteps = D / 16;  // products of 16 dims of keys, and of values by 32 dims and 16 tokens
     const rocknpu_kv_cache& c = p.c;
     const rocknpu_kv_attention_args& a = p.a;

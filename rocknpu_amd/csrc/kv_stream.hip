@@ -273,74 +273,88 @@ __global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
     }
 }
 
-// Joins the splits of a tile's rows: the first workgroups take a row each, its
-// splits' sums read side by side (all of a row's loads are in flight together),
-// the others (with block weights) a block per thread.
-template <int TYPE, int D>
+// Joins the splits of a tile's rows: the first workgroups take 4 / WAVES rows
+// each, a row's splits read side by side, the others (with block weights) a block
+// per thread. A row of many splits takes a workgroup, so that its loads are all
+// in flight together; of few, a wave (2048 rows of 8 heads in 2 splits: a
+// workgroup each took 45 us).
+template <int TYPE, int D, int WAVES>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups) {
     using K = KvType<TYPE>;
     using T = typename K::T;
-    constexpr int kPer = D / 4;                 // threads that read a split's row
-    constexpr int kBeside = 256 / kPer;         // splits read side by side
+    constexpr int kPer = D / 4;         // lanes that read a split's row
+    constexpr int kBeside = 64 / kPer;  // splits that a wave reads side by side
     const rocknpu_kv_cache& c = p.c;
     const rocknpu_kv_attention_args& a = p.a;
     __shared__ float final_state[kKvMaxWeightRows][2];
-    __shared__ float keep[kMaxSplits];
-    __shared__ alignas(16) float part[kBeside][D];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.y, b = blockIdx.z;
+    __shared__ float keep[4 / WAVES][kMaxSplits];
+    __shared__ alignas(16) float part[WAVES][D];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = blockIdx.y, b = blockIdx.z;
     const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
     const int rows = s.n * p.group;
     const int64_t seq = static_cast<int64_t>(b) * c.kv_heads + h;
-    if (static_cast<int>(blockIdx.x) < row_groups && static_cast<int>(blockIdx.x) >= rows) return;
+    const bool joins = static_cast<int>(blockIdx.x) < row_groups;
+    if (joins && static_cast<int>(blockIdx.x) * (4 / WAVES) >= rows) return;
     const KvSlot slot = kv_slot(p, -1 - b);
     const auto slot_of = [&](int r) { return (static_cast<int64_t>(h) * p.row_tiles + r / p.tile_rows) * p.slots + slot.first; };
     const auto state_of = [&](int r) {
         return reinterpret_cast<const float2*>(p.part_state) + slot_of(r) * p.tile_rows + r % p.tile_rows;
     };
-    if (static_cast<int>(blockIdx.x) < row_groups) {
-        const int r = blockIdx.x;
+    if (joins) {
+        const int r = blockIdx.x * (4 / WAVES) + wave / WAVES, nth = wave % WAVES, mine = wave / WAVES;
         if (slot.splits <= 1) return;  // its only workgroup wrote the row
-        if (wave == 0) {
+        float4v acc = {0, 0, 0, 0};
+        if (r < rows) {
             const float2* st = state_of(r);
             float most = -__builtin_inff(), total = 0.0f;
-            float2 mine[kMaxSplits / 64];
+            float2 state[kMaxSplits / 64];
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 64; ++k) {
                 const int i = k * 64 + lane;
-                mine[k] = i < slot.splits ? st[i * p.tile_rows] : make_float2(-__builtin_inff(), 0.0f);
-                most = fmaxf(most, mine[k].x);
+                state[k] = i < slot.splits ? st[i * p.tile_rows] : make_float2(-__builtin_inff(), 0.0f);
+                most = fmaxf(most, state[k].x);
             }
             most = wave_max(most);
             const float ref = most == -__builtin_inff() ? 0.0f : most;
 #pragma unroll
-            for (int k = 0; k < kMaxSplits / 64; ++k) total += mine[k].y * exp2_fast(mine[k].x - ref);
+            for (int k = 0; k < kMaxSplits / 64; ++k) total += state[k].y * exp2_fast(state[k].x - ref);
 #pragma unroll
             for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
             // a split without blocks wrote no sums: its factor is 0 and its sums are not read
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 64; ++k)
                 if (k * 64 + lane < slot.splits)
-                    keep[k * 64 + lane] = mine[k].y == 0.0f ? 0.0f : exp2_fast(mine[k].x - ref) / total;
-        }
-        __syncthreads();
-        const int d = tid % kPer * 4, beside = tid / kPer;
-        float4v acc = {0, 0, 0, 0};
-        if (beside < kBeside) {
-            const float* from = p.part_out + (slot_of(r) * p.tile_rows + r % p.tile_rows) * D + d;
+                    keep[mine][k * 64 + lane] = state[k].y == 0.0f ? 0.0f : exp2_fast(state[k].x - ref) / total;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+            const int beside = lane / kPer;
+            const float* from = p.part_out + (slot_of(r) * p.tile_rows + r % p.tile_rows) * D + lane % kPer * 4;
+            if (beside < kBeside) {
 #pragma unroll 4
-            for (int i = beside; i < slot.splits; i += kBeside) {
-                const float f = keep[i];
-                if (f != 0.0f) acc += f * *reinterpret_cast<const float4v*>(from + static_cast<int64_t>(i) * p.tile_rows * D);
+                for (int i = nth * kBeside + beside; i < slot.splits; i += WAVES * kBeside) {
+                    const float f = keep[mine][i];
+                    if (f != 0.0f) acc += f * *reinterpret_cast<const float4v*>(from + static_cast<int64_t>(i) * p.tile_rows * D);
+                }
             }
-            *reinterpret_cast<float4v*>(&part[beside][d]) = acc;
-        }
-        __syncthreads();
-        if (tid < D) {
-            float x = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kBeside; ++i) x += part[i][tid];
+            for (int g = kPer; g < 64 && kBeside > 1; g *= 2)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], g, 64);
+        }
+        if constexpr (WAVES > 1) {
+            if (lane < kPer) *reinterpret_cast<float4v*>(&part[nth][lane * 4]) = acc;
+            __syncthreads();
+            if (nth > 0) return;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w)
+                if (lane < kPer) acc += *reinterpret_cast<float4v*>(&part[w][lane * 4]);
+        }
+        if (r < rows && lane < kPer) {
             const int hd = h * p.group + r % p.group;
-            static_cast<T*>(a.out)[(s.row0 + r / p.group) * a.out_row + hd * a.out_head + tid] = K::from_f32(x);
+            T* out = static_cast<T*>(a.out) + (s.row0 + r / p.group) * a.out_row + hd * a.out_head + lane * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = K::from_f32(acc[e]);
         }
         return;
     }
@@ -392,10 +406,17 @@ int launch(const KvAttend& p, hipStream_t stream) {
 
 template <int TYPE, int D>
 int launch_join(const KvAttend& p, hipStream_t stream) {
-    const int row_groups = p.part_out ? static_cast<int>(p.a.max_new) * p.group : 0;
+    // a sequence's splits are about share / batch
+    const bool many = p.share > 12 * p.c.batch;
+    const int rows = p.part_out ? static_cast<int>(p.a.max_new) * p.group : 0;
+    const int row_groups = many ? rows : (rows + 3) / 4;
     const int weight_groups = p.a.weights_out ? (p.c.max_blocks + 255) / 256 : 0;
-    if (row_groups + weight_groups > 0)
-        kv_join_kernel<TYPE, D><<<dim3(row_groups + weight_groups, p.c.kv_heads, p.c.batch), 256, 0, stream>>>(p, row_groups);
+    const dim3 grid(row_groups + weight_groups, p.c.kv_heads, p.c.batch);
+    if (grid.x == 0) return kStatusOk;
+    if (many)
+        kv_join_kernel<TYPE, D, 4><<<grid, 256, 0, stream>>>(p, row_groups);
+    else
+        kv_join_kernel<TYPE, D, 1><<<grid, 256, 0, stream>>>(p, row_groups);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 

@@ -64,14 +64,9 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
     const int lead = max(s.past - j * kKvBlock, 0);          // tokens the block held before
     const int end = min(s.past + s.n - j * kKvBlock, kKvBlock);
     if (end <= lead) return;
-    const int64_t entry_row = (static_cast<int64_t>(b) * a.c.kv_heads + h) * a.c.max_blocks;
-    const int at = j - a.c.dropped[b];
-    if (at < 0 || at >= a.c.max_blocks) return;
-    const int page = a.c.table[entry_row + at];
-    if (page < 0 || page >= a.c.n_pages) return;
-    uint8_t* keys = a.c.pages + static_cast<int64_t>(page) * (2 * kKvBlock * D);
     const int64_t row = s.row0 + (j * kKvBlock - s.past);     // the row of the block's token 0
 
+    // the rows' loads go out before the table's, which they do not wait for
     float x[2][kRounds][16];
     uint32_t top[2] = {0, 0};
 #pragma unroll
@@ -83,10 +78,27 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
             const int i = tid + r * kAppendThreads, t = i / (D / 16), c = i % (D / 16);
             if (t >= lead && t < end) {
                 load16<TYPE>(src + (row + t) * stride + c * 16, a.vec, x[w][r]);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top[w] = max(top[w], __float_as_uint(x[w][r][e]) & 0x7fffffffu);
+                for (int e = 0; e < 16; ++e) x[w][r][e] = 0.0f;
             }
         }
+    }
+    const int64_t entry_row = (static_cast<int64_t>(b) * a.c.kv_heads + h) * a.c.max_blocks;
+    const int at = j - a.c.dropped[b];
+    if (at < 0 || at >= a.c.max_blocks) return;
+    const int page = a.c.table[entry_row + at];
+    if (page < 0 || page >= a.c.n_pages) return;
+    uint8_t* keys = a.c.pages + static_cast<int64_t>(page) * (2 * kKvBlock * D);
+    float before[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) before[w] = lead > 0 ? a.c.scales[2 * static_cast<int64_t>(page) + w] : 0.0f;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top[w] = max(top[w], __float_as_uint(x[w][r][e]) & 0x7fffffffu);
         top[w] = wave_max_u32(top[w]);
         if ((tid & 63) == 0) red[w][tid >> 6] = top[w];
     }
@@ -96,12 +108,11 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
         top[w] = red[w][0];
 #pragma unroll
         for (int i = 1; i < kAppendThreads / 64; ++i) top[w] = max(top[w], red[w][i]);
-        const float before = lead > 0 ? a.c.scales[2 * static_cast<int64_t>(page) + w] : 0.0f;
         const float amax = __uint_as_float(top[w]);
         // bit patterns above FLT_MAX are infinities and NaNs
-        const bool bad = top[w] > 0x7f7fffffu || !(before <= 3.402823466e38f);
-        const float scale = bad ? __builtin_nanf("") : fmaxf(fmaxf(amax / 127.0f, before), kKvScaleFloor);
-        const float inv = bad ? 0.0f : 1.0f / scale, again = bad ? 0.0f : before / scale;
+        const bool bad = top[w] > 0x7f7fffffu || !(before[w] <= 3.402823466e38f);
+        const float scale = bad ? __builtin_nanf("") : fmaxf(fmaxf(amax / 127.0f, before[w]), kKvScaleFloor);
+        const float inv = bad ? 0.0f : 1.0f / scale, again = bad ? 0.0f : before[w] / scale;
         int8_t* out = reinterpret_cast<int8_t*>(keys) + w * (kKvBlock * D);
         // new codes: keys straight to their place, values to LDS
 #pragma unroll
@@ -144,8 +155,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
                 *reinterpret_cast<uint4*>(out + i * 16) = *reinterpret_cast<uint4*>(q);
             }
         }
-        // all threads have read the scale before it is replaced
-        __syncthreads();
+        // all threads read the scales before the barrier above
         if (tid == 0) a.c.scales[2 * static_cast<int64_t>(page) + w] = scale;
     }
     if (tid == 0 && lead == 0) {
@@ -168,8 +178,9 @@ __device__ __forceinline__ int find_block(const int32_t* starts, int n, int star
     return lo < n && starts[lo] == start ? lo : -1;
 }
 
-// One workgroup per 32 positions of a sequence and head, a thread per 16 dims
-// of a position.
+// One workgroup per block of a sequence and head that holds a position asked for,
+// through LDS, so that both the page and the rows are whole runs of 16 bytes a
+// lane. Bound by the bytes of codes and rows.
 template <int TYPE, int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(rocknpu_kv_cache c, const int32_t* __restrict__ first,
                                                       const int32_t* __restrict__ tokens, int64_t count,
@@ -177,49 +188,72 @@ __global__ __launch_bounds__(256) void kv_read_kernel(rocknpu_kv_cache c, const 
                                                       typename KvType<TYPE>::T* __restrict__ v) {
     using K = KvType<TYPE>;
     using T = typename K::T;
-    const int b = blockIdx.z, h = blockIdx.y;
+    constexpr int kChunks = kKvBlock * D / 16;
+    __shared__ alignas(16) int8_t codes[2][kKvBlock][D + 4];
+    const int tid = threadIdx.x, b = blockIdx.z, h = blockIdx.y;
     const int total = min(max(tokens[b], 0), 0x3fffffff);
     const int gone = max(c.dropped[b], 0);
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
     const int64_t entry_row = (static_cast<int64_t>(b) * c.kv_heads + h) * c.max_blocks;
-    for (int i = threadIdx.x; i < kKvBlock * D / 16; i += 256) {
-        const int64_t o = static_cast<int64_t>(blockIdx.x) * kKvBlock + i / (D / 16);
-        const int d = i % (D / 16) * 16;
-        if (o >= count) continue;
-        const int64_t pos = first[b] + o;
-        float xk[16] = {}, xv[16] = {};
-        if (pos >= 0 && pos < total) {
-            const int start = static_cast<int>(pos) / kKvBlock * kKvBlock, t = static_cast<int>(pos) % kKvBlock;
-            int at = start / kKvBlock;
-            if (gone) at = find_block(c.starts + entry_row, held, start);
-            const int page = at >= 0 && at < held ? c.table[entry_row + at] : -1;
-            if (page >= 0 && page < c.n_pages) {
-                const int8_t* keys = reinterpret_cast<const int8_t*>(c.pages) + static_cast<int64_t>(page) * (2 * kKvBlock * D);
-                const int8_t* values = keys + kKvBlock * D;
-                const float sk = c.scales[2 * static_cast<int64_t>(page)], sv = c.scales[2 * static_cast<int64_t>(page) + 1];
+    const int64_t from = first[b];
+    const int64_t start = ((from - (from < 0 ? kKvBlock - 1 : 0)) / kKvBlock + blockIdx.x) * kKvBlock;
+    if (start >= from + count) return;
+    int page = -1;
+    if (start >= 0 && start < total) {
+        int at = static_cast<int>(start / kKvBlock);
+        if (gone) at = find_block(c.starts + entry_row, held, static_cast<int>(start));
+        page = at >= 0 && at < held ? c.table[entry_row + at] : -1;
+        if (page >= c.n_pages) page = -1;
+    }
+    const int8_t* keys = reinterpret_cast<const int8_t*>(c.pages) + static_cast<int64_t>(max(page, 0)) * (2 * kKvBlock * D);
+    const float2 scale = reinterpret_cast<const float2*>(c.scales)[max(page, 0)];
+    constexpr int kRounds = (kChunks + 255) / 256, kPer = 16 / sizeof(T);
+    struct alignas(16) Quad {
+        T e[kPer];
+    };
+    uint4 key[kRounds] = {}, value[kRounds] = {};
+    if (page >= 0) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    xk[e] = static_cast<float>(keys[kv_key_at(t, d + e)]) * sk;
-                    xv[e] = static_cast<float>(values[kv_value_at(t, d + e)]) * sv;
-                }
+        for (int r = 0; r < kRounds; ++r) {
+            const int i = tid + r * 256;
+            if (i < kChunks) {
+                key[r] = *reinterpret_cast<const uint4*>(keys + i * 16);
+                value[r] = *reinterpret_cast<const uint4*>(keys + kKvBlock * D + i * 16);
             }
         }
-        const int64_t to = ((static_cast<int64_t>(b) * count + o) * c.kv_heads + h) * D + d;
-        struct alignas(16) Quad {
-            T e[16 / sizeof(T)];
-        };
-        constexpr int kPer = 16 / sizeof(T);
+    }
+    // keys: token i / 4 % 32, dims 64 (i / 128) + 16 (i % 4); values: 8 tokens of dims d and d + 16
 #pragma unroll
-        for (int p = 0; p < 16 / kPer; ++p) {
-            Quad qk, qv;
+    for (int r = 0; r < kRounds; ++r) {
+        const int i = tid + r * 256;
+        if (i < kChunks) {
+            uint32_t* row = reinterpret_cast<uint32_t*>(&codes[0][i / 4 % kKvBlock][i / 128 * 64 + i % 4 * 16]);
+            row[0] = key[r].x;
+            row[1] = key[r].y;
+            row[2] = key[r].z;
+            row[3] = key[r].w;
+            const int d = i / 64 * 32 + i / 4 % 16, t4 = i % 4 * 4;
+            const int8_t* q = reinterpret_cast<const int8_t*>(&value[r]);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                qk.e[e] = K::from_f32(xk[p * kPer + e]);
-                qv.e[e] = K::from_f32(xv[p * kPer + e]);
-            }
-            reinterpret_cast<Quad*>(k + to)[p] = qk;
-            reinterpret_cast<Quad*>(v + to)[p] = qv;
+            for (int e = 0; e < 16; ++e) codes[1][e / 4 % 2 * 16 + t4 + e % 4][d + e / 8 * 16] = q[e];
         }
+    }
+    __syncthreads();
+    // 16 bytes of a row a thread
+    for (int i = tid; i < 2 * kKvBlock * D / kPer; i += 256) {
+        const int w = i / (kKvBlock * D / kPer), t = i / (D / kPer) % kKvBlock, d = i % (D / kPer) * kPer;
+        const int64_t o = start + t - from;
+        if (o < 0 || o >= count) continue;
+        const bool there = page >= 0 && start + t < total;
+        Quad quad;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            float x = static_cast<float>(codes[w][t][d + e]) * (w ? scale.y : scale.x);
+            // the f32 product is the value: not joined with the conversion to f16, which would round it once only
+            asm("" : "+v"(x));
+            quad.e[e] = K::from_f32(there ? x : 0.0f);
+        }
+        *reinterpret_cast<Quad*>((w ? v : k) + ((static_cast<int64_t>(b) * count + o) * c.kv_heads + h) * D + d) = quad;
     }
 }
 
@@ -230,9 +264,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The sum of `v` over the threads before this one; `total` over all of them.
+// The sum of `v` over the threads before this one.
 template <int THREADS>
-__device__ __forceinline__ int exclusive_sum(int v, int* part, int& total) {
+__device__ __forceinline__ int exclusive_sum(int v, int* part) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int x = v;
 #pragma unroll
@@ -243,118 +277,128 @@ __device__ __forceinline__ int exclusive_sum(int v, int* part, int& total) {
     if (lane == 63) part[wave] = x;
     __syncthreads();
     int before = 0;
-    total = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-        if (w < wave) before += part[w];
-        total += part[w];
-    }
-    __syncthreads();
+    for (int w = 0; w < THREADS / 64; ++w) before += w < wave ? part[w] : 0;
     return before + x - v;
 }
 
-// One workgroup per row of the table, every thread with ITEMS consecutive
-// entries in registers. The budget-th greatest key is found a byte at a time
-// from the top (a histogram of the entries that match the bytes found so far),
-// then two sums over the threads place every entry. Everything is read before
-// the first write, so outputs may be the inputs. Bound by the latency of its
-// steps: a row is a few kilobytes.
+// One workgroup per row of the table, entry i * THREADS + thread in register i of
+// a thread. The budget-th greatest key is found by digits of 11, 11 and 10 bits
+// from the top (a histogram in LDS of the entries that match the digits found so
+// far): the first digit holds the exponent and two more bits, so that few of a
+// wave's lanes meet in one bin (with digits of 8 bits 512 rows of 4098 took 30 us,
+// with these 20). Then ballots and one sum over (register, wave) place every
+// entry. Everything is read before the first write, so outputs may be the inputs.
+// Bound by the latency of its steps where rows are few, else by its bytes.
 template <int THREADS, int ITEMS>
 __global__ __launch_bounds__(THREADS) void kv_evict_kernel(rocknpu_kv_evict_args a) {
-    __shared__ int hist[256];
-    __shared__ int part[THREADS / 64];
-    __shared__ int pick[2];  // the byte found, and how many entries rank above it
-    const int tid = threadIdx.x;
+    constexpr int kWaves = THREADS / 64, kBins = 2048, kGroups = ITEMS * kWaves;
+    static_assert(kGroups <= THREADS);
+    __shared__ int hist[kBins];
+    __shared__ int part[kWaves];
+    __shared__ int pick[2];                   // the digit found, and how many entries rank above it
+    __shared__ int count[kGroups][2];         // by register and wave: entries above the key found, and equal to it
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x;
     const int b = static_cast<int>(r / a.kv_heads);
     const int64_t base = r * a.max_blocks;
+    int32_t page[ITEMS], start[ITEMS];
+    float w[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int at = min(i * THREADS + tid, a.max_blocks - 1);
+        w[i] = a.weights[base + at];
+        page[i] = a.table[base + at];
+        start[i] = a.starts[base + at];
+    }
     const int total = min(max(a.tokens[b], 0), 0x3fffffff);
     const int gone = max(a.dropped[b], 0);
     const int n = min(max((total + kKvBlock - 1) / kKvBlock - gone, 0), a.max_blocks);
-    int32_t page[ITEMS], start[ITEMS];
-    float w[ITEMS];
     uint32_t key[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int at = tid * ITEMS + i;
-        const bool in = at < a.max_blocks;
-        page[i] = in ? a.table[base + at] : 0;
-        start[i] = in ? a.starts[base + at] : 0;
-        w[i] = in ? a.weights[base + at] : 0.0f;
+        const int at = i * THREADS + tid;
         key[i] = at < a.sinks || at >= n - a.recent ? 0xffffffffu : weight_key(w[i]);
     }
-    __syncthreads();
+    int to[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) to[i] = i * THREADS + tid;
     if (n > a.budget) {
         uint32_t found = 0;
         int above = 0;  // entries known to rank above the budget-th
 #pragma unroll
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+            for (int i = tid; i < bins; i += THREADS) hist[i] = 0;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
-                if (tid * ITEMS + i < n && (shift == 24 || key[i] >> ((shift + 8) & 31) == found))
-                    atomicAdd(&hist[key[i] >> shift & 255], 1);
+                if (i * THREADS + tid < n && (pass == 0 || key[i] >> (pass == 1 ? 21 : 10) == found))
+                    atomicAdd(&hist[key[i] >> shift & (bins - 1)], 1);
             __syncthreads();
-            if (tid < 64) {  // lane l: bins 255 - 4 l down to 252 - 4 l
-                int c[4], sum = 0;
+            // this thread's bins, from the top
+            constexpr int kMost = kBins / THREADS > 0 ? kBins / THREADS : 1;
+            const int mine = bins / THREADS > 0 ? bins / THREADS : 1;
+            int c[kMost], sum = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - 4 * tid - i];
-                int x = sum;
+            for (int i = 0; i < kMost; ++i) {
+                c[i] = i < mine && tid * mine + i < bins ? hist[bins - 1 - tid * mine - i] : 0;
+                sum += c[i];
+            }
+            int up = above + exclusive_sum<THREADS>(sum, part);
 #pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int y = __shfl_up(x, o, 64);
-                    if (tid >= o) x += y;
+            for (int i = 0; i < kMost; ++i) {
+                if (up < a.budget && up + c[i] >= a.budget) {
+                    pick[0] = bins - 1 - tid * mine - i;
+                    pick[1] = up;
                 }
-                int up = above + x - sum;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (up < a.budget && up + c[i] >= a.budget) {
-                        pick[0] = 255 - 4 * tid - i;
-                        pick[1] = up;
-                    }
-                    up += c[i];
-                }
+                up += c[i];
             }
             __syncthreads();
-            found = found << 8 | static_cast<uint32_t>(pick[0]);
+            found = found << (pass == 2 ? 10 : 11) | static_cast<uint32_t>(pick[0]);
             above = pick[1];
         }
-        // of the entries equal to the budget-th key the first budget - above stay
-        int equal = 0, kept = 0, sum;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) equal += tid * ITEMS + i < n && key[i] == found;
-        int rank = exclusive_sum<THREADS>(equal, part, sum);
-        bool keep[ITEMS];
+        // Of the entries equal to the budget-th key the first `need` stay: an entry has as many kept ones before it as there
+        // are above the key, and equal to it but no more than `need`.
+        const int need = a.budget - above;
+        uint64_t over[ITEMS], same[ITEMS];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const bool in = tid * ITEMS + i < n;
-            keep[i] = in && (key[i] > found || (key[i] == found && rank < a.budget - above));
-            rank += in && key[i] == found;
-            kept += keep[i];
-        }
-        int before = exclusive_sum<THREADS>(kept, part, sum);
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int at = tid * ITEMS + i;
-            const int to = at >= n ? at : keep[i] ? before : a.budget + at - before;
-            before += keep[i];
-            if (at < a.max_blocks) {
-                a.table_out[base + to] = page[i];
-                a.starts_out[base + to] = start[i];
-                a.weights_out[base + to] = w[i];
+            const bool in = i * THREADS + tid < n;
+            over[i] = __ballot(in && key[i] > found);
+            same[i] = __ballot(in && key[i] == found);
+            if (lane == 0) {
+                count[i * kWaves + wave][0] = __popcll(over[i]);
+                count[i * kWaves + wave][1] = __popcll(same[i]);
             }
+        }
+        __syncthreads();
+        // both sums in one number: neither reaches 2^16
+        const int packed = tid < kGroups ? count[tid][0] << 16 | count[tid][1] : 0;
+        const int before = exclusive_sum<THREADS>(packed, part);
+        if (tid < kGroups) {
+            count[tid][0] = before >> 16;
+            count[tid][1] = before & 0xffff;
+        }
+        __syncthreads();
+        const uint64_t lower = (uint64_t{1} << lane) - 1;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int at = i * THREADS + tid;
+            const int equal = count[i * kWaves + wave][1] + __popcll(same[i] & lower);
+            const int kept = count[i * kWaves + wave][0] + __popcll(over[i] & lower) + min(equal, need);
+            const bool keep = (over[i] >> lane & 1) || ((same[i] >> lane & 1) && equal < need);
+            if (at < n) to[i] = keep ? kept : a.budget + at - kept;
         }
     } else {
+        __syncthreads();
+    }
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int at = tid * ITEMS + i;
-            if (at < a.max_blocks) {
-                a.table_out[base + at] = page[i];
-                a.starts_out[base + at] = start[i];
-                a.weights_out[base + at] = w[i];
-            }
-        }
+    for (int i = 0; i < ITEMS; ++i) {
+        if (i * THREADS + tid >= a.max_blocks) break;
+        a.table_out[base + to[i]] = page[i];
+        a.starts_out[base + to[i]] = start[i];
+        a.weights_out[base + to[i]] = w[i];
     }
     if (tid == 0 && r % a.kv_heads == 0) a.dropped_out[b] = a.dropped[b] + max(n - a.budget, 0);
 }
@@ -377,7 +421,8 @@ template <int TYPE>
 void launch_read(const rocknpu_kv_cache& c, const int32_t* first, const int32_t* tokens, int64_t count, void* k, void* v,
                  hipStream_t s) {
     using T = typename KvType<TYPE>::T;
-    const dim3 grid(static_cast<unsigned>((count + kKvBlock - 1) / kKvBlock), c.kv_heads, c.batch);
+    // a run of `count` positions touches at most this many blocks, wherever in a block it begins
+    const dim3 grid(static_cast<unsigned>((count + 2 * kKvBlock - 2) / kKvBlock), c.kv_heads, c.batch);
     T *kt = static_cast<T*>(k), *vt = static_cast<T*>(v);
     switch (c.head_dim) {
         case 64: kv_read_kernel<TYPE, 64><<<grid, 256, 0, s>>>(c, first, tokens, count, kt, vt); break;

@@ -13,24 +13,22 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return __float_as_uint(wave_max_nonneg(__uint_as_float(v)));
 }
 
-// 16 consecutive elements as f32. `vec`: 16-byte aligned.
+// 16 bytes of elements as f32. `vec`: 16-byte aligned.
 template <int TYPE>
-__device__ __forceinline__ void load16(const typename KvType<TYPE>::T* p, bool vec, float (&x)[16]) {
+__device__ __forceinline__ void load_piece(const typename KvType<TYPE>::T* p, bool vec,
+                                           float (&x)[16 / sizeof(typename KvType<TYPE>::T)]) {
     using K = KvType<TYPE>;
+    constexpr int kPer = 16 / sizeof(typename K::T);
     if (vec) {
-        constexpr int kPer = 16 / sizeof(typename K::T);
         struct alignas(16) Quad {
             typename K::T e[kPer];
         };
+        const Quad v = *reinterpret_cast<const Quad*>(p);
 #pragma unroll
-        for (int i = 0; i < 16 / kPer; ++i) {
-            const Quad v = reinterpret_cast<const Quad*>(p)[i];
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) x[i * kPer + j] = K::to_f32(v.e[j]);
-        }
+        for (int e = 0; e < kPer; ++e) x[e] = K::to_f32(v.e[e]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = K::to_f32(p[i]);
+        for (int e = 0; e < kPer; ++e) x[e] = K::to_f32(p[e]);
     }
 }
 
@@ -47,17 +45,18 @@ struct AppendArgs {
     bool vec;
 };
 
-// One workgroup per touched block of a sequence and head. Keys are the first
-// pass, values the second: the new rows' largest magnitude over the workgroup,
-// the block's scale, then its bytes in page order. Values are transposed
-// through LDS. Bound by the bytes of the rows and codes.
+// One workgroup per touched block of a sequence and head: the new rows, 16 bytes
+// a lane, stay in registers while the workgroup finds their largest magnitudes;
+// their codes pass through LDS and leave in page order, 16 bytes a lane. Bound by
+// the bytes of the rows and codes.
 template <int TYPE, int D>
 __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a) {
     using T = typename KvType<TYPE>::T;
-    constexpr int kChunks = kKvBlock * D / 16;                               // 16-byte pieces of keys, and of values
-    constexpr int kRounds = (kChunks + kAppendThreads - 1) / kAppendThreads;
+    constexpr int kPer = 16 / sizeof(T);                          // elements of a piece of a row
+    constexpr int kPieces = kKvBlock * D / kPer, kRounds = (kPieces + kAppendThreads - 1) / kAppendThreads;
+    constexpr int kChunks = kKvBlock * D / 16;                    // 16-byte pieces of a page's keys, and of its values
     __shared__ uint32_t red[2][kAppendThreads / 64];
-    __shared__ alignas(16) int8_t codes[kKvBlock][D + 4];
+    __shared__ alignas(16) int8_t codes[2][kKvBlock][D + 4];
     const int tid = threadIdx.x, b = blockIdx.z, h = blockIdx.y;
     const KvSpan s = kv_span(a.past, a.cu, b, a.rows, a.max_new);
     const int j = s.past / kKvBlock + blockIdx.x;
@@ -67,96 +66,99 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
     const int64_t row = s.row0 + (j * kKvBlock - s.past);     // the row of the block's token 0
 
     // the rows' loads go out before the table's, which they do not wait for
-    float x[2][kRounds][16];
-    uint32_t top[2] = {0, 0};
+    float x[2][kRounds][kPer];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         const T* src = static_cast<const T*>(w ? a.v : a.k) + h * (w ? a.v_head : a.k_head);
         const int64_t stride = w ? a.v_row : a.k_row;
 #pragma unroll
         for (int r = 0; r < kRounds; ++r) {
-            const int i = tid + r * kAppendThreads, t = i / (D / 16), c = i % (D / 16);
+            const int i = tid + r * kAppendThreads, t = i / (D / kPer);
             if (t >= lead && t < end) {
-                load16<TYPE>(src + (row + t) * stride + c * 16, a.vec, x[w][r]);
+                load_piece<TYPE>(src + (row + t) * stride + i % (D / kPer) * kPer, a.vec, x[w][r]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[w][r][e] = 0.0f;
+                for (int e = 0; e < kPer; ++e) x[w][r][e] = 0.0f;
             }
         }
     }
     const int64_t entry_row = (static_cast<int64_t>(b) * a.c.kv_heads + h) * a.c.max_blocks;
-    const int at = j - a.c.dropped[b];
+    const int at = j - max(a.c.dropped[b], 0);
     if (at < 0 || at >= a.c.max_blocks) return;
     const int page = a.c.table[entry_row + at];
     if (page < 0 || page >= a.c.n_pages) return;
-    uint8_t* keys = a.c.pages + static_cast<int64_t>(page) * (2 * kKvBlock * D);
+    int8_t* keys = reinterpret_cast<int8_t*>(a.c.pages) + static_cast<int64_t>(page) * (2 * kKvBlock * D);
     float before[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) before[w] = lead > 0 ? a.c.scales[2 * static_cast<int64_t>(page) + w] : 0.0f;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
+        uint32_t top = 0;
 #pragma unroll
         for (int r = 0; r < kRounds; ++r)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top[w] = max(top[w], __float_as_uint(x[w][r][e]) & 0x7fffffffu);
-        top[w] = wave_max_u32(top[w]);
-        if ((tid & 63) == 0) red[w][tid >> 6] = top[w];
+            for (int e = 0; e < kPer; ++e) top = max(top, __float_as_uint(x[w][r][e]) & 0x7fffffffu);
+        top = wave_max_u32(top);
+        if ((tid & 63) == 0) red[w][tid >> 6] = top;
     }
     __syncthreads();
+    float again[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        top[w] = red[w][0];
+        uint32_t top = red[w][0];
 #pragma unroll
-        for (int i = 1; i < kAppendThreads / 64; ++i) top[w] = max(top[w], red[w][i]);
-        const float amax = __uint_as_float(top[w]);
+        for (int i = 1; i < kAppendThreads / 64; ++i) top = max(top, red[w][i]);
         // bit patterns above FLT_MAX are infinities and NaNs
-        const bool bad = top[w] > 0x7f7fffffu || !(before[w] <= 3.402823466e38f);
-        const float scale = bad ? __builtin_nanf("") : fmaxf(fmaxf(amax / 127.0f, before[w]), kKvScaleFloor);
-        const float inv = bad ? 0.0f : 1.0f / scale, again = bad ? 0.0f : before[w] / scale;
-        int8_t* out = reinterpret_cast<int8_t*>(keys) + w * (kKvBlock * D);
-        // new codes: keys straight to their place, values to LDS
-#pragma unroll
-        for (int r = 0; r < kRounds; ++r) {
-            const int i = tid + r * kAppendThreads, t = i / (D / 16), c = i % (D / 16);
-            if (t >= lead && t < end) {
-                alignas(16) int8_t q[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) q[e] = bad ? int8_t{0} : code_of(x[w][r][e], inv);
-                if (w == 0) {
-                    *reinterpret_cast<uint4*>(out + kv_key_at(t, c * 16)) = *reinterpret_cast<uint4*>(q);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        reinterpret_cast<uint32_t*>(&codes[t][c * 16])[e] = reinterpret_cast<uint32_t*>(q)[e];
-                }
-            } else if (w == 0 && t < lead && again != 1.0f) {
-                alignas(16) int8_t q[16];
-                *reinterpret_cast<uint4*>(q) = *reinterpret_cast<uint4*>(out + kv_key_at(t, c * 16));
-#pragma unroll
-                for (int e = 0; e < 16; ++e) q[e] = code_of(static_cast<float>(q[e]), again);
-                *reinterpret_cast<uint4*>(out + kv_key_at(t, c * 16)) = *reinterpret_cast<uint4*>(q);
-            }
-        }
-        if (w == 1) {
-            __syncthreads();
-            // values in page order: 16 bytes are 8 tokens of dims d and d + 16
-            for (int i = tid; i < kChunks; i += kAppendThreads) {
-                const int d = i / 64 * 32 + i / 4 % 16, t4 = i % 4 * 4;
-                alignas(16) int8_t q[16];
-                if (lead > 0) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<uint4*>(out + i * 16);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int t = e / 4 % 2 * 16 + t4 + e % 4;
-                    if (t < lead)
-                        q[e] = code_of(static_cast<float>(q[e]), again);
-                    else
-                        q[e] = t < end ? codes[t][d + e / 8 * 16] : int8_t{0};
-                }
-                *reinterpret_cast<uint4*>(out + i * 16) = *reinterpret_cast<uint4*>(q);
-            }
-        }
+        const bool bad = top > 0x7f7fffffu || !(before[w] <= 3.402823466e38f);
+        const float scale = bad ? __builtin_nanf("") : fmaxf(fmaxf(__uint_as_float(top) / 127.0f, before[w]), kKvScaleFloor);
+        const float inv = bad ? 0.0f : 1.0f / scale;
+        again[w] = bad ? 0.0f : before[w] / scale;
         // all threads read the scales before the barrier above
         if (tid == 0) a.c.scales[2 * static_cast<int64_t>(page) + w] = scale;
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const int i = tid + r * kAppendThreads, t = i / (D / kPer);
+            if (t < kKvBlock) {
+                uint32_t* to = reinterpret_cast<uint32_t*>(&codes[w][t][i % (D / kPer) * kPer]);
+#pragma unroll
+                for (int e = 0; e < kPer / 4; ++e) {
+                    uint32_t q = 0;
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                        q |= bad ? 0u : static_cast<uint32_t>(code_of(x[w][r][e * 4 + f], inv) & 0xff) << (8 * f);
+                    to[e] = q;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < kChunks; i += kAppendThreads) {
+        // keys: token i / 4 % 32, dims 64 (i / 128) + 16 (i % 4)
+        const int t = i / 4 % kKvBlock;
+        if (t >= lead && t < end) {
+            const uint32_t* row_lds = reinterpret_cast<const uint32_t*>(&codes[0][t][i / 128 * 64 + i % 4 * 16]);
+            *reinterpret_cast<uint4*>(keys + i * 16) = make_uint4(row_lds[0], row_lds[1], row_lds[2], row_lds[3]);
+        } else if (t < lead && again[0] != 1.0f) {
+            alignas(16) int8_t q[16];
+            *reinterpret_cast<uint4*>(q) = *reinterpret_cast<uint4*>(keys + i * 16);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) q[e] = code_of(static_cast<float>(q[e]), again[0]);
+            *reinterpret_cast<uint4*>(keys + i * 16) = *reinterpret_cast<uint4*>(q);
+        }
+        // values: 8 tokens of dims d and d + 16
+        const int d = i / 64 * 32 + i / 4 % 16, t4 = i % 4 * 4;
+        int8_t* values = keys + kKvBlock * D + i * 16;
+        alignas(16) int8_t q[16];
+        if (lead > 0) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<uint4*>(values);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int tv = e / 4 % 2 * 16 + t4 + e % 4;
+            if (tv < lead)
+                q[e] = code_of(static_cast<float>(q[e]), again[1]);
+            else
+                q[e] = codes[1][tv][d + e / 8 * 16];
+        }
+        *reinterpret_cast<uint4*>(values) = *reinterpret_cast<uint4*>(q);
     }
     if (tid == 0 && lead == 0) {
         a.c.starts[entry_row + at] = j * kKvBlock;

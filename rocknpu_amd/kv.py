@@ -17,7 +17,6 @@ HIP graph.
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -60,27 +59,36 @@ class _EvictStruct(ctypes.Structure):
                 ("kv_heads", _i32), ("max_blocks", _i32), ("budget", _i32), ("sinks", _i32), ("recent", _i32)]
 
 
-def _is(t, shape, dtype, what, device=None):
+# A serving step makes these calls per layer and token: their checks are kept to a
+# few comparisons.
+def _is(t, shape, dtype, what, device):
     """`t` is a contiguous tensor of that shape and type, on that device."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{what} has to be a contiguous {dtype} tensor of shape {tuple(shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the cache on {device}")
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or t.device != device
+            or not t.is_contiguous()):
+        raise ValueError(f"{what} has to be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
     return t
 
 
 def _rows(t, heads, head_dim, what, device):
-    """`t` is [rows, heads, head_dim] of a known type with a contiguous last dimension: its strides."""
-    if t.dtype not in _TYPES:
-        raise ValueError(f"{what} is {t.dtype}: float32, float16 or bfloat16 is wanted")
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != head_dim:
-        raise ValueError(f"{what} has to be [rows, {'heads' if heads is None else heads}, {head_dim}], not {tuple(t.shape)}")
+    """`t` is [rows, heads, head_dim] of a known type with a contiguous last dimension: its shape and strides."""
+    shape = t.shape
+    if t.dtype not in _TYPES or len(shape) != 3 or shape[2] != head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what} has to be float32, float16 or bfloat16 [rows, {'heads' if heads is None else heads}, "
+                         f"{head_dim}], not {t.dtype} {tuple(shape)}")
     row, head, one = t.stride()
     if one != 1 and t.numel():
         raise ValueError(f"{what} has to be contiguous in its last dimension")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, the cache on {device}")
-    return row, head
+    return shape[0], shape[1], row, head
+
+
+def _stream(device: torch.device) -> int:
+    """The device's current stream, as hip._stream gives it, without its object where torch offers that."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return raw(device.index)
 
 
 class Cache:
@@ -101,18 +109,21 @@ class Cache:
         n = pages.shape[0]
         if n == 0:
             raise ValueError("a cache needs at least one page")
-        self.pages = _is(pages, (n, 2 * BLOCK * head_dim), pages.dtype, "pages", at)
-        self.scales = _is(scales, (n, 2), torch.float32, "scales", at)
-        self.table = _is(table, table.shape, torch.int32, "table", at)
-        self.starts = _is(starts, table.shape, torch.int32, "starts", at)
-        self.dropped = _is(dropped, table.shape[:1], torch.int32, "dropped", at)
-        self.weights = None if weights is None else _is(weights, table.shape, torch.float32, "weights", at)
+        self.shape = table.shape
         self.batch, self.kv_heads, self.max_blocks = table.shape
         self.head_dim, self.device = head_dim, at
+        self._lengths, self._offsets = torch.Size((self.batch,)), torch.Size((self.batch + 1,))
+        self.pages = _is(pages, torch.Size((n, 2 * BLOCK * head_dim)), pages.dtype, "pages", at)
+        self.scales = _is(scales, torch.Size((n, 2)), torch.float32, "scales", at)
+        self.table = _is(table, table.shape, torch.int32, "table", at)
+        self.starts = _is(starts, table.shape, torch.int32, "starts", at)
+        self.dropped = _is(dropped, self._lengths, torch.int32, "dropped", at)
+        self.weights = None if weights is None else _is(weights, table.shape, torch.float32, "weights", at)
         self._struct = _CacheStruct(
             pages.data_ptr(), scales.data_ptr(), table.data_ptr(), starts.data_ptr(), dropped.data_ptr(),
             None if weights is None else weights.data_ptr(), n, self.batch, self.kv_heads, head_dim, self.max_blocks)
         self._ref = ctypes.addressof(self._struct)
+        self._needs: dict[tuple, int] = {}  # workspace bytes by the sizes that they depend on
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, head_dim: int, max_blocks: int, device="cuda", weights: bool = True):
@@ -124,11 +135,11 @@ class Cache:
                    torch.zeros(batch, dtype=torch.int32, device=device),
                    torch.zeros(table.shape, device=device) if weights else None, head_dim=head_dim)
 
-    def lengths(self, t, what):
-        return ctypes.c_void_p(_is(t, (self.batch,), torch.int32, what, self.device).data_ptr())
+    def lengths(self, t, what) -> int:
+        return _is(t, self._lengths, torch.int32, what, self.device).data_ptr()
 
-    def offsets(self, t):
-        return ctypes.c_void_p(_is(t, (self.batch + 1,), torch.int32, "cu", self.device).data_ptr())
+    def offsets(self, t) -> int:
+        return _is(t, self._offsets, torch.int32, "cu", self.device).data_ptr()
 
 
 def append(cache: Cache, k: torch.Tensor, v: torch.Tensor, past: torch.Tensor, cu: torch.Tensor, max_new: int) -> None:
@@ -137,13 +148,13 @@ def append(cache: Cache, k: torch.Tensor, v: torch.Tensor, past: torch.Tensor, c
     the rows of any one sequence. A partly filled block's scale only grows, and
     its older codes are rounded anew when it does; a value that is not finite
     makes its block NaN."""
-    k_row, k_head = _rows(k, cache.kv_heads, cache.head_dim, "k", cache.device)
-    v_row, v_head = _rows(v, cache.kv_heads, cache.head_dim, "v", cache.device)
-    if k.dtype != v.dtype or k.shape != v.shape:
-        raise ValueError("k and v differ in type or shape")
+    rows, _, k_row, k_head = _rows(k, cache.kv_heads, cache.head_dim, "k", cache.device)
+    v_rows, _, v_row, v_head = _rows(v, cache.kv_heads, cache.head_dim, "v", cache.device)
+    if k.dtype is not v.dtype or rows != v_rows:
+        raise ValueError("k and v differ in type or rows")
     hip._check(_lib.load().rocknpu_hip_kv_append(
-        cache._ref, _TYPES[k.dtype], k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, k.shape[0],
-        cache.lengths(past, "past"), cache.offsets(cu), max_new, hip._stream()), "kv_append")
+        cache._ref, _TYPES[k.dtype], k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, rows,
+        cache.lengths(past, "past"), cache.offsets(cu), max_new, _stream(cache.device)), "kv_append")
 
 
 def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dtype: torch.dtype = torch.float32):
@@ -152,11 +163,10 @@ def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dt
     tokens[b] and in evicted blocks."""
     if dtype not in _TYPES:
         raise ValueError(f"{dtype}: float32, float16 or bfloat16 is wanted")
-    k, v = (torch.empty((cache.batch, count, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
-            for _ in range(2))
+    k, v = torch.empty((2, cache.batch, count, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device).unbind(0)
     hip._check(_lib.load().rocknpu_hip_kv_read(
         cache._ref, cache.lengths(first, "first"), cache.lengths(tokens, "tokens"), count, _TYPES[dtype],
-        k.data_ptr(), v.data_ptr(), hip._stream()), "kv_read")
+        k.data_ptr(), v.data_ptr(), _stream(cache.device)), "kv_read")
     return k, v
 
 
@@ -191,32 +201,38 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
     cache.weights; at most 256 rows times heads per kv head). max_tokens, the
     most tokens a sequence is expected to hold, sizes the work split only;
     without it the table's width does."""
-    row, head = _rows(q, None, cache.head_dim, "q", cache.device)
-    rows, heads = q.shape[:2]
+    device, dtype = cache.device, q.dtype
+    rows, heads, row, head = _rows(q, None, cache.head_dim, "q", device)
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads over {cache.kv_heads} kv heads")
     if out is None:
-        out = torch.empty((rows, heads, cache.head_dim), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
-        raise ValueError("out has to have q's type and shape")
-    o_row, o_head = _rows(out, heads, cache.head_dim, "out", cache.device)
+        out = torch.empty(q.shape, dtype=dtype, device=device)
+        o_row, o_head = heads * cache.head_dim, cache.head_dim
+    else:
+        o_rows, _, o_row, o_head = _rows(out, heads, cache.head_dim, "out", device)
+        if out.dtype is not dtype or o_rows != rows:
+            raise ValueError("out has to have q's type and shape")
     args = _AttentionStruct(
         q.data_ptr(), out.data_ptr(), cache.lengths(past, "past"), cache.offsets(cu),
         None if prefix is None else cache.lengths(prefix, "prefix"),
-        None if slopes is None else _is(slopes, (heads,), torch.float32, "slopes", cache.device).data_ptr(),
-        None if weights_out is None else _is(weights_out, cache.table.shape, torch.float32, "weights_out",
-                                             cache.device).data_ptr(),
-        row, head, o_row, o_head, rows, max_new, max_tokens, _TYPES[q.dtype], heads, int(causal), window,
-        1.0 / math.sqrt(cache.head_dim) if scale is None else scale, softcap)
+        None if slopes is None else _is(slopes, torch.Size((heads,)), torch.float32, "slopes", device).data_ptr(),
+        None if weights_out is None else _is(weights_out, cache.shape, torch.float32, "weights_out", device).data_ptr(),
+        row, head, o_row, o_head, rows, max_new, max_tokens, _TYPES[dtype], heads, causal, window,
+        cache.head_dim ** -0.5 if scale is None else scale, softcap)
     lib = _lib.load()
     ref = ctypes.addressof(args)
-    need = ctypes.c_size_t()
-    hip._check(lib.rocknpu_hip_kv_attention_workspace(cache._ref, ref, 0, ctypes.byref(need)), "kv_attention")
+    sizes = (dtype, heads, rows == 0, max_new, max_tokens, window, weights_out is None)
+    need = cache._needs.get(sizes)
+    if need is None:
+        got = ctypes.c_size_t()
+        hip._check(lib.rocknpu_hip_kv_attention_workspace(cache._ref, ref, 0, ctypes.addressof(got)), "kv_attention")
+        need = cache._needs[sizes] = got.value
     ws, nbytes = None, 0
-    if need.value:
-        ws = workspace_for(cache.device, need.value) if workspace is None else workspace
-        nbytes = ws.numel() * ws.element_size()
-    hip._check(lib.rocknpu_hip_kv_attention(cache._ref, ref, hip._ptr(ws), nbytes, hip._stream()), "kv_attention")
+    if need:
+        if workspace is None:
+            workspace = workspace_for(device, need)
+        ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    hip._check(lib.rocknpu_hip_kv_attention(cache._ref, ref, ws, nbytes, _stream(device)), "kv_attention")
     return out
 
 
@@ -238,9 +254,10 @@ def evict(table: torch.Tensor, starts: torch.Tensor, weights: torch.Tensor, toke
     for (t, dtype, what), o in zip(kinds, out):
         _is(t, table.shape, dtype, what, at)
         _is(o, table.shape, dtype, what + "_out", at)
+    size = torch.Size((batch,))
     for t, what in ((tokens, "tokens"), (dropped, "dropped"), (out[3], "dropped_out")):
-        _is(t, (batch,), torch.int32, what, at)
+        _is(t, size, torch.int32, what, at)
     args = _EvictStruct(table.data_ptr(), starts.data_ptr(), weights.data_ptr(), tokens.data_ptr(), dropped.data_ptr(),
                         *[t.data_ptr() for t in out], batch, kv_heads, max_blocks, budget, sinks, recent)
-    hip._check(_lib.load().rocknpu_hip_kv_evict(ctypes.addressof(args), hip._stream()), "kv_evict")
+    hip._check(_lib.load().rocknpu_hip_kv_evict(ctypes.addressof(args), _stream(at)), "kv_evict")
     return out

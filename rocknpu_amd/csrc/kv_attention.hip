@@ -37,7 +37,12 @@ size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 // 106 and 55. f32: 30, 45, 98 and 115 against 51, 55, 83 and 75).
 constexpr int64_t kStreamRows = 32;
 constexpr int64_t kShortBlocks = 32;
-// Blocks of a split, at least: two for each of a workgroup's waves.
+// Up to this many blocks a workgroup takes them alone; and blocks of a split, at
+// least, where they are shared out (8 kv heads of 128, one row, one launch alone
+// against splits and their join: 16 blocks 8.4 and 12.7 us, 32 blocks 11.9 and
+// 13.1, 48 blocks 15.2 and 13.5; 125 blocks in splits of 8, 16 and 32: 14.9, 16.6
+// and 19.2).
+constexpr int kAlone = 32;
 constexpr int kMinChunk = 8;
 // Sequences up to which their blocks are shared out over the workgroups.
 constexpr int kMaxShared = 1024;
@@ -69,12 +74,12 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.min_chunk = kMinChunk;
     // One round of the workgroups that the GPU holds at once: a second round pays every workgroup's start (lookups, the
     // queries, the first blocks' latency) again. Sharing rounds each sequence up, by half a workgroup on average. 32
-    // ragged sequences of 500-4100 tokens, 8 kv heads of 128: 40.4 us; three quarters and one and a half rounds 48.7
-    // and 47.3; a fixed four parts a sequence 51.4. The prompt kernel shares blocks out where that gives every sequence
-    // and tile at least four parts: below, joining costs what it saves.
-    const int64_t resident = (c.head_dim <= 64 && r.stream ? 3 : c.head_dim <= 128 ? 2 : 1) * cus;
+    // ragged sequences of 500-4000 tokens, 8 kv heads of 128: 44 us; one and a half, two and three rounds 53, 55 and
+    // 54. The prompt kernel shares blocks out where that gives every sequence and tile at least four parts: below,
+    // joining costs what it saves.
+    const int64_t resident = (r.stream ? (c.head_dim == 64 ? 3 : 1) : (c.head_dim <= 128 ? 2 : 1)) * static_cast<int64_t>(cus);
     const int64_t share = std::max<int64_t>(resident / (c.kv_heads * p.row_tiles) - c.batch / 2, 1);
-    const bool shared = blocks > p.min_chunk && c.batch <= kMaxShared && rows > 0;
+    const bool shared = blocks > (r.stream ? kAlone : kMinChunk) && c.batch <= kMaxShared && rows > 0;
     p.share = shared && share >= (r.stream ? 2 : 4) ? static_cast<int>(std::min<int64_t>(share, c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk))) : 0;
     p.slots = p.share + c.batch;
     const size_t slots = static_cast<size_t>(p.slots) * c.kv_heads * p.row_tiles * p.tile_rows;

@@ -1,8 +1,8 @@
 // Attention of few rows over a long cache: the cache streams through the matrix
 // units once for up to 16 rows (a kv head's heads times the step's tokens).
 //
-// A workgroup of four waves takes one split of a (sequence, kv head, tile of 16
-// rows); a wave takes every fourth block. Blocks come from memory straight into
+// A workgroup of four or eight waves takes one split of a (sequence, kv head, tile
+// of 16 rows), its waves the split's blocks in turn. Blocks come from memory straight into
 // the operand registers (whole 1 KiB runs per load, the next block's loads in
 // flight behind the current one's work), so LDS is used only to join the waves.
 // Scores: keys (16 tokens x 32 dims) times the rows' queries; they leave in the
@@ -13,7 +13,13 @@
 namespace rk {
 namespace {
 
-constexpr int kWaves = 4;
+// Heads of 128 and 192 take 160 to 240 registers: two waves a SIMD, here as one
+// workgroup of eight, so that a context is cut into half as many splits (32
+// sequences of 500-4000 tokens, 8 kv heads of 128: 44 us against 53 in workgroups
+// of four; 8 of 4000: 26 and 26). Heads of 64 leave room for three waves, heads
+// of 256 for one: four waves (30 us against 35; 85 and 84, f32 with spills).
+template <int D>
+constexpr int kWavesOf = D == 128 || D == 192 ? 8 : 4;
 constexpr int kMaxSplits = kKvMaxSplits;
 
 template <int D>
@@ -47,7 +53,8 @@ __device__ __forceinline__ float sum_over_quads(float x) {
 // of f32 calls as three, which keeps f32's range: an output dim whose greatest
 // weights meet zero codes is as exact as any other.
 template <int TYPE, int D>
-__global__ __launch_bounds__(64 * kWaves) void kv_stream_kernel(KvAttend p) {
+__global__ __launch_bounds__(64 * kWavesOf<D>) void kv_stream_kernel(KvAttend p) {
+    constexpr int kWaves = kWavesOf<D>;
     using K = KvType<TYPE>;
     using T = typename K::T;
     constexpr bool PAIR = TYPE == ROCKNPU_KV_F32;
@@ -400,7 +407,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
 template <int TYPE, int D>
 int launch(const KvAttend& p, hipStream_t stream) {
     if (p.a.rows > 0 && p.a.max_new > 0)
-        kv_stream_kernel<TYPE, D><<<dim3(p.slots, p.c.kv_heads, p.row_tiles), 64 * kWaves, 0, stream>>>(p);
+        kv_stream_kernel<TYPE, D><<<dim3(p.slots, p.c.kv_heads, p.row_tiles), 64 * kWavesOf<D>, 0, stream>>>(p);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 

@@ -226,6 +226,8 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
     if need is None:
         got = ctypes.c_size_t()
         hip._check(lib.rocknpu_hip_kv_attention_workspace(cache._ref, ref, 0, ctypes.addressof(got)), "kv_attention")
+        if len(cache._needs) >= 1024:  # max_tokens may grow from step to step
+            cache._needs.clear()
         need = cache._needs[sizes] = got.value
     ws, nbytes = None, 0
     if need:

@@ -16,6 +16,7 @@ namespace rk {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kKvMaxSplits = 256;  // workgroups that share a tile's blocks, at most
+constexpr int kKvShares = 4;       // lengths of a split that are tried
 constexpr int kKvTileRows = 16;  // rows of a tile of the streaming kernel
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -29,8 +30,11 @@ struct KvAttend {
     int group;       // heads per kv head
     int row_tiles;   // tiles of rows that a sequence and kv head may have
     int tile_rows;
-    int share;       // workgroups that the sequences share, per kv head and row tile; 0: one each
-    int slots;       // workgroups in all per kv head and row tile: share + batch, or batch
+    // per kv head and row tile:
+    int share;       // parts that all sequences' blocks are cut into at least; 0: one workgroup each
+    int slots;       // workgroups: share + batch, or batch
+    int whole;       // workgroups that the GPU holds at once, or as many as there can be work for; at most slots
+    float per_part[kKvShares];  // 1 / parts, rounded up, in the order in which they are tried; the last is share
     int min_chunk;   // blocks per workgroup, at least
     bool vec_q, vec_out;
     // workspace, one entry per (kv head, row tile, slot): sums of the output [rows][head_dim], maxima and sums
@@ -38,6 +42,7 @@ struct KvAttend {
     float* part_out;
     float* part_state;
     float* block_sums;
+    int2* slots_of;  // a sequence's first slot and how many it has
 };
 
 // A page's scale, NaN where there is none or it is not finite.
@@ -91,9 +96,15 @@ __device__ __forceinline__ KvRange kv_range(const rocknpu_kv_attention_args& a, 
 
 // Which sequence a slot works on, and which of the sequence's `splits` parts it
 // takes (seq < 0: none). Every sequence with rows gets one slot for each `chunk`
-// blocks that its rows may see, where chunk is such that all of them come to
-// about p.share slots: a batch of unequal lengths loads the GPU evenly. All
-// slots of a launch, and the join behind them, work out the same division.
+// blocks that its rows may see: a batch of unequal lengths loads the GPU evenly.
+// Each sequence's last slot may be short, so chunk = all / whole can come to whole
+// + batch slots, and what the GPU does not hold at once waits for a round of its
+// own; chunks for whole, whole - batch / 4, ... parts are tried until the slots
+// fit (17 sequences of 700-15200 tokens, 8 kv heads of 128: 59 us, 75 with whole
+// - batch / 2 alone). All workgroups of a launch work out the same division,
+// before their first load of the cache: sums over lanes run
+// through DPP and quotients through the reciprocal (by __shfl and division it
+// cost one sequence of 4000 tokens 1 us of 14).
 struct KvSlot {
     int seq, split, splits, first;
 };
@@ -107,42 +118,59 @@ __device__ __forceinline__ int kv_blocks_estimate(const KvAttend& p, int b) {
     }
     return max(blocks, 1);
 }
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+// Lane l gets the sum over lanes 0 .. l: four steps within rows of 16 lanes, then
+// lane 15 of the odd rows' predecessors and lane 31 into what follows them.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
     return x;
 }
-// `want`: the slot asked for, or -1 - b for sequence b's first slot.
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+// x / y for whole numbers of which the quotient is below 2^20 (a batch has at most
+// kKvShares times as many slots as the GPU holds): by the reciprocal it is off by
+// less than one, which is mended.
+__device__ __forceinline__ int kv_divide(int x, int y) {
+    int q = static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y)));
+    q -= q * y > x;
+    return q + ((q + 1) * y <= x);
+}
 __device__ __forceinline__ KvSlot kv_slot(const KvAttend& p, int want) {
     const int lane = threadIdx.x & 63, batch = p.c.batch;
-    if (p.share == 0) {
-        const int b = want < 0 ? -1 - want : want;
-        return KvSlot{b, 0, 1, b};
+    if (p.share == 0) return KvSlot{want, 0, 1, want};
+    const int mine = lane < batch ? kv_blocks_estimate(p, lane) : 0;
+    int all = mine;
+    for (int base = 64; base < batch; base += 64) all += base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
+    all = wave_sum(all);
+    int chunk = 0;
+#pragma unroll
+    for (int k = 0; k < kKvShares; ++k) {
+        // at least all / parts: the factor and the 1 outdo the rounding
+        chunk = max(p.min_chunk, static_cast<int>(static_cast<float>(all) * p.per_part[k]) + 1);
+        if (k == kKvShares - 1 || batch == 1 || batch > 64) break;
+        if (wave_sum(kv_divide(mine + chunk - 1, chunk)) <= p.whole) break;
     }
-    int all = 0;
-    for (int base = 0; base < batch; base += 64) all += base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
-    all = uniform(wave_sum(all));
-    const int chunk = max(p.min_chunk, (all + p.share - 1) / p.share);
     int before = 0;
     for (int base = 0; base < batch; base += 64) {
-        const int blocks = base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
-        const int splits = min((blocks + chunk - 1) / chunk, kKvMaxSplits);
-        int upto = splits;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += y;
-        }
-        upto += before;
-        const unsigned long long hit = want < 0 ? __ballot(base + lane == -1 - want) : __ballot(want < upto);
+        const int blocks = base == 0 ? mine : base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
+        const int splits = min(kv_divide(blocks + chunk - 1, chunk), kKvMaxSplits);
+        const int upto = before + wave_scan(splits);
+        const unsigned long long hit = __ballot(want < upto);
         if (hit) {
             const int l = uniform(__ffsll(hit) - 1);
             const int end = __builtin_amdgcn_readlane(upto, l), n = __builtin_amdgcn_readlane(splits, l);
-            return KvSlot{base + l, want < 0 ? 0 : want - (end - n), n, end - n};
+            return KvSlot{base + l, want - (end - n), n, end - n};
         }
         before = __builtin_amdgcn_readlane(upto, 63);
     }
     return KvSlot{-1, 0, 0, 0};
+}
+// A sequence's slots, for the join: written by one workgroup of its first slot.
+__device__ __forceinline__ void kv_leave_slot(const KvAttend& p, const KvSlot& s, int h, int tile) {
+    if (p.share && s.split == 0 && h == 0 && tile == 0 && threadIdx.x == 0) p.slots_of[s.seq] = make_int2(s.first, s.splits);
 }
 
 // Whether a row at qpos sees the key at kpos.

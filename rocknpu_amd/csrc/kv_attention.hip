@@ -50,8 +50,8 @@ constexpr int kMaxShared = 1024;
 struct Plan {
     KvAttend p;
     bool stream;
-    size_t out_bytes, state_bytes, sums_bytes;
-    size_t bytes() const { return out_bytes + state_bytes + sums_bytes; }
+    size_t out_bytes, state_bytes, sums_bytes, slot_bytes;
+    size_t bytes() const { return out_bytes + state_bytes + sums_bytes + slot_bytes; }
 };
 
 Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus) {
@@ -73,17 +73,21 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.min_chunk = kMinChunk;
     // One round of the workgroups that the GPU holds at once: a second round pays every workgroup's start (lookups, the
-    // queries, the first blocks' latency) again. Sharing rounds each sequence up, by half a workgroup on average. 32
-    // ragged sequences of 500-4000 tokens, 8 kv heads of 128: 44 us; one and a half, two and three rounds 53, 55 and
-    // 54. The prompt kernel shares blocks out where that gives every sequence and tile at least four parts: below,
+    // queries, the first blocks' latency) again (32
+    // sequences of 500-4000 tokens, 8 kv heads of 128: 44 us; one and a half, two and three rounds 53, 55 and 54). The prompt kernel shares blocks out where that gives every sequence and tile at least four parts: below,
     // joining costs what it saves.
     const int64_t resident = (r.stream ? (c.head_dim == 64 ? 3 : 1) : (c.head_dim <= 128 ? 2 : 1)) * static_cast<int64_t>(cus);
-    const int64_t share = std::max<int64_t>(resident / (c.kv_heads * p.row_tiles) - c.batch / 2, 1);
+    p.whole = static_cast<int>(std::max<int64_t>(
+        std::min<int64_t>(resident / (c.kv_heads * p.row_tiles), c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk)), 1));
+    const int64_t share = std::max<int64_t>(p.whole - static_cast<int64_t>(c.batch) * (kKvShares - 1) / 4, 1);
     const bool shared = blocks > (r.stream ? kAlone : kMinChunk) && c.batch <= kMaxShared && rows > 0;
-    p.share = shared && share >= (r.stream ? 2 : 4) ? static_cast<int>(std::min<int64_t>(share, c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk))) : 0;
+    p.share = shared && share >= (r.stream ? 2 : 4) ? static_cast<int>(share) : 0;
+    for (int k = 0; k < kKvShares; ++k)
+        p.per_part[k] = 1.000001f / static_cast<float>(std::max<int64_t>(p.whole - static_cast<int64_t>(c.batch) * k / 4, 1));
     p.slots = p.share + c.batch;
     const size_t slots = static_cast<size_t>(p.slots) * c.kv_heads * p.row_tiles * p.tile_rows;
     if (p.share) r.out_bytes = padded(slots * c.head_dim * 4);
+    if (p.share) r.slot_bytes = padded(static_cast<size_t>(c.batch) * sizeof(int2));
     if (p.share || a.weights_out) r.state_bytes = padded(slots * 8);
     if (a.weights_out)
         r.sums_bytes = padded(static_cast<size_t>(c.batch) * c.kv_heads * c.max_blocks * p.row_tiles * kKvTileRows * 8);
@@ -114,6 +118,7 @@ extern "C" int rocknpu_hip_kv_attention(const rocknpu_kv_cache* cache, const roc
     if (r.out_bytes) r.p.part_out = reinterpret_cast<float*>(at);
     if (r.state_bytes) r.p.part_state = reinterpret_cast<float*>(at + r.out_bytes);
     if (r.sums_bytes) r.p.block_sums = reinterpret_cast<float*>(at + r.out_bytes + r.state_bytes);
+    if (r.slot_bytes) r.p.slots_of = reinterpret_cast<int2*>(at + r.out_bytes + r.state_bytes + r.sums_bytes);
     const int st = r.stream ? launch_kv_stream(r.p, s) : launch_kv_prompt(r.p, s);
     return st == kStatusOk ? launch_kv_join(r.p, s) : st;
 }

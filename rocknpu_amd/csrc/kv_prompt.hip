@@ -148,6 +148,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
     const int rows = s.n * p.group, r0 = tile * kTile;
     if (r0 >= rows) return;
+    kv_leave_slot(p, mine, h, tile);
     const int total = s.past + s.n, gone = uniform(max(c.dropped[b], 0));
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
     const int prefix = a.prefix ? uniform(a.prefix[b]) : 0;

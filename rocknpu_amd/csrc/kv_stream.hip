@@ -71,6 +71,7 @@ __global__ __launch_bounds__(64 * kWavesOf<D>) void kv_stream_kernel(KvAttend p)
     const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
     const int rows = s.n * p.group, r0 = tile * kKvTileRows;
     if (r0 >= rows) return;
+    kv_leave_slot(p, mine, h, tile);
     const int total = s.past + s.n, gone = uniform(max(c.dropped[b], 0));
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
     const int prefix = a.prefix ? uniform(a.prefix[b]) : 0;
@@ -302,14 +303,16 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     const int64_t seq = static_cast<int64_t>(b) * c.kv_heads + h;
     const bool joins = static_cast<int>(blockIdx.x) < row_groups;
     if (joins && static_cast<int>(blockIdx.x) * (4 / WAVES) >= rows) return;
-    const KvSlot slot = kv_slot(p, -1 - b);
-    const auto slot_of = [&](int r) { return (static_cast<int64_t>(h) * p.row_tiles + r / p.tile_rows) * p.slots + slot.first; };
+    // a sequence without rows has no slots, and left none
+    const int2 slots = p.share && rows > 0 ? p.slots_of[b] : make_int2(b, 1);
+    const int first = uniform(slots.x), splits = uniform(slots.y);
+    const auto slot_of = [&](int r) { return (static_cast<int64_t>(h) * p.row_tiles + r / p.tile_rows) * p.slots + first; };
     const auto state_of = [&](int r) {
         return reinterpret_cast<const float2*>(p.part_state) + slot_of(r) * p.tile_rows + r % p.tile_rows;
     };
     if (joins) {
         const int r = blockIdx.x * (4 / WAVES) + wave / WAVES, nth = wave % WAVES, mine = wave / WAVES;
-        if (slot.splits <= 1) return;  // its only workgroup wrote the row
+        if (splits <= 1) return;  // its only workgroup wrote the row
         float4v acc = {0, 0, 0, 0};
         if (r < rows) {
             const float2* st = state_of(r);
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 64; ++k) {
                 const int i = k * 64 + lane;
-                state[k] = i < slot.splits ? st[i * p.tile_rows] : make_float2(-__builtin_inff(), 0.0f);
+                state[k] = i < splits ? st[i * p.tile_rows] : make_float2(-__builtin_inff(), 0.0f);
                 most = fmaxf(most, state[k].x);
             }
             most = wave_max(most);
@@ -330,7 +333,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
             // a split without blocks wrote no sums: its factor is 0 and its sums are not read
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 64; ++k)
-                if (k * 64 + lane < slot.splits)
+                if (k * 64 + lane < splits)
                     keep[mine][k * 64 + lane] = state[k].y == 0.0f ? 0.0f : exp2_fast(state[k].x - ref) / total;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
             __builtin_amdgcn_wave_barrier();
@@ -339,7 +342,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
             const float* from = p.part_out + (slot_of(r) * p.tile_rows + r % p.tile_rows) * D + lane % kPer * 4;
             if (beside < kBeside) {
 #pragma unroll 4
-                for (int i = nth * kBeside + beside; i < slot.splits; i += WAVES * kBeside) {
+                for (int i = nth * kBeside + beside; i < splits; i += WAVES * kBeside) {
                     const float f = keep[mine][i];
                     if (f != 0.0f) acc += f * *reinterpret_cast<const float4v*>(from + static_cast<int64_t>(i) * p.tile_rows * D);
                 }
@@ -368,10 +371,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     for (int r = wave; r < rows; r += 4) {
         const float2* st = state_of(r);
         float most = -__builtin_inff(), total = 0.0f;
-        for (int i = lane; i < slot.splits; i += 64) most = fmaxf(most, st[i * p.tile_rows].x);
+        for (int i = lane; i < splits; i += 64) most = fmaxf(most, st[i * p.tile_rows].x);
         most = wave_max(most);
         const float ref = most == -__builtin_inff() ? 0.0f : most;
-        for (int i = lane; i < slot.splits; i += 64) total += st[i * p.tile_rows].y * exp2_fast(st[i * p.tile_rows].x - ref);
+        for (int i = lane; i < splits; i += 64) total += st[i * p.tile_rows].y * exp2_fast(st[i * p.tile_rows].x - ref);
 #pragma unroll
         for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
         if (lane == 0) {

@@ -30,6 +30,7 @@ struct KvAttend {
     int group;       // heads per kv head
     int row_tiles;   // tiles of rows that a sequence and kv head may have
     int tile_rows;
+    int waves;       // of a streaming workgroup
     // per kv head and row tile:
     int share;       // parts that all sequences' blocks are cut into at least; 0: one workgroup each
     int slots;       // workgroups: share + batch, or batch

@@ -13,15 +13,6 @@
 namespace rk {
 namespace {
 
-// Heads of 128 and 192 take 160 to 240 registers: two waves a SIMD, here as one
-// workgroup of eight, so that a context is cut into half as many splits (32
-// sequences of 500-4000 tokens, 8 kv heads of 128: 44 us against 53 in workgroups
-// of four; 8 of 4000: 26 and 26). Heads of 64 leave room for three waves, heads
-// of 256 for one: four waves (30 us against 35; 85 and 84, f32 with spills).
-template <int D>
-constexpr int kWavesOf = D == 128 || D == 192 ? 8 : 4;
-constexpr int kMaxSplits = kKvMaxSplits;
-
 template <int D>
 struct BlockRegs {
     uint4 k[2][D / 64];  // token tile, 64 dims
@@ -52,17 +43,16 @@ __device__ __forceinline__ float sum_over_quads(float x) {
 // Queries enter as f16, those of f32 calls as hi + lo; weights as two bf16, those
 // of f32 calls as three, which keeps f32's range: an output dim whose greatest
 // weights meet zero codes is as exact as any other.
-template <int TYPE, int D>
-__global__ __launch_bounds__(64 * kWavesOf<D>) void kv_stream_kernel(KvAttend p) {
-    constexpr int kWaves = kWavesOf<D>;
+template <int TYPE, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
     using K = KvType<TYPE>;
     using T = typename K::T;
     constexpr bool PAIR = TYPE == ROCKNPU_KV_F32;
     constexpr int kParts = PAIR ? 2 : 1, kWeightParts = PAIR ? 3 : 2;
     const rocknpu_kv_cache& c = p.c;
     const rocknpu_kv_attention_args& a = p.a;
-    __shared__ float state[kWaves][kKvTileRows][2];
-    __shared__ alignas(16) float sums[kWaves][kKvTileRows][D + 4];
+    __shared__ float state[WAVES][kKvTileRows][2];
+    __shared__ alignas(16) float sums[WAVES][kKvTileRows][D + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane % 16, quad = lane / 16;
     const int h = blockIdx.y, tile = blockIdx.z;
     const KvSlot mine = kv_slot(p, blockIdx.x);
@@ -122,9 +112,9 @@ __global__ __launch_bounds__(64 * kWavesOf<D>) void kv_stream_kernel(KvAttend p)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[i] = float4v{0, 0, 0, 0};
 
-    for (int base = begin; base < end; base += 64 * kWaves) {
+    for (int base = begin; base < end; base += 64 * WAVES) {
         // lane l looks up the wave's l-th block
-        const int nth = base + lane * kWaves + wave;
+        const int nth = base + lane * WAVES + wave;
         int my_page = 0, my_start = 0;
         float my_sk = 0.0f, my_sv = 0.0f;
         if (nth < end) {
@@ -137,7 +127,7 @@ __global__ __launch_bounds__(64 * kWavesOf<D>) void kv_stream_kernel(KvAttend p)
             my_sk = kv_scale(sc.x, ok);
             my_sv = kv_scale(sc.y, ok);
         }
-        const int here = (min(end - base, 64 * kWaves) - wave + kWaves - 1) / kWaves;  // the wave's blocks
+        const int here = (min(end - base, 64 * WAVES) - wave + WAVES - 1) / WAVES;  // the wave's blocks
         BlockRegs<D> next;
         if (here > 0) load_block<D>(c.pages, __builtin_amdgcn_readlane(my_page, 0), lane, next);
         for (int k = 0; k < here; ++k) {
@@ -220,7 +210,7 @@ __global__ __launch_bounds__(64 * kWavesOf<D>) void kv_stream_kernel(KvAttend p)
             if (p.block_sums) {
                 const float all = sum_over_quads(got);
                 if (quad == 0 && r0 + n < rows) {
-                    const int64_t at = (entry_row + range.entry(base + k * kWaves + wave)) * (p.row_tiles * kKvTileRows) + r0 + n;
+                    const int64_t at = (entry_row + range.entry(base + k * WAVES + wave)) * (p.row_tiles * kKvTileRows) + r0 + n;
                     reinterpret_cast<float2*>(p.block_sums)[at] = make_float2(all, ref);
                 }
             }
@@ -244,26 +234,26 @@ __global__ __launch_bounds__(64 * kWavesOf<D>) void kv_stream_kernel(KvAttend p)
     __syncthreads();
     float most = state[0][n][0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, state[w][n][0]);
+    for (int w = 1; w < WAVES; ++w) most = fmaxf(most, state[w][n][0]);
     const float ref = most == -__builtin_inff() ? 0.0f : most;
     const float keep = exp2_fast(top - ref);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
         *reinterpret_cast<float4v*>(&sums[wave][n][i * 16 + quad * 4]) = o[i] * keep;
     __syncthreads();
-    for (int i = tid; i < kKvTileRows * D / 4; i += 64 * kWaves) {
+    for (int i = tid; i < kKvTileRows * D / 4; i += 64 * WAVES) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         if (r0 + r >= rows) break;
         float4v acc = *reinterpret_cast<float4v*>(&sums[0][r][d]);
         float m = state[0][r][0], l = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) {
+        for (int w = 1; w < WAVES; ++w) {
             acc += *reinterpret_cast<float4v*>(&sums[w][r][d]);
             m = fmaxf(m, state[w][r][0]);
         }
         const float at = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) l += state[w][r][1] * exp2_fast(state[w][r][0] - at);
+        for (int w = 0; w < WAVES; ++w) l += state[w][r][1] * exp2_fast(state[w][r][0] - at);
         if (mine.splits > 1 || p.block_sums) {
             if (d == 0) {
                 p.part_state[(slot * kKvTileRows + r) * 2] = m;
@@ -295,7 +285,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     const rocknpu_kv_cache& c = p.c;
     const rocknpu_kv_attention_args& a = p.a;
     __shared__ float final_state[kKvMaxWeightRows][2];
-    __shared__ float keep[4 / WAVES][kMaxSplits];
+    __shared__ float keep[4 / WAVES][kKvMaxSplits];
     __shared__ alignas(16) float part[WAVES][D];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = blockIdx.y, b = blockIdx.z;
     const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
@@ -317,9 +307,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
         if (r < rows) {
             const float2* st = state_of(r);
             float most = -__builtin_inff(), total = 0.0f;
-            float2 state[kMaxSplits / 64];
+            float2 state[kKvMaxSplits / 64];
 #pragma unroll
-            for (int k = 0; k < kMaxSplits / 64; ++k) {
+            for (int k = 0; k < kKvMaxSplits / 64; ++k) {
                 const int i = k * 64 + lane;
                 state[k] = i < splits ? st[i * p.tile_rows] : make_float2(-__builtin_inff(), 0.0f);
                 most = fmaxf(most, state[k].x);
@@ -327,12 +317,12 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
             most = wave_max(most);
             const float ref = most == -__builtin_inff() ? 0.0f : most;
 #pragma unroll
-            for (int k = 0; k < kMaxSplits / 64; ++k) total += state[k].y * exp2_fast(state[k].x - ref);
+            for (int k = 0; k < kKvMaxSplits / 64; ++k) total += state[k].y * exp2_fast(state[k].x - ref);
 #pragma unroll
             for (int g = 32; g >= 1; g >>= 1) total += __shfl_xor(total, g, 64);
             // a split without blocks wrote no sums: its factor is 0 and its sums are not read
 #pragma unroll
-            for (int k = 0; k < kMaxSplits / 64; ++k)
+            for (int k = 0; k < kKvMaxSplits / 64; ++k)
                 if (k * 64 + lane < splits)
                     keep[mine][k * 64 + lane] = state[k].y == 0.0f ? 0.0f : exp2_fast(state[k].x - ref) / total;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
@@ -409,8 +399,15 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
 
 template <int TYPE, int D>
 int launch(const KvAttend& p, hipStream_t stream) {
-    if (p.a.rows > 0 && p.a.max_new > 0)
-        kv_stream_kernel<TYPE, D><<<dim3(p.slots, p.c.kv_heads, p.row_tiles), 64 * kWavesOf<D>, 0, stream>>>(p);
+    const dim3 grid(p.slots, p.c.kv_heads, p.row_tiles);
+    if (p.a.rows > 0 && p.a.max_new > 0) {
+        if constexpr (D == 128 || D == 192) {
+            if (p.waves == 8) kv_stream_kernel<TYPE, D, 8><<<grid, 512, 0, stream>>>(p);
+        }
+        if constexpr (D != 192) {
+            if (p.waves == 4) kv_stream_kernel<TYPE, D, 4><<<grid, 256, 0, stream>>>(p);
+        }
+    }
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 

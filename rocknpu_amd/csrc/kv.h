@@ -70,6 +70,18 @@ __device__ __forceinline__ KvSpan kv_span(const int32_t* past, const int32_t* cu
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ KvSpan uniform(KvSpan s) { return KvSpan{uniform(s.past), uniform(s.row0), uniform(s.n)}; }
 
+// Lane l gets the sum over lanes 0 .. l: four steps within rows of 16 lanes, then
+// lane 15 of the odd rows' predecessors and lane 31 into what follows them.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
+    return x;
+}
+
 // Whether a cache description is one that the kernels can take. kv_cache.hip.
 bool kv_cache_ok(const rocknpu_kv_cache* c);
 

@@ -121,11 +121,6 @@ __device__ __forceinline__ float max_of_halves(float x) {
 }
 __device__ __forceinline__ float sum_of_halves(float x) { return x + __shfl_xor(x, 32, 64); }
 
-__device__ __forceinline__ float tanh_fast(float x) {
-    // 1 - 2 / (1 + e^2x): its error is of 1, not of small results
-    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + exp2_fast(2.0f * kLog2e * x));
-}
-
 template <int TYPE, int D>
 __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel(KvAttend p, int tiles) {
     using K = KvType<TYPE>;
@@ -304,7 +299,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
                     const int kpos = meta.start + r / 4 * 8 + half * 4 + r % 4;
                     float y = (x[r] - lower) * to_score;
                     if (!plain) {
-                        if (a.softcap != 0.0f) y = a.softcap * (PAIR ? tanhf(y / a.softcap) : tanh_fast(y / a.softcap));
+                        if (a.softcap != 0.0f) y = kv_cap<PAIR>(y, a.softcap);
                         if (a.slopes) y += slope * static_cast<float>(kpos - qpos);
                         y *= kLog2e;
                     }

@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float y = x[t][i] * (unit * sk);
-                        if (a.softcap != 0.0f) y = a.softcap * tanhf(y / a.softcap);
+                        if (a.softcap != 0.0f) y = kv_cap<PAIR>(y, a.softcap);
                         if (a.slopes) y += slope * static_cast<float>(start + t * 16 + quad * 4 + i - qpos);
                         x[t][i] = y;
                     }

@@ -270,12 +270,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 template <int THREADS>
 __device__ __forceinline__ int exclusive_sum(int v, int* part) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
+    const int x = wave_scan(v);
     if (lane == 63) part[wave] = x;
     __syncthreads();
     int before = 0;
@@ -288,15 +283,17 @@ __device__ __forceinline__ int exclusive_sum(int v, int* part) {
 // a thread. The budget-th greatest key is found by digits of 11, 11 and 10 bits
 // from the top (a histogram in LDS of the entries that match the digits found so
 // far): the first digit holds the exponent and two more bits, so that few of a
-// wave's lanes meet in one bin (with digits of 8 bits 512 rows of 4098 took 30 us,
-// with these 20). Then ballots and one sum over (register, wave) place every
+// wave's lanes meet in one bin (with digits of 8 bits 512 rows of 4098 took 10 us
+// more). The histograms are cleared while the row's loads are in flight, and sums
+// over threads run through DPP (15 us; cleared pass by pass and by __shfl 20, of
+// which 50 MB take 11 at a large copy's rate). Then ballots and one sum over (register, wave) place every
 // entry. Everything is read before the first write, so outputs may be the inputs.
 // Bound by the latency of its steps where rows are few, else by its bytes.
 template <int THREADS, int ITEMS>
 __global__ __launch_bounds__(THREADS) void kv_evict_kernel(rocknpu_kv_evict_args a) {
     constexpr int kWaves = THREADS / 64, kBins = 2048, kGroups = ITEMS * kWaves;
     static_assert(kGroups <= THREADS);
-    __shared__ int hist[kBins];
+    __shared__ int hists[3][kBins];
     __shared__ int part[kWaves];
     __shared__ int pick[2];                   // the digit found, and how many entries rank above it
     __shared__ int count[kGroups][2];         // by register and wave: entries above the key found, and equal to it
@@ -315,6 +312,8 @@ __global__ __launch_bounds__(THREADS) void kv_evict_kernel(rocknpu_kv_evict_args
     }
     const int total = min(max(a.tokens[b], 0), 0x3fffffff);
     const int gone = max(a.dropped[b], 0);
+    for (int i = tid; i < 3 * kBins; i += THREADS) hists[0][i] = 0;
+    __syncthreads();
     const int n = min(max((total + kKvBlock - 1) / kKvBlock - gone, 0), a.max_blocks);
     uint32_t key[ITEMS];
 #pragma unroll
@@ -331,8 +330,7 @@ __global__ __launch_bounds__(THREADS) void kv_evict_kernel(rocknpu_kv_evict_args
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-            for (int i = tid; i < bins; i += THREADS) hist[i] = 0;
-            __syncthreads();
+            int* hist = hists[pass];
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
                 if (i * THREADS + tid < n && (pass == 0 || key[i] >> (pass == 1 ? 21 : 10) == found))

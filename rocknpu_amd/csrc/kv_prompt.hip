@@ -10,11 +10,14 @@
 // product, values (32 dims x 16 tokens) times weights, as they stand.
 //
 // Per block a wave has D/8 products of 32 cycles; for each of a lane's 16 scores
-// a fused multiply-add, an exponential (16 cycles), half a maximum, conversion
-// and sum; and its share of the conversion. Both units stay busy because a wave
-// takes block j's exponentials between the products of block j + 1's scores and
-// the conversion of block j + 2 between the products of block j's values, and
-// because the CU's two workgroups are not in step.
+// a fused multiply-add, an exponential (9 cycles), half a maximum, conversion and
+// sum; and its share of the conversion. Both units stay busy because a wave takes
+// block j's maximum and exponentials between the products of block j + 1's scores
+// and the conversion of block j + 2 between the products of block j's values, and
+// because the CU's two workgroups are not in step: the wave that is in its
+// products has priority over one that works on a maximum or waits for blocks.
+// 4096 rows of 32/8 heads of 128, bf16: 168 us (817 TF/s), 180 without priorities
+// and with the maximum before the products.
 #include <type_traits>
 
 #include "kv_attend.h"
@@ -127,8 +130,10 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     using T = typename K::T;
     constexpr bool PAIR = TYPE == ROCKNPU_KV_F32;
     constexpr int kParts = PAIR ? 2 : 1;
+    constexpr int kEarly = 2;             // products of the next block's scores that the maximum is taken between
     constexpr int kAhead = PAIR ? 2 : 4;  // operands are read from LDS this many steps before they are used
     constexpr int kSteps = D / 16;  // products of 16 dims of keys, and of values by 32 dims and 16 tokens
+    static_assert(kAhead <= kSteps && kEarly < kSteps);
     const rocknpu_kv_cache& c = p.c;
     const rocknpu_kv_attention_args& a = p.a;
     __shared__ alignas(16) uint8_t lds[3][block_bytes_lds<D>()];
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     // Block j of the workgroup's part: its bytes are loaded in iteration j - 4 (a trip to memory takes longer than an
     // iteration) and go to LDS in iteration j - 2. Page numbers, positions and scales are looked up 64 blocks at a time, a
     // block per lane, half a batch ahead. (Looked up block by block they were what an iteration waited for: 4096 tokens,
-    // 32/8 heads of 128, bf16: 197 us instead of TIME.)
+    // 32/8 heads of 128, bf16: 197 us; 180 with this and rows stored whole.)
     struct Batch {
         int page, start;
         float sk, sv;
@@ -282,16 +287,42 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
         const bool before = meta.start + kKvBlock <= pre;
         const bool any = active && ((meta.start <= some_high && meta.start + kKvBlock > some_low) || meta.start < pre);
         x_1 = float16v{};
+        half8 key[kSteps];
+        Value value[kSteps];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) key[k] = read_key(at_1, k);
+        // operand k + kAhead of the scores' products, behind them the first of the values'
+        const auto read_ahead = [&](int k) {
+            if (k + kAhead < kSteps)
+                key[k + kAhead] = read_key(at_1, k + kAhead);
+            else
+                value[k + kAhead - kSteps] = read_value(at, k + kAhead - kSteps);
+        };
         if (__builtin_expect(any, 1)) {
             // scores to exponents over the row's reference, which follows the maximum
             const float lift = __log2f(sv);
             float factor = unit * sk * kLog2e, off = __builtin_fmaf(-lower, factor, lift), most;
             if (__builtin_expect(plain && (before || (meta.start >= full_low && meta.start + kKvBlock - 1 <= full_high)), 1)) {
-                most = x[0];
+                float m[kEarly];
 #pragma unroll
-                for (int r = 1; r < 16; ++r) most = fmaxf(most, x[r]);
+                for (int k = 0; k < kEarly; ++k) {
+                    read_ahead(k);
+                    product(key[k], k, x_1);
+                    m[k] = x[k * (16 / kEarly)];
+#pragma unroll
+                    for (int r = 1; r < 16 / kEarly; ++r) m[k] = fmaxf(m[k], x[k * (16 / kEarly) + r]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                most = m[0];
+#pragma unroll
+                for (int k = 1; k < kEarly; ++k) most = fmaxf(most, m[k]);
                 most = __builtin_fmaf(most, factor, off);
             } else {
+#pragma unroll
+                for (int k = 0; k < kEarly; ++k) {
+                    read_ahead(k);
+                    product(key[k], k, x_1);
+                }
                 most = kNothing;
                 const float to_score = plain ? factor : unit * sk;
 #pragma unroll
@@ -320,20 +351,16 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             }
             off += (PAIR ? 0.0f : kBias) - ref;
 
+            __builtin_amdgcn_s_setprio(1);
             // the next block's scores, and between them this one's weights
-            half8 w[2], key[kSteps];
-            Value value[kSteps];
+            half8 w[2];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) key[k] = read_key(at_1, k);
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                if (k + kAhead < kSteps)
-                    key[k + kAhead] = read_key(at_1, k + kAhead);
-                else
-                    value[k + kAhead - kSteps] = read_value(at, k + kAhead - kSteps);
+            for (int k = kEarly; k < kSteps; ++k) {
+                read_ahead(k);
                 product(key[k], k, x_1);
 #pragma unroll
-                for (int e = 16 * k / kSteps; e < 16 * (k + 1) / kSteps; ++e) x[e] = exp2_fast(__builtin_fmaf(x[e], factor, off));
+                for (int e = 16 * (k - kEarly) / (kSteps - kEarly); e < 16 * (k + 1 - kEarly) / (kSteps - kEarly); ++e)
+                    x[e] = exp2_fast(__builtin_fmaf(x[e], factor, off));
             }
             bhalf8 ww[2][3];
             float got = 0.0f;
@@ -365,6 +392,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             sum += got == 0.0f ? 0.0f : got * __builtin_amdgcn_rcpf(sv);
             // Values times weights, and between them the later block's conversion. Its bytes are first touched here: moved
             // up, the conversion would wait for them at the iteration's start.
+            __builtin_amdgcn_s_setprio(2);
             __builtin_amdgcn_sched_barrier(0);
             hold<D>(two);
 #pragma unroll
@@ -383,11 +411,12 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) product(read_key(at_1, k), k, x_1);
+            for (int k = 0; k < kSteps; ++k) product(k < kAhead ? key[k] : read_key(at_1, k), k, x_1);
             hold<D>(two);
 #pragma unroll
             for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(two, i, wave, lds[later]);
         }
+        __builtin_amdgcn_s_setprio(0);
         meta = meta_1;
         meta_1 = meta_of(j + 2);
         fetch_block(j + 4, two);

@@ -15,9 +15,11 @@
 // block j's maximum and exponentials between the products of block j + 1's scores
 // and the conversion of block j + 2 between the products of block j's values, and
 // because the CU's two workgroups are not in step: the wave that is in its
-// products has priority over one that works on a maximum or waits for blocks.
-// 4096 rows of 32/8 heads of 128, bf16: 168 us (817 TF/s), 180 without priorities
-// and with the maximum before the products.
+// products has priority over one that works on a maximum or waits for blocks
+// (not with slopes or capped scores, where the vector unit is the longer one: 148
+// against 143 us).
+// 4096 rows of 32/8 heads of 128, bf16: 165 us (834 TF/s), 180 without priorities
+// and with the maximum before the products; 8192 rows: 603 us (911 TF/s).
 #include <type_traits>
 
 #include "kv_attend.h"
@@ -124,7 +126,9 @@ __device__ __forceinline__ float max_of_halves(float x) {
 }
 __device__ __forceinline__ float sum_of_halves(float x) { return x + __shfl_xor(x, 32, 64); }
 
-template <int TYPE, int D>
+// PLAIN: neither slopes nor capped scores, whose code costs calls without them 3%
+// (170 and 165 us).
+template <int TYPE, int D, bool PLAIN>
 __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel(KvAttend p, int tiles) {
     using K = KvType<TYPE>;
     using T = typename K::T;
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     // The wave's rows are w0 + n. A row sees [low, low + span] and what lies before `pre`; `full` and `some`: what every
     // row and some row of the wave sees.
     const int w0 = r0 + wave * 32;
-    const bool active = w0 < rows, windowed = a.window != 0, plain = a.softcap == 0.0f && !a.slopes;
+    const bool active = w0 < rows, windowed = a.window != 0;
     const int q0 = s.past + min(w0, rows - 1) / p.group, q1 = s.past + (min(w0 + 32, rows) - 1) / p.group;
     const int pre = min(prefix, total), newest = total - 1;
     const int full_low = windowed ? max(q1 - a.window + 1, 0) : 0, full_high = a.causal ? min(q0, newest) : newest;
@@ -175,7 +179,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     const int row = min(w0 + n, rows - 1), head = h * p.group + row % p.group, qpos = s.past + row / p.group;
     const int low = windowed ? max(qpos - a.window + 1, 0) : 0;
     const unsigned span = static_cast<unsigned>((a.causal ? min(qpos, newest) : newest) - low);
-    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    const float slope = !PLAIN && a.slopes ? a.slopes[head] : 0.0f;
     // Block j of the workgroup's part: its bytes are loaded in iteration j - 4 (a trip to memory takes longer than an
     // iteration) and go to LDS in iteration j - 2. Page numbers, positions and scales are looked up 64 blocks at a time, a
     // block per lane, half a batch ahead. (Looked up block by block they were what an iteration waited for: 4096 tokens,
@@ -302,7 +306,8 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             // scores to exponents over the row's reference, which follows the maximum
             const float lift = __log2f(sv);
             float factor = unit * sk * kLog2e, off = __builtin_fmaf(-lower, factor, lift), most;
-            if (__builtin_expect(plain && (before || (meta.start >= full_low && meta.start + kKvBlock - 1 <= full_high)), 1)) {
+            const bool full = before || (meta.start >= full_low && meta.start + kKvBlock - 1 <= full_high);
+            if (__builtin_expect(full && PLAIN, 1)) {
                 float m[kEarly];
 #pragma unroll
                 for (int k = 0; k < kEarly; ++k) {
@@ -317,6 +322,26 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
 #pragma unroll
                 for (int k = 1; k < kEarly; ++k) most = fmaxf(most, m[k]);
                 most = __builtin_fmaf(most, factor, off);
+                __builtin_amdgcn_s_setprio(1);
+            } else if (!PLAIN && full && a.softcap == 0.0f) {
+                // a distance's share of the exponent is the block's plus a multiple of the slope (5 prompts of up to 1500
+                // tokens, 32/4 heads of 64, f32: 102 us, with
+                // the general form's operations 143)
+                const float rise = slope * kLog2e;
+                const float at_0 = __builtin_fmaf(rise, static_cast<float>(meta.start + half * 4 - qpos), off);
+                most = kNothing;
+#pragma unroll
+                for (int k = 0; k < kEarly; ++k) {
+                    read_ahead(k);
+                    product(key[k], k, x_1);
+#pragma unroll
+                    for (int r = k * (16 / kEarly); r < (k + 1) * (16 / kEarly); ++r) {
+                        x[r] = __builtin_fmaf(x[r], factor, __builtin_fmaf(rise, static_cast<float>(r / 4 * 8 + r % 4), at_0));
+                        most = fmaxf(most, x[r]);
+                    }
+                }
+                factor = 1.0f;
+                off = 0.0f;
             } else {
 #pragma unroll
                 for (int k = 0; k < kEarly; ++k) {
@@ -324,12 +349,12 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
                     product(key[k], k, x_1);
                 }
                 most = kNothing;
-                const float to_score = plain ? factor : unit * sk;
+                const float to_score = PLAIN ? factor : unit * sk;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int kpos = meta.start + r / 4 * 8 + half * 4 + r % 4;
                     float y = (x[r] - lower) * to_score;
-                    if (!plain) {
+                    if constexpr (!PLAIN) {
                         if (a.softcap != 0.0f) y = kv_cap<PAIR>(y, a.softcap);
                         if (a.slopes) y += slope * static_cast<float>(kpos - qpos);
                         y *= kLog2e;
@@ -351,7 +376,6 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             }
             off += (PAIR ? 0.0f : kBias) - ref;
 
-            __builtin_amdgcn_s_setprio(1);
             // the next block's scores, and between them this one's weights
             half8 w[2];
 #pragma unroll
@@ -392,7 +416,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             sum += got == 0.0f ? 0.0f : got * __builtin_amdgcn_rcpf(sv);
             // Values times weights, and between them the later block's conversion. Its bytes are first touched here: moved
             // up, the conversion would wait for them at the iteration's start.
-            __builtin_amdgcn_s_setprio(2);
+            if constexpr (PLAIN) __builtin_amdgcn_s_setprio(2);
             __builtin_amdgcn_sched_barrier(0);
             hold<D>(two);
 #pragma unroll
@@ -416,7 +440,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
 #pragma unroll
             for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(two, i, wave, lds[later]);
         }
-        __builtin_amdgcn_s_setprio(0);
+        if constexpr (PLAIN) __builtin_amdgcn_s_setprio(0);
         meta = meta_1;
         meta_1 = meta_of(j + 2);
         fetch_block(j + 4, two);
@@ -526,7 +550,10 @@ template <int TYPE, int D>
 int launch(const KvAttend& p, hipStream_t stream) {
     const int64_t grid = static_cast<int64_t>(p.row_tiles) * p.slots * p.c.kv_heads;
     if (grid > 0x7fffffff) return kStatusInvalid;
-    kv_prompt_kernel<TYPE, D><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, p.row_tiles);
+    if (p.a.softcap == 0.0f && !p.a.slopes)
+        kv_prompt_kernel<TYPE, D, true><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, p.row_tiles);
+    else
+        kv_prompt_kernel<TYPE, D, false><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, p.row_tiles);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 

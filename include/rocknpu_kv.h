@@ -117,11 +117,8 @@ typedef struct rocknpu_kv_attention_args {
  * sees, and 0 where it sees nothing. Scores, the running maximum and sum and the
  * products' sums are f32. The codes enter the matrix instructions exactly, q as
  * f16 for f16 and bf16 calls and as a pair of f16 (22 bits) for f32 calls (each
- * row scaled by a power of two first), the weights with 24 bits for f32 calls
- * and 11 or more for f16 and bf16 calls. f16 and bf16 calls of more than 32 rows
- * times heads per kv head may hold weights as f16: one below 2^-23 of the row's
- * greatest exp(x) times its block's value scale has fewer bits, one below about
- * 2^-33 counts as 0; all others keep f32's range.
+ * row scaled by a power of two first), the weights with 16 bits for f16 and bf16
+ * calls and 24 for f32 calls, over f32's range.
  * With weights_out, also weights_out = cache->weights + the weight that each
  * block got from all rows and the kv head's heads (entries past the blocks in
  * use are copied); at most 256 rows times heads per kv head.

@@ -28,15 +28,19 @@ bool attention_ok(const rocknpu_kv_cache* c, const rocknpu_kv_attention_args* a)
 
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 
-// The streaming kernel reads the cache once per 16 rows, the prompt kernel once
-// per 128, with several times the work for a block. Streaming serves calls of at
-// most 32 rows a kv head; and short contexts in launches that leave the prompt
-// kernel too few tiles, up to kShortBlocks blocks and four 16-row tiles a CU
-// (32/8 heads of 128, bf16, one sequence, 512 rows over 512 and 912 tokens: 38
-// and 42 us, prompt kernel 44 and 49; over 2512: 87 and 63; 64 rows over 16000:
-// 106 and 55. f32: 30, 45, 98 and 115 against 51, 55, 83 and 75).
+// The streaming kernel reads the cache once per tile of 16 rows, the prompt kernel
+// once per 128, with several times the work for a block and a longer start.
+// Streaming serves calls of at most 32 rows a kv head, and launches of up to four
+// tiles a CU and, in tiles times blocks of 128 dims, 64 a CU (f32 calls 108: their
+// prompt kernel takes five products for two). 8 kv heads of 128, 4 heads each,
+// bf16, streaming and prompt kernel: 16 rows x 4 over 4000 tokens 15.0 and 18.4
+// us, over 16000 25.5 and 28.0, 32 x 4 over 16000 37.7 and 33.1, 512 x 4 over 0
+// 22.0 and 21.1, over 2000 78 and 49, two times 512 x 4 over 0 39 and 21. f32: 32
+// x 4 over 4000 19.6 and 26.9, over 16000 41.8 and 42.9, 512 x 4 over 2000 86 and
+// 68; 4 kv heads of 64, 8 heads each, 256 x 8 over 1500 23.9 and 31.1, 64 x 8 over
+// 16000 52 and 42.
 constexpr int64_t kStreamRows = 32;
-constexpr int64_t kShortBlocks = 32;
+constexpr int64_t kStreamTiles = 4, kStreamWork = 64 * 128, kStreamWorkF32 = 108 * 128;
 // Up to this many blocks a workgroup takes them alone; and blocks of a split, at
 // least, where they are shared out (8 kv heads of 128, one row, one launch alone
 // against splits and their join: 16 blocks 8.4 and 12.7 us, 32 blocks 11.9 and
@@ -68,7 +72,9 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     if (a.window > 0) blocks = std::min<int64_t>(blocks, (static_cast<int64_t>(a.window) + a.max_new) / kKvBlock + 2);
     blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, c.max_blocks));
     const int64_t tiles = (rows + kKvTileRows - 1) / kKvTileRows * c.batch * c.kv_heads;
-    r.stream = rows <= kStreamRows || a.weights_out || (blocks <= kShortBlocks && tiles <= 4 * cus);
+    r.stream = rows <= kStreamRows || a.weights_out ||
+               (tiles <= kStreamTiles * cus &&
+                tiles * blocks * c.head_dim <= (a.type == ROCKNPU_KV_F32 ? kStreamWorkF32 : kStreamWork) * cus);
     p.tile_rows = r.stream ? kKvTileRows : kv_prompt_tile();
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.min_chunk = kMinChunk;

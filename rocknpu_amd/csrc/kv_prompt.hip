@@ -18,8 +18,11 @@
 // products has priority over one that works on a maximum or waits for blocks
 // (not with slopes or capped scores, where the vector unit is the longer one: 148
 // against 143 us).
-// 4096 rows of 32/8 heads of 128, bf16: 165 us (834 TF/s), 180 without priorities
-// and with the maximum before the products; 8192 rows: 603 us (911 TF/s).
+// Weights enter as two bf16 (f32 calls: three), which keeps f32's range: as one
+// f16 they cost less (165 us where two bf16 take 203), but a row whose greatest
+// weights meet zero codes lost the bits of its result below 2^-23 of them. 4096
+// rows of 32/8 heads of 128, bf16: 203 us (677 TF/s); 8192 rows: 762 (721 TF/s).
+// Priorities and the maximum between the products took 12 of 180 us off.
 #include <type_traits>
 
 #include "kv_attend.h"
@@ -28,12 +31,11 @@ namespace rk {
 namespace {
 
 typedef float float16v __attribute__((ext_vector_type(16)));
-typedef float float2v __attribute__((ext_vector_type(2)));
 
-// f16 weights are held times 2^kBias, and the row's reference M follows the
-// maximum only when that grows by more than kSlack: rescaling the output costs
-// as much as a block's exponentials. 2^(kBias + kSlack) stays below f16's 65504.
-constexpr float kBias = 9.0f, kSlack = 6.0f;
+// The row's reference M follows the maximum only when that grows by more than
+// kSlack: rescaling the output costs as much as a block's exponentials, and
+// weights, sums and outputs have room for 2^kSlack.
+constexpr float kSlack = 30.0f;
 // the reference of a row that has seen nothing yet: 2^-inf over it is 0, and so is 2^it over any other
 constexpr float kNothing = -1e30f;
 // bytes of a 512-byte run of operands in LDS, padded so that the writers' 8
@@ -85,10 +87,10 @@ __device__ __forceinline__ half8 codes_to_half_raised(uint32_t lo, uint32_t hi) 
     return r.v;
 }
 
-// Converts piece i into LDS. Values become bf16 for f32 calls, else f16. Keys of
-// f16 and bf16 calls stay raised by 1152 (their scores come down by 1152 times
-// the row's sum, which rounds a score by about 2^-24 of that: less than those
-// calls' weights are rounded by); f32 calls take them exactly.
+// Converts piece i into LDS: keys into f16, values into bf16. Keys of f16 and bf16
+// calls stay raised by 1152 (their scores come down by 1152 times the row's sum,
+// which rounds a score by about 2^-24 of that: less than those calls' weights are
+// rounded by); f32 calls take them exactly.
 template <int D, bool PAIR>
 __device__ __forceinline__ void place(const BlockPieces<D>& r, int i, int wave, uint8_t* to) {
     const int piece = threadIdx.x + i * kThreads;
@@ -102,13 +104,8 @@ __device__ __forceinline__ void place(const BlockPieces<D>& r, int i, int wave, 
     } else {  // values: dims d and d + 16, 8 tokens
         const int v = piece - kKeys;
         uint8_t* p = to + key_bytes<D>() + (v / 64 * 4 + v % 4) * kValueRun + v / 4 % 16 * 16;
-        if constexpr (PAIR) {
-            *reinterpret_cast<bhalf8*>(p) = codes_to_bhalf(w.x, w.y);
-            *reinterpret_cast<bhalf8*>(p + 256) = codes_to_bhalf(w.z, w.w);
-        } else {
-            *reinterpret_cast<half8*>(p) = codes_to_half(w.x, w.y);
-            *reinterpret_cast<half8*>(p + 256) = codes_to_half(w.z, w.w);
-        }
+        *reinterpret_cast<bhalf8*>(p) = codes_to_bhalf(w.x, w.y);
+        *reinterpret_cast<bhalf8*>(p + 256) = codes_to_bhalf(w.z, w.w);
     }
 }
 
@@ -127,15 +124,15 @@ __device__ __forceinline__ float max_of_halves(float x) {
 __device__ __forceinline__ float sum_of_halves(float x) { return x + __shfl_xor(x, 32, 64); }
 
 // PLAIN: neither slopes nor capped scores, whose code costs calls without them 3%
-// (170 and 165 us).
+// (170 and 165 us, with weights as f16).
 template <int TYPE, int D, bool PLAIN>
 __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel(KvAttend p, int tiles) {
     using K = KvType<TYPE>;
     using T = typename K::T;
     constexpr bool PAIR = TYPE == ROCKNPU_KV_F32;
-    constexpr int kParts = PAIR ? 2 : 1;
+    constexpr int kParts = PAIR ? 2 : 1, kWeightParts = PAIR ? 3 : 2;
     constexpr int kEarly = 2;             // products of the next block's scores that the maximum is taken between
-    constexpr int kAhead = PAIR ? 2 : 4;  // operands are read from LDS this many steps before they are used
+    constexpr int kAhead = 2;  // operands are read from LDS this many steps before they are used
     constexpr int kSteps = D / 16;  // products of 16 dims of keys, and of values by 32 dims and 16 tokens
     static_assert(kAhead <= kSteps && kEarly < kSteps);
     const rocknpu_kv_cache& c = p.c;
@@ -268,14 +265,13 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     for (int d = 0; d < D / 32; ++d) o[d] = float16v{};
     float ref = kNothing, sum = 0.0f;
 
-    using Value = typename std::conditional<PAIR, bhalf8, half8>::type;
     // operand k of the scores' products (16 dims), and of the values': all tiles of 32 dims with 16 of the tokens, then with
     // the others
     const auto read_key = [&](const uint8_t* at, int k) {
         return *reinterpret_cast<const half8*>(at + half * kKeyRun + n * 16 + k * 2 * kKeyRun);
     };
     const auto read_value = [&](const uint8_t* at, int k) {
-        return *reinterpret_cast<const Value*>(at + key_bytes<D>() + half * kValueRun + n * 16 +
+        return *reinterpret_cast<const bhalf8*>(at + key_bytes<D>() + half * kValueRun + n * 16 +
                                                (k % (kSteps / 2) * 2 + k / (kSteps / 2)) * 2 * kValueRun);
     };
     // x[r]: token 8 (r / 4) + 4 half + r % 4 of the block, row n
@@ -296,7 +292,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
         const bool any = active && ((meta.start <= some_high && meta.start + kKvBlock > some_low) || meta.start < pre);
         x_1 = float16v{};
         half8 key[kSteps];
-        Value value[kSteps];
+        bhalf8 value[kSteps];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) key[k] = read_key(at_1, k);
         // operand k + kAhead of the scores' products, behind them the first of the values'
@@ -378,10 +374,9 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) o[d] *= keep;
             }
-            off += (PAIR ? 0.0f : kBias) - ref;
+            off -= ref;
 
             // the next block's scores, and between them this one's weights
-            half8 w[2];
 #pragma unroll
             for (int k = kEarly; k < kSteps; ++k) {
                 read_ahead(k);
@@ -390,32 +385,17 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
                 for (int e = 16 * (k - kEarly) / (kSteps - kEarly); e < 16 * (k + 1 - kEarly) / (kSteps - kEarly); ++e)
                     x[e] = exp2_fast(__builtin_fmaf(x[e], factor, off));
             }
-            bhalf8 ww[2][3];
+            bhalf8 w[2][kWeightParts];
             float got = 0.0f;
 #pragma unroll
             for (int h2 = 0; h2 < 2; ++h2) {
-                if constexpr (PAIR) {
-                    float part[8];
+                float part[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        part[i] = x[i / 4 * 8 + h2 * 4 + i % 4];
-                        got += part[i];
-                    }
-                    split_bhalf(part, ww[h2]);
-                } else {
-                    union {
-                        half2v h[4];
-                        half8 v;
-                    } u;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = i / 2 * 8 + h2 * 4 + i % 2 * 2;
-                        u.h[i] = __builtin_convertvector(float2v{x[r], x[r + 1]}, half2v);
-                        got = __builtin_amdgcn_fdot2(u.h[i], half2v{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, got,
-                                                     false);
-                    }
-                    w[h2] = u.v;
+                for (int i = 0; i < 8; ++i) {
+                    part[i] = x[i / 4 * 8 + h2 * 4 + i % 4];
+                    got += part[i];
                 }
+                split_bhalf(part, w[h2]);
             }
             sum += got == 0.0f ? 0.0f : got * __builtin_amdgcn_rcpf(sv);
             // Values times weights, and between them the later block's conversion. Its bytes are first touched here: moved
@@ -427,13 +407,9 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             for (int k = 0; k < kSteps; ++k) {
                 const int h2 = k / (kSteps / 2), d = k % (kSteps / 2);
                 if (k + kAhead < kSteps) value[k + kAhead] = read_value(at, k + kAhead);
-                if constexpr (PAIR) {
 #pragma unroll
-                    for (int part = 0; part < 3; ++part)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value[k], ww[h2][part], o[d], 0, 0, 0);
-                } else {
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value[k], w[h2], o[d], 0, 0, 0);
-                }
+                for (int part = 0; part < kWeightParts; ++part)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value[k], w[h2][part], o[d], 0, 0, 0);
                 if (k % (kSteps / BlockPieces<D>::kEach) == 0)
                     place<D, PAIR>(two, k / (kSteps / BlockPieces<D>::kEach), wave, lds[later]);
             }

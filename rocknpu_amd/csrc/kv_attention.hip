@@ -95,7 +95,9 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.whole = static_cast<int>(std::max<int64_t>(
         std::min<int64_t>(resident / (c.kv_heads * p.row_tiles), c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk)), 1));
     const int64_t share = std::max<int64_t>(p.whole - static_cast<int64_t>(c.batch) * (kKvShares - 1) / 4, 1);
-    const bool shared = blocks > (r.stream ? kAlone : kMinChunk) && c.batch <= kMaxShared && rows > 0;
+    // the device adds up all sequences' blocks in 32 bits
+    const bool shared = blocks > (r.stream ? kAlone : kMinChunk) && c.batch <= kMaxShared && rows > 0 &&
+                        static_cast<int64_t>(c.batch) * c.max_blocks < (1 << 30);
     p.share = shared && share >= (r.stream ? 2 : 4) ? static_cast<int>(share) : 0;
     for (int k = 0; k < kKvShares; ++k)
         p.per_part[k] = 1.000001f / static_cast<float>(std::max<int64_t>(p.whole - static_cast<int64_t>(c.batch) * k / 4, 1));

@@ -298,9 +298,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     const int64_t seq = static_cast<int64_t>(b) * c.kv_heads + h;
     const bool joins = static_cast<int>(blockIdx.x) < row_groups;
     if (joins && static_cast<int>(blockIdx.x) * (4 / WAVES) >= rows) return;
-    // a sequence without rows has no slots, and left none
+    // A sequence without rows has no slots, and left none. What was left is held to the workspace's bounds: lengths that
+    // change under a call (a caller's missing wait) may leave a sequence here whose slots nothing wrote.
     const int2 slots = p.share && rows > 0 ? p.slots_of[b] : make_int2(b, 1);
-    const int first = uniform(slots.x), splits = uniform(slots.y);
+    const int first = uniform(min(max(slots.x, 0), p.slots - 1));
+    const int splits = uniform(min(max(slots.y, 1), min(p.slots - first, kKvMaxSplits)));
     const auto slot_of = [&](int r) { return (static_cast<int64_t>(h) * p.row_tiles + r / p.tile_rows) * p.slots + first; };
     const auto state_of = [&](int r) {
         return reinterpret_cast<const float2*>(p.part_state) + slot_of(r) * p.tile_rows + r % p.tile_rows;

@@ -164,3 +164,20 @@ def test_strides_and_repeated_calls():
             assert torch.equal(out[:, :, :d], want) and not out[:, :, d:].any()
         ref = kv_ref.Ref(c).attention(q.double().cpu().numpy(), past, cu)
         check_attention(want, ref, kind, d, max(p + n for p, n in zip(past, new)))
+
+
+def test_a_workspace_may_hold_anything():
+    """Splits, their states and the sequences' parts are written before they are read, also where some have no rows."""
+    for new, heads in (([1, 0, 1, 1], 8), ([64, 0, 3, 33], 32)):
+        c = random_cache(52, 4, 8, 128, 130)
+        past, cu = [4000, 4000, 70, 2050], offsets(new)
+        q = torch.randn((cu[-1], heads, 128), device=DEV)
+        weigh = max(new) == 1
+        results = []
+        for fill in (0, 0x7f, 0xff):
+            ws = torch.full((1 << 28,), fill, dtype=torch.uint8, device=DEV)
+            wo = torch.empty_like(c.weights) if weigh else None
+            results.append((kv.attention(c, q, ints(past), ints(cu), max(new), max_tokens=4100, workspace=ws, weights_out=wo), wo))
+        for o, wo in results[1:]:
+            assert torch.equal(o, results[0][0]) and (wo is None or torch.equal(wo, results[0][1]))
+        assert torch.isfinite(results[0][0]).all()

@@ -31,16 +31,13 @@ size_t padded(size_t n) { return (n + 255) / 256 * 256; }
 // The streaming kernel reads the cache once per tile of 16 rows, the prompt kernel
 // once per 128, with several times the work for a block and a longer start.
 // Streaming serves calls of at most 32 rows a kv head, and launches of up to four
-// tiles a CU and, in tiles times blocks of 128 dims, 64 a CU (f32 calls 108: their
-// prompt kernel takes five products for two). 8 kv heads of 128, 4 heads each,
-// bf16, streaming and prompt kernel: 16 rows x 4 over 4000 tokens 15.0 and 18.4
-// us, over 16000 25.5 and 28.0, 32 x 4 over 16000 37.7 and 33.1, 512 x 4 over 0
-// 22.0 and 21.1, over 2000 78 and 49, two times 512 x 4 over 0 39 and 21. f32: 32
-// x 4 over 4000 19.6 and 26.9, over 16000 41.8 and 42.9, 512 x 4 over 2000 86 and
-// 68; 4 kv heads of 64, 8 heads each, 256 x 8 over 1500 23.9 and 31.1, 64 x 8 over
-// 16000 52 and 42.
-constexpr int64_t kStreamRows = 32;
-constexpr int64_t kStreamTiles = 4, kStreamWork = 64 * 128, kStreamWorkF32 = 108 * 128;
+// tiles and, in tiles times blocks of 128 dims, 100 a CU. 8 kv heads of 128, 4
+// heads each, bf16, streaming and prompt kernel: 16 rows x 4 over 4000 tokens 15.0
+// and 20.1 us, over 16000 25.6 and 29.5, 32 x 4 over 16000 37.6 and 35.3, 256 x 4
+// over 1500 33.5 and 37.5 (110 a CU), 512 x 4 over 2000 75 and 54, two times 512 x
+// 4 over 0 39 and 25 (eight tiles a CU). f32: 20 x 4 over 16000 32.2 and 37.0, 12
+// x 4 of 8 sequences over 4000 46.7 and 44.5 (94), 512 x 4 over 2000 85 and 66.
+constexpr int64_t kStreamRows = 32, kStreamTiles = 4, kStreamWork = 100 * 128;
 // Up to this many blocks a workgroup takes them alone; and blocks of a split, at
 // least, where they are shared out (8 kv heads of 128, one row, one launch alone
 // against splits and their join: 16 blocks 8.4 and 12.7 us, 32 blocks 11.9 and
@@ -73,8 +70,7 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, c.max_blocks));
     const int64_t tiles = (rows + kKvTileRows - 1) / kKvTileRows * c.batch * c.kv_heads;
     r.stream = rows <= kStreamRows || a.weights_out ||
-               (tiles <= kStreamTiles * cus &&
-                tiles * blocks * c.head_dim <= (a.type == ROCKNPU_KV_F32 ? kStreamWorkF32 : kStreamWork) * cus);
+               (tiles <= kStreamTiles * cus && tiles * blocks * c.head_dim <= kStreamWork * cus);
     p.tile_rows = r.stream ? kKvTileRows : kv_prompt_tile();
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.min_chunk = kMinChunk;

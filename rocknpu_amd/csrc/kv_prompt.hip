@@ -23,8 +23,6 @@
 // weights meet zero codes lost the bits of its result below 2^-23 of them. 4096
 // rows of 32/8 heads of 128, bf16: 203 us (677 TF/s); 8192 rows: 762 (721 TF/s).
 // Priorities and the maximum between the products took 12 of 180 us off.
-#include <type_traits>
-
 #include "kv_attend.h"
 
 namespace rk {

@@ -163,7 +163,7 @@ def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dt
     tokens[b] and in evicted blocks."""
     if dtype not in _TYPES:
         raise ValueError(f"{dtype}: float32, float16 or bfloat16 is wanted")
-    k, v = torch.empty((2, cache.batch, count, cache.kv_heads, cache.head_dim), dtype=dtype, device=cache.device).unbind(0)
+    k, v = cache.scales.new_empty((2, cache.batch, count, cache.kv_heads, cache.head_dim), dtype=dtype).unbind(0)
     hip._check(_lib.load().rocknpu_hip_kv_read(
         cache._ref, cache.lengths(first, "first"), cache.lengths(tokens, "tokens"), count, _TYPES[dtype],
         k.data_ptr(), v.data_ptr(), _stream(cache.device)), "kv_read")
@@ -206,7 +206,7 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads over {cache.kv_heads} kv heads")
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         o_row, o_head = heads * cache.head_dim, cache.head_dim
     else:
         o_rows, _, o_row, o_head = _rows(out, heads, cache.head_dim, "out", device)
@@ -250,16 +250,18 @@ def evict(table: torch.Tensor, starts: torch.Tensor, weights: torch.Tensor, toke
         raise ValueError("table has to be [batch, kv_heads, max_blocks]")
     at = table.device
     batch, kv_heads, max_blocks = table.shape
-    kinds = ((table, torch.int32, "table"), (starts, torch.int32, "starts"), (weights, torch.float32, "weights"))
     if out is None:
         out = (torch.empty_like(table), torch.empty_like(starts), torch.empty_like(weights), torch.empty_like(dropped))
-    for (t, dtype, what), o in zip(kinds, out):
-        _is(t, table.shape, dtype, what, at)
-        _is(o, table.shape, dtype, what + "_out", at)
-    size = torch.Size((batch,))
-    for t, what in ((tokens, "tokens"), (dropped, "dropped"), (out[3], "dropped_out")):
+    table_out, starts_out, weights_out, dropped_out = out
+    shape, size = table.shape, torch.Size((batch,))
+    for t, what in ((table, "table"), (table_out, "table_out"), (starts, "starts"), (starts_out, "starts_out")):
+        _is(t, shape, torch.int32, what, at)
+    for t, what in ((weights, "weights"), (weights_out, "weights_out")):
+        _is(t, shape, torch.float32, what, at)
+    for t, what in ((tokens, "tokens"), (dropped, "dropped"), (dropped_out, "dropped_out")):
         _is(t, size, torch.int32, what, at)
     args = _EvictStruct(table.data_ptr(), starts.data_ptr(), weights.data_ptr(), tokens.data_ptr(), dropped.data_ptr(),
-                        *[t.data_ptr() for t in out], batch, kv_heads, max_blocks, budget, sinks, recent)
+                        table_out.data_ptr(), starts_out.data_ptr(), weights_out.data_ptr(), dropped_out.data_ptr(),
+                        batch, kv_heads, max_blocks, budget, sinks, recent)
     hip._check(_lib.load().rocknpu_hip_kv_evict(ctypes.addressof(args), _stream(at)), "kv_evict")
     return out

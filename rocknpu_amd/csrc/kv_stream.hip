@@ -85,6 +85,32 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
         return;
     }
 
+    // Lane l looks up the wave's l-th block from `base` on. The first blocks are looked up and their bytes asked for before
+    // the queries are converted: the chain of trips to memory is what a short context waits for.
+    int my_page = 0, my_start = 0;
+    float my_sk = 0.0f, my_sv = 0.0f;
+    BlockRegs<D> next;
+    const auto look_up = [&](int base) {
+        const int nth = base + lane * WAVES + wave;
+        if (nth < end) {
+            const int at = range.entry(nth);
+            my_page = c.table[entry_row + at];
+            my_start = c.starts[entry_row + at];
+        }
+    };
+    const auto blocks_from = [&](int base) { return (min(end - base, 64 * WAVES) - wave + WAVES - 1) / WAVES; };
+    const auto fetch_first = [&](int base) {
+        const bool ok = my_page >= 0 && my_page < c.n_pages;
+        my_page = ok ? my_page : 0;
+        if (base + lane * WAVES + wave < end) {
+            const float2 sc = reinterpret_cast<const float2*>(c.scales)[my_page];
+            my_sk = kv_scale(sc.x, ok);
+            my_sv = kv_scale(sc.y, ok);
+        }
+        if (blocks_from(base) > 0) load_block<D>(c.pages, __builtin_amdgcn_readlane(my_page, 0), lane, next);
+    };
+    if (begin < end) look_up(begin);
+
     // this lane's row: column n of the products
     const int row = min(r0 + n, rows - 1), head = h * p.group + row % p.group;
     const int qpos = s.past + row / p.group;
@@ -94,11 +120,12 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
         const T* src = static_cast<const T*>(a.q) + (s.row0 + row / p.group) * a.q_row + head * a.q_head;
         float x[D / 32][8], top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            load8<TYPE>(src + i / 2 * 64 + quad * 16 + i % 2 * 8, p.vec_q, x[i]);
+        for (int i = 0; i < D / 32; ++i) load8<TYPE>(src + i / 2 * 64 + quad * 16 + i % 2 * 8, p.vec_q, x[i]);
+        if (begin < end) fetch_first(begin);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
-        }
         const float power = row_power(max_over_quads(top));
         unit = a.scale / power;
 #pragma unroll
@@ -118,23 +145,11 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
     for (int i = 0; i < D / 16; ++i) o[i] = float4v{0, 0, 0, 0};
 
     for (int base = begin; base < end; base += 64 * WAVES) {
-        // lane l looks up the wave's l-th block
-        const int nth = base + lane * WAVES + wave;
-        int my_page = 0, my_start = 0;
-        float my_sk = 0.0f, my_sv = 0.0f;
-        if (nth < end) {
-            const int at = range.entry(nth);
-            const int page = c.table[entry_row + at];
-            const bool ok = page >= 0 && page < c.n_pages;
-            my_page = ok ? page : 0;
-            my_start = c.starts[entry_row + at];
-            const float2 sc = reinterpret_cast<const float2*>(c.scales)[my_page];
-            my_sk = kv_scale(sc.x, ok);
-            my_sv = kv_scale(sc.y, ok);
+        if (base != begin) {
+            look_up(base);
+            fetch_first(base);
         }
-        const int here = (min(end - base, 64 * WAVES) - wave + WAVES - 1) / WAVES;  // the wave's blocks
-        BlockRegs<D> next;
-        if (here > 0) load_block<D>(c.pages, __builtin_amdgcn_readlane(my_page, 0), lane, next);
+        const int here = blocks_from(base);  // the wave's blocks
         for (int k = 0; k < here; ++k) {
             const BlockRegs<D> cur = next;
             if (k + 1 < here) load_block<D>(c.pages, __builtin_amdgcn_readlane(my_page, k + 1), lane, next);

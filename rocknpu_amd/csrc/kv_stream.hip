@@ -63,13 +63,13 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
     const KvSlot mine = kv_slot(p, slot_at);
     const int b = mine.seq;
     if (b < 0) return;
+    const int dropped = c.dropped[b], kept = a.prefix ? a.prefix[b] : 0;
     const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
     const int rows = s.n * p.group, r0 = tile * kKvTileRows;
+    const int total = s.past + s.n, gone = uniform(max(dropped, 0)), prefix = uniform(kept);
     if (r0 >= rows) return;
     kv_leave_slot(p, mine, h, tile);
-    const int total = s.past + s.n, gone = uniform(max(c.dropped[b], 0));
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
-    const int prefix = a.prefix ? uniform(a.prefix[b]) : 0;
     const int64_t entry_row = (static_cast<int64_t>(b) * c.kv_heads + h) * c.max_blocks;
     const int q0 = s.past + r0 / p.group, q1 = s.past + (min(r0 + kKvTileRows, rows) - 1) / p.group;
     const KvRange range = kv_range(a, c.starts + entry_row, held, gone, q0, q1, prefix);

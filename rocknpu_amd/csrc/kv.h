@@ -57,12 +57,18 @@ struct KvType<ROCKNPU_KV_BF16> {
 struct KvSpan {
     int past, row0, n;
 };
-__device__ __forceinline__ KvSpan kv_span(const int32_t* past, const int32_t* cu, int b, int rows, int max_new) {
+// The four are asked for before any is waited for, and before a branch on one of
+// them: a kernel's start is a chain of trips to memory, this makes them one.
+__device__ __forceinline__ KvSpan kv_span(const int32_t* past, const int32_t* cu, const int32_t* dropped, int b, int rows,
+                                          int max_new, int& gone) {
+    int had = past[b], first = cu[b], last = cu[b + 1], lost = dropped[b];
+    asm volatile("" : "+v"(had), "+v"(first), "+v"(last), "+v"(lost));
     KvSpan s;
-    s.past = min(max(past[b], 0), 0x3fffffff);
-    s.row0 = min(max(cu[b], 0), rows);
-    const int end = min(max(cu[b + 1], s.row0), rows);
+    s.past = min(max(had, 0), 0x3fffffff);
+    s.row0 = min(max(first, 0), rows);
+    const int end = min(max(last, s.row0), rows);
     s.n = min(end - s.row0, max_new);
+    gone = max(lost, 0);
     return s;
 }
 

@@ -110,9 +110,10 @@ struct KvSlot {
     int seq, split, splits, first;
 };
 __device__ __forceinline__ int kv_blocks_estimate(const KvAttend& p, int b) {
-    const KvSpan s = kv_span(p.a.past, p.a.cu, b, static_cast<int>(p.a.rows), static_cast<int>(p.a.max_new));
+    int gone;
+    const KvSpan s = kv_span(p.a.past, p.a.cu, p.c.dropped, b, static_cast<int>(p.a.rows), static_cast<int>(p.a.max_new), gone);
     if (s.n == 0) return 0;
-    int blocks = min((s.past + s.n + kKvBlock - 1) / kKvBlock - max(p.c.dropped[b], 0), p.c.max_blocks);
+    int blocks = min((s.past + s.n + kKvBlock - 1) / kKvBlock - gone, p.c.max_blocks);
     if (p.a.window > 0) {
         const int prefix = p.a.prefix ? min(max(p.a.prefix[b], 0), 0x3fffffff) : 0;
         blocks = min(blocks, min(p.a.window, 0x3fffffff) / kKvBlock + (s.n + prefix) / kKvBlock + 3);

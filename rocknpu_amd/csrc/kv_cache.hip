@@ -59,7 +59,8 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
     __shared__ uint32_t red[2][kAppendThreads / 64];
     __shared__ alignas(16) int8_t codes[2][kKvBlock][D + 4];
     const int tid = threadIdx.x, b = blockIdx.z, h = blockIdx.y;
-    const KvSpan s = kv_span(a.past, a.cu, b, a.rows, a.max_new);
+    int gone;
+    const KvSpan s = kv_span(a.past, a.cu, a.c.dropped, b, a.rows, a.max_new, gone);
     const int j = s.past / kKvBlock + blockIdx.x;
     const int lead = max(s.past - j * kKvBlock, 0);          // tokens the block held before
     const int end = min(s.past + s.n - j * kKvBlock, kKvBlock);
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
         }
     }
     const int64_t entry_row = (static_cast<int64_t>(b) * a.c.kv_heads + h) * a.c.max_blocks;
-    const int at = j - max(a.c.dropped[b], 0);
+    const int at = j - gone;
     if (at < 0 || at >= a.c.max_blocks) return;
     const int page = a.c.table[entry_row + at];
     if (page < 0 || page >= a.c.n_pages) return;

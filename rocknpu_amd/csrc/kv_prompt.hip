@@ -148,11 +148,12 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     const KvSlot mine = kv_slot(p, slot_at);
     const int b = mine.seq;
     if (b < 0) return;
-    const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
+    int lost;
+    const KvSpan s = uniform(kv_span(a.past, a.cu, c.dropped, b, static_cast<int>(a.rows), static_cast<int>(a.max_new), lost));
     const int rows = s.n * p.group, r0 = tile * kTile;
     if (r0 >= rows) return;
     kv_leave_slot(p, mine, h, tile);
-    const int total = s.past + s.n, gone = uniform(max(c.dropped[b], 0));
+    const int total = s.past + s.n, gone = uniform(lost);
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
     const int prefix = a.prefix ? uniform(a.prefix[b]) : 0;
     const int64_t entry_row = (static_cast<int64_t>(b) * c.kv_heads + h) * c.max_blocks;

@@ -63,10 +63,11 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
     const KvSlot mine = kv_slot(p, slot_at);
     const int b = mine.seq;
     if (b < 0) return;
-    const int dropped = c.dropped[b], kept = a.prefix ? a.prefix[b] : 0;
-    const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
+    const int kept = a.prefix ? a.prefix[b] : 0;
+    int lost;
+    const KvSpan s = uniform(kv_span(a.past, a.cu, c.dropped, b, static_cast<int>(a.rows), static_cast<int>(a.max_new), lost));
     const int rows = s.n * p.group, r0 = tile * kKvTileRows;
-    const int total = s.past + s.n, gone = uniform(max(dropped, 0)), prefix = uniform(kept);
+    const int total = s.past + s.n, gone = uniform(lost), prefix = uniform(kept);
     if (r0 >= rows) return;
     kv_leave_slot(p, mine, h, tile);
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
@@ -308,7 +309,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     __shared__ float keep[4 / WAVES][kKvMaxSplits];
     __shared__ alignas(16) float part[WAVES][D];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), h = blockIdx.y, b = blockIdx.z;
-    const KvSpan s = uniform(kv_span(a.past, a.cu, b, static_cast<int>(a.rows), static_cast<int>(a.max_new)));
+    int lost;
+    const KvSpan s = uniform(kv_span(a.past, a.cu, c.dropped, b, static_cast<int>(a.rows), static_cast<int>(a.max_new), lost));
     const int rows = s.n * p.group;
     const int64_t seq = static_cast<int64_t>(b) * c.kv_heads + h;
     const bool joins = static_cast<int>(blockIdx.x) < row_groups;
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     if (at >= c.max_blocks) return;
     const int64_t entry = seq * c.max_blocks + at;
     float got = 0.0f;
-    const int total = s.past + s.n, gone = uniform(max(c.dropped[b], 0));
+    const int total = s.past + s.n, gone = uniform(lost);
     if (at < min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks)) {
         const int start = c.starts[entry], prefix = a.prefix ? uniform(a.prefix[b]) : 0;
         for (int tile = 0; tile * p.tile_rows < rows; ++tile) {

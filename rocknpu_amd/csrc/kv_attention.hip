@@ -74,19 +74,21 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.tile_rows = r.stream ? kKvTileRows : kv_prompt_tile();
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.min_chunk = kMinChunk;
-    // A streaming workgroup's waves. Heads of 128 take 160 registers and heads of 192 up to 240: two waves a SIMD.
-    // Eight in one workgroup cut a context into half as many splits, two workgroups of four even out unequal lengths
-    // better where sequences times kv heads come near the CUs (8 kv heads of 128, bf16, in workgroups of eight and of
-    // four: one sequence of 16000 tokens 17.7 and 20.3 us, 8 of 1000-3400 19.9 and 20.4, 24 of 600-4000 37.5 and 34.5,
-    // 32 of 800-3900 40.1 and 36.9; 32 of 4100 each, which the host cannot tell from them, 66 and 77). Heads of 192
-    // would have one workgroup of four a CU; heads of 64 leave room for three waves a SIMD, heads of 256 for one.
+    // A streaming workgroup's waves. Eight cut a context into half as many splits and shorten a short one; four even out
+    // unequal lengths better where sequences times kv heads come near the CUs (8 kv heads of 128, bf16, in workgroups of
+    // eight and of four: one sequence of 16000 tokens 17.7 and 20.3 us, 8 of 1000-3400 19.9 and 20.4, 24 of 600-4000 37.5
+    // and 34.5, 32 of 800-3900 40.1 and 36.9; 32 of 4100 each, which the host cannot tell from them, 66 and 77; 4 kv heads
+    // of 64, f32, one of 512 7.5 and 7.9, of 900 10.0 and 11.3). Heads of 192 take up to 240 registers: two waves a SIMD,
+    // which workgroups of four would not reach; heads of 256 take all of them: one.
     const bool busy = static_cast<int64_t>(c.batch) * c.kv_heads * p.row_tiles >= cus / 2;
-    p.waves = c.head_dim == 192 || (c.head_dim == 128 && !busy) ? 8 : 4;
+    p.waves = c.head_dim == 192 || (c.head_dim <= 128 && !busy) ? 8 : 4;
     // One round of the workgroups that the GPU holds at once: a second round pays every workgroup's start (lookups, the
     // queries, the first blocks' latency) again (32 sequences of 500-4000 tokens, 8 kv heads of 128, workgroups of
     // eight: 44 us; one and a half, two and three rounds 53, 55 and 54). The prompt kernel shares blocks out where that
     // gives every sequence and tile at least four parts: below, joining costs what it saves.
-    const int held = !r.stream ? (c.head_dim <= 128 ? 2 : 1) : c.head_dim == 64 ? 3 : c.head_dim == 128 && busy ? 2 : 1;
+    const int held = !r.stream          ? (c.head_dim <= 128 ? 2 : 1)
+                     : c.head_dim == 64 ? (busy ? 3 : 2)
+                     : c.head_dim == 128 && busy ? 2 : 1;
     const int64_t resident = static_cast<int64_t>(held) * cus;
     p.whole = static_cast<int>(std::max<int64_t>(
         std::min<int64_t>(resident / (c.kv_heads * p.row_tiles), c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk)), 1));

@@ -440,7 +440,7 @@ template <int TYPE, int D>
 int launch(const KvAttend& p, hipStream_t stream) {
     const dim3 grid(p.c.kv_heads, p.row_tiles, p.slots);
     if (p.a.rows > 0 && p.a.max_new > 0) {
-        if constexpr (D == 128 || D == 192) {
+        if constexpr (D != 256) {
             if (p.waves == 8) kv_stream_kernel<TYPE, D, 8><<<grid, 512, 0, stream>>>(p);
         }
         if constexpr (D != 192) {

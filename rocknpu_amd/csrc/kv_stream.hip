@@ -9,7 +9,7 @@
 // layout in which the next product takes weights: values (16 dims x 32 tokens)
 // times weights. Bound by the cache's bytes: one row of two sequences of 100000
 // tokens, 8 kv heads of 128, 420 MB in 79 us (5.3 TB/s, above a large copy's 4.7);
-// by the longest part where lengths differ: 32 of 500-4100 tokens, 145 MB in 39.
+// by the longest part where lengths differ: 32 of 500-4100 tokens, 145 MB in 38.
 #include "kv_attend.h"
 
 namespace rk {

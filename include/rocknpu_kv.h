@@ -134,6 +134,14 @@ int rocknpu_hip_kv_attention(const rocknpu_kv_cache * cache, const rocknpu_kv_at
 int rocknpu_hip_kv_attention_workspace(const rocknpu_kv_cache * cache, const rocknpu_kv_attention_args * args, int cus,
                                        size_t * bytes);
 
+/* How such a call is shared out over workgroups where the rows of sequence b may
+ * see blocks[b] blocks (0: it has no rows): parts[b] of them take sequence b, each
+ * a part of its blocks, per kv head and tile of rows. All parts together are at
+ * most `slots`, what the launch holds. blocks and parts are HOST arrays of batch
+ * entries; host code only, `cus` as above. */
+int rocknpu_hip_kv_attention_parts(const rocknpu_kv_cache * cache, const rocknpu_kv_attention_args * args, int cus,
+                                   const int32_t * blocks, int32_t * parts, int64_t * slots);
+
 typedef struct rocknpu_kv_evict_args {
     const int32_t * table;   /* [batch][kv_heads][max_blocks], as in the cache */
     const int32_t * starts;

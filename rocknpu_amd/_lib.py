@@ -91,6 +91,7 @@ SIGNATURES = {
     "rocknpu_hip_kv_read": (_i, [_vp, _vp, _vp, _sz, _u32, _vp, _vp, _vp]),
     "rocknpu_hip_kv_attention": (_i, [_vp, _vp, _vp, _sz, _vp]),
     "rocknpu_hip_kv_attention_workspace": (_i, [_vp, _vp, _i, _vp]),
+    "rocknpu_hip_kv_attention_parts": (_i, [_vp, _vp, _i, _vp, _vp, _vp]),
     "rocknpu_hip_kv_evict": (_i, [_vp, _vp]),
 }
 

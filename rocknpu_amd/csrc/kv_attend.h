@@ -129,6 +129,25 @@ __device__ __forceinline__ int kv_divide(int x, int y) {
     q -= q * y > x;
     return q + ((q + 1) * y <= x);
 }
+// Blocks of a split, where all sequences' rows may see `all` blocks together;
+// `needed` gives the slots that a chunk comes to. The last chunk fits `slots`
+// whatever the sequences' lengths are; a longer one may take more and has to be
+// counted. That is done for up to 64 sequences, one a lane: more of them take the
+// last chunk. The host asks the same function how a call is shared out.
+template <class Needed>
+__host__ __device__ __forceinline__ int kv_chunk(const KvAttend& p, int all, const Needed& needed) {
+    int chunk = 0;
+#pragma unroll
+    for (int k = 0; k < kKvShares; ++k) {
+        if (p.c.batch > 64 && k < kKvShares - 1) continue;
+        // at least all / parts: the factor and the 1 outdo the rounding
+        chunk = static_cast<int>(static_cast<float>(all) * p.per_part[k]) + 1;
+        chunk = chunk > p.min_chunk ? chunk : p.min_chunk;
+        if (k == kKvShares - 1 || p.c.batch == 1) break;
+        if (needed(chunk) <= p.whole) break;
+    }
+    return chunk;
+}
 __device__ __forceinline__ KvSlot kv_slot(const KvAttend& p, int want) {
     const int lane = threadIdx.x & 63, batch = p.c.batch;
     if (p.share == 0) return KvSlot{want, 0, 1, want};
@@ -136,14 +155,7 @@ __device__ __forceinline__ KvSlot kv_slot(const KvAttend& p, int want) {
     int all = mine;
     for (int base = 64; base < batch; base += 64) all += base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;
     all = wave_sum(all);
-    int chunk = 0;
-#pragma unroll
-    for (int k = 0; k < kKvShares; ++k) {
-        // at least all / parts: the factor and the 1 outdo the rounding
-        chunk = max(p.min_chunk, static_cast<int>(static_cast<float>(all) * p.per_part[k]) + 1);
-        if (k == kKvShares - 1 || batch == 1 || batch > 64) break;
-        if (wave_sum(kv_divide(mine + chunk - 1, chunk)) <= p.whole) break;
-    }
+    const int chunk = kv_chunk(p, all, [&](int c) { return wave_sum(kv_divide(mine + c - 1, c)); });
     int before = 0;
     for (int base = 0; base < batch; base += 64) {
         const int blocks = base == 0 ? mine : base + lane < batch ? kv_blocks_estimate(p, base + lane) : 0;

@@ -120,6 +120,28 @@ extern "C" int rocknpu_hip_kv_attention_workspace(const rocknpu_kv_cache* cache,
     return kStatusOk;
 }
 
+extern "C" int rocknpu_hip_kv_attention_parts(const rocknpu_kv_cache* cache, const rocknpu_kv_attention_args* args,
+                                              int cus, const int32_t* blocks, int32_t* parts, int64_t* slots) {
+    using namespace rk;
+    if (!blocks || !parts || !slots || !attention_ok(cache, args)) return kStatusInvalid;
+    const KvAttend p = plan(*cache, *args, cus > 0 ? cus : device_cu_count()).p;
+    *slots = p.slots;
+    const auto held = [&](int b) { return std::min(std::max(blocks[b], 0), cache->max_blocks); };
+    int64_t all = 0;
+    for (int b = 0; b < cache->batch; ++b) all += held(b);
+    if (p.share == 0) {
+        std::fill(parts, parts + cache->batch, 1);
+        return kStatusOk;
+    }
+    const int chunk = kv_chunk(p, static_cast<int>(all), [&](int c) {
+        int n = 0;
+        for (int b = 0; b < cache->batch; ++b) n += (held(b) + c - 1) / c;
+        return n;
+    });
+    for (int b = 0; b < cache->batch; ++b) parts[b] = std::min((held(b) + chunk - 1) / chunk, kKvMaxSplits);
+    return kStatusOk;
+}
+
 extern "C" int rocknpu_hip_kv_attention(const rocknpu_kv_cache* cache, const rocknpu_kv_attention_args* args,
                                         void* workspace, size_t workspace_bytes, void* stream) {
     using namespace rk;

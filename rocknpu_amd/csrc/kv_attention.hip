@@ -91,7 +91,7 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
                      : c.head_dim == 128 && busy ? 2 : 1;
     const int64_t resident = static_cast<int64_t>(held) * cus;
     p.whole = static_cast<int>(std::max<int64_t>(
-        std::min<int64_t>(resident / (c.kv_heads * p.row_tiles), c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk)), 1));
+        std::min<int64_t>(resident / (static_cast<int64_t>(c.kv_heads) * p.row_tiles), c.batch * ((blocks + p.min_chunk - 1) / p.min_chunk)), 1));
     const int64_t share = std::max<int64_t>(p.whole - static_cast<int64_t>(c.batch) * (kKvShares - 1) / 4, 1);
     // the device adds up all sequences' blocks in 32 bits
     const bool shared = blocks > (r.stream ? kAlone : kMinChunk) && c.batch <= kMaxShared && rows > 0 &&

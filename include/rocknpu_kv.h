@@ -69,9 +69,9 @@ typedef struct rocknpu_kv_cache {
 
 /* Quantises a step's key and value rows (type ROCKNPU_KV_*, [rows][kv_heads]
  * [head_dim], strides in elements, the last dimension contiguous) into their
- * blocks. max_new bounds the rows of any one sequence. A block's scale is the
- * largest of amax / 127 over the new values, the scale it had if it held tokens
- * before, and 2^-100; codes are rint(x * (1 / scale)), codes that the block held
+ * blocks. max_new bounds the rows of any one sequence (above `rows` it is
+ * `rows`). A block's scale is the largest of amax / 127 over the new values, the
+ * scale it had if it held tokens before, and 2^-100; codes are rint(x * (1 / scale)), codes that the block held
  * before become rint(code * (old scale / scale)) when the scale grows. A new
  * value that is not finite makes the block's scale NaN and its codes zero, and
  * NaN it stays until the block is started anew. The first token of a block sets
@@ -98,7 +98,7 @@ typedef struct rocknpu_kv_attention_args {
     float * weights_out;     /* [batch][kv_heads][max_blocks], or NULL; may be cache->weights itself */
     int64_t q_row, q_head, out_row, out_head;
     int64_t rows;
-    int64_t max_new;         /* bounds the rows of any one sequence */
+    int64_t max_new;         /* bounds the rows of any one sequence; above `rows` it is `rows` */
     int64_t max_tokens;      /* what past + rows are expected to reach: sizes the work split, not the result; 0: unknown */
     uint32_t type;
     int32_t heads;           /* a multiple of kv_heads; head h reads kv head h / (heads / kv_heads) */

@@ -21,7 +21,7 @@ bool attention_ok(const rocknpu_kv_cache* c, const rocknpu_kv_attention_args* a)
     if (a->rows > 0 && (!a->q || !a->out)) return false;
     if (!aligned(a->q, size) || !aligned(a->out, size) || a->q_row < 0 || a->q_head < 0 || a->out_row < 0 || a->out_head < 0)
         return false;
-    if (a->max_new * (a->heads / c->kv_heads) > INT_MAX) return false;
+    if (std::min(a->max_new, a->rows) * (a->heads / c->kv_heads) > INT_MAX) return false;
     if (a->weights_out && (!c->weights || a->max_new * (a->heads / c->kv_heads) > kKvMaxWeightRows)) return false;
     return true;
 }
@@ -60,13 +60,14 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     KvAttend& p = r.p;
     p.c = c;
     p.a = a;
+    p.a.max_new = std::min(a.max_new, a.rows);
     p.group = a.heads / c.kv_heads;
     const int64_t per = a.type == ROCKNPU_KV_F32 ? 4 : 8;
     p.vec_q = aligned(a.q, 16) && a.q_row % per == 0 && a.q_head % per == 0;
     p.vec_out = aligned(a.out, 16) && a.out_row % per == 0 && a.out_head % per == 0;
-    const int64_t rows = std::max<int64_t>(a.max_new, 1) * p.group;
+    const int64_t rows = std::max<int64_t>(p.a.max_new, 1) * p.group;
     int64_t blocks = a.max_tokens > 0 ? (a.max_tokens + kKvBlock - 1) / kKvBlock : c.max_blocks;
-    if (a.window > 0) blocks = std::min<int64_t>(blocks, (static_cast<int64_t>(a.window) + a.max_new) / kKvBlock + 2);
+    if (a.window > 0) blocks = std::min<int64_t>(blocks, (static_cast<int64_t>(a.window) + p.a.max_new) / kKvBlock + 2);
     blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, c.max_blocks));
     const int64_t tiles = (rows + kKvTileRows - 1) / kKvTileRows * c.batch * c.kv_heads;
     r.stream = rows <= kStreamRows || a.weights_out ||

@@ -461,6 +461,7 @@ extern "C" int rocknpu_hip_kv_append(const rocknpu_kv_cache* cache, uint32_t typ
     if (!k || !v || k_row < 0 || k_head < 0 || v_row < 0 || v_head < 0) return kStatusInvalid;
     const int size = element_size(type);
     if (!aligned(k, size) || !aligned(v, size)) return kStatusInvalid;
+    max_new = std::min(max_new, rows);
     AppendArgs a{k, v, k_row, k_head, v_row, v_head, past, cu, *cache, static_cast<int>(rows), static_cast<int>(max_new), false};
     const int64_t per = 16 / size;
     a.vec = aligned(k, 16) && aligned(v, 16) && k_row % per == 0 && k_head % per == 0 && v_row % per == 0 && v_head % per == 0;

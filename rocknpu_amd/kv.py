@@ -221,7 +221,7 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
         cache.head_dim ** -0.5 if scale is None else scale, softcap)
     lib = _lib.load()
     ref = ctypes.addressof(args)
-    sizes = (dtype, heads, rows == 0, max_new, max_tokens, window, weights_out is None)
+    sizes = (dtype, heads, min(max_new, rows), max_tokens, window, weights_out is None)
     need = cache._needs.get(sizes)
     if need is None:
         got = ctypes.c_size_t()

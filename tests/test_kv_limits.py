@@ -24,3 +24,22 @@ def test_the_workspace_of_calls_of_any_size(kv_heads, heads, max_new, batch, kin
     status, n = workspace(c, a)
     # far more tiles than the GPU holds workgroups: nothing is shared out, so nothing is joined
     assert (status, n) == (0, 0)
+
+
+@pytest.mark.parametrize("max_new", [3, 4, 1000, 10 ** 6, 2 ** 31 - 1])
+@pytest.mark.parametrize("weights", [False, True])
+def test_no_sequence_has_more_rows_than_the_step(max_new, weights):
+    """A bound above the step's rows, as a caller gives that keeps one for all its steps, is the step's rows."""
+    lib = _lib.load()
+    if weights and max_new * 2 > 256:
+        return  # over the limit of such calls
+    c = cache_struct(batch=7, max_blocks=500)
+    kw = dict(rows=3, weights_out=1 << 20 if weights else 0, heads=4)
+    exact, loose = attention_struct(max_new=3, **kw), attention_struct(max_new=max_new, **kw)
+    assert workspace(c, loose) == workspace(c, exact)
+    blocks, parts, slots = (ctypes.c_int32 * 7)(*[400] * 7), (ctypes.c_int32 * 7)(), ctypes.c_int64()
+    got = []
+    for a in (exact, loose):
+        assert lib.rocknpu_hip_kv_attention_parts(ctypes.byref(c), ctypes.byref(a), 256, blocks, parts, ctypes.byref(slots)) == 0
+        got.append((list(parts), slots.value))
+    assert got[0] == got[1]

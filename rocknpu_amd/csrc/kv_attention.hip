@@ -66,7 +66,7 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.vec_q = aligned(a.q, 16) && a.q_row % per == 0 && a.q_head % per == 0;
     p.vec_out = aligned(a.out, 16) && a.out_row % per == 0 && a.out_head % per == 0;
     const int64_t rows = std::max<int64_t>(p.a.max_new, 1) * p.group;
-    int64_t blocks = a.max_tokens > 0 ? (a.max_tokens + kKvBlock - 1) / kKvBlock : c.max_blocks;
+    int64_t blocks = a.max_tokens > 0 ? (a.max_tokens - 1) / kKvBlock + 1 : c.max_blocks;
     if (a.window > 0) blocks = std::min<int64_t>(blocks, (static_cast<int64_t>(a.window) + p.a.max_new) / kKvBlock + 2);
     blocks = std::max<int64_t>(1, std::min<int64_t>(blocks, c.max_blocks));
     const int64_t tiles = (rows + kKvTileRows - 1) / kKvTileRows * c.batch * c.kv_heads;

@@ -43,3 +43,10 @@ def test_no_sequence_has_more_rows_than_the_step(max_new, weights):
         assert lib.rocknpu_hip_kv_attention_parts(ctypes.byref(c), ctypes.byref(a), 256, blocks, parts, ctypes.byref(slots)) == 0
         got.append((list(parts), slots.value))
     assert got[0] == got[1]
+
+
+@pytest.mark.parametrize("max_tokens", [2 ** 31 - 1, 2 ** 40, 2 ** 63 - 32, 2 ** 63 - 1])
+def test_expecting_more_tokens_than_the_table_holds(max_tokens):
+    """An expectation without limit plans for the table's width, as none does."""
+    c = cache_struct(batch=2, max_blocks=4000)
+    assert workspace(c, attention_struct(max_tokens=max_tokens)) == workspace(c, attention_struct(max_tokens=0))

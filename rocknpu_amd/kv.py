@@ -83,6 +83,13 @@ def _rows(t, heads, head_dim, what, device):
     return shape[0], shape[1], row, head
 
 
+def _size(n: int, what: str, below: int = 1 << 31) -> int:
+    """`n`, where the field that takes it holds it: ctypes cuts larger ones to their low bits."""
+    if not 0 <= n < below:
+        raise ValueError(f"{what} {n} is not in [0, {below})")
+    return n
+
+
 def _stream(device: torch.device) -> int:
     """The device's current stream, as hip._stream gives it, without its object where torch offers that."""
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -154,7 +161,7 @@ def append(cache: Cache, k: torch.Tensor, v: torch.Tensor, past: torch.Tensor, c
         raise ValueError("k and v differ in type or rows")
     hip._check(_lib.load().rocknpu_hip_kv_append(
         cache._ref, _TYPES[k.dtype], k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, rows,
-        cache.lengths(past, "past"), cache.offsets(cu), max_new, _stream(cache.device)), "kv_append")
+        cache.lengths(past, "past"), cache.offsets(cu), _size(max_new, "max_new"), _stream(cache.device)), "kv_append")
 
 
 def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dtype: torch.dtype = torch.float32):
@@ -163,6 +170,7 @@ def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dt
     tokens[b] and in evicted blocks."""
     if dtype not in _TYPES:
         raise ValueError(f"{dtype}: float32, float16 or bfloat16 is wanted")
+    _size(count, "count")
     k, v = cache.scales.new_empty((2, cache.batch, count, cache.kv_heads, cache.head_dim), dtype=dtype).unbind(0)
     hip._check(_lib.load().rocknpu_hip_kv_read(
         cache._ref, cache.lengths(first, "first"), cache.lengths(tokens, "tokens"), count, _TYPES[dtype],
@@ -217,7 +225,8 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
         None if prefix is None else cache.lengths(prefix, "prefix"),
         None if slopes is None else _is(slopes, torch.Size((heads,)), torch.float32, "slopes", device).data_ptr(),
         None if weights_out is None else _is(weights_out, cache.shape, torch.float32, "weights_out", device).data_ptr(),
-        row, head, o_row, o_head, rows, max_new, max_tokens, _TYPES[dtype], heads, causal, window,
+        row, head, o_row, o_head, rows, _size(max_new, "max_new"),
+        _size(max_tokens, "max_tokens", 1 << 63), _TYPES[dtype], heads, causal, _size(window, "window"),
         cache.head_dim ** -0.5 if scale is None else scale, softcap)
     lib = _lib.load()
     ref = ctypes.addressof(args)
@@ -262,6 +271,6 @@ def evict(table: torch.Tensor, starts: torch.Tensor, weights: torch.Tensor, toke
         _is(t, size, torch.int32, what, at)
     args = _EvictStruct(table.data_ptr(), starts.data_ptr(), weights.data_ptr(), tokens.data_ptr(), dropped.data_ptr(),
                         table_out.data_ptr(), starts_out.data_ptr(), weights_out.data_ptr(), dropped_out.data_ptr(),
-                        batch, kv_heads, max_blocks, budget, sinks, recent)
+                        batch, kv_heads, max_blocks, _size(budget, "budget"), _size(sinks, "sinks"), _size(recent, "recent"))
     hip._check(_lib.load().rocknpu_hip_kv_evict(ctypes.addressof(args), _stream(at)), "kv_evict")
     return out

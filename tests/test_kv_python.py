@@ -1,0 +1,38 @@
+"""The Python entry points of the key/value cache on the CPU: what they refuse, and what they make."""
+import pytest
+import torch
+
+from rocknpu_amd import kv
+from tests.test_kv import small_cache
+
+
+def lengths(n):
+    return torch.zeros(n, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("what,bad", [("window", 2 ** 31), ("window", 2 ** 32 + 5), ("window", -1), ("max_new", 2 ** 64 + 1),
+                                      ("max_new", -1), ("max_tokens", 2 ** 64 + 9), ("max_tokens", -5)])
+def test_sizes_that_an_attention_call_does_not_hold(what, bad):
+    """They are refused by name: none is cut to its low bits."""
+    c, q = small_cache(), torch.zeros((2, 1, 64))
+    kw = {"max_new": 1, what: bad}
+    with pytest.raises(ValueError, match=what):
+        kv.attention(c, q, lengths(2), lengths(3), kw.pop("max_new"), **kw)
+
+
+def test_sizes_that_an_append_or_a_read_does_not_hold():
+    c, k = small_cache(), torch.zeros((2, 1, 64))
+    for bad in (2 ** 64 + 1, -1):
+        with pytest.raises(ValueError, match="max_new"):
+            kv.append(c, k, k, lengths(2), lengths(3), bad)
+    for bad in (2 ** 31, -1):
+        with pytest.raises(ValueError, match="count"):
+            kv.read(c, lengths(2), lengths(2), bad)
+
+
+@pytest.mark.parametrize("what,bad", [("budget", 2 ** 32 + 2), ("sinks", 2 ** 32), ("recent", 2 ** 32 + 1), ("budget", -1)])
+def test_sizes_that_an_eviction_does_not_hold(what, bad):
+    t = torch.zeros((2, 1, 5), dtype=torch.int32)
+    kw = {"budget": 2, "sinks": 0, "recent": 1, what: bad}
+    with pytest.raises(ValueError, match=what):
+        kv.evict(t, t, torch.zeros(t.shape), lengths(2), lengths(2), kw.pop("budget"), **kw)

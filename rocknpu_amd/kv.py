@@ -242,6 +242,8 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
     if need:
         if workspace is None:
             workspace = workspace_for(device, need)
+        elif workspace.device != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace has to be a contiguous tensor on {device}")
         ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     hip._check(lib.rocknpu_hip_kv_attention(cache._ref, ref, ws, nbytes, _stream(device)), "kv_attention")
     return out

@@ -36,3 +36,12 @@ def test_sizes_that_an_eviction_does_not_hold(what, bad):
     kw = {"budget": 2, "sinks": 0, "recent": 1, what: bad}
     with pytest.raises(ValueError, match=what):
         kv.evict(t, t, torch.zeros(t.shape), lengths(2), lengths(2), kw.pop("budget"), **kw)
+
+
+@pytest.mark.parametrize("bad", ["elsewhere", "strided"])
+def test_a_workspace_that_the_kernels_cannot_write(bad):
+    """Its address goes to the kernels: it has to be the cache's device's memory, all of it."""
+    c = small_cache(weights=torch.zeros((2, 1, 3)))
+    ws = torch.empty(1 << 21, dtype=torch.uint8, device="meta") if bad == "elsewhere" else torch.zeros(1 << 21, dtype=torch.uint8)[::2]
+    with pytest.raises(ValueError, match="workspace"):
+        kv.attention(c, torch.zeros((2, 1, 64)), lengths(2), lengths(3), 1, weights_out=c.weights, workspace=ws)

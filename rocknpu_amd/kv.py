@@ -138,9 +138,9 @@ class Cache:
         n = batch * kv_heads * max_blocks
         table = torch.arange(n, dtype=torch.int32, device=device).view(batch, kv_heads, max_blocks)
         return cls(torch.zeros((n, 2 * BLOCK * head_dim), dtype=torch.int8, device=device),
-                   torch.full((n, 2), 2.0 ** -100, device=device), table, torch.zeros_like(table),
+                   torch.full((n, 2), 2.0 ** -100, dtype=torch.float32, device=device), table, torch.zeros_like(table),
                    torch.zeros(batch, dtype=torch.int32, device=device),
-                   torch.zeros(table.shape, device=device) if weights else None, head_dim=head_dim)
+                   torch.zeros(table.shape, dtype=torch.float32, device=device) if weights else None, head_dim=head_dim)
 
     def lengths(self, t, what) -> int:
         return _is(t, self._lengths, torch.int32, what, self.device).data_ptr()

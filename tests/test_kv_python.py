@@ -45,3 +45,14 @@ def test_a_workspace_that_the_kernels_cannot_write(bad):
     ws = torch.empty(1 << 21, dtype=torch.uint8, device="meta") if bad == "elsewhere" else torch.zeros(1 << 21, dtype=torch.uint8)[::2]
     with pytest.raises(ValueError, match="workspace"):
         kv.attention(c, torch.zeros((2, 1, 64)), lengths(2), lengths(3), 1, weights_out=c.weights, workspace=ws)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
+def test_an_empty_cache_is_f32_whatever_torch_makes_by_default(dtype):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        c = kv.Cache.empty(2, 1, 64, 3, device="cpu")
+    finally:
+        torch.set_default_dtype(before)
+    assert c.scales.dtype is torch.float32 and c.weights.dtype is torch.float32

@@ -103,7 +103,16 @@ class Cache:
     [n_pages, 64 * head_dim], `scales` f32 [n_pages, 2], `table` and `starts`
     int32 [batch, kv_heads, max_blocks], `dropped` int32 [batch], `weights` f32
     [batch, kv_heads, max_blocks] or None. The tensors are used in place and
-    kept alive by the object."""
+    kept alive by the object; write into them, or make a new Cache of others (an
+    assignment is refused)."""
+
+    _FIXED = frozenset(("pages", "scales", "table", "starts", "dropped", "weights", "shape", "batch", "kv_heads",
+                        "max_blocks", "head_dim", "device"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and name in self.__dict__:
+            raise AttributeError(f"the kernels use the {name} that the cache was made with: write into it, or make a new Cache")
+        object.__setattr__(self, name, value)
 
     def __init__(self, pages, scales, table, starts, dropped, weights=None, *, head_dim: int):
         if head_dim not in HEAD_DIMS:
@@ -256,7 +265,9 @@ def evict(table: torch.Tensor, starts: torch.Tensor, weights: torch.Tensor, toke
     (equal weights: the lowest place). Returns new (table, starts, weights,
     dropped), or fills `out`; each row holds the kept entries in order, then the
     evicted, whose pages the sequence's next blocks take, then the rest. out[:3]
-    may be the inputs themselves, out[3] must not be `dropped`."""
+    may be the inputs themselves, out[3] must not be `dropped`. A Cache keeps the
+    tensors that it was made with: give its own as out[:3] and copy out[3] into
+    its `dropped`, or make a new Cache of what is returned."""
     if table.dim() != 3 or 0 in table.shape:
         raise ValueError("table has to be [batch, kv_heads, max_blocks]")
     at = table.device

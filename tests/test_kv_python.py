@@ -56,3 +56,14 @@ def test_an_empty_cache_is_f32_whatever_torch_makes_by_default(dtype):
     finally:
         torch.set_default_dtype(before)
     assert c.scales.dtype is torch.float32 and c.weights.dtype is torch.float32
+
+
+@pytest.mark.parametrize("name", ["pages", "scales", "table", "starts", "dropped", "weights", "head_dim", "max_blocks"])
+def test_a_cache_does_not_take_other_tensors(name):
+    """The kernels use the buffers that it was made with: an assignment would change what Python shows alone."""
+    c = small_cache()
+    value = getattr(c, name)
+    with pytest.raises(AttributeError, match="new Cache"):
+        setattr(c, name, value)
+    c.table[:] = 1  # its contents are the caller's
+    assert getattr(c, name) is value and int(c.table.sum()) == 6

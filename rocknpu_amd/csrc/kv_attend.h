@@ -69,6 +69,12 @@ __device__ __forceinline__ int starts_below(const int32_t* starts, int n, int va
     return lo;
 }
 
+// The positions before this one are seen whatever the window; held to a range in
+// which sums of positions and sizes stay within 32 bits, as `past` is.
+__device__ __forceinline__ int kv_prefix(const rocknpu_kv_attention_args& a, int b) {
+    return a.prefix ? min(max(a.prefix[b], 0), 0x3fffffff) : 0;
+}
+
 // The blocks that rows at positions q0 .. q1 see: entries [0, first) and
 // [from, to) of the table's row.
 struct KvRange {
@@ -115,7 +121,7 @@ __device__ __forceinline__ int kv_blocks_estimate(const KvAttend& p, int b) {
     if (s.n == 0) return 0;
     int blocks = min((s.past + s.n + kKvBlock - 1) / kKvBlock - gone, p.c.max_blocks);
     if (p.a.window > 0) {
-        const int prefix = p.a.prefix ? min(max(p.a.prefix[b], 0), 0x3fffffff) : 0;
+        const int prefix = kv_prefix(p.a, b);
         blocks = min(blocks, min(p.a.window, 0x3fffffff) / kKvBlock + (s.n + prefix) / kKvBlock + 3);
     }
     return max(blocks, 1);

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     kv_leave_slot(p, mine, h, tile);
     const int total = s.past + s.n, gone = uniform(lost);
     const int held = min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks);
-    const int prefix = a.prefix ? uniform(a.prefix[b]) : 0;
+    const int prefix = uniform(kv_prefix(a, b));
     const int64_t entry_row = (static_cast<int64_t>(b) * c.kv_heads + h) * c.max_blocks;
     const KvRange range = kv_range(a, c.starts + entry_row, held, gone, s.past + r0 / p.group,
                                    s.past + (min(r0 + kTile, rows) - 1) / p.group, prefix);

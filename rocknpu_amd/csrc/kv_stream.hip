@@ -63,7 +63,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
     const KvSlot mine = kv_slot(p, slot_at);
     const int b = mine.seq;
     if (b < 0) return;
-    const int kept = a.prefix ? a.prefix[b] : 0;
+    const int kept = kv_prefix(a, b);
     int lost;
     const KvSpan s = uniform(kv_span(a.past, a.cu, c.dropped, b, static_cast<int>(a.rows), static_cast<int>(a.max_new), lost));
     const int rows = s.n * p.group, r0 = tile * kKvTileRows;
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
     float got = 0.0f;
     const int total = s.past + s.n, gone = uniform(lost);
     if (at < min((total + kKvBlock - 1) / kKvBlock - gone, c.max_blocks)) {
-        const int start = c.starts[entry], prefix = a.prefix ? uniform(a.prefix[b]) : 0;
+        const int start = c.starts[entry], prefix = uniform(kv_prefix(a, b));
         for (int tile = 0; tile * p.tile_rows < rows; ++tile) {
             const int r0 = tile * p.tile_rows, r1 = min(r0 + p.tile_rows, rows);
             // the blocks that kv_range gave the tile

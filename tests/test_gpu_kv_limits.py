@@ -25,3 +25,20 @@ def test_a_bound_above_the_rows(max_new):
     same_cache(c, r, [43, 2])
     check_attention(o, r.attention(q.double().numpy(), past, cu), "f32", 64, 43)
     assert torch.equal(o, kv.attention(c, q.to(DEV), ints(past), ints(cu), 3))
+
+
+@pytest.mark.parametrize("prefix", [2 ** 31 - 1, 2 ** 31 - 31, 2 ** 30, -1, -2 ** 31])
+@pytest.mark.parametrize("new", [1, 3, 60])
+@pytest.mark.parametrize("lost", [0, 4])
+def test_prefixes_beyond_every_position(prefix, new, lost):
+    """With a window too: a prefix of 2^31 - 1 keeps all keys, a negative one none."""
+    past, cu = [700, 90], [0, new, 2 * new]
+    c = random_cache(72, 2, 2, 64, 26, [lost, 0], past)
+    q = torch.randn((2 * new, 8, 64), generator=torch.Generator().manual_seed(73))
+    wo = torch.full_like(c.weights, float("nan")) if new < 60 else None
+    o = kv.attention(c, q.to(DEV), ints(past), ints(cu), new, window=40, prefix=ints([prefix] * 2), weights_out=wo)
+    r = kv_ref.Ref(c)
+    want = r.attention(q.double().numpy(), past, cu, window=40, prefix=[prefix] * 2)
+    check_attention(o, want, "f32", 64, 760)
+    if wo is not None:
+        assert (abs(wo.cpu().double().numpy() - r.weights - want[3]) <= 1e-4).all()

@@ -16,7 +16,8 @@
  * or written whatever it holds. A block whose page number is outside
  * [0, n_pages) or whose place is outside the table is skipped by append and reads
  * as zeros. In attention, a page number outside [0, n_pages) or a scale that is
- * not finite gives NaN in the rows that see the block, and in no other.
+ * negative or not finite gives NaN in the rows that see the block, and in no other.
+ * Any other scale counts as it is, zero too.
  *
  * The cache. A page holds one block of 32 tokens of one kv head: 32 * head_dim
  * int8 codes of keys, then as many of values, and in `scales` one f32 for its

@@ -7,7 +7,10 @@
 // for any M: folding a block's value scale into the exponent leaves the codes
 // as they are (exact in f16 and bf16), takes one add per block and row, and one
 // product per block and row for the denominator. M is the row's running maximum
-// of x log2(e) + log2(sv).
+// of x log2(e) + log2(sv). A scale below kKvFoldLeast (blocks of zeros have
+// 2^-100) counts as kKvFoldLeast in M, and its block's denominator is summed apart
+// with that one: with its own, the keys' share would fall below f32's range where
+// other blocks' values are large, and pass it where it is divided by the scale.
 #pragma once
 
 #include "kv.h"
@@ -46,10 +49,15 @@ struct KvAttend {
     int2* slots_of;  // a sequence's first slot and how many it has
 };
 
-// A page's scale, NaN where there is none or it is not finite.
+// A page's scale, NaN where there is none or it is negative or not finite.
 __device__ __forceinline__ float kv_scale(float s, bool ok) {
-    return ok && fabsf(s) <= 3.402823466e38f ? s : __builtin_nanf("");
+    return ok && s >= 0.0f && s <= 3.402823466e38f ? s : __builtin_nanf("");
 }
+
+// Whether the exponents of a block's weights take its value scale as it is (NaN
+// is): the same in every lane.
+constexpr float kKvFoldLeast = 0x1p-40f;
+__device__ __forceinline__ bool kv_folds(float sv) { return !(sv < kKvFoldLeast); }
 
 // How many of a row's n ascending starts are below `value`: 64 probes a round,
 // the same answer in every lane.

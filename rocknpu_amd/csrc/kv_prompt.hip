@@ -303,7 +303,9 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
         };
         if (__builtin_expect(any, 1)) {
             // scores to exponents over the row's reference, which follows the maximum
-            const float lift = __log2f(sv);
+            const bool folds = kv_folds(sv);
+            const float lift = __log2f(folds ? sv : kKvFoldLeast);
+            float inverse = __builtin_amdgcn_rcpf(sv);
             float factor = unit * sk * kLog2e, off = __builtin_fmaf(-lower, factor, lift), most;
             const bool full = before || (meta.start >= full_low && meta.start + kKvBlock - 1 <= full_high);
             if (__builtin_expect(full && PLAIN, 1)) {
@@ -365,13 +367,21 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
                 off = 0.0f;
             }
             most = max_of_halves(most);
-            if (__builtin_expect(__any(most > ref + kSlack), 0)) {
+            if (__builtin_expect(__any(most > ref + kSlack || !folds), 0)) {
                 const float to = fmaxf(ref, most);
                 const float keep = exp2_fast(ref - to);
                 ref = to;
                 sum *= keep;
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) o[d] *= keep;
+                if (!folds) {
+                    float apart = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) apart += exp2_fast(__builtin_fmaf(x[r], factor, off - ref));
+                    sum += apart / kKvFoldLeast;
+                    inverse = 0.0f;
+                    off += __log2f(sv / kKvFoldLeast);
+                }
             }
             off -= ref;
 
@@ -396,7 +406,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
                 }
                 split_bhalf(part, w[h2]);
             }
-            sum += got == 0.0f ? 0.0f : got * __builtin_amdgcn_rcpf(sv);
+            sum += got == 0.0f ? 0.0f : got * inverse;
             // Values times weights, and between them the later block's conversion. Its bytes are first touched here: moved
             // up, the conversion would wait for them at the iteration's start.
             if constexpr (PLAIN) __builtin_amdgcn_s_setprio(2);

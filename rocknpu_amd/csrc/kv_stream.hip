@@ -185,7 +185,8 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
                     }
                 factor = kLog2e;
             }
-            const float lift = __log2f(sv);
+            const bool folds = kv_folds(sv);
+            const float lift = __log2f(folds ? sv : kKvFoldLeast);
             float most = -__builtin_inff();
             const bool folded = !kv_all_seen(a, start, q0, q1, prefix, total);
             if (!folded) {
@@ -208,14 +209,22 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
             most = max_over_quads(most);
             const float now = fmaxf(top, most);
             const float ref = now == -__builtin_inff() ? 0.0f : now;
-            if (__any(now != top)) {
+            float shift = (folded ? 0.0f : lift) - ref, apart = 0.0f;
+            if (__any(now != top || !folds)) {
                 const float keep = exp2_fast(top - ref);
                 sum *= keep;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) o[i] *= keep;
                 top = now;
+                if (!folds) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) apart += exp2_fast(__builtin_fmaf(x[t][i], factor, shift));
+                    apart /= kKvFoldLeast;
+                    shift += __log2f(sv / kKvFoldLeast);
+                }
             }
-            const float shift = (folded ? 0.0f : lift) - ref;
             float e[8], got = 0.0f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -226,7 +235,7 @@ __global__ __launch_bounds__(64 * WAVES) void kv_stream_kernel(KvAttend p) {
                 }
             bhalf8 w[kWeightParts];
             split_bhalf(e, w);
-            got = got == 0.0f ? 0.0f : got / sv;
+            got = !folds ? apart : got == 0.0f ? 0.0f : got / sv;
             sum += got;
             if (p.block_sums) {
                 const float all = sum_over_quads(got);

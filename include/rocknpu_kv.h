@@ -74,8 +74,9 @@ typedef struct rocknpu_kv_cache {
  * `rows`). A block's scale is the largest of amax / 127 over the new values, the
  * scale it had if it held tokens before, and 2^-100; codes are rint(x * (1 / scale)), codes that the block held
  * before become rint(code * (old scale / scale)) when the scale grows. A new
- * value that is not finite makes the block's scale NaN and its codes zero, and
- * NaN it stays until the block is started anew. The first token of a block sets
+ * value that is not finite, or an old scale that is negative or not finite, makes
+ * the block's scale NaN and its codes zero, and NaN it stays until the block is
+ * started anew. The first token of a block sets
  * its entry of `starts` and clears its entry of `weights` (if not NULL). Past
  * tokens must not share a partly filled block with another sequence. */
 int rocknpu_hip_kv_append(const rocknpu_kv_cache * cache, uint32_t type, const void * k, int64_t k_row,

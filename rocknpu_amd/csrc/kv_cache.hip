@@ -110,8 +110,8 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(AppendArgs a)
         uint32_t top = red[w][0];
 #pragma unroll
         for (int i = 1; i < kAppendThreads / 64; ++i) top = max(top, red[w][i]);
-        // bit patterns above FLT_MAX are infinities and NaNs
-        const bool bad = top > 0x7f7fffffu || !(before[w] <= 3.402823466e38f);
+        // bit patterns above FLT_MAX are infinities and NaNs; so is a scale below 0 to the readers
+        const bool bad = top > 0x7f7fffffu || !(before[w] >= 0.0f && before[w] <= 3.402823466e38f);
         const float scale = bad ? __builtin_nanf("") : fmaxf(fmaxf(__uint_as_float(top) / 127.0f, before[w]), kKvScaleFloor);
         const float inv = bad ? 0.0f : 1.0f / scale;
         again[w] = bad ? 0.0f : before[w] / scale;

@@ -90,3 +90,25 @@ def test_negative_scales_count_as_not_finite(kind, which):
             outs.append(kv.attention(c, q.to(DEV), ints(past), ints(cu), max(new), window=40).cpu())
         torch.testing.assert_close(outs[0], outs[1], rtol=0, atol=0, equal_nan=True)
         assert torch.isnan(outs[0]).any() and not torch.isnan(outs[0]).all()
+
+
+@pytest.mark.parametrize("old", [0.0, -0.0, 2.0 ** -130, 3.0, -0.03, float("-inf"), float("inf"), float("nan")])
+def test_appending_to_blocks_of_any_scale(old):
+    """A block's older values are kept to half a step of its new scale; a scale that is negative or not finite leaves NaN."""
+    c = random_cache(92, 1, 2, 64, 3)
+    page = c.table[0, :, 0].long()
+    c.scales[page] = old
+    r = kv_ref.Ref(c)
+    k = torch.randn((5, 2, 64), generator=torch.Generator().manual_seed(93))
+    kv.append(c, k.to(DEV), k.to(DEV), ints([20]), ints([0, 5]), 5)
+    got = kv_ref.Ref(c)
+    for h in range(2):
+        scale = got.scales[got.table[0, h, 0]]
+        if not (np.isfinite(old) and old >= 0):
+            assert np.isnan(scale).all()
+            continue
+        top = k[:, h].abs().max().numpy() / np.float32(127)
+        assert np.all(scale == max(top, np.float32(old)))
+        for x, y in zip(got.values(got.table[0, h, 0]), r.values(r.table[0, h, 0])):
+            assert np.all(np.abs(x[:20] - y[:20]) <= 0.5001 * scale[0])
+            assert np.all(np.abs(x[20:25] - k[:, h].numpy()) <= 0.5001 * scale[0])

@@ -70,26 +70,8 @@ __device__ __forceinline__ void hold(BlockPieces<D>& r) {
         asm volatile("" : "+v"(r.raw[i].x), "+v"(r.raw[i].y), "+v"(r.raw[i].z), "+v"(r.raw[i].w));
 }
 
-// Eight signed bytes as f16 plus 1152.
-__device__ __forceinline__ half8 codes_to_half_raised(uint32_t lo, uint32_t hi) {
-    union {
-        uint32_t u[4];
-        half8 v;
-    } r;
-    lo ^= 0x80808080u;
-    hi ^= 0x80808080u;
-    r.u[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u);
-    r.u[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u);
-    r.u[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u);
-    r.u[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u);
-    return r.v;
-}
-
-// Converts piece i into LDS: keys into f16, values into bf16. Keys of f16 and bf16
-// calls stay raised by 1152 (their scores come down by 1152 times the row's sum,
-// which rounds a score by about 2^-24 of that: less than those calls' weights are
-// rounded by); f32 calls take them exactly.
-template <int D, bool PAIR>
+// Converts piece i into LDS, exactly: keys into f16, values into bf16.
+template <int D>
 __device__ __forceinline__ void place(const BlockPieces<D>& r, int i, int wave, uint8_t* to) {
     const int piece = threadIdx.x + i * kThreads;
     const uint4 w = r.raw[i];
@@ -97,8 +79,8 @@ __device__ __forceinline__ void place(const BlockPieces<D>& r, int i, int wave, 
     // whole waves take keys or values, and where a round of the workgroup does, that is known here
     if ((i + 1) * kThreads <= kKeys || (i * kThreads < kKeys && wave * 64 + i * kThreads < kKeys)) {  // keys: token, 16 dims
         uint8_t* p = to + (piece / 128 * 4 + piece % 4) * 2 * kKeyRun + piece / 4 % 32 * 16;
-        *reinterpret_cast<half8*>(p) = PAIR ? codes_to_half(w.x, w.y) : codes_to_half_raised(w.x, w.y);
-        *reinterpret_cast<half8*>(p + kKeyRun) = PAIR ? codes_to_half(w.z, w.w) : codes_to_half_raised(w.z, w.w);
+        *reinterpret_cast<half8*>(p) = codes_to_half(w.x, w.y);
+        *reinterpret_cast<half8*>(p + kKeyRun) = codes_to_half(w.z, w.w);
     } else {  // values: dims d and d + 16, 8 tokens
         const int v = piece - kKeys;
         uint8_t* p = to + key_bytes<D>() + (v / 64 * 4 + v % 4) * kValueRun + v / 4 % 16 * 16;
@@ -227,7 +209,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
     BlockPieces<D> even, odd;
     look_up(0, batch);
     half8 q[kParts][kSteps];
-    float unit, lower = 0.0f;  // of a product: its weight in the score; what it is too large by
+    float unit;  // a product's weight in the score
     {
         const T* src = static_cast<const T*>(a.q) + (s.row0 + row / p.group) * a.q_row + head * a.q_head + half * 8;
         float x[kSteps][8], top = 0.0f;
@@ -251,12 +233,8 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             for (int e = 0; e < 8; ++e) {
                 const float v = x[i][e] * signed_power;
                 q[0][i][e] = static_cast<_Float16>(v);
-                if constexpr (PAIR)
-                    q[1][i][e] = static_cast<_Float16>(v - static_cast<float>(q[0][i][e]));
-                else
-                    lower += static_cast<float>(q[0][i][e]);
+                if constexpr (PAIR) q[1][i][e] = static_cast<_Float16>(v - static_cast<float>(q[0][i][e]));
             }
-        if constexpr (!PAIR) lower = 1152.0f * sum_of_halves(lower);
     }
 
     float16v o[D / 32];
@@ -306,7 +284,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
             const bool folds = kv_folds(sv);
             const float lift = __log2f(folds ? sv : kKvFoldLeast);
             float inverse = __builtin_amdgcn_rcpf(sv);
-            float factor = unit * sk * kLog2e, off = __builtin_fmaf(-lower, factor, lift), most;
+            float factor = unit * sk * kLog2e, off = lift, most;
             const bool full = before || (meta.start >= full_low && meta.start + kKvBlock - 1 <= full_high);
             if (__builtin_expect(full && PLAIN, 1)) {
                 float m[kEarly];
@@ -354,7 +332,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int kpos = meta.start + r / 4 * 8 + half * 4 + r % 4;
-                    float y = (x[r] - lower) * to_score;
+                    float y = x[r] * to_score;
                     if constexpr (!PLAIN) {
                         if (a.softcap != 0.0f) y = kv_cap<PAIR>(y, a.softcap);
                         if (a.slopes) y += slope * static_cast<float>(kpos - qpos);
@@ -420,14 +398,14 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
                 for (int part = 0; part < kWeightParts; ++part)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value[k], w[h2][part], o[d], 0, 0, 0);
                 if (k % (kSteps / BlockPieces<D>::kEach) == 0)
-                    place<D, PAIR>(two, k / (kSteps / BlockPieces<D>::kEach), wave, lds[later]);
+                    place<D>(two, k / (kSteps / BlockPieces<D>::kEach), wave, lds[later]);
             }
         } else {
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) product(k < kAhead ? key[k] : read_key(at_1, k), k, x_1);
             hold<D>(two);
 #pragma unroll
-            for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(two, i, wave, lds[later]);
+            for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D>(two, i, wave, lds[later]);
         }
         if constexpr (PLAIN) __builtin_amdgcn_s_setprio(0);
         meta = meta_1;
@@ -449,10 +427,10 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
         meta = meta_of(0);
         meta_1 = meta_of(1);
 #pragma unroll
-        for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(even, i, wave, lds[0]);
+        for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D>(even, i, wave, lds[0]);
         fetch_block(2, even);
 #pragma unroll
-        for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D, PAIR>(odd, i, wave, lds[1]);
+        for (int i = 0; i < BlockPieces<D>::kEach; ++i) place<D>(odd, i, wave, lds[1]);
         fetch_block(3, odd);
     }
     lds_barrier();

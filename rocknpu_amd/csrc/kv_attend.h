@@ -25,6 +25,8 @@ constexpr int kKvTileRows = 16;  // rows of a tile of the streaming kernel
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bhalf2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 struct KvAttend {
@@ -254,9 +256,10 @@ __device__ __forceinline__ bhalf8 codes_to_bhalf(uint32_t lo, uint32_t hi) {
     return r.v;
 }
 
-// Non-negative x as the sum of PARTS bf16 (8 bits each, cut off; the last one's
-// rest is dropped), eight at a time: 16 bits in two, f32's 24 in three, over
-// f32's whole range.
+// x as the sum of PARTS bf16, eight at a time, each part what the ones before it
+// leave, rounded to nearest: 17 bits in two (an error of 2^-18 at most), f32's 24
+// in three, over f32's whole range. (Cut off, which costs as much, two hold 16 bits
+// and leave outputs closer to 0 by 2^-17 in the mean.)
 template <int PARTS>
 __device__ __forceinline__ void split_bhalf(const float (&x)[8], bhalf8 (&part)[PARTS]) {
     float rest[8];
@@ -266,15 +269,19 @@ __device__ __forceinline__ void split_bhalf(const float (&x)[8], bhalf8 (&part)[
     for (int p = 0; p < PARTS; ++p) {
         union {
             uint32_t u[4];
+            bhalf2v h[4];
             bhalf8 v;
         } r;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            r.u[i] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * i + 1]), __float_as_uint(rest[2 * i]), 0x07060302u);
+            r.h[i] = __builtin_convertvector((float2v{rest[2 * i], rest[2 * i + 1]}), bhalf2v);
         part[p] = r.v;
         if (p + 1 < PARTS) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xffff0000u);
+            for (int i = 0; i < 4; ++i) {
+                rest[2 * i] -= __uint_as_float(r.u[i] << 16);
+                rest[2 * i + 1] -= __uint_as_float(r.u[i] & 0xffff0000u);
+            }
         }
     }
 }

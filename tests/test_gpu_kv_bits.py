@@ -36,7 +36,7 @@ def check(c, q, past, new, kind, d, more=0.0, **kw):
 
 def case(seed, d, new):
     past, news = [100] * BATCH, [new] * BATCH
-    assert new == 1 or many_tiles(news)
+    assert new <= 8 or many_tiles(news)
     c = random_cache(seed, BATCH, KV_HEADS, d, 6)
     g = torch.Generator().manual_seed(seed + 1)
     return c, torch.randn((BATCH * new, HEADS, d), generator=g), past, news
@@ -59,3 +59,19 @@ def test_biased_queries_and_a_strong_key_channel(kind, new, d):
     q[..., 5] = 0
     c.scales[:, 0] = 0.05
     check(c, q.to(TYPES[kind]), past, news, kind, d)
+
+
+@pytest.mark.parametrize("new", [8, 41])
+def test_outputs_do_not_lean(new):
+    """The outputs' mean relative error: rounding to f16 leaves 2^-12 over the square root of their number at most, six of
+    that are allowed, and 2^-20 for what the weights' 16 bits may leave in the mean when they are rounded, not cut off
+    (cut off they leave 2^-17)."""
+    c, q, past, news = case(104, 64, new)
+    c.pages[:, 32 * 64:] = torch.randint(60, 128, (c.pages.shape[0], 32 * 64), dtype=torch.int8, device=DEV)
+    q = q.to(torch.float16)
+    cu = offsets(news)
+    got = kv.attention(c, q.to(DEV), ints(past), ints(cu), new).cpu().double().numpy()
+    out = kv_ref.Ref(c).attention(q.double().numpy(), past, cu)[0]
+    mean = float(((got - out) / out).mean())
+    print(f"mean {mean:.3g}", flush=True)
+    assert abs(mean) <= 2.0 ** -20 + 6 * 2.0 ** -12 / np.sqrt(out.size)

@@ -194,16 +194,21 @@ __device__ __forceinline__ void kv_leave_slot(const KvAttend& p, const KvSlot& s
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// cap tanh(x / cap). With 1 - 2 / (1 + e^2z) for tanh the error is of 1, not of small
-// results, so of a score up to 2^-22 cap: it is used where weights are rounded to
-// 16 bits anyway (8 sequences' 4 rows under a window of 4096 tokens, f16: 25.3
-// and 26.8 us, 23.3 without a cap).
+// cap tanh(x / cap), to a few units of the last place however small x / cap is.
+// 16-bit calls take tanh z as a quotient: of its continued fraction's fifth
+// convergent, z (945 + 105 z^2 + z^4) / (945 + 420 z^2 + 15 z^4), up to 1, and
+// (e^2z - 1) / (e^2z + 1) above, which for small z would leave 2^-24 of the cap.
+// (8 sequences of 4 rows under a window of 4096 tokens, f16: 23.5 us; by
+// 1 - 2 / (1 + e^2z) throughout 23.1.)
 template <bool EXACT>
 __device__ __forceinline__ float kv_cap(float x, float cap) {
-    if constexpr (EXACT)
-        return cap * tanhf(x / cap);
-    else
-        return cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + exp2_fast(2.0f * kLog2e * x * __builtin_amdgcn_rcpf(cap))));
+    if constexpr (EXACT) return cap * tanhf(x / cap);
+    const float z = x * __builtin_amdgcn_rcpf(cap), z2 = z * z;
+    const float e = exp2_fast(2.0f * kLog2e * fminf(fmaxf(z, -20.0f), 20.0f));
+    const bool large = fabsf(z) > 1.0f;  // not NaN
+    const float over = large ? e - 1.0f : z * __builtin_fmaf(z2, z2 + 105.0f, 945.0f);
+    const float under = large ? e + 1.0f : __builtin_fmaf(z2, __builtin_fmaf(15.0f, z2, 420.0f), 945.0f);
+    return cap * (over * __builtin_amdgcn_rcpf(under));
 }
 
 // Whether a row at qpos sees the key at kpos.

@@ -61,6 +61,9 @@ Plan plan(const rocknpu_kv_cache& c, const rocknpu_kv_attention_args& a, int cus
     p.c = c;
     p.a = a;
     p.a.max_new = std::min(a.max_new, a.rows);
+    // Below 2^52 such a cap changes a score by less than its last place, and above f32's spacing leaves the softmax the
+    // largest alone, capped or not; its reciprocal could fall below f32's range.
+    if (a.softcap > 0x1p64f) p.a.softcap = 0.0f;
     p.group = a.heads / c.kv_heads;
     const int64_t per = a.type == ROCKNPU_KV_F32 ? 4 : 8;
     p.vec_q = aligned(a.q, 16) && a.q_row % per == 0 && a.q_head % per == 0;

@@ -75,3 +75,20 @@ def test_outputs_do_not_lean(new):
     mean = float(((got - out) / out).mean())
     print(f"mean {mean:.3g}", flush=True)
     assert abs(mean) <= 2.0 ** -20 + 6 * 2.0 ** -12 / np.sqrt(out.size)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("new", [1, 41])
+@pytest.mark.parametrize("cap", [0.02, 1.0, 50.0, 1e4, 1e6, 1e20, 3e38])
+def test_caps_of_any_size(cap, new, kind):
+    """A capped score has the bits that it has without a cap, however large the cap."""
+    c, q, past, news = case(106, 64, new)
+    check(c, q.to(TYPES[kind]), past, news, kind, 64, softcap=cap)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("new", [1, 41])
+def test_capped_scores_from_zero_to_far_beyond_the_cap(new, kind):
+    c, q, past, news = case(108, 64, new)
+    q = q * 2.0 ** torch.arange(-8, 8).view(1, HEADS, 1)
+    check(c, q.to(TYPES[kind]), past, news, kind, 64, softcap=2.0)

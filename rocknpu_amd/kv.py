@@ -83,11 +83,11 @@ def _rows(t, heads, head_dim, what, device):
     return shape[0], shape[1], row, head
 
 
-def _size(n: int, what: str, below: int = 1 << 31) -> int:
-    """`n`, where the field that takes it holds it: ctypes cuts larger ones to their low bits."""
-    if not 0 <= n < below:
-        raise ValueError(f"{what} {n} is not in [0, {below})")
-    return n
+def _sizes(below: int = 1 << 31, **sizes: int) -> None:
+    """Refuses by name what a C field does not hold: ctypes cuts it to its low bits. (Callers ask (a | b) >> 31 first.)"""
+    for what, n in sizes.items():
+        if not 0 <= n < below:
+            raise ValueError(f"{what} {n} is not in [0, {below})")
 
 
 def _stream(device: torch.device) -> int:
@@ -168,9 +168,11 @@ def append(cache: Cache, k: torch.Tensor, v: torch.Tensor, past: torch.Tensor, c
     v_rows, _, v_row, v_head = _rows(v, cache.kv_heads, cache.head_dim, "v", cache.device)
     if k.dtype is not v.dtype or rows != v_rows:
         raise ValueError("k and v differ in type or rows")
+    if max_new >> 31:
+        _sizes(max_new=max_new)
     hip._check(_lib.load().rocknpu_hip_kv_append(
         cache._ref, _TYPES[k.dtype], k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, rows,
-        cache.lengths(past, "past"), cache.offsets(cu), _size(max_new, "max_new"), _stream(cache.device)), "kv_append")
+        cache.lengths(past, "past"), cache.offsets(cu), max_new, _stream(cache.device)), "kv_append")
 
 
 def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dtype: torch.dtype = torch.float32):
@@ -179,7 +181,8 @@ def read(cache: Cache, first: torch.Tensor, tokens: torch.Tensor, count: int, dt
     tokens[b] and in evicted blocks."""
     if dtype not in _TYPES:
         raise ValueError(f"{dtype}: float32, float16 or bfloat16 is wanted")
-    _size(count, "count")
+    if count >> 31:
+        _sizes(count=count)
     k, v = cache.scales.new_empty((2, cache.batch, count, cache.kv_heads, cache.head_dim), dtype=dtype).unbind(0)
     hip._check(_lib.load().rocknpu_hip_kv_read(
         cache._ref, cache.lengths(first, "first"), cache.lengths(tokens, "tokens"), count, _TYPES[dtype],
@@ -222,6 +225,9 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
     rows, heads, row, head = _rows(q, None, cache.head_dim, "q", device)
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads over {cache.kv_heads} kv heads")
+    if (max_new | window) >> 31 or max_tokens >> 63:
+        _sizes(max_new=max_new, window=window)
+        _sizes(1 << 63, max_tokens=max_tokens)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         o_row, o_head = heads * cache.head_dim, cache.head_dim
@@ -234,8 +240,7 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
         None if prefix is None else cache.lengths(prefix, "prefix"),
         None if slopes is None else _is(slopes, torch.Size((heads,)), torch.float32, "slopes", device).data_ptr(),
         None if weights_out is None else _is(weights_out, cache.shape, torch.float32, "weights_out", device).data_ptr(),
-        row, head, o_row, o_head, rows, _size(max_new, "max_new"),
-        _size(max_tokens, "max_tokens", 1 << 63), _TYPES[dtype], heads, causal, _size(window, "window"),
+        row, head, o_row, o_head, rows, max_new, max_tokens, _TYPES[dtype], heads, causal, window,
         cache.head_dim ** -0.5 if scale is None else scale, softcap)
     lib = _lib.load()
     ref = ctypes.addressof(args)
@@ -282,8 +287,10 @@ def evict(table: torch.Tensor, starts: torch.Tensor, weights: torch.Tensor, toke
         _is(t, shape, torch.float32, what, at)
     for t, what in ((tokens, "tokens"), (dropped, "dropped"), (dropped_out, "dropped_out")):
         _is(t, size, torch.int32, what, at)
+    if (budget | sinks | recent) >> 31:
+        _sizes(budget=budget, sinks=sinks, recent=recent)
     args = _EvictStruct(table.data_ptr(), starts.data_ptr(), weights.data_ptr(), tokens.data_ptr(), dropped.data_ptr(),
                         table_out.data_ptr(), starts_out.data_ptr(), weights_out.data_ptr(), dropped_out.data_ptr(),
-                        batch, kv_heads, max_blocks, _size(budget, "budget"), _size(sinks, "sinks"), _size(recent, "recent"))
+                        batch, kv_heads, max_blocks, budget, sinks, recent)
     hip._check(_lib.load().rocknpu_hip_kv_evict(ctypes.addressof(args), _stream(at)), "kv_evict")
     return out

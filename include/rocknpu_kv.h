@@ -62,10 +62,10 @@ typedef struct rocknpu_kv_cache {
     const int32_t * dropped; /* [batch] */
     float * weights;         /* [batch][kv_heads][max_blocks], or NULL */
     int64_t n_pages;
-    int32_t batch;
-    int32_t kv_heads;
+    int32_t batch;           /* at most 4095 */
+    int32_t kv_heads;        /* at most 65535 */
     int32_t head_dim;
-    int32_t max_blocks;
+    int32_t max_blocks;      /* at most 2^26 - 1 */
 } rocknpu_kv_cache;
 
 /* Quantises a step's key and value rows (type ROCKNPU_KV_*, [rows][kv_heads]

@@ -21,15 +21,8 @@ namespace rk {
 constexpr int kKvBlock = 32;
 constexpr float kKvScaleFloor = 0x1p-100f;
 constexpr int kKvMaxWeightRows = 256;
-constexpr int kKvMaxBatch = 4095;  // times 16 row tiles fits a grid dimension
+constexpr int kKvMaxBatch = 4095;  // sequences, or their slots (a few thousand more), are a grid's z, which ends at 65535
 constexpr int kKvEvictMaxBlocks = 16384;
-
-// Byte of key dim d of token t within a page's keys, and of value dim d within
-// its values.
-__host__ __device__ constexpr int kv_key_at(int t, int d) { return (d / 64 * kKvBlock + t) * 64 + d % 64; }
-__host__ __device__ constexpr int kv_value_at(int t, int d) {
-    return ((d / 32 * 16 + d % 16) * 4 + t / 4 % 4) * 16 + (d / 16 % 2) * 8 + t / 16 * 4 + t % 4;
-}
 
 template <int TYPE>
 struct KvType;

@@ -92,7 +92,7 @@ int rocknpu_hip_kv_read(const rocknpu_kv_cache * cache, const int32_t * first, c
 
 typedef struct rocknpu_kv_attention_args {
     const void * q;          /* [rows][heads][head_dim] of `type`, strides in elements, last dimension contiguous */
-    void * out;              /* the same shape and type, strides its own */
+    void * out;              /* the same shape and type, strides its own, without overlap */
     const int32_t * past;    /* [batch] */
     const int32_t * cu;      /* [batch + 1] */
     const int32_t * prefix;  /* [batch], or NULL */

@@ -21,6 +21,7 @@ bool attention_ok(const rocknpu_kv_cache* c, const rocknpu_kv_attention_args* a)
     if (a->rows > 0 && (!a->q || !a->out)) return false;
     if (!aligned(a->q, size) || !aligned(a->out, size) || a->q_row < 0 || a->q_head < 0 || a->out_row < 0 || a->out_head < 0)
         return false;
+    if ((a->rows > 1 && a->out_row < c->head_dim) || (a->heads > 1 && a->out_head < c->head_dim)) return false;
     if (std::min(a->max_new, a->rows) * (a->heads / c->kv_heads) > INT_MAX) return false;
     if (a->weights_out && (!c->weights || a->max_new * (a->heads / c->kv_heads) > kKvMaxWeightRows)) return false;
     return true;

@@ -50,3 +50,13 @@ def test_expecting_more_tokens_than_the_table_holds(max_tokens):
     """An expectation without limit plans for the table's width, as none does."""
     c = cache_struct(batch=2, max_blocks=4000)
     assert workspace(c, attention_struct(max_tokens=max_tokens)) == workspace(c, attention_struct(max_tokens=0))
+
+
+@pytest.mark.parametrize("bad", [dict(out_row=0), dict(out_row=63), dict(out_head=0), dict(out_head=63)], ids=str)
+def test_outputs_that_overlap(bad):
+    """Rows or heads that share elements would be written in no order, as an expanded tensor's."""
+    c = cache_struct()
+    assert workspace(c, attention_struct(**bad))[0] == -1
+    # a single row's or head's stride does not matter; another order of the two is one
+    assert workspace(cache_struct(kv_heads=1), attention_struct(rows=1, heads=1, **bad))[0] == 0
+    assert workspace(c, attention_struct(out_row=64, out_head=128))[0] == 0

@@ -37,7 +37,8 @@ def test_every_sequence_gets_its_parts(batch, d):
         for group, new, kind in ((1, 1, 0), (4, 1, 2), (8, 5, 1), (4, 12, 2), (4, 64, 0)):
             for most, cus in ((33, 256), (127, 256), (500, 256), (5000, 256), (127, 304), (127, 64)):
                 c = cache_struct(batch=batch, kv_heads=kv_heads, head_dim=d, max_blocks=most)
-                a = attention_struct(heads=kv_heads * group, max_new=new, rows=batch * new, type=kind)
+                a = attention_struct(heads=kv_heads * group, max_new=new, rows=batch * new, type=kind, out_head=d,
+                                     out_row=kv_heads * group * d)
                 for blocks in lengths(g, batch, most):
                     parts, slots = parts_of(c, a, blocks, cus)
                     what = (kv_heads, group, new, most, cus)

@@ -6,7 +6,9 @@ its budget.
 
 runs TinyLlama-1.1B's layer shapes (2048 wide, 32 heads of 64 over 4 kv heads)
 with synthetic weights: prompts of unequal lengths in pieces, then tokens of all
-sequences at once, the decode step as one captured graph.
+sequences at once, the decode step as one captured graph. Positions enter as a
+distance bias; a model that rotates its queries and keys does so between their
+projections and the append, with the rows at positions past[b] + i.
 """
 from __future__ import annotations
 

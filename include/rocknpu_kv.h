@@ -118,9 +118,10 @@ typedef struct rocknpu_kv_attention_args {
  * and prefix must then be absent). out = sum(exp(x) v) / sum(exp(x)) over what it
  * sees, and 0 where it sees nothing. Scores, the running maximum and sum and the
  * products' sums are f32. The codes enter the matrix instructions exactly, q as
- * f16 for f16 and bf16 calls and as a pair of f16 (to one unit of f32's last
- * place) for f32 calls (each row scaled by a power of two first), the weights
- * rounded to 17 bits for f16 and bf16 calls and 24 for f32 calls, over f32's range.
+ * f16 for f16 and bf16 calls and as a pair of f16 (to a unit of f32's last place,
+ * or 2^-38 of the row's largest) for f32 calls (each row scaled by a power of two
+ * first), the weights rounded to 17 bits for f16 and bf16 calls and 24 for f32
+ * calls, over f32's range.
  * With weights_out, also weights_out = cache->weights + the weight that each
  * block got from all rows and the kv head's heads (entries past the blocks in
  * use are copied); at most 256 rows times heads per kv head.
@@ -166,8 +167,9 @@ typedef struct rocknpu_kv_evict_args {
  * its last `recent` and, of the others, the budget - sinks - recent of greatest
  * weight (equal weights: the lowest place; NaN ranks lowest). Its entries of
  * table, starts and weights become the kept ones in order, then the evicted ones
- * in order (their pages are the next to be reused), then the rest as they were;
- * dropped_out = dropped + n - budget. Other sequences are copied. */
+ * in order (their pages are the next to be reused: pages that another sequence
+ * shares have to be replaced there before the next append), then the rest as they
+ * were; dropped_out = dropped + n - budget. Other sequences are copied. */
 int rocknpu_hip_kv_evict(const rocknpu_kv_evict_args * args, void * stream);
 
 #ifdef __cplusplus

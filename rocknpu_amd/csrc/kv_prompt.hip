@@ -9,19 +9,23 @@
 // lane but for one exchange, and the weights are the second operand of the next
 // product, values (32 dims x 16 tokens) times weights, as they stand.
 //
-// Per block a wave has D/8 products of 32 cycles; for each of a lane's 16 scores
-// a fused multiply-add, an exponential (9 cycles), half a maximum, conversion and
-// sum; and its share of the conversion. Both units stay busy because a wave takes
-// block j's maximum and exponentials between the products of block j + 1's scores
-// and the conversion of block j + 2 between the products of block j's values, and
-// because the CU's two workgroups are not in step: the wave that is in its
-// products has priority over one that works on a maximum or waits for blocks
-// (not with slopes or capped scores, where the vector unit is the longer one: 148
-// against 143 us).
+// Per block a wave has 3 D/16 products of 32 cycles (D/16 for the scores, twice
+// that for the values, with two parts of a weight; f32 calls 5 D/16); for each of
+// a lane's 16 scores a fused multiply-add, an exponential (9 cycles), half a
+// maximum, conversion and sum; and its share of the conversion. The matrix and
+// vector units overlap because a wave takes block j's maximum and exponentials
+// between the products of block j + 1's scores and the conversion of block j + 2
+// between the products of block j's values, and because the CU's two workgroups
+// are not in step: the wave that is in its products has priority over one that
+// works on a maximum or waits for blocks (not with slopes or capped scores, where
+// the vector unit is the longer one: 148 against 143 us). Over 4096 rows of 32/8
+// heads of 128, bf16, they are busy 42% and 56% of the time; over ragged f32
+// prompts with slopes, heads of 64, 19% and 37%, the rest waits and uneven tiles.
 // Weights enter as two bf16 (f32 calls: three), which keeps f32's range: as one
 // f16 they cost less (165 us where two bf16 take 203), but a row whose greatest
 // weights meet zero codes lost the bits of its result below 2^-23 of them. 4096
-// rows of 32/8 heads of 128, bf16: 203 us (677 TF/s); 8192 rows: 762 (721 TF/s).
+// rows of 32/8 heads of 128, bf16: 206 us (667 TF/s); 8192 rows: 783 (702 TF/s);
+// 4096 rows, f32: 319 us, where the compiler keeps 9 registers in memory.
 // Priorities and the maximum between the products took 12 of 180 us off.
 #include "kv_attend.h"
 
@@ -304,8 +308,7 @@ __global__ __launch_bounds__(kThreads, (D <= 128 ? 2 : 1)) void kv_prompt_kernel
                 __builtin_amdgcn_s_setprio(1);
             } else if (!PLAIN && full && a.softcap == 0.0f) {
                 // a distance's share of the exponent is the block's plus a multiple of the slope (5 prompts of up to 1500
-                // tokens, 32/4 heads of 64, f32: 102 us, with
-                // the general form's operations 143)
+                // tokens, 32/4 heads of 64, f32: 102 us, with the general form's operations 143)
                 const float rise = slope * kLog2e;
                 const float at_0 = __builtin_fmaf(rise, static_cast<float>(meta.start + half * 4 - qpos), off);
                 most = kNothing;

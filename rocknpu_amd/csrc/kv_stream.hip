@@ -392,8 +392,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttend p, int row_groups
         return;
     }
     // The rows' maxima and sums over their splits, all rows at once: as many lanes a row as there are (rows one after the
-    // other: 64 rows of 8 splits with 501 blocks 34 us
-    // instead of 17).
+    // other: 64 rows of 8 splits with 501 blocks 34 us instead of 17).
     int lanes = 64;
     while (lanes > 1 && 256 / lanes < rows) lanes /= 2;
     {

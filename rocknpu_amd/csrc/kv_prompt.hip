@@ -20,7 +20,7 @@
 // works on a maximum or waits for blocks (not with slopes or capped scores, where
 // the vector unit is the longer one: 148 against 143 us). Over 4096 rows of 32/8
 // heads of 128, bf16, they are busy 42% and 56% of the time; over ragged f32
-// prompts with slopes, heads of 64, 19% and 37%, the rest waits and uneven tiles.
+// prompts with slopes, heads of 64, 19% and 38%, the rest waits and uneven tiles.
 // Weights enter as two bf16 (f32 calls: three), which keeps f32's range: as one
 // f16 they cost less (165 us where two bf16 take 203), but a row whose greatest
 // weights meet zero codes lost the bits of its result below 2^-23 of them. 4096

@@ -40,6 +40,36 @@ int rocknpu_hip_repack_w8(uint32_t kind, const uint8_t * blocks, size_t blocks_b
 int rocknpu_hip_quantize_a8(const float * a, size_t m, size_t k, size_t lda, size_t k_pad,
                             int8_t * a8, float * scales, void * stream);
 
+#define ROCKNPU_TYPE_F32 0
+#define ROCKNPU_TYPE_F16 1
+#define ROCKNPU_TYPE_BF16 2
+#define ROCKNPU_NORM_MAX_K 65536
+
+typedef struct rocknpu_norm_args {
+    const void * x;        /* [rows][k] of `type`, rows x_row elements apart */
+    const void * residual; /* the same, rows residual_row apart, or NULL */
+    const void * weight;   /* [k] of `weight_type` */
+    void * hidden;         /* x + residual, of `type`, or NULL; may be x or residual itself, or overlap nothing */
+    void * out;            /* the normed rows, of `type`, or NULL; may be x or residual (not hidden), or overlap nothing */
+    int8_t * a8;           /* [rows][k_pad], columns k .. k_pad - 1 are written as zeros */
+    float * scales;        /* [rows] */
+    int64_t rows, k, k_pad;
+    int64_t x_row, residual_row, hidden_row, out_row;
+    uint32_t type, weight_type; /* ROCKNPU_TYPE_*; the weight is f32 or of x's type */
+    float eps;                  /* at least 1e-30 */
+} rocknpu_norm_args;
+
+/* Root-mean-square norm into A8 rows, behind the residual's addition. Of a row:
+ * h = x + residual in f32 (hidden holds it rounded), u = h * weight in f32,
+ * s0 = max|u| / 127 (1 for a row of zeros), a8 = u / s0 rounded half away from
+ * zero as rocknpu_hip_quantize_a8 does, f = 1 / sqrt(mean(h^2) + eps),
+ * scales = s0 * f, out = u * f rounded. The codes do not depend on f, so they
+ * are exact. A row of which a u is not finite gets scale NaN, zero codes and,
+ * in `out`, NaN. k is at most ROCKNPU_NORM_MAX_K; rows = 0 does nothing. The
+ * reference norms on the host (crates/rocknpu-llm/src/lib.rs) and quantises
+ * in crates/rocknpu-capi/src/lib.rs:1776-1791. */
+int rocknpu_hip_norm_a8(const rocknpu_norm_args * args, void * stream);
+
 /* Kernel (c): out[m, ldo] = (f32(A8 W8^T) * a_scales[m]) * w_scales[n] on int8
  * MFMA; if out_i32 is non-NULL the exact int32 accumulators are also written
  * there as [m, n]. Replaces Int8DecodePool::execute_prepared_mtile_direct

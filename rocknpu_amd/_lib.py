@@ -63,6 +63,7 @@ SIGNATURES = {
     # rocknpu_hip.h — device-pointer launch layer
     "rocknpu_hip_repack_w8": (_i, [_u32, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp]),
     "rocknpu_hip_quantize_a8": (_i, [_vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp]),
+    "rocknpu_hip_norm_a8": (_i, [_vp, _vp]),
     "rocknpu_hip_gemm_w8a8": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
     "rocknpu_hip_gemm_route": (_i, [_sz, _sz, _sz, _i, _vp, _vp, _vp]),
     "rocknpu_hip_gemm_column_split": (_i, [_sz, _sz, _sz, _i, _vp]),

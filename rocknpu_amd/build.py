@@ -46,7 +46,7 @@ CFLAGS = [
     f"-I{CSRC}",
 ]
 
-SOURCES = ["repack.hip", "quant.hip", "gemm.hip", "gemm_skinny.hip", "gemv.hip", "gemv_mfma.hip", "gemv_tiled.hip", "launch.hip", "matmul.hip", "capi.hip", "sidecar.hip", "route.hip",
+SOURCES = ["repack.hip", "quant.hip", "norm.hip", "gemm.hip", "gemm_skinny.hip", "gemv.hip", "gemv_mfma.hip", "gemv_tiled.hip", "launch.hip", "matmul.hip", "capi.hip", "sidecar.hip", "route.hip",
            "kv_cache.hip", "kv_stream.hip", "kv_prompt.hip", "kv_attention.hip"]
 
 

@@ -26,6 +26,29 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+class on_device:
+    """Gives the current stream of `device` and makes that device the current
+    one for the launch where it is another."""
+
+    __slots__ = ("device", "back")
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+    def __enter__(self) -> int:
+        if self.device.type != "cuda":
+            raise ValueError(f"the tensors are on {self.device}: a GPU's are wanted")
+        now, index = torch.cuda.current_device(), self.device.index
+        self.back = now if index is not None and index != now else None
+        if self.back is not None:
+            torch.cuda.set_device(index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *_):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+
+
 def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
@@ -72,6 +95,68 @@ def quantize_a8(a: torch.Tensor, k_pad: int | None = None, a8: torch.Tensor | No
     _check(_lib.load().rocknpu_hip_quantize_a8(_ptr(a), m, k, _ld(a), kp, _ptr(a8), _ptr(scales),
                                                _stream()), "quantize_a8")
     return a8, scales
+
+
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class _NormStruct(ctypes.Structure):
+    """rocknpu_norm_args (include/rocknpu_hip.h)."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "residual", "weight", "hidden", "out", "a8", "scales")]
+                + [(n, ctypes.c_int64) for n in ("rows", "k", "k_pad", "x_row", "residual_row", "hidden_row", "out_row")]
+                + [("type", ctypes.c_uint32), ("weight_type", ctypes.c_uint32), ("eps", ctypes.c_float)])
+
+
+def _like(t, x, what):
+    """`t` has x's shape, type and device, and rows that are contiguous: its row stride."""
+    if t.shape != x.shape or t.dtype is not x.dtype or t.device != x.device or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{what} has to be {x.dtype} {tuple(x.shape)} on {x.device} with contiguous rows")
+    return _ld(t)
+
+
+def norm_a8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: torch.Tensor | None = None, *,
+            hidden: torch.Tensor | None = None, out: torch.Tensor | None = None, k_pad: int | None = None,
+            a8: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """Root-mean-square norm of x + residual [m, k] (f32, f16 or bf16) times
+    weight [k] (f32 or x's type), quantised per row for the product that
+    follows: returns (A8 [m, k_pad] int8, scales [m] f32, hidden), hidden the
+    sum x + residual in x's type (`hidden` if given: it may be x or residual
+    itself) and None without a residual. `out`, if given, takes the normed rows
+    in x's type as well. The codes are those of the row x + residual times
+    weight, the norm's factor is in the scales alone."""
+    if x.dim() != 2 or x.dtype not in TYPES:
+        raise ValueError(f"x has to be float32, float16 or bfloat16 [m, k], not {x.dtype} {tuple(x.shape)}")
+    m, k = x.shape
+    at = x.device
+    if weight.shape != (k,) or not weight.is_contiguous() or weight.device != at or weight.dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"weight has to be contiguous float32 or {x.dtype} [{k}] on {at}")
+    if hidden is not None and residual is None:
+        raise ValueError("hidden is x + residual: it needs a residual")
+    if out is not None and hidden is not None and out.data_ptr() == hidden.data_ptr() and m:
+        raise ValueError("out and hidden are the same memory")
+    kp = k_pad_of(k) if k_pad is None else k_pad
+    if kp < k or kp >> 31:
+        raise ValueError(f"k_pad {kp} is not in [{k}, 2^31)")
+    if a8 is None:
+        a8 = torch.empty((m, kp), dtype=torch.int8, device=at)
+    elif a8.shape != (m, kp) or a8.dtype is not torch.int8 or a8.device != at or not a8.is_contiguous():
+        raise ValueError(f"a8 has to be contiguous int8 [{m}, {kp}] on {at}")
+    if scales is None:
+        scales = torch.empty(m, dtype=torch.float32, device=at)
+    elif scales.shape != (m,) or scales.dtype is not torch.float32 or scales.device != at or not scales.is_contiguous():
+        raise ValueError(f"scales have to be contiguous float32 [{m}] on {at}")
+    if residual is not None and hidden is None:
+        hidden = torch.empty((m, k), dtype=x.dtype, device=at)
+    args = _NormStruct(
+        x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
+        None if hidden is None else hidden.data_ptr(), None if out is None else out.data_ptr(), a8.data_ptr(),
+        scales.data_ptr(), m, k, kp, _like(x, x, "x"), 0 if residual is None else _like(residual, x, "residual"),
+        0 if hidden is None else _like(hidden, x, "hidden"), 0 if out is None else _like(out, x, "out"),
+        TYPES[x.dtype], TYPES[weight.dtype], eps)
+    with on_device(at) as stream:
+        _check(_lib.load().rocknpu_hip_norm_a8(ctypes.addressof(args), stream), "norm_a8")
+    return a8, scales, hidden
 
 
 def gemm_workspace(m: int, n: int, k_pad: int, cus: int = 0) -> tuple[int, int]:

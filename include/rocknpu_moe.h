@@ -1,0 +1,75 @@
+/*
+ * rocknpu_moe.h — a feed-forward made of experts, on device buffers: which
+ * experts a token goes to, and the experts' W8A8 products.
+ *
+ * No counterpart in the reference, whose plugin takes plain MUL_MAT nodes only
+ * (adapters/ggml-rocknpu/src/ggml-rocknpu.cpp:614-715); the products' arithmetic
+ * is that of its W8A8 route (crates/rocknpu-capi/src/lib.rs:614-709), as in
+ * rocknpu_hip_quantize_a8 and rocknpu_hip_gemm_w8a8.
+ *
+ * Every pointer inside the structures is a DEVICE pointer, the structures
+ * themselves are host memory read during the call; `stream` is a hipStream_t.
+ * Calls validate what the host can see, enqueue and return without
+ * synchronising or allocating. Status codes are those of rocknpu.h (0 ok, -1
+ * invalid argument, -3 launch failure). Types are ROCKNPU_TYPE_* of
+ * rocknpu_hip.h.
+ */
+#ifndef ROCKNPU_MOE_H
+#define ROCKNPU_MOE_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "rocknpu_hip.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define ROCKNPU_MOE_SOFTMAX 0
+#define ROCKNPU_MOE_SIGMOID 1
+#define ROCKNPU_MOE_MAX_EXPERTS 1024
+#define ROCKNPU_MOE_MAX_TOP_K 64
+#define ROCKNPU_MOE_MAX_GROUPS 64
+#define ROCKNPU_MOE_MAX_ROWS (1 << 28) /* tokens * top_k */
+
+typedef struct rocknpu_moe_route_args {
+    const void * logits; /* [tokens][experts] of `type`, rows logits_row elements apart */
+    const float * bias;  /* [experts], added to the scores for the choice only, or NULL */
+    int32_t * ids;       /* [tokens][top_k] */
+    float * weights;     /* [tokens][top_k] */
+    int32_t * plan;      /* rocknpu_hip_moe_plan_words words: the rows in order of expert, for rocknpu_hip_moe_experts */
+    int64_t tokens, logits_row;
+    uint32_t type;
+    int32_t experts, top_k;
+    int32_t groups;      /* of experts / groups neighbours each; 1: none */
+    int32_t top_groups;  /* groups that a token may choose from; their experts are at least top_k */
+    int32_t group_top;   /* a group's rank: 1, its best expert's rank; 2, the sum of its two best scores + bias */
+    int32_t score;       /* ROCKNPU_MOE_SOFTMAX over the token's logits, or ROCKNPU_MOE_SIGMOID of each */
+    int32_t normalise;   /* weights are divided by their sum + 1e-20 */
+    float factor;        /* and multiplied by this */
+} rocknpu_moe_route_args;
+
+/* Chooses top_k experts for every token. Experts are ranked by score + bias in 64
+ * bits, without a bias by the logits themselves, equal ones by index; a logit of
+ * -inf, or a bias of -inf or NaN, is an expert that cannot be chosen. With groups
+ * only the experts of the top_groups groups of highest rank can (equal groups by
+ * index; a group without group_top experts that can be chosen ranks lowest). ids
+ * are in order of rank; weights are the chosen scores (without bias), normalised and multiplied. Where
+ * less than top_k experts can be chosen the last ids are -1 and their weights 0.
+ * A row that holds a NaN or +inf has its lowest experts and NaN weights.
+ *
+ * The plan begins with 16 words of its own, then offsets [experts + 1] and order
+ * [tokens * top_k]: order[offsets[e]] .. order[offsets[e + 1] - 1] are, ascending,
+ * the numbers token * top_k + place of the choices that fell on expert e, and what
+ * follows offsets[experts] is -1. The rest is the library's. */
+int rocknpu_hip_moe_route(const rocknpu_moe_route_args * args, void * stream);
+
+/* Words of such a plan. Host code only. */
+int rocknpu_hip_moe_plan_words(int64_t tokens, int32_t experts, int32_t top_k, size_t * words);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif

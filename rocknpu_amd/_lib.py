@@ -1,5 +1,5 @@
 """ctypes binding of librocknpu_capi.so (include/rocknpu.h, rocknpu_ggml.h,
-rocknpu_hip.h, rocknpu_kv.h, rocknpu_sidecar.h, rocknpu_route.h).
+rocknpu_hip.h, rocknpu_kv.h, rocknpu_moe.h, rocknpu_sidecar.h, rocknpu_route.h).
 
 The library is loaded from this package directory only. A missing library is
 an error, never a fallback: every compute path in this package goes through
@@ -94,6 +94,9 @@ SIGNATURES = {
     "rocknpu_hip_kv_attention_workspace": (_i, [_vp, _vp, _i, _vp]),
     "rocknpu_hip_kv_attention_parts": (_i, [_vp, _vp, _i, _vp, _vp, _vp]),
     "rocknpu_hip_kv_evict": (_i, [_vp, _vp]),
+    # rocknpu_moe.h — experts: routing and products
+    "rocknpu_hip_moe_route": (_i, [_vp, _vp]),
+    "rocknpu_hip_moe_plan_words": (_i, [_i64, ctypes.c_int32, ctypes.c_int32, _vp]),
 }
 
 

@@ -47,7 +47,8 @@ CFLAGS = [
 ]
 
 SOURCES = ["repack.hip", "quant.hip", "norm.hip", "gemm.hip", "gemm_skinny.hip", "gemv.hip", "gemv_mfma.hip", "gemv_tiled.hip", "launch.hip", "matmul.hip", "capi.hip", "sidecar.hip", "route.hip",
-           "kv_cache.hip", "kv_stream.hip", "kv_prompt.hip", "kv_attention.hip"]
+           "kv_cache.hip", "kv_stream.hip", "kv_prompt.hip", "kv_attention.hip",
+           "moe_route.hip"]
 
 
 def _run(cmd: list[str]) -> None:

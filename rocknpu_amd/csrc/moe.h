@@ -1,0 +1,67 @@
+// What the kernels of an expert feed-forward share: the plan, which the routing
+// writes and the products read (include/rocknpu_moe.h).
+#pragma once
+
+#include "common.h"
+#include "rocknpu_moe.h"
+
+namespace rk {
+
+// A plan's parts, all int32. `tiles` lists the products' row tiles, two words
+// each: the expert and the tile's first row in `order`; a tile ends after tile_rows
+// rows or with its expert's. `place` is where each choice stands in `order` (-1:
+// nothing was chosen). `counts` is the routing's own: each block's choices by expert.
+struct MoePlan {
+    int32_t* tile_count;  // [1], the first of the header's words
+    int32_t* offsets;     // [experts + 1]
+    int32_t* order;       // [rows]
+    int32_t* place;       // [rows]
+    int32_t* tiles;       // [max_tiles][2]
+    int32_t* counts;      // [blocks][experts]
+    int rows, experts, top_k;
+    int tile_rows, max_tiles;
+    int block, blocks;  // entries of a counting block (a multiple of 64), and blocks
+};
+
+constexpr int kMoeHeader = 16;
+constexpr int kMoeCountThreads = 1024;
+
+// Rows of a product's tile.
+inline int moe_tile_rows(int64_t rows, int experts) {
+    (void)rows;
+    (void)experts;
+    return 64;
+}
+
+// The plan of such a call at `base` (which may be null), and its words.
+inline MoePlan moe_plan(int64_t tokens, int experts, int top_k, int32_t* base, size_t* words) {
+    MoePlan p{};
+    p.rows = static_cast<int>(tokens * top_k);
+    p.experts = experts;
+    p.top_k = top_k;
+    p.tile_rows = moe_tile_rows(p.rows, experts);
+    p.max_tiles = p.rows / p.tile_rows + (p.rows < experts ? p.rows : experts);
+    // at most 64 blocks: every one reads all blocks' counts
+    p.block = (p.rows + 63) / 64;
+    p.block = p.block < 4096 ? 4096 : (p.block + kMoeCountThreads - 1) / kMoeCountThreads * kMoeCountThreads;
+    p.blocks = (p.rows + p.block - 1) / p.block;
+    size_t at = 0;
+    const auto take = [&](size_t n) {
+        int32_t* q = base ? base + at : nullptr;
+        at += n;
+        return q;
+    };
+    p.tile_count = take(kMoeHeader);
+    p.offsets = take(static_cast<size_t>(experts) + 1);
+    p.order = take(p.rows);
+    p.place = take(p.rows);
+    p.tiles = take(static_cast<size_t>(p.max_tiles) * 2);
+    p.counts = take(p.blocks > 1 ? static_cast<size_t>(p.blocks) * experts : 0);
+    if (words) *words = at;
+    return p;
+}
+
+// Whether a plan of that size is one that the kernels can take. moe_route.hip.
+bool moe_size_ok(int64_t tokens, int32_t experts, int32_t top_k);
+
+}  // namespace rk

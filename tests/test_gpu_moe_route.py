@@ -1,0 +1,152 @@
+"""moe.route on the GPU against its definition: ids, offsets and order are equal; a weight has the 64-bit score's
+rounding to f32, half a unit of its last place (with a share of another 2^-30 for the scores' own errors)."""
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from rocknpu_amd import moe
+from tests import moe_ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def check(x, top_k, what="", **kw):
+    print("route", what, tuple(x.shape), x.dtype, top_k, {k: v for k, v in kw.items() if k != "bias"}, "bias" if "bias" in kw else "", flush=True)
+    r = moe.route(x, top_k, **kw)
+    torch.cuda.synchronize()
+    ids, weights, offsets, order = moe_ref.route(x, top_k, **kw)
+    assert np.array_equal(r.ids.cpu().numpy(), ids)
+    w = r.weights.cpu().double().numpy()
+    assert np.array_equal(np.isnan(w), np.isnan(weights))
+    assert (np.nan_to_num(np.abs(w - weights) - (2.0 ** -24 + 2.0 ** -30) * np.abs(weights)) <= 2.0 ** -149).all()
+    assert np.array_equal(r.offsets.cpu().numpy(), offsets)
+    assert np.array_equal(r.order.cpu().numpy(), order)
+    return r
+
+
+def logits(seed, tokens, experts, kind="f32", spread=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (spread * torch.randn((tokens, experts), generator=g)).to(TYPES[kind]).to(DEV)
+
+
+def bias(seed, experts, spread=0.2):
+    return (spread * torch.randn(experts, generator=torch.Generator().manual_seed(seed))).to(DEV)
+
+
+@pytest.mark.parametrize("experts", [1, 2, 3, 8, 15, 16, 17, 60, 64, 65, 96, 128, 160, 255, 256, 257, 384, 512, 513, 1000, 1024])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_sizes(experts, kind):
+    for i, (score, with_bias, normalise) in enumerate(itertools.product(("softmax", "sigmoid"), (False, True), (False, True))):
+        kw = {"bias": bias(i, experts)} if with_bias else {}
+        check(logits(experts + i, 13, experts, kind), min(experts, (1, 8, 2, 6, 64, 3, 10, 4)[i]), score=score, normalise=normalise, factor=1.0 + i, **kw)
+
+
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [(256, 8, 4, 8), (60, 4, 2, 6), (64, 64, 9, 9), (128, 2, 1, 64), (512, 16, 3, 10), (24, 3, 2, 3),
+                                                            (16, 8, 8, 16), (1024, 32, 5, 33), (9, 3, 1, 3), (32, 1, 1, 4), (48, 16, 3, 8), (160, 8, 3, 6)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_groups(experts, groups, top_groups, top_k, kind):
+    for i, (score, with_bias) in enumerate(itertools.product(("softmax", "sigmoid"), (False, True))):
+        for group_top in (1, 2) if experts // groups > 1 else (1,):
+            kw = {"bias": bias(i, experts)} if with_bias else {}
+            check(logits(i, 40, experts, kind), top_k, score=score, groups=groups, top_groups=top_groups, group_top=group_top, **kw)
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 2, 3, 4, 5, 63, 64, 65, 100, 511, 512, 513, 1024, 1500])
+def test_token_counts(tokens):
+    check(logits(tokens, tokens, 64), 8)
+    check(logits(tokens, tokens, 24, "f16"), 3, score="sigmoid", bias=bias(1, 24), groups=4, top_groups=2, group_top=2)
+
+
+@pytest.mark.parametrize("tokens,experts,top_k", [(9000, 8, 2), (5000, 256, 8), (40000, 60, 1), (3000, 1024, 16)])
+def test_long(tokens, experts, top_k):
+    """More choices than one workgroup counts: offsets and order against the ids, whose first rows are checked in full."""
+    x = logits(7, tokens, experts)
+    x[::17] = -math.inf
+    r = moe.route(x, top_k)
+    check(x[:200], top_k)
+    torch.cuda.synchronize()
+    ids = r.ids.cpu()
+    want = x.cpu().sort(dim=1, descending=True, stable=True)
+    want = torch.where(want.values[:, :top_k] == -math.inf, -1, want.indices[:, :top_k])
+    assert torch.equal(ids.long(), want)
+    flat = ids.reshape(-1).long()
+    kept = (flat >= 0).sum().item()
+    order = torch.where(flat < 0, experts, flat).sort(stable=True).indices[:kept]
+    assert torch.equal(r.order.cpu().long(), torch.cat((order, torch.full((flat.numel() - kept,), -1))))
+    assert torch.equal(r.offsets.cpu().long(), torch.cat((torch.zeros(1, dtype=torch.long), torch.bincount(flat[flat >= 0], minlength=experts).cumsum(0))))
+
+
+@pytest.mark.parametrize("experts", [5, 64, 200, 700])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_masks_and_values_at_the_ends(experts, score, with_bias):
+    x = logits(experts, 24, experts)
+    x[0] = -math.inf
+    x[1, 1:] = -math.inf
+    x[2, :experts - 1] = -math.inf
+    x[3, 2], x[4, 0], x[5, experts - 1] = math.nan, math.inf, math.nan
+    x[6] = 0.0
+    x[7] = torch.finfo(torch.float32).min
+    x[8, ::2] = torch.finfo(torch.float32).max
+    x[9] = -0.0
+    x[9, ::2] = 0.0
+    x[10] = 80.0 + torch.arange(experts)            # sigmoids that are 1
+    x[11] = -800.0 - torch.arange(experts)          # and 0
+    x[12, ::3] = -math.inf
+    x[13] = -45.0 - 0.1 * torch.arange(experts)
+    x[14] = 1e-7 * torch.arange(experts)            # closer than f32 scores could tell
+    x[15] = 3.0 + 2.4e-7 * (torch.arange(experts) % 7)
+    x[16] = torch.arange(experts) % 3
+    b = {"bias": bias(3, experts)} if with_bias else {}
+    check(x, min(experts, 6), score=score, **b)
+    check(x, min(experts, 6), score=score, normalise=False, **b)
+    if experts % 5 == 0:
+        for group_top in (1, 2) if experts > 5 else (1,):
+            check(x, 2, score=score, groups=5, top_groups=2, group_top=group_top, **b)
+    if with_bias:
+        b["bias"][0], b["bias"][1], b["bias"][2] = math.nan, -math.inf, math.inf
+        check(x, min(experts, 3), score=score, **b)
+        b["bias"][3:] *= 1e4
+        check(x, min(experts, 3), score=score, **b)
+        b["bias"] = torch.zeros(experts, device=DEV)
+        check(x, min(experts, 6), score=score, **b)
+
+
+def test_equal_logits_go_by_index():
+    x = torch.zeros((3, 300), device=DEV)
+    r = check(x, 64)
+    assert r.ids[0].tolist() == list(range(64))
+    check(x.half(), 8, score="sigmoid", bias=torch.zeros(300, device=DEV), groups=10, top_groups=3, group_top=2)
+
+
+def test_strides():
+    wide = logits(1, 20, 300)
+    for at, n in ((0, 64), (1, 64), (3, 250)):
+        check(wide[:, at:at + n], 5)
+    check(wide[::2, :128], 5)
+    check(logits(2, 1, 64).expand(6, 64), 5)
+
+
+def test_streams_and_graphs():
+    x = logits(3, 777, 60)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        check(x, 4)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            r = moe.route(x, 4)
+    for seed in range(4):
+        x.copy_(logits(30 + seed, 777, 60))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        now = check(x, 4)
+        for a, b in ((r.ids, now.ids), (r.weights, now.weights), (r.offsets, now.offsets), (r.order, now.order)):
+            assert torch.equal(a, b)

@@ -68,6 +68,41 @@ int rocknpu_hip_moe_route(const rocknpu_moe_route_args * args, void * stream);
 /* Words of such a plan. Host code only. */
 int rocknpu_hip_moe_plan_words(int64_t tokens, int32_t experts, int32_t top_k, size_t * words);
 
+typedef struct rocknpu_moe_experts_args {
+    const int8_t * a8;          /* [tokens][hidden_pad], as rocknpu_hip_norm_a8 or rocknpu_hip_quantize_a8 give it; 16-byte aligned */
+    const float * a_scales;     /* [tokens] */
+    const int8_t * gate;        /* W8 [experts][ffn][hidden_pad]; 16-byte aligned, as up and down */
+    const int8_t * up;          /* W8 [experts][ffn][hidden_pad] */
+    const int8_t * down;        /* W8 [experts][hidden][ffn_pad] */
+    const float * gate_scales;  /* [experts][ffn] */
+    const float * up_scales;    /* [experts][ffn] */
+    const float * down_scales;  /* [experts][hidden] */
+    const float * weights;      /* [tokens][top_k], as rocknpu_hip_moe_route gives them */
+    const int32_t * plan;       /* of a rocknpu_hip_moe_route with these tokens, experts and top_k */
+    void * out;                 /* [tokens][hidden] of out_type, rows out_row elements apart */
+    int64_t tokens, out_row;
+    int32_t experts, top_k;
+    int32_t hidden, hidden_pad; /* pads are multiples of 64, at most 133120, and what they add is zero in A8 or W8 */
+    int32_t ffn, ffn_pad;
+    uint32_t out_type;
+} rocknpu_moe_experts_args;
+
+/* The feed-forward of every token's chosen experts: for choice s of token t, on
+ * expert e, g and u are the W8A8 products of the token's row with gate[e] and
+ * up[e] (f32(f32(sum) * row's scale) * column's scale, as rocknpu_hip_gemm_w8a8),
+ * v = f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, v's row is
+ * quantised as rocknpu_hip_quantize_a8 does, d is its product with down[e], and
+ * out[t] = sum over s of weights[t][s] * d, in f32 in the order of s, rounded
+ * once. Choices of id -1 are left out; a token without any gets zeros. A row of A8
+ * whose scale is NaN gives NaN in its token's output and in no other.
+ * The workspace (rocknpu_hip_moe_experts_workspace bytes, 256-byte aligned, any
+ * contents) is free again when the call's kernels are done. The same call gives
+ * the same bits. */
+int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args * args, void * workspace, size_t workspace_bytes, void * stream);
+
+/* Bytes of workspace for such a call (only its sizes are read). Host code only. */
+int rocknpu_hip_moe_experts_workspace(const rocknpu_moe_experts_args * args, size_t * bytes);
+
 #ifdef __cplusplus
 }
 #endif

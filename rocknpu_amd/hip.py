@@ -15,6 +15,7 @@ from . import _lib
 
 QK = 256
 Q8K_BYTES = 292
+MAX_K = 133120  # the largest padded K whose int32 sums are exact
 BLOCK_BYTES = {4: 144, 5: 176, 6: 210}
 
 

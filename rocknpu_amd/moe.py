@@ -37,6 +37,16 @@ class _RouteStruct(ctypes.Structure):
                 ("top_groups", _i32), ("group_top", _i32), ("score", _i32), ("normalise", _i32), ("factor", ctypes.c_float)]
 
 
+class _ExpertsStruct(ctypes.Structure):
+    """rocknpu_moe_experts_args (include/rocknpu_moe.h)."""
+
+    _fields_ = ([(n, _vp) for n in ("a8", "a_scales", "gate", "up", "down", "gate_scales", "up_scales", "down_scales",
+                                    "weights", "plan", "out")]
+                + [("tokens", _i64), ("out_row", _i64)]
+                + [(n, _i32) for n in ("experts", "top_k", "hidden", "hidden_pad", "ffn", "ffn_pad")]
+                + [("out_type", ctypes.c_uint32)])
+
+
 class Routing:
     """What route returns: `ids` int32 and `weights` f32 [tokens, top_k], and the
     plan of the experts' products, of which `offsets` int32 [experts + 1] and
@@ -115,3 +125,100 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     with hip.on_device(at) as stream:
         hip._check(_lib.load().rocknpu_hip_moe_route(ctypes.addressof(args), stream), "moe_route")
     return Routing(ids, weights, plan, experts)
+
+
+def _pair(pair, shape, what, device):
+    """A W8 stack and its scales, as hip.repack_w8 gives them for a stack of matrices."""
+    w8, scales = pair
+    if w8.dtype is not torch.int8 or tuple(w8.shape) != shape or not w8.is_contiguous() or w8.device != device:
+        raise ValueError(f"{what} has to be contiguous int8 {shape} on {device}, not {w8.dtype} {tuple(w8.shape)} on {w8.device}")
+    if scales.dtype is not torch.float32 or tuple(scales.shape) != shape[:2] or not scales.is_contiguous() or scales.device != device:
+        raise ValueError(f"{what}'s scales have to be contiguous float32 {shape[:2]} on {device}")
+    return w8, scales
+
+
+class Experts:
+    """A layer's experts: `gate`, `up` and `down`, each a pair of W8 int8 and
+    scales f32: gate and up [experts, ffn, hidden_pad] and [experts, ffn], down
+    [experts, hidden, ffn_pad] and [experts, hidden], the pads zeros up to a
+    multiple of 64. hip.repack_w8 makes them of a stack of GGUF matrices, taken as
+    one matrix of experts * ffn (or hidden) rows. The tensors are used in place
+    and kept alive by the object."""
+
+    __slots__ = ("gate", "up", "down", "experts", "hidden", "hidden_pad", "ffn", "ffn_pad", "device", "_needs")
+
+    def __init__(self, gate, up, down, *, hidden: int, ffn: int):
+        experts = gate[0].shape[0] if gate[0].dim() == 3 else 0
+        if not 1 <= experts <= MAX_EXPERTS or hidden < 1 or ffn < 1:
+            raise ValueError(f"{experts} experts of {hidden} x {ffn}: gate has to be [experts, ffn, hidden_pad], of 1 to {MAX_EXPERTS} experts")
+        self.hidden_pad, self.ffn_pad = gate[0].shape[2], down[0].shape[-1]
+        for what, n, pad in (("hidden", hidden, self.hidden_pad), ("ffn", ffn, self.ffn_pad)):
+            if pad < n or pad % 64 or pad > hip.MAX_K:
+                raise ValueError(f"{what} {n} in rows of {pad}: a multiple of 64 from {n} to {hip.MAX_K} is wanted")
+        self.device = gate[0].device
+        self.gate = _pair(gate, (experts, ffn, self.hidden_pad), "gate", self.device)
+        self.up = _pair(up, (experts, ffn, self.hidden_pad), "up", self.device)
+        self.down = _pair(down, (experts, hidden, self.ffn_pad), "down", self.device)
+        self.experts, self.hidden, self.ffn = experts, hidden, ffn
+        self._needs: dict[tuple[int, int], int] = {}  # workspace bytes by tokens and top_k
+
+
+# Workspaces of the products, one per (device, stream); a call needs nothing of
+# what an earlier one left there. A replaced one is kept for the graphs that hold
+# its address, as the K-split workspaces are.
+_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
+    ws = hip._stream_workspace(_workspaces, device, nbytes, 1 << 20)
+    if ws is None:
+        raise LaunchError("experts under graph capture need this stream's workspace: make one eager call of the same "
+                          "size on the capturing stream first")
+    return ws
+
+
+def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing: Routing, *,
+            dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+            workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The chosen experts' feed-forward of every row of a8 [tokens, hidden_pad]
+    (int8, with a_scales f32 [tokens]: hip.norm_a8 or hip.quantize_a8), weighted
+    by the routing and summed: [tokens, hidden] of `dtype` (f32, f16 or bf16), or
+    into `out`. Products are W8A8 as hip.gemm_w8a8's, between them SwiGLU and
+    the quantisation of its rows."""
+    at = weights.device
+    tokens, top_k = routing.ids.shape
+    if a8.dtype is not torch.int8 or a8.shape != (tokens, weights.hidden_pad) or not a8.is_contiguous() or a8.device != at:
+        raise ValueError(f"a8 has to be contiguous int8 [{tokens}, {weights.hidden_pad}] on {at}")
+    if a_scales.dtype is not torch.float32 or a_scales.shape != (tokens,) or not a_scales.is_contiguous() or a_scales.device != at:
+        raise ValueError(f"a_scales have to be contiguous float32 [{tokens}] on {at}")
+    if routing.experts != weights.experts or routing.plan.device != at:
+        raise ValueError(f"the routing is of {routing.experts} experts on {routing.plan.device}, not {weights.experts} on {at}")
+    if out is None:
+        if dtype not in TYPES:
+            raise ValueError(f"{dtype}: float32, float16 or bfloat16 is wanted")
+        out = torch.empty((tokens, weights.hidden), dtype=dtype, device=at)
+    elif out.dtype not in TYPES or out.shape != (tokens, weights.hidden) or out.device != at or (out.stride(1) != 1 and weights.hidden > 1):
+        raise ValueError(f"out has to be float32, float16 or bfloat16 [{tokens}, {weights.hidden}] on {at} with contiguous rows")
+    args = _ExpertsStruct(
+        a8.data_ptr(), a_scales.data_ptr(), weights.gate[0].data_ptr(), weights.up[0].data_ptr(), weights.down[0].data_ptr(),
+        weights.gate[1].data_ptr(), weights.up[1].data_ptr(), weights.down[1].data_ptr(), routing.weights.data_ptr(),
+        routing.plan.data_ptr(), out.data_ptr(), tokens, hip._ld(out), weights.experts, top_k, weights.hidden,
+        weights.hidden_pad, weights.ffn, weights.ffn_pad, TYPES[out.dtype])
+    lib, ref = _lib.load(), ctypes.addressof(args)
+    with hip.on_device(at) as stream:
+        need = weights._needs.get((tokens, top_k))
+        if need is None:
+            got = ctypes.c_size_t()
+            hip._check(lib.rocknpu_hip_moe_experts_workspace(ref, ctypes.addressof(got)), "moe_experts_workspace")
+            if len(weights._needs) >= 1024:
+                weights._needs.clear()
+            need = weights._needs[tokens, top_k] = got.value
+        ws, nbytes = None, 0
+        if need:
+            if workspace is None:
+                workspace = workspace_for(at, need)
+            elif workspace.device != at or not workspace.is_contiguous():
+                raise ValueError(f"workspace has to be a contiguous tensor on {at}")
+            ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        hip._check(lib.rocknpu_hip_moe_experts(ref, ws, nbytes, stream), "moe_experts")
+    return out

@@ -50,3 +50,40 @@ def route(logits, top_k, *, score="softmax", bias=None, groups=1, top_groups=Non
         at += len(mine)
         offsets[e + 1] = at
     return ids, weights, offsets, order
+
+
+def a8(v):
+    """Codes and scales of the rows of v (f32) by rocknpu_hip_quantize_a8's definition."""
+    v = v.astype(np.float32)
+    fine = np.isfinite(v).all(1) if v.shape[1] else np.ones(len(v), bool)
+    v = np.where(fine[:, None], v, np.float32(0))
+    peak = np.abs(v).max(1)
+    step = np.where(peak == 0, np.float32(1), peak / np.float32(127)).astype(np.float32)
+    q = (v / step[:, None]).astype(np.float64)
+    codes = np.clip(np.copysign(np.floor(np.abs(q) + 0.5), q), -127, 127)
+    return codes, np.where(fine, step, np.float32(np.nan))
+
+
+def product(a, sa, w, sw):
+    """(f32(sum) * row's scale) * column's scale, each in f32."""
+    with np.errstate(all="ignore"):
+        return ((a @ w.T).astype(np.float32) * sa[:, None].astype(np.float32)) * sw[None].astype(np.float32)
+
+
+def experts(codes, scales, ids, weights, gate, up, down, hidden, ffn):
+    """(out, the sum of its terms' magnitudes), 64 bits [tokens, hidden]; codes, scales and the pairs as moe.experts takes them."""
+    c, sc = codes.cpu().numpy().astype(np.float64), scales.cpu().numpy()
+    g, sg, u, su, d, sd = (x.cpu().numpy() for pair in (gate, up, down) for x in pair)
+    out, size = np.zeros((c.shape[0], hidden)), np.zeros((c.shape[0], hidden))
+    with np.errstate(all="ignore"):
+        for e in range(g.shape[0]):
+            t, s = np.nonzero(ids == e)
+            if not len(t):
+                continue
+            x = product(c[t], sc[t], g[e].astype(np.float64), sg[e]).astype(np.float64)
+            y = product(c[t], sc[t], u[e].astype(np.float64), su[e]).astype(np.float64)
+            v, sv = a8((x * y / (1.0 + np.exp(-x))).astype(np.float32))
+            r = product(v, sv, d[e][:, :ffn].astype(np.float64), sd[e]).astype(np.float64) * weights[t, s][:, None].astype(np.float64)
+            np.add.at(out, t, r)
+            np.add.at(size, t, np.abs(r))
+    return out, size

@@ -75,7 +75,7 @@ def test_the_plain_form():
 
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not installed")
-@pytest.mark.parametrize("name,struct", [("rocknpu_moe_route_args", moe._RouteStruct)], ids=str)
+@pytest.mark.parametrize("name,struct", [("rocknpu_moe_route_args", moe._RouteStruct), ("rocknpu_moe_experts_args", moe._ExpertsStruct)], ids=str)
 def test_struct_layouts(name, struct, tmp_path):
     fields = [f for f, _ in struct._fields_]
     src = tmp_path / "layout.c"
@@ -85,3 +85,52 @@ def test_struct_layouts(name, struct, tmp_path):
     subprocess.run(["gcc", "-std=c99", f"-I{ROOT / 'include'}", str(src), "-o", str(tmp_path / "layout")], check=True)
     got = [int(v) for v in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [ctypes.sizeof(struct)] + [getattr(struct, f).offset for f in fields]
+
+
+def experts_struct(**kw):
+    names = ("a8", "a_scales", "gate", "up", "down", "gate_scales", "up_scales", "down_scales", "weights", "plan", "out")
+    base = dict.fromkeys(names, AT) | dict(tokens=5, out_row=100, experts=8, top_k=2, hidden=100, hidden_pad=128, ffn=60, ffn_pad=64, out_type=0)
+    return moe._ExpertsStruct(**{**base, **kw})
+
+
+@pytest.mark.parametrize("bad", [
+    *(dict([(n, 0)]) for n, _ in moe._ExpertsStruct._fields_[:11]), *(dict([(n, AT + 8)]) for n in ("a8", "gate", "up", "down")),
+    *(dict([(n, AT + 2)]) for n in ("a_scales", "gate_scales", "up_scales", "down_scales", "weights", "plan", "out")), dict(out_type=2, out=AT + 1),
+    dict(out_type=3), dict(tokens=-1), dict(tokens=1 << 28), dict(out_row=-1), dict(out_row=99), dict(experts=0), dict(experts=1025), dict(top_k=0),
+    dict(top_k=9), dict(hidden=0), dict(hidden=129), dict(hidden_pad=120), dict(hidden_pad=0), dict(hidden_pad=133184), dict(ffn=0), dict(ffn=65),
+    dict(ffn_pad=100), dict(ffn_pad=133184), dict(workspace=0), dict(workspace=AT + 16), dict(short=1)], ids=str)
+def test_refused_experts(bad):
+    lib, need = _lib.load(), ctypes.c_size_t()
+    assert lib.rocknpu_hip_moe_experts_workspace(ctypes.byref(experts_struct()), ctypes.byref(need)) == 0
+    bad = dict(bad)
+    ws, short = bad.pop("workspace", AT), bad.pop("short", 0)
+    assert lib.rocknpu_hip_moe_experts(ctypes.byref(experts_struct(**bad)), ws, need.value - short, None) == -1
+
+
+def test_experts_without_tokens_or_arguments():
+    lib, need = _lib.load(), ctypes.c_size_t()
+    assert lib.rocknpu_hip_moe_experts(None, None, 0, None) == -1
+    assert lib.rocknpu_hip_moe_experts_workspace(None, ctypes.byref(need)) == -1
+    assert lib.rocknpu_hip_moe_experts_workspace(ctypes.byref(experts_struct()), None) == -1
+    assert lib.rocknpu_hip_moe_experts(ctypes.byref(experts_struct(tokens=0, a8=0, a_scales=0, out=0)), None, 0, None) == 0
+
+
+def test_refused_experts_in_python():
+    i8 = lambda *s: torch.zeros(s, dtype=torch.int8)  # noqa: E731
+    f = torch.zeros
+    good = dict(gate=(i8(4, 60, 128), f(4, 60)), up=(i8(4, 60, 128), f(4, 60)), down=(i8(4, 100, 64), f(4, 100)), hidden=100, ffn=60)
+    w = moe.Experts(**good)
+    for kw in (dict(gate=(i8(60, 128), f(60))), dict(gate=(i8(4, 60, 120), f(4, 60))), dict(up=(i8(4, 61, 128), f(4, 61))), dict(up=(i8(4, 60, 192), f(4, 60))),
+               dict(up=(f(4, 60, 128), f(4, 60))), dict(up=(i8(4, 60, 128), f(4, 60).double())), dict(up=(i8(4, 60, 128), f(240))), dict(down=(i8(4, 100, 50), f(4, 100))),
+               dict(down=(i8(4, 101, 64), f(4, 101))), dict(hidden=0), dict(hidden=129), dict(ffn=0), dict(ffn=59), dict(gate=(i8(1025, 1, 64), f(1025, 1)), ffn=1, hidden=1),
+               dict(gate=(i8(4, 128, 60).transpose(1, 2), f(4, 60)))):
+        with pytest.raises(ValueError):
+            moe.Experts(**{**good, **kw})
+    r = moe.Routing(torch.zeros((3, 2), dtype=torch.int32), f(3, 2), torch.zeros(100, dtype=torch.int32), 4)
+    args = dict(weights=w, a8=i8(3, 128), a_scales=f(3), routing=r)
+    for kw in (dict(a8=i8(2, 128)), dict(a8=i8(3, 64)), dict(a8=f(3, 128)), dict(a8=i8(128, 3).T), dict(a_scales=f(2)), dict(a_scales=f(3).double()),
+               dict(routing=moe.Routing(r.ids, r.weights, r.plan, 5)), dict(dtype=torch.float64), dict(out=f(3, 99)), dict(out=f(3, 100).double()),
+               dict(out=f(100, 3).T), {}):
+        a = {**args, **kw}
+        with pytest.raises(ValueError):
+            moe.experts(a.pop("weights"), a.pop("a8"), a.pop("a_scales"), a.pop("routing"), **a)

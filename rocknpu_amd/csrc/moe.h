@@ -28,9 +28,7 @@ constexpr int kMoeCountThreads = 1024;
 
 // Rows of a product's tile.
 inline int moe_tile_rows(int64_t rows, int experts) {
-    (void)rows;
-    (void)experts;
-    return 64;
+    return rows >= static_cast<int64_t>(96) * experts ? 256 : 64;
 }
 
 // The plan of such a call at `base` (which may be null), and its words.

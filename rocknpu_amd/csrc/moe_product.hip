@@ -1,0 +1,318 @@
+// The experts' W8A8 products: grouped by the routing's plan, gate and up in one
+// pass with SwiGLU.
+//
+// out[r][c] = (f32(sum_k A[row of r][k] * W[e][c][k]) * a_scale) * w_scale for
+// every row r in order of expert (e is its expert), or for gate and up together
+// out[r][c] = f32(g * u / (1 + exp(-g))). Sums are exact int32.
+//
+// Tiling, stages and waits are gemm.hip's: BM x BN tiles of 32x32 fragments of
+// v_mfma_i32_32x32x32_i8, operands through LDS stage buffers that direct loads
+// fill. What differs:
+//   - A workgroup takes a tile of the plan: up to BM rows of one expert. For gate
+//     and up the rows are gathered: each lane's source addresses are looked up
+//     once, the direct loads take any.
+//   - An expert's last tile has fewer rows. Rows are dealt to the WM waves of a
+//     column by fragments of 32 in turn, so a tile of at most BM' rows runs as a
+//     BM' x BN tile on the same buffers: fewer loads, reads and products.
+//   - Gate's and up's columns alternate by fragments of 32 in a tile, so a lane
+//     holds g and u of the same output, and no pass over [rows][2 ffn] follows.
+#include "gemm_dma.h"
+#include "moe.h"
+#include "moe_product.h"
+
+namespace rk {
+namespace {
+
+// f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, to 2^-50 of the value:
+// exp(-g) = 2^n 2^r with n = rint(-g log2(e)), |r| <= 1/2 in two parts of log2(e),
+// 2^r by the polynomial through its values at the 11 Chebyshev nodes of [-1/2, 1/2]
+// (off by 2^-51.5 at most), the division by the reciprocal's Newton step and one
+// of the quotient. -g log2(e) is held to 2^1000, where the value is 0 in f32.
+__device__ __forceinline__ float swiglu(float gate, float up) {
+    const double g = static_cast<double>(gate), x = g * static_cast<double>(up);
+    const double a = fmin(fmax(g * -0x1.71547652b82fep+0, -1000.0), 1000.0);
+    const double n = rint(a);
+    double r = fma(g, -0x1.71547652b82fep+0, -n);
+    r = fma(g, -0x1.777d0ffda0d24p-56, r);
+    r = fmin(fmax(r, -0.5001), 0.5001);  // where a was held
+    double p = 0x1.e6063f7217bc6p-28;
+    p = fma(p, r, 0x1.b675bca4eeebbp-24);
+    p = fma(p, r, 0x1.62bfd47773353p-20);
+    p = fma(p, r, 0x1.ffcb54062e698p-17);
+    p = fma(p, r, 0x1.430913096fd9fp-13);
+    p = fma(p, r, 0x1.5d87fe9d7a584p-10);
+    p = fma(p, r, 0x1.3b2ab6fba1ddap-7);
+    p = fma(p, r, 0x1.c6b08d703ce49p-5);
+    p = fma(p, r, 0x1.ebfbdff82c598p-3);
+    p = fma(p, r, 0x1.62e42fefa3a19p-1);
+    p = fma(p, r, 1.0);
+    const double d = 1.0 + ldexp(p, static_cast<int>(n));
+    double y = __builtin_amdgcn_rcp(d);
+    y = fma(fma(-d, y, 1.0), y, y);
+    const double q = x * y;
+    return static_cast<float>(fma(fma(-d, q, x), y, q));
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// One tile: rows r0 .. end - 1 (at most BME) of the plan's order, expert e, output
+// columns from c0. `stages(A?, stage)` names the stage buffers, distinct arrays, so
+// that a wait for one does not wait for all.
+template <int BME, int BN, int WM, int WN, int ST, int KB, bool GATED, typename SA, typename SB>
+__device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t* __restrict__ order, int rows, int e, int r0,
+                                             int end, int c0, SA stage_a, SB stage_b, float* lsc) {
+    using Cfg = DmaTile<BME, BN, WM, WN, KB>;
+    constexpr int TN = BN / WN, FM = BME / WM / 32, FN = TN / 32;
+    constexpr int SUB = KB / 64, CPR = KB / 16, THREADS = WM * WN * 64;
+    static_assert(FM * WM * 32 == BME && FN * WN * 32 == BN && (!GATED || FN % 2 == 0), "whole fragments, gate's and up's in pairs");
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int k = p.k;
+    // the row of A behind tile row r: rows past the tile re-read its last one
+    const auto source = [&](int r) {
+        const int at = min(r0 + r, end - 1);
+        return GATED ? min(max(order[at], 0), rows - 1) / p.top_k : at;
+    };
+    // the row of W (of which matrix) behind tile column c; columns past the matrix re-read its last one
+    const auto column = [&](int c) { return min(c0 + (GATED ? (c >> 6) * 32 + (c & 31) : c), p.n - 1); };
+    const int64_t first = static_cast<int64_t>(e) * p.n;
+
+    // Addresses of the direct loads: a base that is the same for the wave and 32 bits
+    // a lane (half the registers and none of the additions of 64-bit pointers). A
+    // segment's rows lie in one fragment, so in one matrix.
+    const int8_t* abase = GATED ? p.a : p.a + static_cast<int64_t>(r0) * k;
+    const int8_t* bbase[Cfg::B_SEG];
+    uint32_t aoff[Cfg::A_SEG], boff[Cfg::B_SEG];
+#pragma unroll
+    for (int q = 0; q < Cfg::A_SEG; ++q) {
+        const int r = ((wave * Cfg::A_SEG + q) % Cfg::A_ROWSEG) * Cfg::RPI + lane / CPR;
+        const int c = (lane % CPR) ^ ((r >> 1) & (CPR - 1));
+        aoff[q] = static_cast<uint32_t>(source(r) - (GATED ? 0 : r0)) * static_cast<uint32_t>(k) + c * 16;
+    }
+#pragma unroll
+    for (int q = 0; q < Cfg::B_SEG; ++q) {
+        const int r0q = ((wave * Cfg::B_SEG + q) % Cfg::B_ROWSEG) * Cfg::RPI, r = r0q + lane / CPR;
+        const int c = (lane % CPR) ^ ((r >> 1) & (CPR - 1));
+        bbase[q] = (GATED && (r0q & 32) ? p.w[1] : p.w[0]) + (first + c0) * k;
+        boff[q] = static_cast<uint32_t>(column(r) - c0) * static_cast<uint32_t>(k) + c * 16;
+    }
+    auto issue = [&](auto st, int ks) {
+        int8_t* la = stage_a(st);
+        int8_t* lb = stage_b(st);
+        const int at = ks * KB;
+#pragma unroll
+        for (int q = 0; q < Cfg::A_SEG; ++q)
+            dma16(abase + at + aoff[q], la + ((wave * Cfg::A_SEG + q) % Cfg::A_ROWSEG) * 1024);
+#pragma unroll
+        for (int q = 0; q < Cfg::B_SEG; ++q)
+            dma16(bbase[q] + at + boff[q], lb + ((wave * Cfg::B_SEG + q) % Cfg::B_ROWSEG) * 1024);
+    };
+
+    v16i acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = v16i{};
+
+    const int KS = k / KB;  // stages
+    const int KT = k / 64;  // 64-deep steps
+    using S0 = std::integral_constant<int, 0>;
+    using H0 = std::integral_constant<int, 0>;
+    using H1 = std::integral_constant<int, 1>;
+    using R0 = std::integral_constant<int, 0>;
+    constexpr int PER_STAGE = Cfg::A_SEG + Cfg::B_SEG;
+    v4i fa[2][2][FM], fb[2][2][FN];  // [register set][32-deep half][fragment]
+    // lane l supplies row l % 32 and the 16 bytes of chunk 4 u + 2 h + l / 32; fragment i of
+    // wave column wm holds tile rows 32 (WM i + wm) ..
+    auto read_half = [&](auto st, auto set, auto u, auto h) {
+        constexpr int R = decltype(set)::value, H = decltype(h)::value, SU = decltype(u)::value;
+        const int8_t* la = stage_a(st);
+        const int8_t* lb = stage_b(st);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            fa[R][H][i] = *reinterpret_cast<const v4i*>(la + swz_kb<KB>((i * WM + wm) * 32 + (lane & 31), 4 * SU + 2 * H + half));
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            fb[R][H][j] = *reinterpret_cast<const v4i*>(lb + swz_kb<KB>(wn * TN + j * 32 + (lane & 31), 4 * SU + 2 * H + half));
+    };
+    auto read_frags = [&](auto st, auto set, auto u) {
+        read_half(st, set, u, H0{});
+        read_half(st, set, u, H1{});
+    };
+    auto mfma_half = [&](auto set, auto h) {
+        constexpr int R = decltype(set)::value, H = decltype(h)::value;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[R][H][i], fb[R][H][j], acc[i][j], 0, 0, 0);
+    };
+    // The tile's scales: each thread loads one or two before the stages (older than
+    // their loads, so the waits' counts hold) and writes them to LDS once the first
+    // stage has landed; the loop's barriers publish them.
+    constexpr int NSC = BME + BN, SCP = (NSC + THREADS - 1) / THREADS;
+    float scv[SCP];
+#pragma unroll
+    for (int u = 0; u < SCP; ++u) {
+        const int idx = threadIdx.x + u * THREADS, c = min(idx, NSC - 1) - BME;
+        const float* sc = idx < BME ? p.a_scales + source(idx) : (GATED && (c & 32) ? p.w_scales[1] : p.w_scales[0]) + first + column(c);
+        scv[u] = *sc;
+    }
+    // prologue: stages 0 .. ST-2 in flight, wait for stage 0, then stage ST-1
+    unroll_seq([&](auto i) { issue(i, min(static_cast<int>(decltype(i)::value), KS - 1)); }, std::make_integer_sequence<int, ST - 1>{});
+    wait_vm<(ST - 2) * PER_STAGE>();
+#pragma unroll
+    for (int u = 0; u < SCP; ++u) {
+        const int idx = threadIdx.x + u * THREADS;
+        if (idx < NSC) lsc[idx] = scv[u];
+    }
+    __builtin_amdgcn_s_barrier();
+    issue(std::integral_constant<int, ST - 1>{}, min(ST - 1, KS - 1));
+    read_frags(S0{}, R0{}, S0{});
+    // One 64-deep step, as in gemm.hip: the fragments of step j were read in step j-1;
+    // the last step of a stage waits for the next one, passes the barrier that frees
+    // the stage's buffer, and refills it.
+    auto step = [&](auto set, auto next_st, auto next_u, auto refill_st, auto last_of_stage, int q) {
+        using NSET = std::integral_constant<int, 1 - decltype(set)::value>;
+        constexpr bool LAST = decltype(last_of_stage)::value;
+        wait_lgkm0();
+        if constexpr (LAST) {
+            wait_vm<(ST - 2) * PER_STAGE>();
+            __builtin_amdgcn_s_barrier();
+            issue(refill_st, min(q + ST, KS - 1));
+        }
+        read_frags(next_st, NSET{}, next_u);
+        mfma_half(set, H0{});
+        mfma_half(set, H1{});
+        constexpr int READS = 2 * (FM + FN), MFMAS = 2 * FM * FN;
+        if constexpr (LAST && READS % PER_STAGE == 0 && MFMAS % PER_STAGE == 0) {
+#pragma unroll
+            for (int i = 0; i < PER_STAGE; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                  // VMEM read (direct load)
+                __builtin_amdgcn_sched_group_barrier(0x100, READS / PER_STAGE, 0);  // DS read
+                __builtin_amdgcn_sched_group_barrier(0x008, MFMAS / PER_STAGE, 0);  // MFMA
+            }
+        } else if constexpr (!LAST && MFMAS % READS == 0) {
+#pragma unroll
+            for (int i = 0; i < READS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);              // DS read
+                __builtin_amdgcn_sched_group_barrier(0x008, MFMAS / READS, 0);  // MFMA
+            }
+        }
+    };
+    auto step_i = [&](auto i, int kt) {
+        constexpr int I = decltype(i)::value;
+        step(std::integral_constant<int, I % 2>{}, std::integral_constant<int, ((I + 1) / SUB) % ST>{},
+             std::integral_constant<int, (I + 1) % SUB>{}, std::integral_constant<int, (I / SUB) % ST>{},
+             std::integral_constant<bool, (I + 1) % SUB == 0>{}, (kt + I) / SUB);
+    };
+    constexpr int U = (ST * SUB) % 2 == 0 ? ST * SUB : 2 * ST * SUB;
+    const int KTA = KT - KT % U;
+    for (int kt = 0; kt < KTA; kt += U) unroll_seq([&](auto i) { step_i(i, kt); }, std::make_integer_sequence<int, U>{});
+    unroll_seq([&](auto i) { if (KTA + decltype(i)::value < KT) step_i(i, KTA); }, std::make_integer_sequence<int, U - 1>{});
+    wait_vm<0>();  // no direct load is in flight when the workgroup's LDS is given back
+    wait_lgkm0();
+
+    // Epilogue. lane l holds column l % 32 of each fragment, rows (i % 4) + 4 (l / 32) +
+    // 8 (i / 4): a store is two whole runs of 128 bytes.
+    constexpr int STEP = GATED ? 2 : 1;
+#pragma unroll
+    for (int j = 0; j < FN; j += STEP) {
+        const int tc = wn * TN + j * 32 + (lane & 31);
+        const int col = c0 + (GATED ? (tc >> 6) * 32 + (tc & 31) : tc);
+        const float ws0 = lsc[BME + tc], ws1 = GATED ? lsc[BME + tc + 32] : 0.0f;
+        if (col >= p.n) continue;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int r = (i * WM + wm) * 32 + (x & 3) + 4 * half + 8 * (x >> 2);
+                const float as = lsc[r];
+                float v = (static_cast<float>(acc[i][j][x]) * as) * ws0;
+                if constexpr (GATED) v = swiglu(v, (static_cast<float>(acc[i][j + STEP - 1][x]) * as) * ws1);
+                if (r0 + r < end) p.out[static_cast<int64_t>(r0 + r) * p.n + col] = v;
+            }
+        }
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
+__global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p, const MoePlan plan) {
+    static_assert(ST >= 2 && ST <= 4, "two to four stage buffers");
+    __shared__ __align__(16) int8_t la0[BM * KB], la1[BM * KB], la2[ST > 2 ? BM * KB : 16], la3[ST > 3 ? BM * KB : 16];
+    __shared__ __align__(16) int8_t lb0[BN * KB], lb1[BN * KB], lb2[ST > 2 ? BN * KB : 16], lb3[ST > 3 ? BN * KB : 16];
+    __shared__ float lsc[BM + BN];
+    auto stage_a = [&](auto st) -> int8_t* {
+        constexpr int S = decltype(st)::value;
+        if constexpr (S == 0) return la0; else if constexpr (S == 1) return la1;
+        else if constexpr (S == 2) return la2; else return la3;
+    };
+    auto stage_b = [&](auto st) -> int8_t* {
+        constexpr int S = decltype(st)::value;
+        if constexpr (S == 0) return lb0; else if constexpr (S == 1) return lb1;
+        else if constexpr (S == 2) return lb2; else return lb3;
+    };
+    // Workgroup b runs on XCD b % 8: each XCD takes a contiguous range of (row tile,
+    // column tile) pairs, in groups of 4 row tiles, which share W in its L2 where
+    // they are one expert's.
+    constexpr int BC = GATED ? BN / 2 : BN;  // output columns of a tile
+    const int tiles_m = uniform(min(*plan.tile_count, plan.max_tiles)), tiles_n = (p.n + BC - 1) / BC;
+    const int total = tiles_m * tiles_n;
+    const int bid = blockIdx.x;
+    if (bid >= total) return;
+    const int xcd = bid & 7, per = total >> 3, rem = total & 7;
+    const int t = xcd * per + min(xcd, rem) + (bid >> 3);
+    constexpr int GM = 4;
+    const int group = t / (GM * tiles_n), first_m = group * GM;
+    const int gsize = min(tiles_m - first_m, GM);
+    const int tm = first_m + (t % (GM * tiles_n)) % gsize, tn = (t % (GM * tiles_n)) / gsize;
+    const int e = uniform(min(max(plan.tiles[2 * tm], 0), plan.experts - 1));
+    const int r0 = uniform(min(max(plan.tiles[2 * tm + 1], 0), plan.rows));
+    const int end = uniform(min(min(plan.offsets[e + 1], plan.rows), r0 + BM));
+    const int n = end - r0;
+    if (n <= 0) return;
+#define RK_TILE(BME) \
+    product_tile<BME, BN, WM, WN, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, end, tn * BC, stage_a, stage_b, lsc)
+    if constexpr (BM == 256) {
+        if (n > 192) return RK_TILE(256);
+        if (n > 128) return RK_TILE(192);
+    }
+    if constexpr (BM >= 128)
+        if (n > 64) return RK_TILE(128);
+    if constexpr (BM >= 64 && WM == 1) {
+        if (n > 32) return RK_TILE(64);
+        return RK_TILE(32);
+    } else {
+        return RK_TILE(64);
+    }
+#undef RK_TILE
+}
+
+template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
+int launch(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
+    constexpr int BC = GATED ? BN / 2 : BN;
+    const int64_t grid = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
+    if (grid > 0x7fffffff) return kStatusInvalid;
+    product_kernel<BM, BN, WM, WN, ST, KB, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
+    return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
+}
+
+template <bool GATED>
+int route(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
+    // 128-byte stages need K % 128 == 0 (a stage never reads past a row)
+    if (plan.tile_rows == 256) {
+        if (p.k % 128 == 0) return launch<256, 256, 2, 2, 2, 128, GATED>(p, plan, stream);
+        return launch<256, 256, 2, 2, 4, 64, GATED>(p, plan, stream);
+    }
+    if (p.k % 128 == 0) return launch<64, 128, 1, 2, 3, 128, GATED>(p, plan, stream);
+    return launch<64, 128, 1, 2, 4, 64, GATED>(p, plan, stream);
+}
+
+}  // namespace
+
+int launch_moe_product(const MoeProduct& p, bool gated, const MoePlan& plan, hipStream_t stream) {
+    return gated ? route<true>(p, plan, stream) : route<false>(p, plan, stream);
+}
+
+}  // namespace rk

@@ -27,14 +27,14 @@ namespace {
 // exp(-g) = 2^n 2^r with n = rint(-g log2(e)), |r| <= 1/2 in two parts of log2(e),
 // 2^r by the polynomial through its values at the 11 Chebyshev nodes of [-1/2, 1/2]
 // (off by 2^-51.5 at most), the division by the reciprocal's Newton step and one
-// of the quotient. -g log2(e) is held to 2^1000, where the value is 0 in f32.
+// of the quotient. In the exponential g is held to +-693, where the value is that of
+// 1 + exp(-g) = 1, or 0 in f32.
 __device__ __forceinline__ float swiglu(float gate, float up) {
-    const double g = static_cast<double>(gate), x = g * static_cast<double>(up);
-    const double a = fmin(fmax(g * -0x1.71547652b82fep+0, -1000.0), 1000.0);
-    const double n = rint(a);
+    const double x = static_cast<double>(gate) * static_cast<double>(up);
+    const double g = static_cast<double>(__builtin_amdgcn_fmed3f(gate, -693.0f, 693.0f));
+    const double n = rint(g * -0x1.71547652b82fep+0);
     double r = fma(g, -0x1.71547652b82fep+0, -n);
     r = fma(g, -0x1.777d0ffda0d24p-56, r);
-    r = fmin(fmax(r, -0.5001), 0.5001);  // where a was held
     double p = 0x1.e6063f7217bc6p-28;
     p = fma(p, r, 0x1.b675bca4eeebbp-24);
     p = fma(p, r, 0x1.62bfd47773353p-20);
@@ -215,23 +215,35 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
     wait_lgkm0();
 
     // Epilogue. lane l holds column l % 32 of each fragment, rows (i % 4) + 4 (l / 32) +
-    // 8 (i / 4): a store is two whole runs of 128 bytes.
-    constexpr int STEP = GATED ? 2 : 1;
+    // 8 (i / 4): a store is two whole runs of 128 bytes. Eight values at a time, so that
+    // their chains of 64-bit operations overlap.
+    constexpr int STEP = GATED ? 2 : 1, X = 8;
+    float* out = p.out + static_cast<int64_t>(r0) * p.n + c0;
 #pragma unroll
     for (int j = 0; j < FN; j += STEP) {
         const int tc = wn * TN + j * 32 + (lane & 31);
-        const int col = c0 + (GATED ? (tc >> 6) * 32 + (tc & 31) : tc);
+        const int col = GATED ? (tc >> 6) * 32 + (tc & 31) : tc;
         const float ws0 = lsc[BME + tc], ws1 = GATED ? lsc[BME + tc + 32] : 0.0f;
-        if (col >= p.n) continue;
+        const int last = c0 + col < p.n ? end - r0 : 0;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const int r = (i * WM + wm) * 32 + (x & 3) + 4 * half + 8 * (x >> 2);
-                const float as = lsc[r];
-                float v = (static_cast<float>(acc[i][j][x]) * as) * ws0;
-                if constexpr (GATED) v = swiglu(v, (static_cast<float>(acc[i][j + STEP - 1][x]) * as) * ws1);
-                if (r0 + r < end) p.out[static_cast<int64_t>(r0 + r) * p.n + col] = v;
+            for (int x0 = 0; x0 < 16; x0 += X) {
+                float v[X];
+#pragma unroll
+                for (int x = 0; x < X; ++x) {
+                    const int f = x0 + x;
+                    const float as = lsc[(i * WM + wm) * 32 + (f & 3) + 4 * half + 8 * (f >> 2)];
+                    v[x] = (static_cast<float>(acc[i][j][f]) * as) * ws0;
+                    if constexpr (GATED) v[x] = swiglu(v[x], (static_cast<float>(acc[i][j + STEP - 1][f]) * as) * ws1);
+                }
+                // all of them before the first store's condition, or each would wait for its own chain
+                asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]));
+#pragma unroll
+                for (int x = 0; x < X; ++x) {
+                    const int f = x0 + x, r = (i * WM + wm) * 32 + (f & 3) + 4 * half + 8 * (f >> 2);
+                    if (r < last) out[static_cast<uint32_t>(r * p.n + col)] = v[x];
+                }
             }
         }
     }

@@ -15,7 +15,8 @@ struct MoeProduct {
     const float* w_scales[2];
     float* out;
     int n, k, top_k;
+    int xcd_cus;  // CUs of an XCD, filled in by the launch
 };
-int launch_moe_product(const MoeProduct& p, bool gated, const MoePlan& plan, hipStream_t stream);
+int launch_moe_product(MoeProduct p, bool gated, const MoePlan& plan, hipStream_t stream);
 
 }  // namespace rk

@@ -267,36 +267,54 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
     };
     // Workgroup b runs on XCD b % 8: each XCD takes a contiguous range of (row tile,
     // column tile) pairs, in groups of 4 row tiles, which share W in its L2 where
-    // they are one expert's.
+    // they are one expert's. What its CUs would run in a last round that is at most
+    // half full runs in halves (of the columns), at most a quarter full in quarters.
     constexpr int BC = GATED ? BN / 2 : BN;  // output columns of a tile
     const int tiles_m = uniform(min(*plan.tile_count, plan.max_tiles)), tiles_n = (p.n + BC - 1) / BC;
     const int total = tiles_m * tiles_n;
-    const int bid = blockIdx.x;
-    if (bid >= total) return;
-    const int xcd = bid & 7, per = total >> 3, rem = total & 7;
-    const int t = xcd * per + min(xcd, rem) + (bid >> 3);
+    const int xcd = blockIdx.x & 7, per = total >> 3, rem = total & 7;
+    const int mine = per + (xcd < rem), rest = BM == 256 ? mine % p.xcd_cus : 0;
+    const int parts = 2 * rest > p.xcd_cus || rest == 0 ? 1 : 4 * rest > p.xcd_cus ? 2 : 4;
+    int i = blockIdx.x >> 3, part = 0;
+    if (i >= mine - rest) {
+        const int j = i - (mine - rest);
+        i = mine - rest + j / parts;
+        part = j % parts;
+    }
+    if (i >= mine) return;
+    const int t = xcd * per + min(xcd, rem) + i;
     constexpr int GM = 4;
     const int group = t / (GM * tiles_n), first_m = group * GM;
     const int gsize = min(tiles_m - first_m, GM);
     const int tm = first_m + (t % (GM * tiles_n)) % gsize, tn = (t % (GM * tiles_n)) / gsize;
     const int e = uniform(min(max(plan.tiles[2 * tm], 0), plan.experts - 1));
-    const int r0 = uniform(min(max(plan.tiles[2 * tm + 1], 0), plan.rows));
+    int r0 = uniform(min(max(plan.tiles[2 * tm + 1], 0), plan.rows));
     const int end = uniform(min(min(plan.offsets[e + 1], plan.rows), r0 + BM));
+    int c0 = tn * BC;
+    if (BM == 256 && i >= mine - rest && parts > 1) {
+        c0 += part % 2 * (BC / 2);
+        r0 += part / 2 * (BM / 2);
+        if (r0 >= end || c0 >= p.n) return;
+        const int last = parts == 4 ? min(end, r0 + BM / 2) : end, n = last - r0;
+#define RK_PART(BME) product_tile<BME, BN / 2, WM, WN, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, last, c0, stage_a, stage_b, lsc)
+        if constexpr (BM == 256) {
+            if (n > 128) return RK_PART(256);
+            if (n > 64) return RK_PART(128);
+            return RK_PART(64);
+        }
+#undef RK_PART
+    }
     const int n = end - r0;
     if (n <= 0) return;
-#define RK_TILE(BME) \
-    product_tile<BME, BN, WM, WN, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, end, tn * BC, stage_a, stage_b, lsc)
+#define RK_TILE(BME) product_tile<BME, BN, WM, WN, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, end, c0, stage_a, stage_b, lsc)
     if constexpr (BM == 256) {
         if (n > 192) return RK_TILE(256);
         if (n > 128) return RK_TILE(192);
-    }
-    if constexpr (BM >= 128)
         if (n > 64) return RK_TILE(128);
-    if constexpr (BM >= 64 && WM == 1) {
+        return RK_TILE(64);
+    } else {
         if (n > 32) return RK_TILE(64);
         return RK_TILE(32);
-    } else {
-        return RK_TILE(64);
     }
 #undef RK_TILE
 }
@@ -304,7 +322,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
 template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
 int launch(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
     constexpr int BC = GATED ? BN / 2 : BN;
-    const int64_t grid = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
+    // a split last round has up to as many workgroups as the GPU has CUs
+    int64_t grid = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
+    if (BM == 256) grid = (grid + 7) / 8 * 8 + 8 * static_cast<int64_t>(p.xcd_cus);
     if (grid > 0x7fffffff) return kStatusInvalid;
     product_kernel<BM, BN, WM, WN, ST, KB, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
@@ -323,7 +343,8 @@ int route(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
 
 }  // namespace
 
-int launch_moe_product(const MoeProduct& p, bool gated, const MoePlan& plan, hipStream_t stream) {
+int launch_moe_product(MoeProduct p, bool gated, const MoePlan& plan, hipStream_t stream) {
+    p.xcd_cus = device_cu_count() >= 8 ? device_cu_count() / 8 : 1;
     return gated ? route<true>(p, plan, stream) : route<false>(p, plan, stream);
 }
 

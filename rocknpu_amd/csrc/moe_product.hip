@@ -55,6 +55,8 @@ __device__ __forceinline__ float swiglu(float gate, float up) {
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+constexpr int kMoeManyTiles = 64;
+
 // One tile: rows r0 .. end - 1 (at most BME) of the plan's order, expert e, output
 // columns from c0. `stages(A?, stage)` names the stage buffers, distinct arrays, so
 // that a wait for one does not wait for all.
@@ -265,15 +267,22 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
         if constexpr (S == 0) return lb0; else if constexpr (S == 1) return lb1;
         else if constexpr (S == 2) return lb2; else return lb3;
     };
-    // Workgroup b runs on XCD b % 8: each XCD takes a contiguous range of (row tile,
-    // column tile) pairs, in groups of 4 row tiles, which share W in its L2 where
-    // they are one expert's. What its CUs would run in a last round that is at most
-    // half full runs in halves (of the columns), at most a quarter full in quarters.
+    // Workgroup b runs on XCD b % 8, which walks its share of the (row tile, column
+    // tile) pairs in groups of 4 row tiles: they share W in its L2 where they are one
+    // expert's, and their A over the columns. With many row tiles a share is a
+    // contiguous range; with few, in which a range's full and partly filled tiles
+    // would not even out, an eighth of the columns of every row tile (and a range of
+    // the columns that are left over). What an XCD's CUs would run in a last round
+    // that is at most half full runs in halves (of the columns), at most a quarter
+    // full in quarters.
     constexpr int BC = GATED ? BN / 2 : BN;  // output columns of a tile
+    constexpr int GM = 4;
     const int tiles_m = uniform(min(*plan.tile_count, plan.max_tiles)), tiles_n = (p.n + BC - 1) / BC;
-    const int total = tiles_m * tiles_n;
-    const int xcd = blockIdx.x & 7, per = total >> 3, rem = total & 7;
-    const int mine = per + (xcd < rem), rest = BM == 256 ? mine % p.xcd_cus : 0;
+    const int xcd = blockIdx.x & 7;
+    const int eighth = tiles_m < kMoeManyTiles ? tiles_n >> 3 : 0;  // columns of each XCD's own
+    const int own = eighth * tiles_m, shared = (tiles_n - 8 * eighth) * tiles_m;
+    const int per = shared >> 3, rem = shared & 7;
+    const int mine = own + per + (xcd < rem), rest = BM == 256 ? mine % p.xcd_cus : 0;
     const int parts = 2 * rest > p.xcd_cus || rest == 0 ? 1 : 4 * rest > p.xcd_cus ? 2 : 4;
     int i = blockIdx.x >> 3, part = 0;
     if (i >= mine - rest) {
@@ -282,11 +291,13 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
         part = j % parts;
     }
     if (i >= mine) return;
-    const int t = xcd * per + min(xcd, rem) + i;
-    constexpr int GM = 4;
-    const int group = t / (GM * tiles_n), first_m = group * GM;
+    const bool is_own = i < own;
+    const int wide = is_own ? eighth : tiles_n - 8 * eighth;
+    const int t = is_own ? i : xcd * per + min(xcd, rem) + i - own;
+    const int group = t / (GM * wide), first_m = group * GM;
     const int gsize = min(tiles_m - first_m, GM);
-    const int tm = first_m + (t % (GM * tiles_n)) % gsize, tn = (t % (GM * tiles_n)) / gsize;
+    const int tm = first_m + (t % (GM * wide)) % gsize;
+    const int tn = (t % (GM * wide)) / gsize + (is_own ? xcd * eighth : 8 * eighth);
     const int e = uniform(min(max(plan.tiles[2 * tm], 0), plan.experts - 1));
     int r0 = uniform(min(max(plan.tiles[2 * tm + 1], 0), plan.rows));
     const int end = uniform(min(min(plan.offsets[e + 1], plan.rows), r0 + BM));
@@ -323,8 +334,8 @@ template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
 int launch(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
     constexpr int BC = GATED ? BN / 2 : BN;
     // a split last round has up to as many workgroups as the GPU has CUs
-    int64_t grid = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
-    if (BM == 256) grid = (grid + 7) / 8 * 8 + 8 * static_cast<int64_t>(p.xcd_cus);
+    const int64_t tiles = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
+    const int64_t grid = (tiles + 7) / 8 * 8 + 8 + (BM == 256 ? 8 * static_cast<int64_t>(p.xcd_cus) : 0);
     if (grid > 0x7fffffff) return kStatusInvalid;
     product_kernel<BM, BN, WM, WN, ST, KB, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;

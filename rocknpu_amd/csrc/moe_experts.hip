@@ -8,19 +8,57 @@
 namespace rk {
 namespace {
 
-// out[t] = sum over the token's choices of weight * row.
-template <typename T>
+// out[t] = sum over the token's choices, in their order, of weight * row. Bound by
+// memory: top_k rows are read for each that is written. A thread takes V columns
+// of a token and asks for four choices' rows before it adds them up.
+template <typename T, int V>
 __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ rows, const float* __restrict__ weights,
-                                                      const MoePlan plan, int hidden, T* __restrict__ out, int64_t out_row) {
-    const int t = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
+                                                      const int32_t* __restrict__ place, int top_k, int hidden, int n_rows,
+                                                      T* __restrict__ out, int64_t out_row) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const int64_t t = blockIdx.x;
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
     if (c >= hidden) return;
-    float sum = 0.0f;
-    for (int s = 0; s < plan.top_k; ++s) {
-        const int i = t * plan.top_k + s, at = plan.place[i];
-        if (at < 0 || at >= plan.rows) continue;
-        sum += weights[i] * rows[static_cast<int64_t>(at) * hidden + c];
+    place += t * top_k;
+    weights += t * top_k;
+    float sum[V] = {};
+    for (int s0 = 0; s0 < top_k; s0 += 4) {
+        vec v[4];
+        float w[4];
+        bool used[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = min(s0 + i, top_k - 1), at = place[s];
+            used[i] = s0 + i < top_k && at >= 0 && at < n_rows;
+            w[i] = weights[s];
+            v[i] = *reinterpret_cast<const vec*>(rows + static_cast<int64_t>(used[i] ? at : 0) * hidden + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (used[i])
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] += w[i] * reinterpret_cast<const float*>(&v[i])[e];
     }
-    out[t * out_row + c] = static_cast<T>(sum);
+    struct alignas(sizeof(T) * V) Out {
+        T e[V];
+    } o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.e[e] = static_cast<T>(sum[e]);
+    *reinterpret_cast<Out*>(out + t * out_row + c) = o;
+}
+
+template <typename T>
+int launch_combine(const float* rows, const float* weights, const MoePlan& plan, int64_t tokens, int hidden, void* out,
+                   int64_t out_row, hipStream_t stream) {
+    T* o = static_cast<T*>(out);
+    const bool vec = hidden % 4 == 0 && out_row % 4 == 0 && reinterpret_cast<uintptr_t>(o) % (4 * sizeof(T)) == 0;
+    const int cols = vec ? hidden / 4 : hidden, nt = std::min(256, (cols + 63) / 64 * 64);
+    const dim3 grid(static_cast<unsigned>(tokens), (cols + nt - 1) / nt);
+    if (vec)
+        combine_kernel<T, 4><<<grid, nt, 0, stream>>>(rows, weights, plan.place, plan.top_k, hidden, plan.rows, o, out_row);
+    else
+        combine_kernel<T, 1><<<grid, nt, 0, stream>>>(rows, weights, plan.place, plan.top_k, hidden, plan.rows, o, out_row);
+    return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -85,12 +123,7 @@ extern "C" int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args* args, voi
     const MoeProduct second{codes, scales, {a.down, nullptr}, {a.down_scales, nullptr}, values, a.hidden, a.ffn_pad, a.top_k};
     st = launch_moe_product(second, false, plan, s);
     if (st != kStatusOk) return st;
-    const dim3 grid(static_cast<unsigned>(a.tokens), (a.hidden + 255) / 256);
-    if (a.out_type == ROCKNPU_TYPE_F32)
-        combine_kernel<<<grid, 256, 0, s>>>(values, a.weights, plan, a.hidden, static_cast<float*>(a.out), a.out_row);
-    else if (a.out_type == ROCKNPU_TYPE_F16)
-        combine_kernel<<<grid, 256, 0, s>>>(values, a.weights, plan, a.hidden, static_cast<_Float16*>(a.out), a.out_row);
-    else
-        combine_kernel<<<grid, 256, 0, s>>>(values, a.weights, plan, a.hidden, static_cast<__bf16*>(a.out), a.out_row);
-    return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
+    if (a.out_type == ROCKNPU_TYPE_F32) return launch_combine<float>(values, a.weights, plan, a.tokens, a.hidden, a.out, a.out_row, s);
+    if (a.out_type == ROCKNPU_TYPE_F16) return launch_combine<_Float16>(values, a.weights, plan, a.tokens, a.hidden, a.out, a.out_row, s);
+    return launch_combine<__bf16>(values, a.weights, plan, a.tokens, a.hidden, a.out, a.out_row, s);
 }

@@ -5,6 +5,8 @@
 #include "common.h"
 #include "rocknpu_moe.h"
 
+#include <algorithm>
+
 namespace rk {
 
 // A plan's parts, all int32. `tiles` lists the products' row tiles, two words
@@ -20,7 +22,7 @@ struct MoePlan {
     int32_t* counts;      // [blocks][experts]
     int rows, experts, top_k;
     int tile_rows, max_tiles;
-    int block, blocks;  // entries of a counting block (a multiple of 64), and blocks
+    int block, blocks;  // choices of a counting block, and blocks
 };
 
 constexpr int kMoeHeader = 16;
@@ -39,10 +41,10 @@ inline MoePlan moe_plan(int64_t tokens, int experts, int top_k, int32_t* base, s
     p.top_k = top_k;
     p.tile_rows = moe_tile_rows(p.rows, experts);
     p.max_tiles = p.rows / p.tile_rows + (p.rows < experts ? p.rows : experts);
-    // at most 64 blocks: every one reads all blocks' counts
-    p.block = (p.rows + 63) / 64;
-    p.block = p.block < 4096 ? 4096 : (p.block + kMoeCountThreads - 1) / kMoeCountThreads * kMoeCountThreads;
-    p.blocks = (p.rows + p.block - 1) / p.block;
+    // 64 tokens a counting block, more where that would be over 256 blocks
+    const int64_t per_block = 64 * std::max<int64_t>((tokens + 64 * 256 - 1) / (64 * 256), 1);
+    p.block = static_cast<int>(per_block * top_k);
+    p.blocks = static_cast<int>((tokens + per_block - 1) / per_block);
     size_t at = 0;
     const auto take = [&](size_t n) {
         int32_t* q = base ? base + at : nullptr;

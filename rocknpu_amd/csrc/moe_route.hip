@@ -3,7 +3,10 @@
 //
 // The ranking is in 64 bits: scores that differ by less than an f32's last place
 // are common among hundreds of experts, and ids have to be the same whoever
-// computes them.
+// computes them. That is route_token, a wave a token. Most tokens need none of it:
+// route_rows ranks by 24-bit whole numbers, 16 lanes a token, notices every token
+// whose choice its rounding could have turned, and hands those to route_token
+// (16384 tokens over 256 experts in groups: 65 us by route_token alone).
 #include "moe.h"
 
 #include <algorithm>
@@ -14,7 +17,67 @@ namespace {
 
 constexpr double kNone = -__builtin_inf();
 
-__device__ __forceinline__ double shfl_xor(double v, int o) { return __shfl_xor(v, o, 64); }
+// The same 16 lanes get the result of these.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = max(v, dpp<0xB1>(v));   // lanes 1 0 3 2
+    v = max(v, dpp<0x4E>(v));   // lanes 2 3 0 1
+    v = max(v, dpp<0x141>(v));  // mirrored within 8
+    return max(v, dpp<0x140>(v));
+}
+__device__ __forceinline__ float dpp_max(float v, uint32_t o) { return fmaxf(v, __uint_as_float(o)); }
+__device__ __forceinline__ float row_max(float v) {
+    v = dpp_max(v, dpp<0xB1>(__float_as_uint(v)));
+    v = dpp_max(v, dpp<0x4E>(__float_as_uint(v)));
+    v = dpp_max(v, dpp<0x141>(__float_as_uint(v)));
+    return dpp_max(v, dpp<0x140>(__float_as_uint(v)));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    v += __uint_as_float(dpp<0xB1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x4E>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x141>(__float_as_uint(v)));
+    return v + __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    const uint64_t b = __double_as_longlong(v);
+    return __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(dpp<CTRL>(static_cast<uint32_t>(b >> 32))) << 32 |
+                                                     dpp<CTRL>(static_cast<uint32_t>(b))));
+}
+__device__ __forceinline__ double row_sum(double v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    return v + dpp<0x140>(v);
+}
+// How many of the row's other lanes hold more.
+template <int R>
+__device__ __forceinline__ void count_above(uint32_t v, int& n) {
+    n += dpp<0x120 + R>(v) > v;  // row_ror
+    if constexpr (R < 15) count_above<R + 1>(v, n);
+}
+
+__device__ __forceinline__ double read_lane(double v, int lane) {
+    const uint64_t b = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
+    return __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+// Every lane gets the wave's.
+__device__ __forceinline__ double wave_max(double v) {
+    v = fmax(v, dpp<0xB1>(v));
+    v = fmax(v, dpp<0x4E>(v));
+    v = fmax(v, dpp<0x141>(v));
+    v = fmax(v, dpp<0x140>(v));
+    return fmax(fmax(read_lane(v, 0), read_lane(v, 16)), fmax(read_lane(v, 32), read_lane(v, 48)));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = row_sum(v);
+    return (read_lane(v, 0) + read_lane(v, 16)) + (read_lane(v, 32) + read_lane(v, 48));
+}
 
 struct RouteParams {
     const void* logits;
@@ -23,17 +86,15 @@ struct RouteParams {
     float* weights;
     int64_t logits_row;
     int tokens, experts, top_k, groups, top_groups, group_top;
+    int normalise;
     float factor;
 };
 
-// One wave a token, lane l holding experts l, l + 64, ..; the ranks of a token's
-// groups go through LDS.
-template <typename T, int P, bool SIGMOID, bool NORMALISE>
-__global__ __launch_bounds__(256) void route_kernel(const RouteParams p) {
-    extern __shared__ double smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int token = blockIdx.x * 4 + wave;
-    if (token >= p.tokens) return;  // a whole wave; no barrier follows
+// One token by one wave, lane l holding experts l, l + 64, ..; `all` are `experts`
+// doubles of the wave's own in LDS, used with groups. Lane i returns choice i.
+template <typename T, int P, bool SIGMOID>
+__device__ __forceinline__ int route_token(const RouteParams& p, int token, double* all) {
+    const int lane = threadIdx.x & 63;
     const T* x = static_cast<const T*>(p.logits) + token * p.logits_row;
     float l[P];
     bool odd = false;
@@ -59,9 +120,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteParams p) {
             score[j] = l[j] == -__builtin_inff() ? 0.0 : exp(static_cast<double>(l[j]) - static_cast<double>(top));
             total += score[j];
         }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) total += shfl_xor(total, o);
-        total = fmax(total, 1e-300);
+        total = fmax(wave_sum(total), 1e-300);
 #pragma unroll
         for (int j = 0; j < P; ++j) score[j] /= total;
     } else {
@@ -78,7 +137,6 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteParams p) {
         }
     }
     if (p.groups > 1) {
-        double* all = smem + wave * p.experts;
         const int size = p.experts / p.groups;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -89,6 +147,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteParams p) {
         // lane g: its group's best and second best; then the groups before it
         double a = kNone, b = kNone;
         if (lane < p.groups)
+#pragma unroll 8
             for (int i = 0; i < size; ++i) {
                 const double v = all[lane * size + i];
                 b = fmax(b, fmin(a, v));
@@ -97,7 +156,7 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteParams p) {
         const double mine = p.group_top == 1 ? a : b == kNone ? kNone : a + b;
         int before = 0;
         for (int g = 0; g < p.groups; ++g) {
-            const double v = __shfl(mine, g, 64);
+            const double v = read_lane(mine, g);
             before += v > mine || (v == mine && g < lane);
         }
         const uint64_t open = __ballot(lane < p.groups && before < p.top_groups);
@@ -107,49 +166,274 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteParams p) {
             if (!(open >> (min(e, p.experts - 1) / size) & 1)) rank[j] = kNone;
         }
     }
-    // top_k times the best that is left; lane i keeps choice i
+    // top_k times the best that is left, the first of equals; lane i keeps choice i
     int id = -1;
     double chosen = 0.0;
     for (int i = 0; i < p.top_k; ++i) {
-        double v = kNone, s = 0.0;
-        int at = INT_MAX;
+        double v = rank[0];
 #pragma unroll
-        for (int j = 0; j < P; ++j)
-            if (rank[j] > v) {
-                v = rank[j];
-                s = score[j];
-                at = lane + 64 * j;
-            }
+        for (int j = 1; j < P; ++j) v = fmax(v, rank[j]);
+        v = wave_max(v);
+        if (v == kNone) break;  // nothing is left
+        int at = -1;
+        double s = 0.0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double ov = shfl_xor(v, o), os = shfl_xor(s, o);
-            const int oa = __shfl_xor(at, o, 64);
-            if (ov > v || (ov == v && oa < at)) {
-                v = ov;
-                s = os;
-                at = oa;
+        for (int j = 0; j < P; ++j) {
+            const uint64_t holds = __ballot(rank[j] == v);
+            if (at < 0 && holds) {
+                const int from = __builtin_ctzll(holds);
+                at = from + 64 * j;
+                s = read_lane(score[j], from);
+                if (lane == from) rank[j] = kNone;
             }
         }
-        if (at == INT_MAX) break;  // nothing is left
-#pragma unroll
-        for (int j = 0; j < P; ++j)
-            if (lane + 64 * j == at) rank[j] = kNone;
         if (lane == i) {
             id = at;
             chosen = s;
         }
     }
-    if constexpr (NORMALISE) {
-        double sum = chosen;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) sum += shfl_xor(sum, o);
-        chosen /= sum + 1e-20;
+    if (p.normalise) {
+        chosen /= wave_sum(chosen) + 1e-20;
     }
     if (lane < p.top_k) {
         const int64_t at = static_cast<int64_t>(token) * p.top_k + lane;
         p.ids[at] = id;
         p.weights[at] = id < 0 ? 0.0f : bad ? __builtin_nanf("") : static_cast<float>(chosen * static_cast<double>(p.factor));
     }
+    return lane < p.top_k ? id : -1;
+}
+
+template <typename T, int P, bool SIGMOID>
+__global__ __launch_bounds__(256) void route_token_kernel(const RouteParams p) {
+    extern __shared__ double smem[];
+    const int wave = threadIdx.x >> 6, token = blockIdx.x * 4 + wave;
+    if (token < p.tokens) route_token<T, P, SIGMOID>(p, token, smem + wave * p.experts);
+}
+
+constexpr int kRowsTopK = 16;      // choices that route_rows holds, one a lane
+constexpr int kRowsExperts = 256;  // experts, 16 a lane and 8 bits of a key
+constexpr float kUnit = 0x1p20f;   // units of a key's value
+
+// What of a routing's plan a block of tokens works out along with its choices.
+struct RouteBlocks {
+    MoePlan plan;
+    int tokens;  // of a block
+    int lanes;   // of a group
+    int vec;     // logits can be loaded 16 bytes at a time
+};
+
+__device__ void place_block(const int32_t* ids, int first, int last, int run, const MoePlan& p, int* hist, int* sums, int all,
+                            int before, bool leads);
+
+// A block of tokens by 16 lanes each, lane l of them holding P neighbouring experts
+// of a group. An expert's key has its rank in the upper 24 bits and 255 - its
+// index in the lower 8, so a maximum is the best and, of equals, the first; 0 is an
+// expert that cannot be chosen. Ranks are
+//   - without a bias, 16-bit logits: their bits, in order: exact;
+//   - without a bias, f32 logits: 2^20 (logit - the token's largest), from -16 up;
+//   - with a bias: 2^20 (score + bias), within +-8.
+// The last two are truncated from f32 values that are within 0.6 of a unit of the
+// 64-bit one (and a softmax's sum of up to 256 within 1.3 units of its share, the
+// same for all): keys that differ by four units or more are in the right order,
+// and sums of two that differ by eight. Where two choices, or the last one and the best that is left,
+// differ by less, or the last open group and the best closed one, or where a
+// value does not fit, the token goes to route_token. The weights are worked out
+// in 64 bits from the chosen logits.
+template <typename T, int P, bool SIGMOID>
+__global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, const RouteBlocks b) {
+    extern __shared__ double smem[];
+    __shared__ int32_t chosen_ids[64 * kRowsTopK];
+    __shared__ int hist[16 * kRowsExperts];
+    __shared__ int sums[17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int l16 = lane & 15;
+    const bool alone = b.plan.blocks == 1;
+    double* all = smem + wave * p.experts;
+    for (int i = threadIdx.x; i < (alone ? waves : 1) * p.experts; i += blockDim.x) hist[i] = 0;
+    __syncthreads();
+    const int size = p.experts / p.groups, group = l16 / b.lanes, at0 = l16 % b.lanes * P;
+    const int base = blockIdx.x * b.tokens, end = min(base + b.tokens, p.tokens);
+    const bool exact = sizeof(T) == 2 && !p.bias;
+    for (int t0 = base + wave * 4; t0 < end; t0 += 4 * waves) {
+        const int token = t0 + (lane >> 4);
+        const bool active = token < end;
+        const T* x = static_cast<const T*>(p.logits) + min(token, end - 1) * p.logits_row;
+        const int e0 = group * size + at0;
+        float l[P];
+        bool odd = false;  // the token goes to route_token
+        if (b.vec) {
+            constexpr int V = P * sizeof(T) >= 16 ? 16 / sizeof(T) : P;
+            struct alignas(V * sizeof(T)) Run {
+                T e[V];
+            };
+#pragma unroll
+            for (int j = 0; j < P; j += V) {
+                Run r = {};
+                if (group < p.groups && at0 + j < size) r = *reinterpret_cast<const Run*>(x + e0 + j);
+#pragma unroll
+                for (int i = 0; i < V; ++i) l[j + i] = static_cast<float>(r.e[i]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < P; ++j) l[j] = group < p.groups && at0 + j < size ? static_cast<float>(x[e0 + j]) : 0.0f;
+        }
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            odd |= !(l[j] < __builtin_inff());
+            if (!(group < p.groups && at0 + j < size)) l[j] = -__builtin_inff();
+            top = fmaxf(top, l[j]);
+        }
+        top = row_max(top);
+        uint32_t key[P];
+        if (exact) {
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const T h = static_cast<T>(l[j] + 0.0f);  // -0 as 0
+                uint16_t u;
+                __builtin_memcpy(&u, &h, 2);
+                const uint32_t o = u & 0x8000 ? u ^ 0xFFFFu : u | 0x8000u;
+                key[j] = l[j] == -__builtin_inff() ? 0 : o << 16 | (255 - (e0 + j));
+            }
+        } else {
+            float y[P];
+            float floor = -8.0f;
+            if (!p.bias) {
+                floor = -16.0f;
+#pragma unroll
+                for (int j = 0; j < P; ++j) y[j] = l[j] - top;
+            } else {
+                float scale = 1.0f;
+                if constexpr (SIGMOID) {
+#pragma unroll
+                    for (int j = 0; j < P; ++j)
+                        y[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -1.44269504f));
+                } else {
+                    float total = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < P; ++j) {
+                        y[j] = __builtin_amdgcn_exp2f((l[j] - top) * 1.44269504f);
+                        total += l[j] == -__builtin_inff() ? 0.0f : y[j];
+                    }
+                    scale = __builtin_amdgcn_rcpf(row_sum(total));
+                }
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    const bool real = l[j] != -__builtin_inff();
+                    y[j] = y[j] * scale + (real ? p.bias[e0 + j] : 0.0f);
+                    odd |= real && !(fabsf(y[j]) < 7.9f);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const int q = static_cast<int>(fmaxf(y[j], floor) * kUnit) - static_cast<int>(floor * kUnit);
+                key[j] = l[j] == -__builtin_inff() ? 0 : static_cast<uint32_t>(min(max(q, 1), 0xFFFFFF)) << 8 | (255 - (e0 + j));
+            }
+        }
+        if (p.groups > 1) {
+            uint32_t a = 0, c = 0;  // the group's best and second best
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                c = max(c, min(a, key[j]));
+                a = max(a, key[j]);
+            }
+            const auto join = [&](uint32_t oa, uint32_t oc) {
+                c = max(min(a, oa), max(c, oc));
+                a = max(a, oa);
+            };
+            if (b.lanes >= 2) join(dpp<0xB1>(a), dpp<0xB1>(c));
+            if (b.lanes >= 4) join(dpp<0x4E>(a), dpp<0x4E>(c));
+            if (b.lanes >= 8) join(dpp<0x141>(a), dpp<0x141>(c));
+            const uint32_t rank = p.group_top == 1 ? a >> 8 : c == 0 ? 0 : (a >> 8) + (c >> 8);
+            int above = 0;
+            count_above<1>(rank << 6 | (63 - group), above);
+            const bool open = above < p.top_groups * b.lanes;
+            const uint32_t closed = row_max(open ? 0 : rank), least = ~row_max(open ? ~rank : 0);
+            odd |= !exact && closed != 0 && least - closed < 8;
+            if (!open)
+#pragma unroll
+                for (int j = 0; j < P; ++j) key[j] = 0;
+        }
+        // lane i keeps choice i, and the two that come behind the last
+        const bool pairs = p.top_k <= kRowsTopK - 2 && (SIGMOID || !p.bias);
+        uint32_t mine = 0, before = 0xFFFFFFFF;
+        bool near = false;  // the choice before may be of lower rank
+        for (int i = 0; i < p.top_k + (exact ? 0 : pairs ? 2 : 1); ++i) {
+            uint32_t best = 0;
+#pragma unroll
+            for (int j = 0; j < P; ++j) best = max(best, key[j]);
+            best = row_max(best);
+            if (l16 == i) {
+                mine = best;
+                near = !exact && i > 0 && best != 0 && (before >> 8) - (best >> 8) < 4;
+            }
+            if (i == kRowsTopK) odd |= !exact && best != 0 && (before >> 8) - (best >> 8) < 4;
+            before = best;
+#pragma unroll
+            for (int j = 0; j < P; ++j) key[j] = key[j] == best ? 0 : key[j];
+        }
+        int id = mine ? 255 - static_cast<int>(mine & 255) : -1;
+        double w = 0.0;
+        if (id >= 0) {
+            const double v = static_cast<double>(static_cast<float>(x[id]));
+            if constexpr (SIGMOID) w = 1.0 / (1.0 + exp(-v));
+            else w = exp(v - static_cast<double>(top));
+        }
+        if (__any(near)) {
+            const uint32_t behind = dpp<0x101>(static_cast<uint32_t>(near));  // of the next choice
+            odd |= near && (behind || !pairs);
+            // one of two near ones: they change places where their 64-bit ranks say so
+            double rank = w;
+            if (id >= 0) rank = p.bias ? w + static_cast<double>(p.bias[id]) : static_cast<double>(static_cast<float>(x[id]));
+            // (all lanes read their neighbours' before any takes one)
+            const double w_up = dpp<0x111>(w), w_down = dpp<0x101>(w), rank_up = dpp<0x111>(rank), rank_down = dpp<0x101>(rank);
+            const double ow = near ? w_up : w_down, orank = near ? rank_up : rank_down;
+            const int up = static_cast<int>(dpp<0x111>(static_cast<uint32_t>(id))), down = static_cast<int>(dpp<0x101>(static_cast<uint32_t>(id)));
+            const int oid = near ? up : down;
+            const bool wrong = near ? rank > orank || (rank == orank && id < oid) : orank > rank || (rank == orank && oid < id);
+            if ((near || behind) && wrong) {
+                id = oid;
+                w = ow;
+            }
+        }
+        if (l16 >= p.top_k) w = 0.0;
+        if (p.normalise) {
+            const double sum = row_sum(w);
+            // softmax: the 1e-20 stands beside the sum over the total, which is 1 to 256
+            if constexpr (!SIGMOID) odd |= id >= 0 && sum < 1e-7;
+            w /= sum + 1e-20;
+        } else if constexpr (!SIGMOID) {
+            double total = 0.0;
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+                if (l[j] != -__builtin_inff()) total += exp(static_cast<double>(l[j]) - static_cast<double>(top));
+            w /= fmax(row_sum(total), 1e-300);
+        }
+        const uint64_t odd_lanes = __ballot(odd);
+        const auto note = [&](int t, int i, int e) {  // choice i of token t fell on e
+            if (alone) chosen_ids[(t - base) * p.top_k + i] = e;
+            else if (e >= 0) atomicAdd(&hist[e], 1);
+        };
+        if (active && l16 < p.top_k && !(odd_lanes >> (lane & 48) & 0xFFFF)) {
+            const int64_t at = static_cast<int64_t>(token) * p.top_k + l16;
+            p.ids[at] = id;
+            p.weights[at] = id < 0 ? 0.0f : static_cast<float>(w * static_cast<double>(p.factor));
+            note(token, l16, id);
+        }
+        for (int q = 0; q < 4; ++q)
+            if ((odd_lanes >> (16 * q) & 0xFFFF) && t0 + q < end) {
+                const int e = route_token<T, P >= 4 ? P / 4 : 1, SIGMOID>(p, t0 + q, all);
+                if (lane < p.top_k) note(t0 + q, lane, e);
+            }
+    }
+    __syncthreads();
+    if (!alone) {
+        for (int e = threadIdx.x; e < p.experts; e += blockDim.x) b.plan.counts[blockIdx.x * p.experts + e] = hist[e];
+        return;
+    }
+    // the only block: place its choices too
+    const int rows = b.plan.rows, run = (rows + 64 * waves - 1) / (64 * waves) * 64;
+    place_block(chosen_ids, 0, rows, run, b.plan, hist, sums, 0, 0, true);
 }
 
 // Lane l gets the sum over lanes 0 .. l.
@@ -163,20 +447,84 @@ __device__ __forceinline__ int scan(int x) {
     return x;
 }
 
-// Exclusive sums over the workgroup's threads; `sums` holds 17 ints.
+// Exclusive sums over the workgroup's threads (at most 1024); `sums` holds 16 ints.
 __device__ __forceinline__ int scan_threads(int x, int* sums, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int in = scan(x);
     if (lane == 63) sums[wave] = in;
     __syncthreads();
     int before = 0, all = 0;
-    for (int w = 0; w < kMoeCountThreads / 64; ++w) {
+    for (int w = 0; w < waves; ++w) {
         before += w < wave ? sums[w] : 0;
         all += sums[w];
     }
     total = all;
     __syncthreads();
     return before + in - x;
+}
+
+// Places choices first .. last - 1 in order: wave w takes the w-th run of them (whole
+// chunks of 64). hist (zeros [waves][experts]) counts a wave's choices of e, then holds
+// where its next one goes. Thread e gives the choices of expert e in all blocks, and
+// in those before; with one block, zeros. The workgroup that leads writes the offsets
+// and the tiles. At least `experts` threads.
+__device__ void place_block(const int32_t* ids, int first, int last, int run, const MoePlan& p, int* hist, int* sums, int all,
+                            int before, bool leads) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, E = p.experts;
+    const int from = min(first + wave * run, last), to = min(from + run, last);
+    for (int i = from + lane; i < to; i += 64) {
+        const int e = ids[i];
+        if (e >= 0 && e < E) atomicAdd(&hist[wave * E + e], 1);
+    }
+    __syncthreads();
+    const int e0 = threadIdx.x;
+    if (e0 < E && p.blocks == 1)
+        for (int w = 0; w < waves; ++w) all += hist[w * E + e0];
+    int total;
+    const int offset = scan_threads(all, sums, total);
+    if (e0 < E) {
+        int at = offset + before;
+        for (int w = 0; w < waves; ++w) {
+            const int c = hist[w * E + e0];
+            hist[w * E + e0] = at;
+            at += c;
+        }
+    }
+    if (leads) {
+        if (e0 < E) p.offsets[e0] = offset;
+        if (e0 == 0) p.offsets[E] = total;
+        const int n = (all + p.tile_rows - 1) / p.tile_rows;
+        int tiles;
+        const int t0 = scan_threads(n, sums, tiles);
+        for (int t = 0; t < n; ++t) {
+            p.tiles[2 * (t0 + t)] = e0;
+            p.tiles[2 * (t0 + t) + 1] = offset + t * p.tile_rows;
+        }
+        if (e0 == 0) *p.tile_count = tiles;
+    }
+    __syncthreads();
+    int bits = 0;
+    while (1 << bits < E) ++bits;
+    for (int i0 = from; i0 < to; i0 += 64) {
+        const int i = i0 + lane;
+        const int e = i < to ? ids[i] : -1;
+        const bool valid = e >= 0 && e < E;
+        // the lanes with the same expert
+        uint64_t same = __ballot(valid);
+        for (int k = 0; k < bits; ++k) {
+            const uint64_t set = __ballot(e >> k & 1);
+            same &= e >> k & 1 ? set : ~set;
+        }
+        const int ahead = __popcll(same & ((uint64_t{1} << lane) - 1));
+        int at = -1;
+        if (valid) at = hist[wave * E + e] + ahead;
+        __builtin_amdgcn_wave_barrier();
+        if (valid && ahead == 0) hist[wave * E + e] += __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+        if (valid) p.order[at] = i;
+        if (i < to) p.place[i] = at;
+    }
+    for (int i = total + blockIdx.x * blockDim.x + threadIdx.x; i < p.rows; i += gridDim.x * blockDim.x) p.order[i] = -1;
 }
 
 // A block's choices by expert.
@@ -194,109 +542,100 @@ __global__ __launch_bounds__(kMoeCountThreads) void count_kernel(const int32_t* 
     for (int e = threadIdx.x; e < experts; e += kMoeCountThreads) counts[blockIdx.x * experts + e] = hist[e];
 }
 
-// Places a block's choices, in order: wave w takes the w-th run of the block.
-// hist[w][e] counts the wave's choices of e, then holds where its next one goes.
-__global__ __launch_bounds__(kMoeCountThreads) void place_kernel(const int32_t* __restrict__ ids, const MoePlan p) {
+// Places `each` counting blocks' choices a workgroup. 1024 / 2^shift threads an expert
+// add up the blocks' counts.
+__global__ __launch_bounds__(kMoeCountThreads) void place_kernel(const int32_t* __restrict__ ids, const MoePlan p, int each,
+                                                                 int shift) {
     constexpr int W = kMoeCountThreads / 64;
-    extern __shared__ int hist[];
-    __shared__ int sums[W + 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, E = p.experts;
-    for (int i = threadIdx.x; i < W * E; i += kMoeCountThreads) hist[i] = 0;
+    extern __shared__ int hist_of_waves[];
+    __shared__ int sums[W], in_all[ROCKNPU_MOE_MAX_EXPERTS], in_before[ROCKNPU_MOE_MAX_EXPERTS];
+    const int t = threadIdx.x, E = p.experts;
+    for (int i = t; i < W * E; i += kMoeCountThreads) hist_of_waves[i] = 0;
+    in_all[t] = in_before[t] = 0;
     __syncthreads();
-    const int run = p.block / W, first = blockIdx.x * p.block + wave * run, last = min(first + run, p.rows);
-    for (int i = first + lane; i < last; i += 64) {
-        const int e = ids[i];
-        if (e >= 0 && e < E) atomicAdd(&hist[wave * E + e], 1);
-    }
-    __syncthreads();
-    // thread e: choices of expert e in all blocks, and in the blocks and waves before
-    const int e0 = threadIdx.x;
-    int all = 0, before = 0;
-    if (e0 < E) {
-        if (p.blocks > 1) {
-            for (int b = 0; b < p.blocks; ++b) {
-                const int c = p.counts[b * E + e0];
+    const int block0 = blockIdx.x * each;
+    if (p.blocks > 1) {
+        const int e = t & ((1 << shift) - 1), parts = kMoeCountThreads >> shift;
+        if (e < E) {
+            int all = 0, before = 0;
+#pragma unroll 8
+            for (int b = t >> shift; b < p.blocks; b += parts) {
+                const int c = p.counts[b * E + e];
                 all += c;
-                before += b < static_cast<int>(blockIdx.x) ? c : 0;
+                before += b < block0 ? c : 0;
             }
-        } else {
-            for (int w = 0; w < W; ++w) all += hist[w * E + e0];
+            atomicAdd(&in_all[e], all);
+            atomicAdd(&in_before[e], before);
         }
+        __syncthreads();
     }
-    int total;
-    const int offset = scan_threads(all, sums, total);
-    if (e0 < E) {
-        int at = offset + before;
-        for (int w = 0; w < W; ++w) {
-            const int c = hist[w * E + e0];
-            hist[w * E + e0] = at;
-            at += c;
-        }
-    }
-    if (blockIdx.x == 0) {
-        if (e0 < E) p.offsets[e0] = offset;
-        if (e0 == 0) p.offsets[E] = total;
-        const int n = (all + p.tile_rows - 1) / p.tile_rows;
-        int tiles;
-        const int t0 = scan_threads(n, sums, tiles);
-        for (int t = 0; t < n; ++t) {
-            p.tiles[2 * (t0 + t)] = e0;
-            p.tiles[2 * (t0 + t) + 1] = offset + t * p.tile_rows;
-        }
-        if (e0 == 0) *p.tile_count = tiles;
-    }
-    __syncthreads();
-    for (int i0 = first; i0 < last; i0 += 64) {
-        const int i = i0 + lane;
-        const int e = i < last ? ids[i] : -1;
-        const bool valid = e >= 0 && e < E;
-        // the lanes with the same expert
-        uint64_t same = __ballot(valid);
-        for (int b = 1; b < E; b <<= 1) {
-            const uint64_t set = __ballot(e & b);
-            same &= e & b ? set : ~set;
-        }
-        const int ahead = __popcll(same & ((uint64_t{1} << lane) - 1));
-        int at = -1;
-        if (valid) at = hist[wave * E + e] + ahead;
-        __builtin_amdgcn_wave_barrier();
-        if (valid && ahead == 0) hist[wave * E + e] += __popcll(same);
-        __builtin_amdgcn_wave_barrier();
-        if (valid) p.order[at] = i;
-        if (i < last) p.place[i] = at;
-    }
-    for (int i = total + blockIdx.x * kMoeCountThreads + threadIdx.x; i < p.rows; i += gridDim.x * kMoeCountThreads)
-        p.order[i] = -1;
+    const int64_t first = static_cast<int64_t>(block0) * p.block;
+    const int last = static_cast<int>(min(first + static_cast<int64_t>(each) * p.block, static_cast<int64_t>(p.rows)));
+    const int span = each * p.block, run = (span + 64 * W - 1) / (64 * W) * 64;
+    place_block(ids, static_cast<int>(first), last, run, p, hist_of_waves, sums, in_all[t], in_before[t], blockIdx.x == 0);
 }
 
 template <typename T, int P>
-int launch_route(const RouteParams& p, bool sigmoid, bool normalise, hipStream_t stream) {
+int launch_tokens(const RouteParams& p, bool sigmoid, hipStream_t stream) {
     const dim3 grid((p.tokens + 3) / 4), block(256);
     const size_t lds = p.groups > 1 ? static_cast<size_t>(4) * p.experts * sizeof(double) : 0;
-    if (sigmoid && normalise) route_kernel<T, P, true, true><<<grid, block, lds, stream>>>(p);
-    else if (sigmoid) route_kernel<T, P, true, false><<<grid, block, lds, stream>>>(p);
-    else if (normalise) route_kernel<T, P, false, true><<<grid, block, lds, stream>>>(p);
-    else route_kernel<T, P, false, false><<<grid, block, lds, stream>>>(p);
+    if (sigmoid) route_token_kernel<T, P, true><<<grid, block, lds, stream>>>(p);
+    else route_token_kernel<T, P, false><<<grid, block, lds, stream>>>(p);
+    return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
+}
+
+template <typename T, int P>
+int launch_rows(const RouteParams& p, const RouteBlocks& b, bool sigmoid, hipStream_t stream) {
+    // 16 waves of four tokens each; a single block takes as many waves as its tokens
+    // and experts need
+    const int threads = b.plan.blocks > 1 ? 1024 : std::max((p.tokens + 3) / 4 * 64, (p.experts + 63) / 64 * 64);
+    const dim3 grid(b.plan.blocks), block(threads);
+    const size_t lds = p.groups > 1 ? static_cast<size_t>(threads / 64) * p.experts * sizeof(double) : 0;
+    if (sigmoid) route_rows_kernel<T, P, true><<<grid, block, lds, stream>>>(p, b);
+    else route_rows_kernel<T, P, false><<<grid, block, lds, stream>>>(p, b);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
 template <typename T>
-int route(const RouteParams& p, bool sigmoid, bool normalise, hipStream_t stream) {
-    if (p.experts <= 64) return launch_route<T, 1>(p, sigmoid, normalise, stream);
-    if (p.experts <= 128) return launch_route<T, 2>(p, sigmoid, normalise, stream);
-    if (p.experts <= 256) return launch_route<T, 4>(p, sigmoid, normalise, stream);
-    if (p.experts <= 512) return launch_route<T, 8>(p, sigmoid, normalise, stream);
-    return launch_route<T, 16>(p, sigmoid, normalise, stream);
+int route(const RouteParams& p, const MoePlan& plan, bool sigmoid, bool* placed, bool* counted, hipStream_t stream) {
+    *placed = *counted = false;
+    // route_rows: groups of whole lanes, and ranks that its keys hold
+    const int lanes = 16 / p.groups, size = p.experts / p.groups;
+    if (p.top_k <= kRowsTopK && p.experts <= kRowsExperts && 16 % p.groups == 0 &&
+        (p.groups == 1 || p.group_top == 1 || p.bias)) {
+        const int each = (size + lanes - 1) / lanes;
+        const int P = each <= 1 ? 1 : each <= 2 ? 2 : each <= 4 ? 4 : each <= 8 ? 8 : 16;
+        const int run = std::min<int>(P * sizeof(T), 16);
+        const RouteBlocks b{plan, plan.block / p.top_k, lanes,
+                            reinterpret_cast<uintptr_t>(p.logits) % run == 0 && p.logits_row * sizeof(T) % run == 0 &&
+                                size % (run / static_cast<int>(sizeof(T))) == 0};
+        *counted = true;
+        *placed = plan.blocks == 1;
+        if (P == 1) return launch_rows<T, 1>(p, b, sigmoid, stream);
+        if (P == 2) return launch_rows<T, 2>(p, b, sigmoid, stream);
+        if (P == 4) return launch_rows<T, 4>(p, b, sigmoid, stream);
+        if (P == 8) return launch_rows<T, 8>(p, b, sigmoid, stream);
+        return launch_rows<T, 16>(p, b, sigmoid, stream);
+    }
+    if (p.experts <= 64) return launch_tokens<T, 1>(p, sigmoid, stream);
+    if (p.experts <= 128) return launch_tokens<T, 2>(p, sigmoid, stream);
+    if (p.experts <= 256) return launch_tokens<T, 4>(p, sigmoid, stream);
+    if (p.experts <= 512) return launch_tokens<T, 8>(p, sigmoid, stream);
+    return launch_tokens<T, 16>(p, sigmoid, stream);
 }
 
-int launch_plan(const int32_t* ids, const MoePlan& p, hipStream_t stream) {
-    const dim3 grid(std::max(p.blocks, 1)), block(kMoeCountThreads);
-    if (p.blocks > 1) {
-        count_kernel<<<grid, block, 0, stream>>>(ids, p.rows, p.experts, p.block, p.counts);
+int launch_plan(const int32_t* ids, const MoePlan& p, bool counted, hipStream_t stream) {
+    if (p.blocks > 1 && !counted) {
+        count_kernel<<<dim3(p.blocks), dim3(kMoeCountThreads), 0, stream>>>(ids, p.rows, p.experts, p.block, p.counts);
         if (hipGetLastError() != hipSuccess) return kStatusExec;
     }
+    // at most 64 workgroups: every one reads all blocks' counts
+    const int each = std::max((p.blocks + 63) / 64, 1);
+    int shift = 0;
+    while (1 << shift < p.experts) ++shift;
+    const dim3 grid(std::max((p.blocks + each - 1) / each, 1));
     const size_t lds = static_cast<size_t>(kMoeCountThreads / 64) * p.experts * sizeof(int);
-    place_kernel<<<grid, block, lds, stream>>>(ids, p);
+    place_kernel<<<grid, dim3(kMoeCountThreads), lds, stream>>>(ids, p, each, shift);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
@@ -335,14 +674,17 @@ extern "C" int rocknpu_hip_moe_route(const rocknpu_moe_route_args* args, void* s
         return kStatusInvalid;
     if (a.tokens > 0 && (!a.logits || !a.ids || !a.weights)) return kStatusInvalid;
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    const MoePlan plan = moe_plan(a.tokens, a.experts, a.top_k, a.plan, nullptr);
+    bool counted = false;
     if (a.tokens > 0) {
         const RouteParams p{a.logits, a.bias, a.ids, a.weights, a.logits_row, static_cast<int>(a.tokens), a.experts, a.top_k,
-                            a.groups, a.top_groups, a.group_top, a.factor};
-        const bool sigmoid = a.score == ROCKNPU_MOE_SIGMOID, norm = a.normalise != 0;
-        const int st = a.type == ROCKNPU_TYPE_F32   ? route<float>(p, sigmoid, norm, s)
-                       : a.type == ROCKNPU_TYPE_F16 ? route<_Float16>(p, sigmoid, norm, s)
-                                                    : route<__bf16>(p, sigmoid, norm, s);
-        if (st != kStatusOk) return st;
+                            a.groups, a.top_groups, a.group_top, a.normalise != 0, a.factor};
+        const bool sigmoid = a.score == ROCKNPU_MOE_SIGMOID;
+        bool placed;
+        const int st = a.type == ROCKNPU_TYPE_F32   ? route<float>(p, plan, sigmoid, &placed, &counted, s)
+                       : a.type == ROCKNPU_TYPE_F16 ? route<_Float16>(p, plan, sigmoid, &placed, &counted, s)
+                                                    : route<__bf16>(p, plan, sigmoid, &placed, &counted, s);
+        if (st != kStatusOk || placed) return st;
     }
-    return launch_plan(a.ids, moe_plan(a.tokens, a.experts, a.top_k, a.plan, nullptr), s);
+    return launch_plan(a.ids, plan, counted, s);
 }

@@ -79,6 +79,8 @@ __device__ __forceinline__ double wave_sum(double v) {
     return (read_lane(v, 0) + read_lane(v, 16)) + (read_lane(v, 32) + read_lane(v, 48));
 }
 
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
 struct RouteParams {
     const void* logits;
     const float* bias;
@@ -210,6 +212,9 @@ __global__ __launch_bounds__(256) void route_token_kernel(const RouteParams p) {
     if (token < p.tokens) route_token<T, P, SIGMOID>(p, token, smem + wave * p.experts);
 }
 
+// All ones, or for a logit of -inf zero (no branch around what it masks).
+__device__ __forceinline__ uint32_t open_mask(float logit) { return logit == -__builtin_inff() ? 0u : ~0u; }
+
 constexpr int kRowsTopK = 16;      // choices that route_rows holds, one a lane
 constexpr int kRowsExperts = 256;  // experts, 16 a lane and 8 bits of a key
 constexpr float kUnit = 0x1p20f;   // units of a key's value
@@ -218,8 +223,9 @@ constexpr float kUnit = 0x1p20f;   // units of a key's value
 struct RouteBlocks {
     MoePlan plan;
     int tokens;  // of a block
-    int lanes;   // of a group
-    int vec;     // logits can be loaded 16 bytes at a time
+    int size;    // experts of a group
+    int shift;   // a group's lanes are 1 << shift
+    int vec;     // logits and bias can be loaded 16 bytes at a time
 };
 
 __device__ void place_block(const int32_t* ids, int first, int last, int run, const MoePlan& p, int* hist, int* sums, int all,
@@ -251,7 +257,7 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
     double* all = smem + wave * p.experts;
     for (int i = threadIdx.x; i < (alone ? waves : 1) * p.experts; i += blockDim.x) hist[i] = 0;
     __syncthreads();
-    const int size = p.experts / p.groups, group = l16 / b.lanes, at0 = l16 % b.lanes * P;
+    const int size = b.size, group = l16 >> b.shift, at0 = (l16 & ((1 << b.shift) - 1)) * P;
     const int base = blockIdx.x * b.tokens, end = min(base + b.tokens, p.tokens);
     const bool exact = sizeof(T) == 2 && !p.bias;
     for (int t0 = base + wave * 4; t0 < end; t0 += 4 * waves) {
@@ -277,6 +283,24 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
 #pragma unroll
             for (int j = 0; j < P; ++j) l[j] = group < p.groups && at0 + j < size ? static_cast<float>(x[e0 + j]) : 0.0f;
         }
+        float bias[P];  // asked for together with the logits
+        if (p.bias) {
+            constexpr int V = P < 4 ? P : 4;
+            struct alignas(V * 4) Run {
+                float e[V];
+            };
+            if (b.vec) {
+#pragma unroll
+                for (int j = 0; j < P; j += V) {
+                    const Run r = *reinterpret_cast<const Run*>(p.bias + min(e0 + j, p.experts - V));
+#pragma unroll
+                    for (int i = 0; i < V; ++i) bias[j + i] = r.e[i];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < P; ++j) bias[j] = p.bias[min(e0 + j, p.experts - 1)];
+            }
+        }
         float top = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -293,7 +317,7 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
                 uint16_t u;
                 __builtin_memcpy(&u, &h, 2);
                 const uint32_t o = u & 0x8000 ? u ^ 0xFFFFu : u | 0x8000u;
-                key[j] = l[j] == -__builtin_inff() ? 0 : o << 16 | (255 - (e0 + j));
+                key[j] = open_mask(l[j]) & (o << 16 | (255 - (e0 + j)));
             }
         } else {
             float y[P];
@@ -320,14 +344,14 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
                     const bool real = l[j] != -__builtin_inff();
-                    y[j] = y[j] * scale + (real ? p.bias[e0 + j] : 0.0f);
+                    y[j] = y[j] * scale + bias[j];
                     odd |= real && !(fabsf(y[j]) < 7.9f);
                 }
             }
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 const int q = static_cast<int>(fmaxf(y[j], floor) * kUnit) - static_cast<int>(floor * kUnit);
-                key[j] = l[j] == -__builtin_inff() ? 0 : static_cast<uint32_t>(min(max(q, 1), 0xFFFFFF)) << 8 | (255 - (e0 + j));
+                key[j] = open_mask(l[j]) & (static_cast<uint32_t>(min(max(q, 1), 0xFFFFFF)) << 8 | (255 - (e0 + j)));
             }
         }
         if (p.groups > 1) {
@@ -341,13 +365,13 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
                 c = max(min(a, oa), max(c, oc));
                 a = max(a, oa);
             };
-            if (b.lanes >= 2) join(dpp<0xB1>(a), dpp<0xB1>(c));
-            if (b.lanes >= 4) join(dpp<0x4E>(a), dpp<0x4E>(c));
-            if (b.lanes >= 8) join(dpp<0x141>(a), dpp<0x141>(c));
+            if (b.shift >= 1) join(dpp<0xB1>(a), dpp<0xB1>(c));
+            if (b.shift >= 2) join(dpp<0x4E>(a), dpp<0x4E>(c));
+            if (b.shift >= 3) join(dpp<0x141>(a), dpp<0x141>(c));
             const uint32_t rank = p.group_top == 1 ? a >> 8 : c == 0 ? 0 : (a >> 8) + (c >> 8);
             int above = 0;
             count_above<1>(rank << 6 | (63 - group), above);
-            const bool open = above < p.top_groups * b.lanes;
+            const bool open = above < p.top_groups << b.shift;
             const uint32_t closed = row_max(open ? 0 : rank), least = ~row_max(open ? ~rank : 0);
             odd |= !exact && closed != 0 && least - closed < 8;
             if (!open)
@@ -606,9 +630,11 @@ int route(const RouteParams& p, const MoePlan& plan, bool sigmoid, bool* placed,
         const int each = (size + lanes - 1) / lanes;
         const int P = each <= 1 ? 1 : each <= 2 ? 2 : each <= 4 ? 4 : each <= 8 ? 8 : 16;
         const int run = std::min<int>(P * sizeof(T), 16);
-        const RouteBlocks b{plan, plan.block / p.top_k, lanes,
-                            reinterpret_cast<uintptr_t>(p.logits) % run == 0 && p.logits_row * sizeof(T) % run == 0 &&
-                                size % (run / static_cast<int>(sizeof(T))) == 0};
+        int shift = 0;
+        while (1 << shift < lanes) ++shift;
+        const RouteBlocks b{plan, plan.block / p.top_k, size, shift,
+                            aligned(p.logits, run) && p.logits_row * sizeof(T) % run == 0 && size % (run / static_cast<int>(sizeof(T))) == 0 &&
+                                size % std::min(P, 4) == 0 && aligned(p.bias, 4 * std::min(P, 4))};
         *counted = true;
         *placed = plan.blocks == 1;
         if (P == 1) return launch_rows<T, 1>(p, b, sigmoid, stream);
@@ -638,8 +664,6 @@ int launch_plan(const int32_t* ids, const MoePlan& p, bool counted, hipStream_t 
     place_kernel<<<grid, dim3(kMoeCountThreads), lds, stream>>>(ids, p, each, shift);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
-
-bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 }  // namespace
 

@@ -77,8 +77,9 @@ typedef struct rocknpu_moe_experts_args {
     const float * gate_scales;  /* [experts][ffn] */
     const float * up_scales;    /* [experts][ffn] */
     const float * down_scales;  /* [experts][hidden] */
-    const float * weights;      /* [tokens][top_k], as rocknpu_hip_moe_route gives them */
-    const int32_t * plan;       /* of a rocknpu_hip_moe_route with these tokens, experts and top_k */
+    const int32_t * ids;        /* [tokens][top_k], as rocknpu_hip_moe_route gives them */
+    const float * weights;      /* [tokens][top_k], its weights or others */
+    const int32_t * plan;       /* the plan that came with the ids */
     void * out;                 /* [tokens][hidden] of out_type, rows out_row elements apart */
     int64_t tokens, out_row;
     int32_t experts, top_k;

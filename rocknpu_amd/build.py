@@ -48,7 +48,7 @@ CFLAGS = [
 
 SOURCES = ["repack.hip", "quant.hip", "norm.hip", "gemm.hip", "gemm_skinny.hip", "gemv.hip", "gemv_mfma.hip", "gemv_tiled.hip", "launch.hip", "matmul.hip", "capi.hip", "sidecar.hip", "route.hip",
            "kv_cache.hip", "kv_stream.hip", "kv_prompt.hip", "kv_attention.hip",
-           "moe_route.hip", "moe_product.hip", "moe_experts.hip"]
+           "moe_route.hip", "moe_product.hip", "moe_decode.hip", "moe_experts.hip"]
 
 
 def _run(cmd: list[str]) -> None:

@@ -79,7 +79,7 @@ struct Space {
 };
 Space space(const rocknpu_moe_experts_args& a) {
     const size_t rows = static_cast<size_t>(a.tokens) * a.top_k;
-    return {padded(rows * std::max(a.ffn, a.hidden) * 4), padded(rows * a.ffn_pad), padded(rows * 4)};
+    return {padded(rows * std::max(a.ffn_pad, a.hidden) * 4), padded(rows * a.ffn_pad), padded(rows * 4)};
 }
 
 }  // namespace
@@ -101,13 +101,13 @@ extern "C" int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args* args, voi
         a.out_type > ROCKNPU_TYPE_BF16 || a.out_row < 0)
         return kStatusInvalid;
     if (!aligned(a.a8, 16) || !aligned(a.gate, 16) || !aligned(a.up, 16) || !aligned(a.down, 16) || !aligned(a.a_scales, 4) ||
-        !aligned(a.gate_scales, 4) || !aligned(a.up_scales, 4) || !aligned(a.down_scales, 4) || !aligned(a.weights, 4) ||
+        !aligned(a.gate_scales, 4) || !aligned(a.up_scales, 4) || !aligned(a.down_scales, 4) || !aligned(a.ids, 4) || !aligned(a.weights, 4) ||
         !aligned(a.plan, 4) || !aligned(a.out, a.out_type == ROCKNPU_TYPE_F32 ? 4 : 2))
         return kStatusInvalid;
     if (a.tokens > 1 && a.out_row < a.hidden) return kStatusInvalid;
     if (a.tokens == 0) return kStatusOk;
     const Space sp = space(a);
-    if (!a.a8 || !a.a_scales || !a.weights || !a.out || !workspace || !aligned(workspace, 256) || workspace_bytes < sp.bytes())
+    if (!a.a8 || !a.a_scales || !a.ids || !a.weights || !a.out || !workspace || !aligned(workspace, 256) || workspace_bytes < sp.bytes())
         return kStatusInvalid;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const MoePlan plan = moe_plan(a.tokens, a.experts, a.top_k, const_cast<int32_t*>(a.plan), nullptr);
@@ -115,6 +115,11 @@ extern "C" int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args* args, voi
     float* values = reinterpret_cast<float*>(at);
     int8_t* codes = reinterpret_cast<int8_t*>(at + sp.values);
     float* scales = reinterpret_cast<float*>(at + sp.values + sp.codes);
+    if (moe_decodes(a.tokens, a.top_k, a.ffn_pad)) {
+        const MoeDecode d{a.a8, a.a_scales, a.gate, a.up, a.down, a.gate_scales, a.up_scales, a.down_scales, a.ids, a.weights,
+                          values, static_cast<int>(a.tokens), a.experts, a.top_k, a.hidden, a.hidden_pad, a.ffn, a.ffn_pad};
+        return launch_moe_decode(d, a.out_type, a.out, a.out_row, s);
+    }
     const MoeProduct first{a.a8, a.a_scales, {a.gate, a.up}, {a.gate_scales, a.up_scales}, values, a.ffn, a.hidden_pad, a.top_k};
     int st = launch_moe_product(first, true, plan, s);
     if (st != kStatusOk) return st;

@@ -23,36 +23,6 @@
 namespace rk {
 namespace {
 
-// f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, to 2^-50 of the value:
-// exp(-g) = 2^n 2^r with n = rint(-g log2(e)), |r| <= 1/2 in two parts of log2(e),
-// 2^r by the polynomial through its values at the 11 Chebyshev nodes of [-1/2, 1/2]
-// (off by 2^-51.5 at most), the division by the reciprocal's Newton step and one
-// of the quotient. In the exponential g is held to +-693, where the value is that of
-// 1 + exp(-g) = 1, or 0 in f32.
-__device__ __forceinline__ float swiglu(float gate, float up) {
-    const double x = static_cast<double>(gate) * static_cast<double>(up);
-    const double g = static_cast<double>(__builtin_amdgcn_fmed3f(gate, -693.0f, 693.0f));
-    const double n = rint(g * -0x1.71547652b82fep+0);
-    double r = fma(g, -0x1.71547652b82fep+0, -n);
-    r = fma(g, -0x1.777d0ffda0d24p-56, r);
-    double p = 0x1.e6063f7217bc6p-28;
-    p = fma(p, r, 0x1.b675bca4eeebbp-24);
-    p = fma(p, r, 0x1.62bfd47773353p-20);
-    p = fma(p, r, 0x1.ffcb54062e698p-17);
-    p = fma(p, r, 0x1.430913096fd9fp-13);
-    p = fma(p, r, 0x1.5d87fe9d7a584p-10);
-    p = fma(p, r, 0x1.3b2ab6fba1ddap-7);
-    p = fma(p, r, 0x1.c6b08d703ce49p-5);
-    p = fma(p, r, 0x1.ebfbdff82c598p-3);
-    p = fma(p, r, 0x1.62e42fefa3a19p-1);
-    p = fma(p, r, 1.0);
-    const double d = 1.0 + ldexp(p, static_cast<int>(n));
-    double y = __builtin_amdgcn_rcp(d);
-    y = fma(fma(-d, y, 1.0), y, y);
-    const double q = x * y;
-    return static_cast<float>(fma(fma(-d, q, x), y, q));
-}
-
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 constexpr int kMoeManyTiles = 64;

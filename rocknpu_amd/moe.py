@@ -41,7 +41,7 @@ class _ExpertsStruct(ctypes.Structure):
     """rocknpu_moe_experts_args (include/rocknpu_moe.h)."""
 
     _fields_ = ([(n, _vp) for n in ("a8", "a_scales", "gate", "up", "down", "gate_scales", "up_scales", "down_scales",
-                                    "weights", "plan", "out")]
+                                    "ids", "weights", "plan", "out")]
                 + [("tokens", _i64), ("out_row", _i64)]
                 + [(n, _i32) for n in ("experts", "top_k", "hidden", "hidden_pad", "ffn", "ffn_pad")]
                 + [("out_type", ctypes.c_uint32)])
@@ -201,7 +201,7 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
         raise ValueError(f"out has to be float32, float16 or bfloat16 [{tokens}, {weights.hidden}] on {at} with contiguous rows")
     args = _ExpertsStruct(
         a8.data_ptr(), a_scales.data_ptr(), weights.gate[0].data_ptr(), weights.up[0].data_ptr(), weights.down[0].data_ptr(),
-        weights.gate[1].data_ptr(), weights.up[1].data_ptr(), weights.down[1].data_ptr(), routing.weights.data_ptr(),
+        weights.gate[1].data_ptr(), weights.up[1].data_ptr(), weights.down[1].data_ptr(), routing.ids.data_ptr(), routing.weights.data_ptr(),
         routing.plan.data_ptr(), out.data_ptr(), tokens, hip._ld(out), weights.experts, top_k, weights.hidden,
         weights.hidden_pad, weights.ffn, weights.ffn_pad, TYPES[out.dtype])
     lib, ref = _lib.load(), ctypes.addressof(args)

@@ -88,14 +88,14 @@ def test_struct_layouts(name, struct, tmp_path):
 
 
 def experts_struct(**kw):
-    names = ("a8", "a_scales", "gate", "up", "down", "gate_scales", "up_scales", "down_scales", "weights", "plan", "out")
+    names = ("a8", "a_scales", "gate", "up", "down", "gate_scales", "up_scales", "down_scales", "ids", "weights", "plan", "out")
     base = dict.fromkeys(names, AT) | dict(tokens=5, out_row=100, experts=8, top_k=2, hidden=100, hidden_pad=128, ffn=60, ffn_pad=64, out_type=0)
     return moe._ExpertsStruct(**{**base, **kw})
 
 
 @pytest.mark.parametrize("bad", [
-    *(dict([(n, 0)]) for n, _ in moe._ExpertsStruct._fields_[:11]), *(dict([(n, AT + 8)]) for n in ("a8", "gate", "up", "down")),
-    *(dict([(n, AT + 2)]) for n in ("a_scales", "gate_scales", "up_scales", "down_scales", "weights", "plan", "out")), dict(out_type=2, out=AT + 1),
+    *(dict([(n, 0)]) for n, _ in moe._ExpertsStruct._fields_[:12]), *(dict([(n, AT + 8)]) for n in ("a8", "gate", "up", "down")),
+    *(dict([(n, AT + 2)]) for n in ("a_scales", "gate_scales", "up_scales", "down_scales", "ids", "weights", "plan", "out")), dict(out_type=2, out=AT + 1),
     dict(out_type=3), dict(tokens=-1), dict(tokens=1 << 28), dict(out_row=-1), dict(out_row=99), dict(experts=0), dict(experts=1025), dict(top_k=0),
     dict(top_k=9), dict(hidden=0), dict(hidden=129), dict(hidden_pad=120), dict(hidden_pad=0), dict(hidden_pad=133184), dict(ffn=0), dict(ffn=65),
     dict(ffn_pad=100), dict(ffn_pad=133184), dict(workspace=0), dict(workspace=AT + 16), dict(short=1)], ids=str)

@@ -8,7 +8,7 @@
 // of whose products row 0 is kept (lanes 0 - 15, first register). Sums over K are
 // exact int32, so waves may share a row's K and add up in LDS.
 //
-// A token's output is worked out by one workgroup per 16 columns, which quantises
+// A token's output is worked out by one workgroup per 8 columns, which quantises
 // the rows of all its choices itself: no launch for that, and none for the weighted
 // sum. Its weights are asked for before.
 #include "gemm_dma.h"
@@ -76,28 +76,32 @@ __global__ __launch_bounds__(kGateWaves * 64) void decode_gate_kernel(const MoeD
 // A barrier for what is in LDS: a fenced one would wait for the weights' loads too.
 __device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// 16 columns of one token's output. LDS: the codes of its choices' rows
-// [top_k][ffn_pad], then the largest magnitudes' bits [top_k] and the sums
-// [top_k][share][16]. `share` of the W waves take a choice's K together.
+// 8 columns of one token's output: the instruction's 16 columns are 8 weight rows
+// twice, with one 64-byte chunk of K and with the next, and its rows 0 and 1 those
+// chunks' codes, so loads are whole 128-byte lines and twice as many workgroups have
+// work (16 columns: 11.7 us for 8 choices of 2048 x 1024). LDS: the codes of
+// its choices' rows [top_k][ffn_pad] and 64 zeros, then the largest magnitudes' bits
+// [top_k] and the sums [top_k][share][16]. `share` of the W waves take a choice's K together.
 template <typename T, int W, int HOLD>
 __global__ __launch_bounds__(W * 64) void decode_down_kernel(const MoeDecode p, int share, T* __restrict__ out, int64_t out_row) {
     extern __shared__ __align__(16) int8_t codes[];
-    const int token = blockIdx.y, c0 = blockIdx.x * 16;
+    const int token = blockIdx.y, c0 = blockIdx.x * 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, q = lane >> 4;
-    const int k = p.ffn_pad, chunks = k / 64, n = p.top_k;
-    uint32_t* peaks = reinterpret_cast<uint32_t*>(codes + static_cast<int64_t>(n) * k);
+    const int col = lane & 7, second = lane >> 3 & 1, q = lane >> 4;
+    const int k = p.ffn_pad, chunks = k / 64, pairs = (chunks + 1) / 2, n = p.top_k;
+    uint32_t* peaks = reinterpret_cast<uint32_t*>(codes + static_cast<int64_t>(n) * k + 64);
     int* sums = reinterpret_cast<int*>(peaks + n);
     const int32_t* ids = p.ids + static_cast<int64_t>(token) * n;
     const int first = wave / share, part = wave % share, step = W / share;
     const int last_row = min(c0 + col, p.hidden - 1);
-    constexpr int R = 2 * kRing;
+    constexpr int R = HOLD <= 2 ? kRing : 2 * kRing;  // pairs of chunks that a wave asks for at once
     v4i ring[R];
     const auto ask = [&](int s, int i0) {  // a wave's next chunks of choice s
         const int e = max(row_of(ids, min(s, n - 1), p.experts), 0);
         const int8_t* w = p.down + (static_cast<int64_t>(e) * p.hidden + last_row) * k + q * 16;
 #pragma unroll
-        for (int i = 0; i < R; ++i) ring[i] = *reinterpret_cast<const v4i*>(w + min(i0 + share * i, chunks - 1) * 64);
+        for (int i = 0; i < R; ++i)
+            ring[i] = *reinterpret_cast<const v4i*>(w + min(2 * (i0 + share * i) + second, chunks - 1) * 64);
     };
     const float* values = p.values + static_cast<int64_t>(token) * n * k;
     const int runs = (k + 255) / 256;
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(W * 64) void decode_down_kernel(const MoeDecode p, 
     // runs do the last one's again. (A row that nothing was chosen for holds anything; its
     // codes and peak are not used.)
     const int mine = min(first, n - 1);
-    const int own = min(static_cast<int>(threadIdx.x >> 4), n - 1);  // thread 16 s + c: choice s, column c
+    const int own = min(static_cast<int>(threadIdx.x >> 3), n - 1);  // thread 8 s + c: choice s, column c
     const int own_e = row_of(ids, own, p.experts);
     float4 held[HOLD];
 #pragma unroll
@@ -121,6 +125,8 @@ __global__ __launch_bounds__(W * 64) void decode_down_kernel(const MoeDecode p, 
     const float own_weight = p.weights[static_cast<int64_t>(token) * n + own];
     const float own_scale = p.down_scales[static_cast<int64_t>(max(own_e, 0)) * p.hidden + last_row];
     if (threadIdx.x < n) peaks[threadIdx.x] = 0;
+    int8_t* zeros = codes + static_cast<int64_t>(n) * k;
+    if (threadIdx.x < 16) reinterpret_cast<int*>(zeros)[threadIdx.x] = 0;
     barrier();
     const auto peak_of = [&](int s, float4 v) {
         const uint32_t b = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
@@ -152,40 +158,36 @@ __global__ __launch_bounds__(W * 64) void decode_down_kernel(const MoeDecode p, 
 
     for (int s = first; s < n; s += step) {
         v4i acc = {};
-        for (int i0 = part; i0 < chunks; i0 += share * R) {
+        for (int i0 = part; i0 < pairs; i0 += share * R) {
             v4i w[R];
 #pragma unroll
             for (int i = 0; i < R; ++i) w[i] = ring[i];
-            const bool more = i0 + share * R < chunks;
-            ask(more ? s : s + step, more ? i0 + share * R : part);
+            const bool more = i0 + share * R < pairs;
+            if (more || s + step < n) ask(more ? s : s + step, more ? i0 + share * R : part);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const int c = i0 + share * i;
-                v4i a = *reinterpret_cast<const v4i*>(codes + static_cast<int64_t>(s) * k + min(c, chunks - 1) * 64 + q * 16);
-                if (c >= chunks) a = v4i{};
+                const int c = 2 * (i0 + share * i) + (lane & 1);  // of the codes' row lane % 16: 0 or 1
+                const v4i a = *reinterpret_cast<const v4i*>((c < chunks ? codes + static_cast<int64_t>(s) * k + c * 64 : zeros) + q * 16);
                 acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, w[i], acc, 0, 0, 0);
             }
         }
-        if (lane < 16) sums[(s * share + part) * 16 + lane] = acc[0];
+        if (lane < 16) sums[(s * share + part) * 16 + lane] = lane < 8 ? acc[0] : acc[1];
     }
     barrier();
     // the choices' weighted values side by side, in place of their sums; then one after the other
     float* terms = reinterpret_cast<float*>(sums);
     const auto term = [&](int s, int e, float weight, float w_scale) {
         int total = 0;
-        for (int j = 0; j < share; ++j) total += sums[(s * share + j) * 16 + col];
+        for (int j = 0; j < share; ++j) total += sums[(s * share + j) * 16 + col] + sums[(s * share + j) * 16 + 8 + col];
         const uint32_t peak = peaks[s];
         const float scale = peak > 0x7f7fffffu ? __builtin_nanf("") : peak == 0 ? 1.0f : __uint_as_float(peak) / 127.0f;
         const float d = (static_cast<float>(total) * scale) * w_scale;
         terms[s * share * 16 + col] = e < 0 ? 0.0f : weight * d;
     };
-    if (threadIdx.x < 16 * n) term(own, own_e, own_weight, own_scale);
-    for (int s = (threadIdx.x >> 4) + 4 * W; s < n; s += 4 * W) {
-        const int e = row_of(ids, s, p.experts);
-        term(s, e, p.weights[static_cast<int64_t>(token) * n + s], p.down_scales[static_cast<int64_t>(max(e, 0)) * p.hidden + last_row]);
-    }
+    static_assert(8 * W >= ROCKNPU_MOE_MAX_TOP_K, "a thread for each choice's column");
+    if (threadIdx.x < 8 * n) term(own, own_e, own_weight, own_scale);
     barrier();
-    if (threadIdx.x < 16 && c0 + col < p.hidden) {
+    if (threadIdx.x < 8 && c0 + col < p.hidden) {
         float sum = 0.0f;
         for (int s = 0; s < n; ++s)
             if (row_of(ids, s, p.experts) >= 0) sum += terms[s * share * 16 + col];
@@ -196,12 +198,12 @@ __global__ __launch_bounds__(W * 64) void decode_down_kernel(const MoeDecode p, 
 constexpr int kDownWaves = 16;
 int share_of(int top_k) { return top_k >= kDownWaves ? 1 : kDownWaves / top_k; }
 size_t down_lds(int top_k, int ffn_pad) {
-    return static_cast<size_t>(top_k) * ffn_pad + static_cast<size_t>(top_k) * 4 * (1 + 16 * share_of(top_k));
+    return static_cast<size_t>(top_k) * ffn_pad + 64 + static_cast<size_t>(top_k) * 4 * (1 + 16 * share_of(top_k));
 }
 
 template <typename T>
 int launch_down(const MoeDecode& p, void* out, int64_t out_row, hipStream_t stream) {
-    const dim3 grid((p.hidden + 15) / 16, p.tokens), block(kDownWaves * 64);
+    const dim3 grid((p.hidden + 7) / 8, p.tokens), block(kDownWaves * 64);
     const int share = share_of(p.top_k), runs = (p.ffn_pad + 255) / 256;
     const size_t lds = down_lds(p.top_k, p.ffn_pad);
     if (runs <= 2 * share)

@@ -7,6 +7,7 @@ memory and streams; the computation is the gfx950 kernels of the library.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 
 import torch
@@ -27,27 +28,23 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-class on_device:
-    """Gives the current stream of `device` and makes that device the current
-    one for the launch where it is another."""
+def stream_of(device: torch.device) -> tuple[int, int]:
+    """(index, current stream) of a GPU."""
+    if device.type != "cuda":
+        raise ValueError(f"the tensors are on {device}: a GPU's are wanted")
+    index = device.index
+    if index is None:
+        index = torch.cuda.current_device()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the stream without its object, where torch offers that
+    return index, torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
 
-    __slots__ = ("device", "back")
 
-    def __init__(self, device: torch.device):
-        self.device = device
-
-    def __enter__(self) -> int:
-        if self.device.type != "cuda":
-            raise ValueError(f"the tensors are on {self.device}: a GPU's are wanted")
-        now, index = torch.cuda.current_device(), self.device.index
-        self.back = now if index is not None and index != now else None
-        if self.back is not None:
-            torch.cuda.set_device(index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *_):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
+def call_on(index: int, function, *args) -> int:
+    """function(*args) with GPU `index` the current one."""
+    if torch.cuda.current_device() == index:
+        return function(*args)
+    with torch.cuda.device(index):
+        return function(*args)
 
 
 def _ptr(t):
@@ -109,11 +106,9 @@ class _NormStruct(ctypes.Structure):
                 + [("type", ctypes.c_uint32), ("weight_type", ctypes.c_uint32), ("eps", ctypes.c_float)])
 
 
-def _like(t, x, what):
-    """`t` has x's shape, type and device, and rows that are contiguous: its row stride."""
-    if t.shape != x.shape or t.dtype is not x.dtype or t.device != x.device or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what} has to be {x.dtype} {tuple(x.shape)} on {x.device} with contiguous rows")
-    return _ld(t)
+# The same bytes without an object: a serving step makes these calls per layer and
+# token, and a ctypes structure costs as much as all their checks.
+_pack_norm = struct.Struct("@7P7q2If0q").pack
 
 
 def norm_a8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: torch.Tensor | None = None, *,
@@ -126,37 +121,48 @@ def norm_a8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: 
     itself) and None without a residual. `out`, if given, takes the normed rows
     in x's type as well. The codes are those of the row x + residual times
     weight, the norm's factor is in the scales alone."""
-    if x.dim() != 2 or x.dtype not in TYPES:
-        raise ValueError(f"x has to be float32, float16 or bfloat16 [m, k], not {x.dtype} {tuple(x.shape)}")
-    m, k = x.shape
-    at = x.device
-    if weight.shape != (k,) or not weight.is_contiguous() or weight.device != at or weight.dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"weight has to be contiguous float32 or {x.dtype} [{k}] on {at}")
-    if hidden is not None and residual is None:
+    kind, shape, at = x.dtype, x.shape, x.device
+    if kind not in TYPES or len(shape) != 2:
+        raise ValueError(f"x has to be float32, float16 or bfloat16 [m, k], not {kind} {tuple(shape)}")
+    m, k = shape
+    if weight.shape != shape[1:] or not weight.is_contiguous() or weight.device != at or weight.dtype not in (torch.float32, kind):
+        raise ValueError(f"weight has to be contiguous float32 or {kind} [{k}] on {at}")
+
+    def rows(t, what):
+        if t.shape != shape or t.dtype is not kind or t.device != at or (t.stride(1) != 1 and k > 1):
+            raise ValueError(f"{what} has to be {kind} {tuple(shape)} on {at} with contiguous rows")
+        return t.data_ptr(), t.stride(0) if m > 1 else k
+
+    x_at, x_row = rows(x, "x")
+    r_at, r_row, h_at, h_row, o_at, o_row = None, 0, None, 0, None, 0
+    if residual is not None:
+        r_at, r_row = rows(residual, "residual")
+        if hidden is None:
+            hidden = torch.empty_like(x) if x_row == k else x.new_empty(shape)
+            h_at, h_row = hidden.data_ptr(), k
+        else:
+            h_at, h_row = rows(hidden, "hidden")
+    elif hidden is not None:
         raise ValueError("hidden is x + residual: it needs a residual")
-    if out is not None and hidden is not None and out.data_ptr() == hidden.data_ptr() and m:
-        raise ValueError("out and hidden are the same memory")
+    if out is not None:
+        o_at, o_row = rows(out, "out")
+        if o_at == h_at and m:
+            raise ValueError("out and hidden are the same memory")
     kp = k_pad_of(k) if k_pad is None else k_pad
     if kp < k or kp >> 31:
         raise ValueError(f"k_pad {kp} is not in [{k}, 2^31)")
     if a8 is None:
-        a8 = torch.empty((m, kp), dtype=torch.int8, device=at)
+        a8 = x.new_empty((m, kp), dtype=torch.int8)
     elif a8.shape != (m, kp) or a8.dtype is not torch.int8 or a8.device != at or not a8.is_contiguous():
         raise ValueError(f"a8 has to be contiguous int8 [{m}, {kp}] on {at}")
     if scales is None:
-        scales = torch.empty(m, dtype=torch.float32, device=at)
+        scales = x.new_empty((m,), dtype=torch.float32)
     elif scales.shape != (m,) or scales.dtype is not torch.float32 or scales.device != at or not scales.is_contiguous():
         raise ValueError(f"scales have to be contiguous float32 [{m}] on {at}")
-    if residual is not None and hidden is None:
-        hidden = torch.empty((m, k), dtype=x.dtype, device=at)
-    args = _NormStruct(
-        x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
-        None if hidden is None else hidden.data_ptr(), None if out is None else out.data_ptr(), a8.data_ptr(),
-        scales.data_ptr(), m, k, kp, _like(x, x, "x"), 0 if residual is None else _like(residual, x, "residual"),
-        0 if hidden is None else _like(hidden, x, "hidden"), 0 if out is None else _like(out, x, "out"),
-        TYPES[x.dtype], TYPES[weight.dtype], eps)
-    with on_device(at) as stream:
-        _check(_lib.load().rocknpu_hip_norm_a8(ctypes.addressof(args), stream), "norm_a8")
+    args = _pack_norm(x_at, r_at or 0, weight.data_ptr(), h_at or 0, o_at or 0, a8.data_ptr(), scales.data_ptr(), m, k, kp,
+                      x_row, r_row, h_row, o_row, TYPES[kind], TYPES[weight.dtype], eps)
+    index, stream = stream_of(at)
+    _check(call_on(index, _lib.load().rocknpu_hip_norm_a8, args, stream), "norm_a8")
     return a8, scales, hidden
 
 

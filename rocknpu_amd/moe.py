@@ -11,6 +11,7 @@ graph.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -45,6 +46,11 @@ class _ExpertsStruct(ctypes.Structure):
                 + [("tokens", _i64), ("out_row", _i64)]
                 + [(n, _i32) for n in ("experts", "top_k", "hidden", "hidden_pad", "ffn", "ffn_pad")]
                 + [("out_type", ctypes.c_uint32)])
+
+
+# The same bytes without an object, as hip's.
+_pack_route = struct.Struct("@5P2qI7if0q").pack
+_pack_experts = struct.Struct("@12P2q6iI0q").pack
 
 
 class Routing:
@@ -116,14 +122,14 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
                          f"most {MAX_GROUPS}, and the chosen ones have to hold top_k experts")
     if not 1 <= group_top <= min(2, experts // groups):
         raise ValueError(f"group_top {group_top} is neither 1 nor 2, or more than a group's experts")
-    ids = torch.empty((tokens, top_k), dtype=torch.int32, device=at)
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=at)
-    plan = torch.empty(words, dtype=torch.int32, device=at)
-    args = _RouteStruct(logits.data_ptr(), None if bias is None else bias.data_ptr(), ids.data_ptr(), weights.data_ptr(),
-                        plan.data_ptr(), tokens, hip._ld(logits), TYPES[logits.dtype], experts, top_k, groups, top_groups,
-                        group_top, SCORES[score], normalise, factor)
-    with hip.on_device(at) as stream:
-        hip._check(_lib.load().rocknpu_hip_moe_route(ctypes.addressof(args), stream), "moe_route")
+    ids = logits.new_empty((tokens, top_k), dtype=torch.int32)
+    weights = logits.new_empty((tokens, top_k), dtype=torch.float32)
+    plan = logits.new_empty((words,), dtype=torch.int32)
+    args = _pack_route(logits.data_ptr(), 0 if bias is None else bias.data_ptr(), ids.data_ptr(), weights.data_ptr(),
+                       plan.data_ptr(), tokens, logits.stride(0) if tokens > 1 else experts, TYPES[logits.dtype], experts, top_k,
+                       groups, top_groups, group_top, SCORES[score], normalise, factor)
+    index, stream = hip.stream_of(at)
+    hip._check(hip.call_on(index, _lib.load().rocknpu_hip_moe_route, args, stream), "moe_route")
     return Routing(ids, weights, plan, experts)
 
 
@@ -145,7 +151,7 @@ class Experts:
     one matrix of experts * ffn (or hidden) rows. The tensors are used in place
     and kept alive by the object."""
 
-    __slots__ = ("gate", "up", "down", "experts", "hidden", "hidden_pad", "ffn", "ffn_pad", "device", "_needs")
+    __slots__ = ("gate", "up", "down", "experts", "hidden", "hidden_pad", "ffn", "ffn_pad", "device", "pointers", "_needs")
 
     def __init__(self, gate, up, down, *, hidden: int, ffn: int):
         experts = gate[0].shape[0] if gate[0].dim() == 3 else 0
@@ -160,6 +166,7 @@ class Experts:
         self.up = _pair(up, (experts, ffn, self.hidden_pad), "up", self.device)
         self.down = _pair(down, (experts, hidden, self.ffn_pad), "down", self.device)
         self.experts, self.hidden, self.ffn = experts, hidden, ffn
+        self.pointers = tuple(pair[i].data_ptr() for i in (0, 1) for pair in (self.gate, self.up, self.down))
         self._needs: dict[tuple[int, int], int] = {}  # workspace bytes by tokens and top_k
 
 
@@ -199,26 +206,27 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
         out = torch.empty((tokens, weights.hidden), dtype=dtype, device=at)
     elif out.dtype not in TYPES or out.shape != (tokens, weights.hidden) or out.device != at or (out.stride(1) != 1 and weights.hidden > 1):
         raise ValueError(f"out has to be float32, float16 or bfloat16 [{tokens}, {weights.hidden}] on {at} with contiguous rows")
-    args = _ExpertsStruct(
-        a8.data_ptr(), a_scales.data_ptr(), weights.gate[0].data_ptr(), weights.up[0].data_ptr(), weights.down[0].data_ptr(),
-        weights.gate[1].data_ptr(), weights.up[1].data_ptr(), weights.down[1].data_ptr(), routing.ids.data_ptr(), routing.weights.data_ptr(),
-        routing.plan.data_ptr(), out.data_ptr(), tokens, hip._ld(out), weights.experts, top_k, weights.hidden,
-        weights.hidden_pad, weights.ffn, weights.ffn_pad, TYPES[out.dtype])
-    lib, ref = _lib.load(), ctypes.addressof(args)
-    with hip.on_device(at) as stream:
-        need = weights._needs.get((tokens, top_k))
-        if need is None:
-            got = ctypes.c_size_t()
-            hip._check(lib.rocknpu_hip_moe_experts_workspace(ref, ctypes.addressof(got)), "moe_experts_workspace")
-            if len(weights._needs) >= 1024:
-                weights._needs.clear()
-            need = weights._needs[tokens, top_k] = got.value
-        ws, nbytes = None, 0
-        if need:
-            if workspace is None:
-                workspace = workspace_for(at, need)
-            elif workspace.device != at or not workspace.is_contiguous():
-                raise ValueError(f"workspace has to be a contiguous tensor on {at}")
-            ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        hip._check(lib.rocknpu_hip_moe_experts(ref, ws, nbytes, stream), "moe_experts")
+    key = hip.stream_of(at)
+    args = _pack_experts(
+        a8.data_ptr(), a_scales.data_ptr(), *weights.pointers, routing.ids.data_ptr(), routing.weights.data_ptr(),
+        routing.plan.data_ptr(), out.data_ptr(), tokens, out.stride(0) if tokens > 1 else weights.hidden, weights.experts, top_k,
+        weights.hidden, weights.hidden_pad, weights.ffn, weights.ffn_pad, TYPES[out.dtype])
+    lib = _lib.load()
+    need = weights._needs.get((tokens, top_k))
+    if need is None:
+        got = ctypes.c_size_t()
+        hip._check(lib.rocknpu_hip_moe_experts_workspace(args, ctypes.addressof(got)), "moe_experts_workspace")
+        if len(weights._needs) >= 1024:
+            weights._needs.clear()
+        need = weights._needs[tokens, top_k] = got.value
+    if workspace is None:
+        workspace = _workspaces.get(key)  # the stream's own
+        if workspace is None or workspace.numel() < need:
+            workspace = workspace_for(at, need)
+        nbytes = workspace.numel()
+    elif workspace.device != at or not workspace.is_contiguous():
+        raise ValueError(f"workspace has to be a contiguous tensor on {at}")
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+    hip._check(hip.call_on(key[0], lib.rocknpu_hip_moe_experts, args, workspace.data_ptr(), nbytes, key[1]), "moe_experts")
     return out

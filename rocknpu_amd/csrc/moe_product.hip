@@ -30,12 +30,12 @@ constexpr int kMoeManyTiles = 64;
 // One tile: rows r0 .. end - 1 (at most BME) of the plan's order, expert e, output
 // columns from c0. `stages(A?, stage)` names the stage buffers, distinct arrays, so
 // that a wait for one does not wait for all.
-template <int BME, int BN, int WM, int WN, int ST, int KB, bool GATED, typename SA, typename SB>
+template <int BME, int BN, int WM, int WN, int ST, int KB, int D, bool GATED, typename SA, typename SB>
 __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t* __restrict__ order, int rows, int e, int r0,
                                              int end, int c0, SA stage_a, SB stage_b, float* lsc) {
     using Cfg = DmaTile<BME, BN, WM, WN, KB>;
     constexpr int TN = BN / WN, FM = BME / WM / 32, FN = TN / 32;
-    constexpr int SUB = KB / 64, CPR = KB / 16, THREADS = WM * WN * 64;
+    constexpr int CPR = KB / 16, THREADS = WM * WN * 64;
     static_assert(FM * WM * 32 == BME && FN * WN * 32 == BN && (!GATED || FN % 2 == 0), "whole fragments, gate's and up's in pairs");
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -87,38 +87,40 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = v16i{};
 
-    const int KS = k / KB;  // stages
-    const int KT = k / 64;  // 64-deep steps
+    // A step multiplies D 32-deep halves of 64 while the fragments of the next step are
+    // read into the other register set.
+    constexpr int SUB = KB / (32 * D);  // steps of a stage
+    const int KS = k / KB;              // stages
+    const int KT = KS * SUB;            // steps
     using S0 = std::integral_constant<int, 0>;
-    using H0 = std::integral_constant<int, 0>;
-    using H1 = std::integral_constant<int, 1>;
     using R0 = std::integral_constant<int, 0>;
     constexpr int PER_STAGE = Cfg::A_SEG + Cfg::B_SEG;
-    v4i fa[2][2][FM], fb[2][2][FN];  // [register set][32-deep half][fragment]
-    // lane l supplies row l % 32 and the 16 bytes of chunk 4 u + 2 h + l / 32; fragment i of
-    // wave column wm holds tile rows 32 (WM i + wm) ..
-    auto read_half = [&](auto st, auto set, auto u, auto h) {
-        constexpr int R = decltype(set)::value, H = decltype(h)::value, SU = decltype(u)::value;
+    v4i fa[2][D][FM], fb[2][D][FN];  // [register set][32-deep half][fragment]
+    // lane l supplies row l % 32 and the 16 bytes of chunk 2 h + l / 32 of half h; fragment i
+    // of wave column wm holds tile rows 32 (WM i + wm) ..
+    auto read_frags = [&](auto st, auto set, auto u) {
+        constexpr int R = decltype(set)::value, SU = decltype(u)::value;
         const int8_t* la = stage_a(st);
         const int8_t* lb = stage_b(st);
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-            fa[R][H][i] = *reinterpret_cast<const v4i*>(la + swz_kb<KB>((i * WM + wm) * 32 + (lane & 31), 4 * SU + 2 * H + half));
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-            fb[R][H][j] = *reinterpret_cast<const v4i*>(lb + swz_kb<KB>(wn * TN + j * 32 + (lane & 31), 4 * SU + 2 * H + half));
-    };
-    auto read_frags = [&](auto st, auto set, auto u) {
-        read_half(st, set, u, H0{});
-        read_half(st, set, u, H1{});
-    };
-    auto mfma_half = [&](auto set, auto h) {
-        constexpr int R = decltype(set)::value, H = decltype(h)::value;
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
+        for (int h = 0; h < D; ++h) {
 #pragma unroll
             for (int i = 0; i < FM; ++i)
-                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[R][H][i], fb[R][H][j], acc[i][j], 0, 0, 0);
+                fa[R][h][i] = *reinterpret_cast<const v4i*>(la + swz_kb<KB>((i * WM + wm) * 32 + (lane & 31), 2 * (D * SU + h) + half));
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                fb[R][h][j] = *reinterpret_cast<const v4i*>(lb + swz_kb<KB>(wn * TN + j * 32 + (lane & 31), 2 * (D * SU + h) + half));
+        }
+    };
+    auto mfma = [&](auto set) {
+        constexpr int R = decltype(set)::value;
+#pragma unroll
+        for (int h = 0; h < D; ++h)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[R][h][i], fb[R][h][j], acc[i][j], 0, 0, 0);
     };
     // The tile's scales: each thread loads one or two before the stages (older than
     // their loads, so the waits' counts hold) and writes them to LDS once the first
@@ -142,7 +144,7 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
     __builtin_amdgcn_s_barrier();
     issue(std::integral_constant<int, ST - 1>{}, min(ST - 1, KS - 1));
     read_frags(S0{}, R0{}, S0{});
-    // One 64-deep step, as in gemm.hip: the fragments of step j were read in step j-1;
+    // A step, as in gemm.hip: the fragments of step j were read in step j-1;
     // the last step of a stage waits for the next one, passes the barrier that frees
     // the stage's buffer, and refills it.
     auto step = [&](auto set, auto next_st, auto next_u, auto refill_st, auto last_of_stage, int q) {
@@ -155,9 +157,8 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
             issue(refill_st, min(q + ST, KS - 1));
         }
         read_frags(next_st, NSET{}, next_u);
-        mfma_half(set, H0{});
-        mfma_half(set, H1{});
-        constexpr int READS = 2 * (FM + FN), MFMAS = 2 * FM * FN;
+        mfma(set);
+        constexpr int READS = D * (FM + FN), MFMAS = D * FM * FN;
         if constexpr (LAST && READS % PER_STAGE == 0 && MFMAS % PER_STAGE == 0) {
 #pragma unroll
             for (int i = 0; i < PER_STAGE; ++i) {
@@ -221,7 +222,7 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
     }
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
+template <int BM, int BN, int WM, int WN, int ST, int KB, int D, bool GATED>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p, const MoePlan plan) {
     static_assert(ST >= 2 && ST <= 4, "two to four stage buffers");
     __shared__ __align__(16) int8_t la0[BM * KB], la1[BM * KB], la2[ST > 2 ? BM * KB : 16], la3[ST > 3 ? BM * KB : 16];
@@ -243,8 +244,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
     // contiguous range; with few, in which a range's full and partly filled tiles
     // would not even out, an eighth of the columns of every row tile (and a range of
     // the columns that are left over). What an XCD's CUs would run in a last round
-    // that is at most half full runs in halves (of the columns), at most a quarter
-    // full in quarters.
+    // that is at most half full runs in halves (of the rows), at most a quarter full in
+    // quarters.
     constexpr int BC = GATED ? BN / 2 : BN;  // output columns of a tile
     constexpr int GM = 4;
     const int tiles_m = uniform(min(*plan.tile_count, plan.max_tiles)), tiles_n = (p.n + BC - 1) / BC;
@@ -270,27 +271,27 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
     const int tn = (t % (GM * wide)) / gsize + (is_own ? xcd * eighth : 8 * eighth);
     const int e = uniform(min(max(plan.tiles[2 * tm], 0), plan.experts - 1));
     int r0 = uniform(min(max(plan.tiles[2 * tm + 1], 0), plan.rows));
-    const int end = uniform(min(min(plan.offsets[e + 1], plan.rows), r0 + BM));
-    int c0 = tn * BC;
-    if (BM == 256 && i >= mine - rest && parts > 1) {
-        c0 += part % 2 * (BC / 2);
-        r0 += part / 2 * (BM / 2);
-        if (r0 >= end || c0 >= p.n) return;
-        const int last = parts == 4 ? min(end, r0 + BM / 2) : end, n = last - r0;
-#define RK_PART(BME) product_tile<BME, BN / 2, WM, WN, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, last, c0, stage_a, stage_b, lsc)
-        if constexpr (BM == 256) {
+    int end = uniform(min(min(plan.offsets[e + 1], plan.rows), r0 + BM));
+    const int c0 = tn * BC;
+    if constexpr (BM == 256)
+        if (parts > 1 && i >= mine - rest) {
+            r0 += part / 2 * (BM / 2);
+            if (parts == 4) end = min(end, r0 + BM / 2);
+            const int c1 = c0 + part % 2 * (BC / 2), n = end - r0;
+            if (n <= 0 || c1 >= p.n) return;
+#define RK_PART(BME) product_tile<BME, BN / 2, WN, WM, ST, KB, D, GATED>(p, plan.order, plan.rows, e, r0, end, c1, stage_a, stage_b, lsc)
             if (n > 128) return RK_PART(256);
-            if (n > 64) return RK_PART(128);
-            return RK_PART(64);
-        }
+            return RK_PART(128);
 #undef RK_PART
-    }
+        }
     const int n = end - r0;
     if (n <= 0) return;
-#define RK_TILE(BME) product_tile<BME, BN, WM, WN, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, end, c0, stage_a, stage_b, lsc)
+#define RK_TILE(BME) product_tile<BME, BN, WM, WN, ST, KB, D, GATED>(p, plan.order, plan.rows, e, r0, end, c0, stage_a, stage_b, lsc)
     if constexpr (BM == 256) {
-        if (n > 192) return RK_TILE(256);
-        if (n > 128) return RK_TILE(192);
+        // (192 rows of 64 bytes are not whole segments for 8 waves)
+        if (n > (KB == 128 ? 192 : 128)) return RK_TILE(256);
+        if constexpr (KB == 128)
+            if (n > 128) return RK_TILE(192);
         if (n > 64) return RK_TILE(128);
         return RK_TILE(64);
     } else {
@@ -300,14 +301,14 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
 #undef RK_TILE
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
+template <int BM, int BN, int WM, int WN, int ST, int KB, int D, bool GATED>
 int launch(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
     constexpr int BC = GATED ? BN / 2 : BN;
     // a split last round has up to as many workgroups as the GPU has CUs
     const int64_t tiles = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
     const int64_t grid = (tiles + 7) / 8 * 8 + 8 + (BM == 256 ? 8 * static_cast<int64_t>(p.xcd_cus) : 0);
     if (grid > 0x7fffffff) return kStatusInvalid;
-    product_kernel<BM, BN, WM, WN, ST, KB, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
+    product_kernel<BM, BN, WM, WN, ST, KB, D, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
@@ -315,11 +316,11 @@ template <bool GATED>
 int route(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
     // 128-byte stages need K % 128 == 0 (a stage never reads past a row)
     if (plan.tile_rows == 256) {
-        if (p.k % 128 == 0) return launch<256, 256, 2, 2, 2, 128, GATED>(p, plan, stream);
-        return launch<256, 256, 2, 2, 4, 64, GATED>(p, plan, stream);
+        if (p.k % 128 == 0) return launch<256, 256, 2, 4, 2, 128, 1, GATED>(p, plan, stream);
+        return launch<256, 256, 2, 4, 4, 64, 1, GATED>(p, plan, stream);
     }
-    if (p.k % 128 == 0) return launch<64, 128, 1, 2, 3, 128, GATED>(p, plan, stream);
-    return launch<64, 128, 1, 2, 4, 64, GATED>(p, plan, stream);
+    if (p.k % 128 == 0) return launch<64, 128, 1, 2, 3, 128, 2, GATED>(p, plan, stream);
+    return launch<64, 128, 1, 2, 4, 64, 2, GATED>(p, plan, stream);
 }
 
 }  // namespace

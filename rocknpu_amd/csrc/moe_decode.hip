@@ -215,9 +215,17 @@ int launch_down(const MoeDecode& p, void* out, int64_t out_row, hipStream_t stre
 
 }  // namespace
 
-// Tokens up to which weights are read once a choice, however many choices share an
-// expert; the rows' codes have to fit LDS.
-bool moe_decodes(int64_t tokens, int top_k, int ffn_pad) { return tokens <= 4 && down_lds(top_k, ffn_pad) <= 128 * 1024; }
+// Whether a call goes choice by choice: one token's choices always, more tokens' while
+// few of them fall on an expert that another has already called for (its weights are
+// read again). By choices and by tiles, us in a graph: 64 experts of 2048 x 1024, top 8,
+// of 1, 3, 4 and 8 tokens 16.4 and 23.2, 37.8 and 40.4, 48.6 and 45.8, 82 and 67; 8 of
+// 4096 x 14336, top 2, of 1, 2 and 3: 83 and 117, 150 and 162, 215 and 194; 128 of 2048 x
+// 768, top 8, of 3 and 4: 34.1 and 35.2, 42.0 and 40.6; 16 of 2048 x 5632, top 1, of 8
+// and 12: 70 and 78, 97 and 84. The rows' codes have to fit LDS.
+bool moe_decodes(int64_t tokens, int experts, int top_k, int ffn_pad) {
+    const int64_t rows = tokens * top_k;
+    return (tokens == 1 || (rows <= 28 && 2 * rows <= experts)) && down_lds(top_k, ffn_pad) <= 128 * 1024;
+}
 
 int launch_moe_decode(const MoeDecode& p, uint32_t out_type, void* out, int64_t out_row, hipStream_t stream) {
     const dim3 grid(p.tokens * p.top_k, p.ffn_pad / 16);

@@ -115,7 +115,7 @@ extern "C" int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args* args, voi
     float* values = reinterpret_cast<float*>(at);
     int8_t* codes = reinterpret_cast<int8_t*>(at + sp.values);
     float* scales = reinterpret_cast<float*>(at + sp.values + sp.codes);
-    if (moe_decodes(a.tokens, a.top_k, a.ffn_pad)) {
+    if (moe_decodes(a.tokens, a.experts, a.top_k, a.ffn_pad)) {
         const MoeDecode d{a.a8, a.a_scales, a.gate, a.up, a.down, a.gate_scales, a.up_scales, a.down_scales, a.ids, a.weights,
                           values, static_cast<int>(a.tokens), a.experts, a.top_k, a.hidden, a.hidden_pad, a.ffn, a.ffn_pad};
         return launch_moe_decode(d, a.out_type, a.out, a.out_row, s);

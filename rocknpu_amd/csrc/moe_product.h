@@ -37,7 +37,7 @@ struct MoeDecode {
     float* values;
     int tokens, experts, top_k, hidden, hidden_pad, ffn, ffn_pad;
 };
-bool moe_decodes(int64_t tokens, int top_k, int ffn_pad);
+bool moe_decodes(int64_t tokens, int experts, int top_k, int ffn_pad);
 int launch_moe_decode(const MoeDecode& p, uint32_t out_type, void* out, int64_t out_row, hipStream_t stream);
 
 // f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, to 2^-50 of the value:

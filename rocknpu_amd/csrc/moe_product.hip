@@ -248,7 +248,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
     // quarters.
     constexpr int BC = GATED ? BN / 2 : BN;  // output columns of a tile
     constexpr int GM = 4;
-    const int tiles_m = uniform(min(*plan.tile_count, plan.max_tiles)), tiles_n = (p.n + BC - 1) / BC;
+    const int tiles_m = uniform(max(min(*plan.tile_count, plan.max_tiles), 0)), tiles_n = (p.n + BC - 1) / BC;
     const int xcd = blockIdx.x & 7;
     const int eighth = tiles_m < kMoeManyTiles ? tiles_n >> 3 : 0;  // columns of each XCD's own
     const int own = eighth * tiles_m, shared = (tiles_n - 8 * eighth) * tiles_m;

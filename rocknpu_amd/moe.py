@@ -1,8 +1,11 @@
 """A feed-forward made of experts (include/rocknpu_moe.h) on device tensors.
 
     a8, a_scales, hidden = hip.norm_a8(x, norm_weight, residual=hidden)
+    logits = hip.gemm_w8a8(a8, a_scales, *router)
     routing = moe.route(logits, top_k)                  # which experts a token goes to
     out = moe.experts(weights, a8, a_scales, routing)   # the chosen experts' products, weighted and summed
+
+or, the four together, feed_forward.
 
 Calls enqueue on the tensors' device's current torch stream and return
 immediately; they read nothing on the host, so a step can be captured in a HIP
@@ -151,7 +154,10 @@ class Experts:
     one matrix of experts * ffn (or hidden) rows. The tensors are used in place
     and kept alive by the object."""
 
-    __slots__ = ("gate", "up", "down", "experts", "hidden", "hidden_pad", "ffn", "ffn_pad", "device", "pointers", "_needs")
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"the kernels use the {name} that the object was made with: make a new Experts")
+        object.__setattr__(self, name, value)
 
     def __init__(self, gate, up, down, *, hidden: int, ffn: int):
         experts = gate[0].shape[0] if gate[0].dim() == 3 else 0
@@ -230,3 +236,19 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
         nbytes = workspace.numel() * workspace.element_size()
     hip._check(hip.call_on(key[0], lib.rocknpu_hip_moe_experts, args, workspace.data_ptr(), nbytes, key[1]), "moe_experts")
     return out
+
+
+def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, router, weights: Experts, top_k: int, *, eps: float = 1e-5,
+                 residual: torch.Tensor | None = None, hidden: torch.Tensor | None = None, out: torch.Tensor | None = None, **routing):
+    """A layer's second half: hip.norm_a8 of x + residual, the router's product
+    (`router`: a W8 pair [experts, hidden_pad] and [experts], for an f32 router
+    hip.quantize_a8 of its rows), route with `routing`'s arguments, and experts.
+    Returns (out [tokens, hidden] in x's type, x + residual or None); the former
+    is the next norm's x, the latter its residual."""
+    a8, a_scales, hidden = hip.norm_a8(x, norm_weight, eps, residual, hidden=hidden)
+    if tuple(router[0].shape) != (weights.experts, weights.hidden_pad) or a8.shape[1] != weights.hidden_pad:
+        raise ValueError(f"x of {x.shape[1]} and a router {tuple(router[0].shape)} for {weights.experts} experts of {weights.hidden_pad}")
+    if x.shape[0] == 0:
+        return x.new_empty((0, weights.hidden)) if out is None else out, hidden
+    logits = hip.gemm_w8a8(a8, a_scales, *router)
+    return experts(weights, a8, a_scales, route(logits, top_k, **routing), dtype=x.dtype, out=out), hidden

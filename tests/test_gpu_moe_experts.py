@@ -241,3 +241,73 @@ def test_a_layer_of_quantised_weights():
     ids, weights, *_ = moe_ref.route(logits, top_k)
     assert np.array_equal(r.ids.cpu().numpy(), ids)
     verify(w, a8, scales, r, out)
+
+
+def whole_layer(dtype=torch.float32, tokens=37, experts=6, hidden=512, ffn=256):
+    g = torch.Generator().manual_seed(23)
+    w = layer(24, experts, hidden, ffn)
+    x, h = (torch.randn((tokens, hidden), generator=g).to(dtype).to(DEV) for _ in range(2))
+    norm = (1 + 0.1 * torch.randn(hidden, generator=g)).to(DEV)
+    return x, h, norm, hip.quantize_a8(torch.randn((experts, hidden), generator=g).to(DEV) / math.sqrt(hidden)), w
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_feed_forward_is_its_parts(dtype):
+    for tokens in (1, 3, 37, 700):
+        x, h, norm, router, w = whole_layer(dtype, tokens)
+        out, hidden = moe.feed_forward(x, norm, router, w, 2, residual=h, score="sigmoid", normalise=False)
+        a8, s, want_h = hip.norm_a8(x, norm, residual=h)
+        r = moe.route(hip.gemm_w8a8(a8, s, *router), 2, score="sigmoid", normalise=False)
+        assert torch.equal(hidden, want_h) and torch.equal(out, moe.experts(w, a8, s, r, dtype=dtype)) and out.dtype is dtype
+        alone, none = moe.feed_forward(x, norm, router, w, 2)
+        assert none is None and alone.shape == x.shape
+    x = x[:0]
+    assert moe.feed_forward(x, norm, router, w, 2, residual=x)[0].shape == (0, 512)
+    with pytest.raises(ValueError):
+        moe.feed_forward(h, norm, (router[0][:5], router[1][:5]), w, 2)
+
+
+def test_layers_in_a_graph():
+    """Two layers of norm, router, choice and experts as one graph, replayed on new rows."""
+    for tokens in (1, 60):
+        x, h, norm, router, w = whole_layer(torch.bfloat16, tokens)
+        second = layer(25, 6, 512, 256)
+
+        def step():
+            o, r = moe.feed_forward(x, norm, router, w, 2, residual=h)
+            return moe.feed_forward(o, norm, router, second, 2, residual=r)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                got = step()
+        for seed in range(4):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(50 + seed)))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(got, step()):
+                assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    """Calls on different streams have workspaces of their own."""
+    w = layer(26, 8, 256, 192)
+    jobs = []
+    for i, tokens in enumerate((300, 290)):
+        a8, s = tokens_of(60 + i, tokens, 256)
+        x = torch.randn((tokens, 8), generator=torch.Generator().manual_seed(70 + i)).to(DEV)
+        jobs.append((a8, s, x, moe.experts(w, a8, s, moe.route(x, 2)), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(8):
+        for i, (a8, s, x, _, stream) in enumerate(jobs):
+            with torch.cuda.stream(stream):
+                outs[i].append(moe.experts(w, a8, s, moe.route(x, 2)))
+    torch.cuda.synchronize()
+    for i, job in enumerate(jobs):
+        assert all(torch.equal(o, job[3]) for o in outs[i])

@@ -150,3 +150,18 @@ def test_streams_and_graphs():
         now = check(x, 4)
         for a, b in ((r.ids, now.ids), (r.weights, now.weights), (r.offsets, now.offsets), (r.order, now.order)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("experts,groups,top_groups,group_top,top_k", [(64, 1, 1, 1, 8), (256, 8, 4, 2, 8), (256, 1, 1, 1, 16), (16, 1, 1, 1, 14), (32, 4, 2, 1, 15), (60, 4, 3, 2, 6)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_scores_closer_than_f32(experts, groups, top_groups, group_top, top_k, score, with_bias):
+    """Logits on a coarse grid with differences around and below f32's last places, in pairs and in clusters."""
+    g = torch.Generator().manual_seed(experts + top_k)
+    x = torch.randint(-6, 7, (400, experts), generator=g) * 0.5 + 2.0 ** -21 * torch.randint(-3, 4, (400, experts), generator=g)
+    x[200:] = 0.25 * torch.randn((200, 1), generator=g) + 10.0 ** -torch.randint(4, 9, (200, experts), generator=g) * torch.randn((200, experts), generator=g)
+    b = {"bias": (torch.randint(0, 2, (experts,), generator=g) * 2.0 ** -20).to(DEV)} if with_bias else {}
+    check(x.to(DEV), top_k, score=score, groups=groups, top_groups=top_groups, group_top=group_top, **b)
+    if with_bias:
+        b["bias"] = 8.0 * b["bias"] * 2.0 ** 20 - 4.0  # beyond the keys' range
+        check(x.to(DEV), top_k, score=score, groups=groups, top_groups=top_groups, group_top=group_top, **b)

@@ -134,3 +134,11 @@ def test_refused_experts_in_python():
         a = {**args, **kw}
         with pytest.raises(ValueError):
             moe.experts(a.pop("weights"), a.pop("a8"), a.pop("a_scales"), a.pop("routing"), **a)
+
+
+def test_experts_keep_their_tensors():
+    i8, f = (lambda *s: torch.zeros(s, dtype=torch.int8)), torch.zeros
+    w = moe.Experts((i8(2, 3, 64), f(2, 3)), (i8(2, 3, 64), f(2, 3)), (i8(2, 5, 64), f(2, 5)), hidden=5, ffn=3)
+    for name in ("gate", "up", "down", "experts", "hidden", "ffn", "device", "pointers"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, None)

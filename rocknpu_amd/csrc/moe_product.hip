@@ -30,7 +30,7 @@ constexpr int kMoeManyTiles = 64;
 // One tile: rows r0 .. end - 1 (at most BME) of the plan's order, expert e, output
 // columns from c0. `stages(A?, stage)` names the stage buffers, distinct arrays, so
 // that a wait for one does not wait for all.
-template <int BME, int BN, int WM, int WN, int ST, int KB, int D, bool GATED, typename SA, typename SB>
+template <int BME, int BN, int WM, int WN, int ST, int KB, bool GATED, typename SA, typename SB>
 __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t* __restrict__ order, int rows, int e, int r0,
                                              int end, int c0, SA stage_a, SB stage_b, float* lsc) {
     using Cfg = DmaTile<BME, BN, WM, WN, KB>;
@@ -87,8 +87,9 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = v16i{};
 
-    // A step multiplies D 32-deep halves of 64 while the fragments of the next step are
-    // read into the other register set.
+    // A step multiplies 64 bytes of K, two 32-deep halves, while the fragments of the next
+    // step are read into the other register set.
+    constexpr int D = 2;
     constexpr int SUB = KB / (32 * D);  // steps of a stage
     const int KS = k / KB;              // stages
     const int KT = KS * SUB;            // steps
@@ -97,20 +98,29 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
     constexpr int PER_STAGE = Cfg::A_SEG + Cfg::B_SEG;
     v4i fa[2][D][FM], fb[2][D][FN];  // [register set][32-deep half][fragment]
     // lane l supplies row l % 32 and the 16 bytes of chunk 2 h + l / 32 of half h; fragment i
-    // of wave column wm holds tile rows 32 (WM i + wm) ..
+    // of wave column wm holds tile rows 32 (WM i + wm) .. A row's swizzle is the same in every
+    // fragment, and another half's place is an exclusive or away: worked out where it is
+    // read (an asm, or the compiler would keep all of them in registers that the
+    // accumulators leave no room for).
+    const int a0 = swz_kb<KB>(wm * 32 + (lane & 31), half), b0 = swz_kb<KB>(wn * TN + (lane & 31), half);
+    const auto at_half = [](int base, auto h) {
+        int at;
+        asm volatile("v_xor_b32 %0, %1, %2" : "=v"(at) : "i"(decltype(h)::value * 32), "v"(base));
+        return at;
+    };
     auto read_frags = [&](auto st, auto set, auto u) {
         constexpr int R = decltype(set)::value, SU = decltype(u)::value;
         const int8_t* la = stage_a(st);
         const int8_t* lb = stage_b(st);
+        unroll_seq([&](auto h) {
+            constexpr int H = decltype(h)::value;
+            using Half = std::integral_constant<int, D * SU + H>;
+            const int pa = at_half(a0, Half{}), pb = at_half(b0, Half{});
 #pragma unroll
-        for (int h = 0; h < D; ++h) {
+            for (int i = 0; i < FM; ++i) fa[R][H][i] = *reinterpret_cast<const v4i*>(la + pa + i * WM * 32 * KB);
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
-                fa[R][h][i] = *reinterpret_cast<const v4i*>(la + swz_kb<KB>((i * WM + wm) * 32 + (lane & 31), 2 * (D * SU + h) + half));
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                fb[R][h][j] = *reinterpret_cast<const v4i*>(lb + swz_kb<KB>(wn * TN + j * 32 + (lane & 31), 2 * (D * SU + h) + half));
-        }
+            for (int j = 0; j < FN; ++j) fb[R][H][j] = *reinterpret_cast<const v4i*>(lb + pb + j * 32 * KB);
+        }, std::make_integer_sequence<int, D>{});
     };
     auto mfma = [&](auto set) {
         constexpr int R = decltype(set)::value;
@@ -222,7 +232,7 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
     }
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int KB, int D, bool GATED>
+template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p, const MoePlan plan) {
     static_assert(ST >= 2 && ST <= 4, "two to four stage buffers");
     __shared__ __align__(16) int8_t la0[BM * KB], la1[BM * KB], la2[ST > 2 ? BM * KB : 16], la3[ST > 3 ? BM * KB : 16];
@@ -279,14 +289,14 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
             if (parts == 4) end = min(end, r0 + BM / 2);
             const int c1 = c0 + part % 2 * (BC / 2), n = end - r0;
             if (n <= 0 || c1 >= p.n) return;
-#define RK_PART(BME) product_tile<BME, BN / 2, WN, WM, ST, KB, D, GATED>(p, plan.order, plan.rows, e, r0, end, c1, stage_a, stage_b, lsc)
+#define RK_PART(BME) product_tile<BME, BN / 2, WN, WM, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, end, c1, stage_a, stage_b, lsc)
             if (n > 128) return RK_PART(256);
             return RK_PART(128);
 #undef RK_PART
         }
     const int n = end - r0;
     if (n <= 0) return;
-#define RK_TILE(BME) product_tile<BME, BN, WM, WN, ST, KB, D, GATED>(p, plan.order, plan.rows, e, r0, end, c0, stage_a, stage_b, lsc)
+#define RK_TILE(BME) product_tile<BME, BN, WM, WN, ST, KB, GATED>(p, plan.order, plan.rows, e, r0, end, c0, stage_a, stage_b, lsc)
     if constexpr (BM == 256) {
         // (192 rows of 64 bytes are not whole segments for 8 waves)
         if (n > (KB == 128 ? 192 : 128)) return RK_TILE(256);
@@ -301,14 +311,14 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const MoeProduct p
 #undef RK_TILE
 }
 
-template <int BM, int BN, int WM, int WN, int ST, int KB, int D, bool GATED>
+template <int BM, int BN, int WM, int WN, int ST, int KB, bool GATED>
 int launch(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
     constexpr int BC = GATED ? BN / 2 : BN;
     // a split last round has up to as many workgroups as the GPU has CUs
     const int64_t tiles = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
     const int64_t grid = (tiles + 7) / 8 * 8 + 8 + (BM == 256 ? 8 * static_cast<int64_t>(p.xcd_cus) : 0);
     if (grid > 0x7fffffff) return kStatusInvalid;
-    product_kernel<BM, BN, WM, WN, ST, KB, D, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
+    product_kernel<BM, BN, WM, WN, ST, KB, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }
 
@@ -316,11 +326,11 @@ template <bool GATED>
 int route(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
     // 128-byte stages need K % 128 == 0 (a stage never reads past a row)
     if (plan.tile_rows == 256) {
-        if (p.k % 128 == 0) return launch<256, 256, 2, 4, 2, 128, 1, GATED>(p, plan, stream);
-        return launch<256, 256, 2, 4, 4, 64, 1, GATED>(p, plan, stream);
+        if (p.k % 128 == 0) return launch<256, 256, 2, 4, 2, 128, GATED>(p, plan, stream);
+        return launch<256, 256, 2, 4, 4, 64, GATED>(p, plan, stream);
     }
-    if (p.k % 128 == 0) return launch<64, 128, 1, 2, 3, 128, 2, GATED>(p, plan, stream);
-    return launch<64, 128, 1, 2, 4, 64, 2, GATED>(p, plan, stream);
+    if (p.k % 128 == 0) return launch<64, 128, 1, 2, 3, 128, GATED>(p, plan, stream);
+    return launch<64, 128, 1, 2, 4, 64, GATED>(p, plan, stream);
 }
 
 }  // namespace

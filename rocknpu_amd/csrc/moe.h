@@ -28,7 +28,12 @@ struct MoePlan {
 constexpr int kMoeHeader = 16;
 constexpr int kMoeCountThreads = 1024;
 
-// Rows of a product's tile.
+// Rows of a product's tile: 256 x 256 tiles where an expert has rows for them, 64 x
+// 128, which stream weights with two workgroups a CU, where it has few. us a call by 64
+// and by 256 at a mean of 64, 80, 96 and 128 rows an expert: 64 experts of 2048 x 1024
+// 141 and 145, 159 and 162, 173 and 169, 199 and 183; 128 of 2048 x 768 214 and 215, 233
+// and 229, 255 and 246, 306 and 274; 8 of 4096 x 14336 408 and 393, 412 and 407, 439 and
+// 424, 515 and 449; 16 of 2048 x 1024 46 and 49, 48 and 52, 49 and 53, 74 and 67.
 inline int moe_tile_rows(int64_t rows, int experts) {
     return rows >= static_cast<int64_t>(96) * experts ? 256 : 64;
 }

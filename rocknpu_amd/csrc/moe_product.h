@@ -8,14 +8,15 @@ namespace rk {
 
 // Rows of `a` [.., k] (of the token of each choice where gated, else of the choice's
 // place in the plan's order) times w[0] (and w[1]) [experts][n][k], into out
-// [rows][n] in the plan's order.
+// [rows][ldo] in the plan's order, zeros behind n; ldo is at most n's next
+// multiple of 64.
 struct MoeProduct {
     const int8_t* a;
     const float* a_scales;
     const int8_t* w[2];
     const float* w_scales[2];
     float* out;
-    int n, k, top_k;
+    int n, k, ldo, top_k;
     int xcd_cus;  // CUs of an XCD, filled in by the launch
 };
 int launch_moe_product(MoeProduct p, bool gated, const MoePlan& plan, hipStream_t stream);

@@ -201,13 +201,14 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
     // 8 (i / 4): a store is two whole runs of 128 bytes. Eight values at a time, so that
     // their chains of 64-bit operations overlap.
     constexpr int STEP = GATED ? 2 : 1, X = 8;
-    float* out = p.out + static_cast<int64_t>(r0) * p.n + c0;
+    float* out = p.out + static_cast<int64_t>(r0) * p.ldo + c0;
 #pragma unroll
     for (int j = 0; j < FN; j += STEP) {
         const int tc = wn * TN + j * 32 + (lane & 31);
         const int col = GATED ? (tc >> 6) * 32 + (tc & 31) : tc;
         const float ws0 = lsc[BME + tc], ws1 = GATED ? lsc[BME + tc + 32] : 0.0f;
-        const int last = c0 + col < p.n ? end - r0 : 0;
+        const int last = c0 + col < p.ldo ? end - r0 : 0;
+        const bool inside = c0 + col < p.n;  // zeros behind it, up to the rows' length
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -225,7 +226,7 @@ __device__ __forceinline__ void product_tile(const MoeProduct& p, const int32_t*
 #pragma unroll
                 for (int x = 0; x < X; ++x) {
                     const int f = x0 + x, r = (i * WM + wm) * 32 + (f & 3) + 4 * half + 8 * (f >> 2);
-                    if (r < last) out[static_cast<uint32_t>(r * p.n + col)] = v[x];
+                    if (r < last) out[static_cast<uint32_t>(r * p.ldo + col)] = inside ? v[x] : 0.0f;
                 }
             }
         }

@@ -14,8 +14,10 @@
 // partial sums in 64 bits; a thread whose own f32 sum comes near the type's end
 // (values beyond 2^48) adds its squares up in 64 bits instead.
 //
-// Bound by memory: a row is read once, into registers, and everything is
-// written from them. One workgroup a row.
+// Bound by memory: a row is read once, into registers, and everything is written
+// from them. One workgroup a row. With a residual (x and r read, hidden and codes
+// written), in a graph: 16384 rows of 4096 f32 152 us, 5.7 TB/s, bf16 88 us, 5.4; of
+// 1024 f32 35 us, 6.3; 16384 rows of 64 f32 8 us; one row of 2048 3.3 us.
 #include "common.h"
 #include "rocknpu_hip.h"
 
@@ -54,7 +56,9 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // Thread t of nt holds R runs of V values, run t + nt j of its row. V > 1: k, the
-// strides and the bases allow whole runs as one load; V = 1: any.
+// strides and the bases allow whole runs as one load; V = 1: any (16384 rows of
+// 2047 f32 90 us, 4.9 TB/s, f16 85, 2.8; runs of 16 bytes with 4- or 2-byte alignment
+// and the last one in parts took 106 and 71, and 1000 rows of f16 8.5 against 6.9).
 template <typename T, typename W, int V, int R>
 __global__ __launch_bounds__(1024) void norm_a8_kernel(const T* x, const T* r, const W* __restrict__ weight,
                                                        int64_t x_row, int64_t r_row, int k, int nt, T* hidden,

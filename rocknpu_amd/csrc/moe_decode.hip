@@ -10,7 +10,10 @@
 //
 // A token's output is worked out by one workgroup per 8 columns, which quantises
 // the rows of all its choices itself: no launch for that, and none for the weighted
-// sum. Its weights are asked for before.
+// sum. Its weights are asked for before. One token, top 8 of 64 experts of 2048 x 1024:
+// 8.0 us gate and up (33.6 MB, 4.2 TB/s), 8.0 us down (16.8 MB; without the quantisation
+// 1.5 us less, without the weights 5.7); by tiles, quantisation and sum 11 + 4 + 8 + 3.
+// Top 2 of 8 of 4096 x 14336: 83 us in a graph, 4.2 TB/s.
 #include "gemm_dma.h"
 #include "moe_product.h"
 

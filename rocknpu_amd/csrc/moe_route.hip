@@ -7,11 +7,12 @@
 // route_rows ranks by 24-bit whole numbers, 16 lanes a token, notices every token
 // whose choice its rounding could have turned, and hands those to route_token.
 //
-// 16384 tokens over 256 experts in groups: 24 us (by route_token alone 65) and 7 to
-// place the choices; 4096 over 64: 7.5 and 7 (17 alone); one token 6.6 to 10 with its
-// plan. Bound by issue and latency: 1540 vector instructions a wave of four tokens of
-// 256 experts, of which ten rounds of choosing take 600 (sorting each lane's keys
-// first instead spilled: 49 us); the bytes would take 4 us.
+// 16384 tokens over 256 experts in groups: 17.7 us (by route_token alone 65) and 7 to
+// place the choices; 4096 over 64: 7.1 and 7 (17 alone); one token 5.8 to 7.9 with its
+// plan. Bound by issue and latency, four waves a SIMD of which each chooses for four
+// tokens; the bytes would take 4 us. A lane's 8 largest keys are sorted first (108
+// operations for 16 keys) and then handed out: 24 us where every choice took the
+// largest of all 16 and cleared it.
 #include "moe.h"
 
 #include <algorithm>
@@ -101,7 +102,8 @@ struct RouteParams {
 // doubles of the wave's own in LDS, used with groups. Lane i returns choice i.
 template <typename T, int P, bool SIGMOID>
 __device__ __forceinline__ int route_token(const RouteParams& p, int token, double* all) {
-    const int lane = threadIdx.x & 63;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // or what depends on it would be worked out ahead of tokens that need none of this
     const T* x = static_cast<const T*>(p.logits) + token * p.logits_row;
     float l[P];
     bool odd = false;
@@ -217,6 +219,54 @@ __global__ __launch_bounds__(256) void route_token_kernel(const RouteParams p) {
     if (token < p.tokens) route_token<T, P, SIGMOID>(p, token, smem + wave * p.experts);
 }
 
+__device__ __forceinline__ void in_order(uint32_t& a, uint32_t& b) {
+    const uint32_t m = min(a, b);
+    a = max(a, b);
+    b = m;
+}
+// The largest kFirst of a lane's keys (all of fewer), the largest first: sorted halves
+// of 8 (Batcher's odd-even merges), of which the larger of each pair from opposite
+// ends are the 8 largest, rising then falling, and a merge of those.
+constexpr int kFirst = 8;
+template <int N>
+__device__ __forceinline__ void sort8(uint32_t* k) {
+    if constexpr (N >= 2) {
+        in_order(k[0], k[1]);
+        if constexpr (N >= 4) in_order(k[2], k[3]);
+        if constexpr (N >= 8) { in_order(k[4], k[5]); in_order(k[6], k[7]); }
+    }
+    if constexpr (N >= 4) {
+        in_order(k[0], k[2]); in_order(k[1], k[3]);
+        if constexpr (N >= 8) { in_order(k[4], k[6]); in_order(k[5], k[7]); }
+        in_order(k[1], k[2]);
+        if constexpr (N >= 8) in_order(k[5], k[6]);
+    }
+    if constexpr (N >= 8) {
+        in_order(k[0], k[4]); in_order(k[1], k[5]); in_order(k[2], k[6]); in_order(k[3], k[7]);
+        in_order(k[2], k[4]); in_order(k[3], k[5]);
+        in_order(k[1], k[2]); in_order(k[3], k[4]); in_order(k[5], k[6]);
+    }
+}
+template <int P, int F>
+__device__ __forceinline__ void first_keys(uint32_t (&key)[P], uint32_t (&f)[F]) {
+    if constexpr (P <= 8) {
+        sort8<P>(key);
+#pragma unroll
+        for (int j = 0; j < F; ++j) f[j] = key[j];
+    } else {
+        sort8<8>(key);
+        sort8<8>(key + 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = max(key[j], key[15 - j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) in_order(f[j], f[j + 4]);
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) { in_order(f[j], f[j + 2]); in_order(f[j + 1], f[j + 3]); }
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) in_order(f[j], f[j + 1]);
+    }
+}
+
 // All ones, or for a logit of -inf zero (no branch around what it masks).
 __device__ __forceinline__ uint32_t open_mask(float logit) { return logit == -__builtin_inff() ? 0u : ~0u; }
 
@@ -242,10 +292,10 @@ __device__ void place_block(const int32_t* ids, int first, int last, int run, co
 // expert that cannot be chosen. Ranks are
 //   - without a bias, 16-bit logits: their bits, in order: exact;
 //   - without a bias, f32 logits: 2^20 (logit - the token's largest), from -16 up;
-//   - with a bias: 2^20 (score + bias), within +-8.
-// The last two are truncated from f32 values that are within 0.6 of a unit of the
-// 64-bit one (and a softmax's sum of up to 256 within 1.3 units of its share, the
-// same for all): keys that differ by four units or more are in the right order,
+//   - with a bias: 2^20 (score + bias), within +-8, or of sigmoids within +-1.9 2^22.
+// The last two are truncated from f32 values that are within 0.6 of a unit (1.1 at
+// 2^22) of the 64-bit one (and a softmax's sum of up to 256 within 1.3 units of its
+// share, the same for all): keys that differ by four units or more are in the right order,
 // and sums of two that differ by eight. Where two choices, or the last one and the best that is left,
 // differ by less, or the last open group and the best closed one, or where a
 // value does not fit, the token goes to route_token. The weights are worked out
@@ -269,7 +319,8 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
         const int token = t0 + (lane >> 4);
         const bool active = token < end;
         const T* x = static_cast<const T*>(p.logits) + min(token, end - 1) * p.logits_row;
-        const int e0 = group * size + at0;
+        int e0 = group * size + at0;
+        asm volatile("" : "+v"(e0));  // or 16 addresses would be kept over the passes, in memory
         float l[P];
         bool odd = false;  // the token goes to route_token
         if (b.vec) {
@@ -326,7 +377,7 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
             }
         } else {
             float y[P];
-            float floor = -8.0f;
+            float floor = -8.0f, unit = kUnit;
             if (!p.bias) {
                 floor = -16.0f;
 #pragma unroll
@@ -355,7 +406,7 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
             }
 #pragma unroll
             for (int j = 0; j < P; ++j) {
-                const int q = static_cast<int>(fmaxf(y[j], floor) * kUnit) - static_cast<int>(floor * kUnit);
+                const int q = static_cast<int>(fmaxf(y[j], floor) * unit) - static_cast<int>(floor * unit);
                 key[j] = open_mask(l[j]) & (static_cast<uint32_t>(min(max(q, 1), 0xFFFFFF)) << 8 | (255 - (e0 + j)));
             }
         }
@@ -385,22 +436,31 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
         }
         // lane i keeps choice i, and the two that come behind the last
         const bool pairs = p.top_k <= kRowsTopK - 2 && (SIGMOID || !p.bias);
+        // every lane's first keys in order: the best that is left is the largest of the
+        // lanes' next
+        constexpr int F = P < kFirst ? P : kFirst;
+        uint32_t next[F];
+        first_keys(key, next);
+        int given = 0;
         uint32_t mine = 0, before = 0xFFFFFFFF;
         bool near = false;  // the choice before may be of lower rank
+#pragma unroll 1
         for (int i = 0; i < p.top_k + (exact ? 0 : pairs ? 2 : 1); ++i) {
-            uint32_t best = 0;
-#pragma unroll
-            for (int j = 0; j < P; ++j) best = max(best, key[j]);
-            best = row_max(best);
-            if (l16 == i) {
-                mine = best;
-                near = !exact && i > 0 && best != 0 && (before >> 8) - (best >> 8) < 4;
-            }
-            if (i == kRowsTopK) odd |= !exact && best != 0 && (before >> 8) - (best >> 8) < 4;
+            const uint32_t best = row_max(next[0]);
+            const bool close = !exact && i > 0 && best != 0 && (before >> 8) - (best >> 8) < 4, here = l16 == i;
+            mine = here ? best : mine;
+            near |= here && close;
+            odd |= i == kRowsTopK && close;
             before = best;
+            // the lane it came from moves on (by masks: a choice between neighbours in an
+            // array would be made an index, and that a chain of choices)
+            const uint32_t taken = next[0] == best ? ~0u : 0u;
+            given += best != 0 ? taken & 1 : 0;
 #pragma unroll
-            for (int j = 0; j < P; ++j) key[j] = key[j] == best ? 0 : key[j];
+            for (int j = 0; j + 1 < F; ++j) next[j] = (next[j + 1] & taken) | (next[j] & ~taken);
+            next[F - 1] &= ~taken;
         }
+        if constexpr (P > kFirst) odd |= given >= kFirst;  // the lane may hold another
         int id = mine ? 255 - static_cast<int>(mine & 255) : -1;
         double w = 0.0;
         if (id >= 0) {

@@ -165,3 +165,22 @@ def test_scores_closer_than_f32(experts, groups, top_groups, group_top, top_k, s
     if with_bias:
         b["bias"] = 8.0 * b["bias"] * 2.0 ** 20 - 4.0  # beyond the keys' range
         check(x.to(DEV), top_k, score=score, groups=groups, top_groups=top_groups, group_top=group_top, **b)
+
+
+@pytest.mark.parametrize("experts,top_k", [(256, 12), (256, 16), (200, 14), (250, 9), (128, 8), (16, 16)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_all_choices_from_neighbours(experts, top_k, with_bias):
+    """The best experts stand side by side, or only neighbours can be chosen at all."""
+    x = logits(experts, 64, experts)
+    for t in range(64):
+        at = (t * 16) % max(experts - 15, 1)
+        if t % 2:
+            x[t, at:at + 16] += 20.0 + torch.arange(16, device=DEV)[:experts - at]
+        else:
+            keep = x[t, at:at + 16].clone()
+            x[t] = -math.inf
+            x[t, at:at + 16] = keep
+    b = {"bias": bias(5, experts)} if with_bias else {}
+    for score in ("softmax", "sigmoid"):
+        check(x, top_k, score=score, **b)
+        check(x.bfloat16(), top_k, score=score, **b)

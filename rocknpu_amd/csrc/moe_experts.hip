@@ -133,8 +133,12 @@ extern "C" int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args* args, voi
     const MoeProduct first{a.a8, a.a_scales, {a.gate, a.up}, {a.gate_scales, a.up_scales}, values, a.ffn, a.hidden_pad, values_row, a.top_k};
     int st = launch_moe_product(first, true, plan, s);
     if (st != kStatusOk) return st;
-    st = launch_quantize_a8(values, plan.rows, values_row, values_row, a.ffn_pad, codes, scales, nullptr, 0, s);
-    if (st != kStatusOk) return st;
+    constexpr int kRowsOnce = 1 << 21;  // a launch holds less than 2^32 threads, a row up to 1024
+    for (int r = 0; r < plan.rows; r += kRowsOnce) {
+        st = launch_quantize_a8(values + static_cast<size_t>(r) * values_row, std::min(plan.rows - r, kRowsOnce), values_row, values_row,
+                                a.ffn_pad, codes + static_cast<size_t>(r) * a.ffn_pad, scales + r, nullptr, 0, s);
+        if (st != kStatusOk) return st;
+    }
     const MoeProduct second{codes, scales, {a.down, nullptr}, {a.down_scales, nullptr}, values, a.hidden, a.ffn_pad, out_row, a.top_k};
     st = launch_moe_product(second, false, plan, s);
     if (st != kStatusOk) return st;

@@ -333,7 +333,7 @@ int launch(const MoeProduct& p, const MoePlan& plan, hipStream_t stream) {
     // a split last round has up to as many workgroups as the GPU has CUs
     const int64_t tiles = static_cast<int64_t>(plan.max_tiles) * ((p.n + BC - 1) / BC);
     const int64_t grid = (tiles + 7) / 8 * 8 + 8 + (BM == 256 ? 8 * static_cast<int64_t>(p.xcd_cus) : 0);
-    if (grid > 0x7fffffff) return kStatusInvalid;
+    if (grid * (WM * WN * 64) > 0xffffffff) return kStatusInvalid;  // (values of that many tiles are over a TB)
     product_kernel<BM, BN, WM, WN, ST, KB, GATED><<<dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), 0, stream>>>(p, plan);
     return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
 }

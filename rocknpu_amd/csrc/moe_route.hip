@@ -215,8 +215,9 @@ __device__ __forceinline__ int route_token(const RouteParams& p, int token, doub
 template <typename T, int P, bool SIGMOID>
 __global__ __launch_bounds__(256) void route_token_kernel(const RouteParams p) {
     extern __shared__ double smem[];
-    const int wave = threadIdx.x >> 6, token = blockIdx.x * 4 + wave;
-    if (token < p.tokens) route_token<T, P, SIGMOID>(p, token, smem + wave * p.experts);
+    const int wave = threadIdx.x >> 6;
+    for (int64_t token = blockIdx.x * 4 + wave; token < p.tokens; token += gridDim.x * 4)
+        route_token<T, P, SIGMOID>(p, static_cast<int>(token), smem + wave * p.experts);
 }
 
 __device__ __forceinline__ void in_order(uint32_t& a, uint32_t& b) {
@@ -666,7 +667,7 @@ __global__ __launch_bounds__(kMoeCountThreads) void place_kernel(const int32_t* 
 
 template <typename T, int P>
 int launch_tokens(const RouteParams& p, bool sigmoid, hipStream_t stream) {
-    const dim3 grid((p.tokens + 3) / 4), block(256);
+    const dim3 grid(std::min((p.tokens + 3) / 4, 1 << 22)), block(256);  // a launch holds less than 2^32 threads
     const size_t lds = p.groups > 1 ? static_cast<size_t>(4) * p.experts * sizeof(double) : 0;
     if (sigmoid) route_token_kernel<T, P, true><<<grid, block, lds, stream>>>(p);
     else route_token_kernel<T, P, false><<<grid, block, lds, stream>>>(p);

@@ -61,7 +61,8 @@ class Routing:
     plan of the experts' products, of which `offsets` int32 [experts + 1] and
     `order` int32 [tokens * top_k] are views: order[offsets[e]:offsets[e + 1]]
     are the numbers token * top_k + place of the choices that fell on expert e,
-    ascending; behind offsets[experts] it is -1."""
+    ascending; behind offsets[experts] it is -1. The plan belongs to its ids; other
+    weights may be put in place of these."""
 
     __slots__ = ("ids", "weights", "plan", "experts")
 
@@ -141,8 +142,8 @@ def _pair(pair, shape, what, device):
     w8, scales = pair
     if w8.dtype is not torch.int8 or tuple(w8.shape) != shape or not w8.is_contiguous() or w8.device != device:
         raise ValueError(f"{what} has to be contiguous int8 {shape} on {device}, not {w8.dtype} {tuple(w8.shape)} on {w8.device}")
-    if scales.dtype is not torch.float32 or tuple(scales.shape) != shape[:2] or not scales.is_contiguous() or scales.device != device:
-        raise ValueError(f"{what}'s scales have to be contiguous float32 {shape[:2]} on {device}")
+    if scales.dtype is not torch.float32 or tuple(scales.shape) != shape[:-1] or not scales.is_contiguous() or scales.device != device:
+        raise ValueError(f"{what}'s scales have to be contiguous float32 {shape[:-1]} on {device}")
     return w8, scales
 
 
@@ -206,6 +207,11 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
         raise ValueError(f"a_scales have to be contiguous float32 [{tokens}] on {at}")
     if routing.experts != weights.experts or routing.plan.device != at:
         raise ValueError(f"the routing is of {routing.experts} experts on {routing.plan.device}, not {weights.experts} on {at}")
+    ids, factors, plan = routing.ids, routing.weights, routing.plan
+    if (ids.dtype is not torch.int32 or not ids.is_contiguous() or ids.device != at or factors.dtype is not torch.float32
+            or factors.shape != ids.shape or not factors.is_contiguous() or factors.device != at or plan.dtype is not torch.int32
+            or not plan.is_contiguous() or plan.numel() != plan_words(tokens, weights.experts, top_k)):
+        raise ValueError(f"the routing's ids and plan have to be route's own, and its weights contiguous float32 {tuple(ids.shape)} on {at}")
     if out is None:
         if dtype not in TYPES:
             raise ValueError(f"{dtype}: float32, float16 or bfloat16 is wanted")
@@ -214,8 +220,8 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
         raise ValueError(f"out has to be float32, float16 or bfloat16 [{tokens}, {weights.hidden}] on {at} with contiguous rows")
     key = hip.stream_of(at)
     args = _pack_experts(
-        a8.data_ptr(), a_scales.data_ptr(), *weights.pointers, routing.ids.data_ptr(), routing.weights.data_ptr(),
-        routing.plan.data_ptr(), out.data_ptr(), tokens, out.stride(0) if tokens > 1 else weights.hidden, weights.experts, top_k,
+        a8.data_ptr(), a_scales.data_ptr(), *weights.pointers, ids.data_ptr(), factors.data_ptr(),
+        plan.data_ptr(), out.data_ptr(), tokens, out.stride(0) if tokens > 1 else weights.hidden, weights.experts, top_k,
         weights.hidden, weights.hidden_pad, weights.ffn, weights.ffn_pad, TYPES[out.dtype])
     lib = _lib.load()
     need = weights._needs.get((tokens, top_k))
@@ -245,10 +251,11 @@ def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, router, weights: Ex
     hip.quantize_a8 of its rows), route with `routing`'s arguments, and experts.
     Returns (out [tokens, hidden] in x's type, x + residual or None); the former
     is the next norm's x, the latter its residual."""
-    a8, a_scales, hidden = hip.norm_a8(x, norm_weight, eps, residual, hidden=hidden)
-    if tuple(router[0].shape) != (weights.experts, weights.hidden_pad) or a8.shape[1] != weights.hidden_pad:
-        raise ValueError(f"x of {x.shape[1]} and a router {tuple(router[0].shape)} for {weights.experts} experts of {weights.hidden_pad}")
+    _pair(router, (weights.experts, weights.hidden_pad), "router", weights.device)
+    if x.dim() != 2 or x.shape[1] != weights.hidden or x.device != weights.device:
+        raise ValueError(f"x has to be [tokens, {weights.hidden}] on {weights.device}, not {tuple(x.shape)} on {x.device}")
+    a8, a_scales, hidden = hip.norm_a8(x, norm_weight, eps, residual, hidden=hidden, k_pad=weights.hidden_pad)
     if x.shape[0] == 0:
         return x.new_empty((0, weights.hidden)) if out is None else out, hidden
-    logits = hip.gemm_w8a8(a8, a_scales, *router)
+    logits = hip.call_on(hip.stream_of(x.device)[0], hip.gemm_w8a8, a8, a_scales, *router)
     return experts(weights, a8, a_scales, route(logits, top_k, **routing), dtype=x.dtype, out=out), hidden

@@ -311,3 +311,30 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i, job in enumerate(jobs):
         assert all(torch.equal(o, job[3]) for o in outs[i])
+
+
+def test_more_rows_than_a_launch_quantises():
+    """2^26 rows and more: over 2^32 threads of one launch, values at offsets past 32 bits."""
+    tokens, n, top_k = (1 << 25) + 3, 64, 2
+    w = layer(5, 3, n, n)
+    g = torch.Generator(DEV).manual_seed(6)
+    a8 = torch.randint(-127, 128, (tokens, n), dtype=torch.int8, device=DEV, generator=g)
+    scales = torch.rand(tokens, device=DEV, generator=g) / 40
+    r = moe.route(torch.randn((tokens, 3), dtype=torch.float16, device=DEV, generator=g), top_k)
+    space = torch.empty(tokens * top_k * (5 * n + 4) + 1024, dtype=torch.uint8, device=DEV)
+    out = moe.experts(w, a8, scales, r, dtype=torch.float16, workspace=space)
+    some = torch.cat([torch.arange(20), torch.randint(0, tokens, (400,), generator=torch.Generator().manual_seed(7)), torch.arange(tokens - 20, tokens)]).to(DEV)
+    part = moe.Routing(r.ids[some], r.weights[some], r.plan, 3)
+    verify(w, a8[some], scales[some], part, out[some])
+
+
+def test_other_weights():
+    w, a8, scales, r, _ = check(9, 50, 6, 3, 128, 64)
+    r.weights = r.weights * 0.25 - 1
+    verify(w, a8, scales, r, moe.experts(w, a8, scales, r))
+    for bad in (r.weights.half(), r.weights[:, :2], r.weights.t().contiguous().t(), r.weights.cpu()):
+        with pytest.raises(ValueError):
+            moe.experts(w, a8, scales, moe.Routing(r.ids, bad, r.plan, 6))
+    for ids, plan in ((r.ids.long(), r.plan), (r.ids, r.plan[:-1]), (r.ids, r.plan.long()), (r.ids[:40], r.plan)):
+        with pytest.raises(ValueError):
+            moe.experts(w, a8, scales, moe.Routing(ids, r.weights, plan, 6))

@@ -184,3 +184,15 @@ def test_all_choices_from_neighbours(experts, top_k, with_bias):
     for score in ("softmax", "sigmoid"):
         check(x, top_k, score=score, **b)
         check(x.bfloat16(), top_k, score=score, **b)
+
+
+def test_more_tokens_than_a_launch_has_waves():
+    """Over 2^26 tokens, a wave each, are more threads than one launch takes."""
+    tokens, experts = (1 << 26) + 7, 257
+    x = torch.randn((1, experts), generator=torch.Generator().manual_seed(1)).to(DEV)
+    r = moe.route(x.expand(tokens, experts), 1, normalise=False)
+    best = int(x.argmax())
+    assert bool((r.ids == best).all()) and bool((r.weights == r.weights[0]).all())
+    assert abs(float(r.weights[0]) - float(torch.softmax(x.double(), 1)[0, best])) < 2.0 ** -24
+    assert torch.equal(r.order, torch.arange(tokens, dtype=torch.int32, device=DEV))
+    assert r.offsets.tolist() == [0] * (best + 1) + [tokens] * (experts - best)

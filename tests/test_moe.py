@@ -142,3 +142,25 @@ def test_experts_keep_their_tensors():
     for name in ("gate", "up", "down", "experts", "hidden", "ffn", "device", "pointers"):
         with pytest.raises(AttributeError):
             setattr(w, name, None)
+
+
+def test_refused_layers():
+    i8, f = (lambda *s: torch.zeros(s, dtype=torch.int8)), torch.zeros
+    w = moe.Experts((i8(4, 60, 128), f(4, 60)), (i8(4, 60, 128), f(4, 60)), (i8(4, 100, 64), f(4, 100)), hidden=100, ffn=60)
+    good = dict(x=f(3, 100), norm_weight=f(100), router=(i8(4, 128), f(4)), weights=w, top_k=2)
+    for kw, what in ((dict(router=(f(4, 128), f(4))), "router"), (dict(router=(i8(4, 128), f(4).double())), "router's scales"), (dict(router=(i8(3, 128), f(3))), "router"),
+                     (dict(router=(i8(128, 4).T, f(4))), "router"), (dict(router=(i8(4, 128), f(3))), "router's scales"), (dict(x=f(3, 128)), "x has"), (dict(x=f(100)), "x has")):
+        with pytest.raises(ValueError, match=what):
+            moe.feed_forward(**{**good, **kw})
+
+
+@pytest.mark.parametrize("kw,what", [(dict(ids=torch.zeros((3, 2), dtype=torch.int64)), "ids"), (dict(weights=torch.zeros((3, 2)).half()), "weights"),
+                                     (dict(weights=torch.zeros((2, 3)).T), "weights"), (dict(plan=torch.zeros(10, dtype=torch.int32)), "plan"), (dict(weights=torch.zeros(3)), "weights")])
+def test_refused_routings(kw, what):
+    i8, f = (lambda *s: torch.zeros(s, dtype=torch.int8)), torch.zeros
+    w = moe.Experts((i8(4, 60, 128), f(4, 60)), (i8(4, 60, 128), f(4, 60)), (i8(4, 100, 64), f(4, 100)), hidden=100, ffn=60)
+    good = dict(ids=torch.zeros((3, 2), dtype=torch.int32), weights=f(3, 2), plan=torch.zeros(moe.plan_words(3, 4, 2), dtype=torch.int32))
+    with pytest.raises(ValueError, match=what):
+        moe.experts(w, i8(3, 128), f(3), moe.Routing(**{**good, **kw}, experts=4))
+    with pytest.raises(ValueError, match="a GPU's are wanted"):
+        moe.experts(w, i8(3, 128), f(3), moe.Routing(**good, experts=4))

@@ -189,11 +189,17 @@ bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p
 
 template <typename T, typename W, int V, int R>
 int launch(const rocknpu_norm_args& a, int nt, hipStream_t stream) {
-    norm_a8_kernel<T, W, V, R><<<dim3(static_cast<unsigned>(a.rows)), dim3(nt), 0, stream>>>(
-        static_cast<const T*>(a.x), static_cast<const T*>(a.residual), static_cast<const W*>(a.weight), a.x_row,
-        a.residual_row, static_cast<int>(a.k), nt, static_cast<T*>(a.hidden), a.hidden_row, static_cast<T*>(a.out),
-        a.out_row, a.a8, a.k_pad, a.scales, a.eps);
-    return hipGetLastError() == hipSuccess ? kStatusOk : kStatusExec;
+    constexpr int64_t kRowsOnce = 1 << 21;  // a launch holds less than 2^32 threads, a row up to 1024
+    for (int64_t row = 0; row < a.rows; row += kRowsOnce) {
+        const auto from = [row](auto* p, int64_t ld) { return p ? p + row * ld : p; };
+        norm_a8_kernel<T, W, V, R><<<dim3(static_cast<unsigned>(std::min(a.rows - row, kRowsOnce))), dim3(nt), 0, stream>>>(
+            from(static_cast<const T*>(a.x), a.x_row), from(static_cast<const T*>(a.residual), a.residual_row),
+            static_cast<const W*>(a.weight), a.x_row, a.residual_row, static_cast<int>(a.k), nt,
+            from(static_cast<T*>(a.hidden), a.hidden_row), a.hidden_row, from(static_cast<T*>(a.out), a.out_row), a.out_row,
+            from(a.a8, a.k_pad), a.k_pad, from(a.scales, 1), a.eps);
+        if (hipGetLastError() != hipSuccess) return kStatusExec;
+    }
+    return kStatusOk;
 }
 
 // Threads a row: two runs each (one for at most 512 rows), in whole waves, at

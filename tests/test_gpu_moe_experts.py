@@ -338,3 +338,9 @@ def test_other_weights():
     for ids, plan in ((r.ids.long(), r.plan), (r.ids, r.plan[:-1]), (r.ids, r.plan.long()), (r.ids[:40], r.plan)):
         with pytest.raises(ValueError):
             moe.experts(w, a8, scales, moe.Routing(ids, r.weights, plan, 6))
+
+
+@pytest.mark.parametrize("experts,top_k,ffn", [(8, 8, 14336), (2, 2, 61440), (2, 2, 70000), (64, 64, 1984), (64, 64, 2048)])
+def test_one_token_of_long_rows(experts, top_k, ffn):
+    """The rows' codes fill most of LDS, or do not fit it."""
+    check(ffn, 1, experts, top_k, 64, ffn)

@@ -176,3 +176,14 @@ def test_streams_and_graphs():
         a8, s, h = hip.norm_a8(x, w, residual=r)
         torch.cuda.synchronize()
         assert torch.equal(out[0], a8) and torch.equal(out[1], s) and torch.equal(out[2], h)
+
+
+def test_more_rows_than_a_launch_has_threads():
+    """2^26 rows of a wave each are 2^32 threads."""
+    rows, k = (1 << 26) + 5, 60
+    x, w = torch.randn((1, k), generator=torch.Generator().manual_seed(1)).to(DEV), torch.ones(k, device=DEV)
+    one, s = hip.norm_a8(x, w)[:2]
+    a8, scales, _ = hip.norm_a8(x.expand(rows, k), w)
+    assert bool((scales == s).all())
+    for part in a8.split(1 << 22):
+        assert bool((part == one).all())

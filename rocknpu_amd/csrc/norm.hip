@@ -10,9 +10,10 @@
 // f = 1 / sqrt(mean(h^2) + eps), scale = s0 * f, out = round(u * f).
 // f multiplies the whole row, so the codes need no f: they are u's, exact to
 // the bit whatever order the sum of squares has, and quantising needs the row's
-// largest |u| alone. f itself is worked out in 64 bits from a sum of f32
-// partial sums in 64 bits; a thread whose own f32 sum comes near the type's end
-// (values beyond 2^48) adds its squares up in 64 bits instead.
+// largest |u| alone. f itself is worked out in 64 bits, the squares' sum included
+// (f32 partial sums of up to 64 squares a thread lose bits where one channel is far above
+// the others, as in residual streams: rms error of the scale 5.9e-8 at 16384 columns
+// where its rounding alone is 2.0e-8), so the scale has one rounding.
 //
 // Bound by memory: a row is read once, into registers, and everything is written
 // from them. One workgroup a row. With a residual (x and r read, hidden and codes
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(1024) void norm_a8_kernel(const T* x, const T* r, c
         }
     }
     float u[N];
-    float part = 0.0f;
+    double sum = 0.0;
     uint32_t um = 0;
 #pragma unroll
     for (int j = 0; j < R; ++j)
@@ -97,14 +98,8 @@ __global__ __launch_bounds__(1024) void norm_a8_kernel(const T* x, const T* r, c
             const float a = static_cast<float>(xv[j].e[e]);
             const float h = r ? a + static_cast<float>(rv[j].e[e]) : a;
             u[V * j + e] = h;
-            part = fmaf(h, h, part);
+            sum = fma(static_cast<double>(h), static_cast<double>(h), sum);
         }
-    double sum = part;
-    if (__any(!(part < 0x1p100f))) {
-        sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum = fma(static_cast<double>(u[i]), static_cast<double>(u[i]), sum);
-    }
     if (hidden) {
         Run<T, V>* hr = reinterpret_cast<Run<T, V>*>(hidden + row * hidden_row);
 #pragma unroll

@@ -93,8 +93,8 @@ typedef struct rocknpu_moe_experts_args {
  * up[e] (f32(f32(sum) * row's scale) * column's scale, as rocknpu_hip_gemm_w8a8),
  * v = f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, v's row is
  * quantised as rocknpu_hip_quantize_a8 does, d is its product with down[e], and
- * out[t] = sum over s of weights[t][s] * d, in f32 in the order of s, rounded
- * once. Choices of id -1 are left out; a token without any gets zeros. A row of A8
+ * out[t] = sum over s of weights[t][s] * d, in 64 bits in the order of s, rounded
+ * to f32 and to out_type. Choices of id -1 are left out; a token without any gets zeros. A row of A8
  * whose scale is NaN gives NaN in its token's output and in no other.
  * The workspace (rocknpu_hip_moe_experts_workspace bytes, 256-byte aligned, any
  * contents) is free again when the call's kernels are done. The same call gives

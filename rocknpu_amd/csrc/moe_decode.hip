@@ -177,24 +177,27 @@ __global__ __launch_bounds__(W * 64) void decode_down_kernel(const MoeDecode p, 
         if (lane < 16) sums[(s * share + part) * 16 + lane] = lane < 8 ? acc[0] : acc[1];
     }
     barrier();
-    // the choices' weighted values side by side, in place of their sums; then one after the other
+    // the choices' values and weights side by side, in place of their sums (each thread
+    // over what it alone has read); then they are added up one after the other, in 64
+    // bits, where every product is exact
     float* terms = reinterpret_cast<float*>(sums);
-    const auto term = [&](int s, int e, float weight, float w_scale) {
+    const auto term = [&](int s, float weight, float w_scale) {
         int total = 0;
         for (int j = 0; j < share; ++j) total += sums[(s * share + j) * 16 + col] + sums[(s * share + j) * 16 + 8 + col];
         const uint32_t peak = peaks[s];
         const float scale = peak > 0x7f7fffffu ? __builtin_nanf("") : peak == 0 ? 1.0f : __uint_as_float(peak) / 127.0f;
-        const float d = (static_cast<float>(total) * scale) * w_scale;
-        terms[s * share * 16 + col] = e < 0 ? 0.0f : weight * d;
+        terms[s * share * 16 + col] = (static_cast<float>(total) * scale) * w_scale;
+        terms[s * share * 16 + 8 + col] = weight;
     };
     static_assert(8 * W >= ROCKNPU_MOE_MAX_TOP_K, "a thread for each choice's column");
-    if (threadIdx.x < 8 * n) term(own, own_e, own_weight, own_scale);
+    if (threadIdx.x < 8 * n) term(own, own_weight, own_scale);
     barrier();
     if (threadIdx.x < 8 && c0 + col < p.hidden) {
-        float sum = 0.0f;
+        double sum = 0.0;
         for (int s = 0; s < n; ++s)
-            if (row_of(ids, s, p.experts) >= 0) sum += terms[s * share * 16 + col];
-        out[token * out_row + c0 + col] = static_cast<T>(sum);
+            if (row_of(ids, s, p.experts) >= 0)
+                sum += static_cast<double>(terms[s * share * 16 + 8 + col]) * static_cast<double>(terms[s * share * 16 + col]);
+        out[token * out_row + c0 + col] = static_cast<T>(static_cast<float>(sum));
     }
 }
 

@@ -8,7 +8,8 @@
 namespace rk {
 namespace {
 
-// out[t] = sum over the token's choices, in their order, of weight * row. Bound by
+// out[t] = sum over the token's choices, in their order, of weight * row, in 64 bits
+// (where every product is exact), rounded to f32 and to out's type. Bound by
 // memory: top_k rows are read for each that is written (32768 rows of 2048 in 51 us,
 // 5.9 TB/s). A thread takes 4 columns of a token and asks for four choices' rows
 // before it adds them up. Rows are ld floats apart, a multiple of 4; VEC: out's
@@ -23,7 +24,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
     if (c >= hidden) return;
     place += t * top_k;
     weights += t * top_k;
-    float sum[4] = {};
+    double sum[4] = {};
     for (int s0 = 0; s0 < top_k; s0 += 4) {
         vec v[4];
         float w[4];
@@ -39,13 +40,13 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
         for (int i = 0; i < 4; ++i)
             if (used[i])
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] += w[i] * v[i][e];
+                for (int e = 0; e < 4; ++e) sum[e] += static_cast<double>(w[i]) * static_cast<double>(v[i][e]);
     }
     struct alignas(sizeof(T) * 4) Out {
         T e[4];
     } o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o.e[e] = static_cast<T>(sum[e]);
+    for (int e = 0; e < 4; ++e) o.e[e] = static_cast<T>(static_cast<float>(sum[e]));
     T* y = out + t * out_row + c;
     if constexpr (VEC) {
         *reinterpret_cast<Out*>(y) = o;

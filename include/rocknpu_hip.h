@@ -65,7 +65,9 @@ typedef struct rocknpu_norm_args {
  * zero as rocknpu_hip_quantize_a8 does, f = 1 / sqrt(mean(h^2) + eps),
  * scales = s0 * f, out = u * f rounded. The codes do not depend on f, so they
  * are exact. A row of which a u is not finite gets scale NaN, zero codes and,
- * in `out`, NaN. k is at most ROCKNPU_NORM_MAX_K; rows = 0 does nothing. The
+ * in `out`, NaN. k is at most ROCKNPU_NORM_MAX_K; rows = 0 does nothing. An output
+ * that overlaps what it must not is refused: rows of one stride may lie between each
+ * other's, those of different strides may not reach into each other's range. The
  * reference norms on the host (crates/rocknpu-llm/src/lib.rs) and quantises
  * in crates/rocknpu-capi/src/lib.rs:1776-1791. */
 int rocknpu_hip_norm_a8(const rocknpu_norm_args * args, void * stream);

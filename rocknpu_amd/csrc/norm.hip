@@ -182,6 +182,43 @@ __global__ __launch_bounds__(1024) void norm_a8_kernel(const T* x, const T* r, c
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
+// Rows of `width` bytes, `step` apart (0 where there is one).
+struct Rows {
+    uintptr_t at;
+    int64_t rows, width, step;
+    __int128 end() const { return static_cast<__int128>(at) + static_cast<__int128>(rows - 1) * step + width; }
+    bool same(const Rows& o) const { return at == o.at && step == o.step; }
+};
+Rows rows_of(const void* p, int64_t rows, int64_t row, int64_t k, int64_t size) {
+    return {reinterpret_cast<uintptr_t>(p), p ? rows : 0, k * size, rows > 1 ? row * size : 0};
+}
+// Whether no byte is in both. Rows as far apart as the other's may lie between them;
+// otherwise what counts is from where to where they reach.
+bool apart(const Rows& a, const Rows& b) {
+    if (a.rows == 0 || b.rows == 0 || a.end() <= b.at || b.end() <= a.at) return true;
+    if (a.step != b.step || a.step == 0) return false;
+    if (b.at < a.at) return apart(b, a);
+    // row i of a and row j of b: b's place less a's is d + (j - i) step
+    const int64_t d = static_cast<int64_t>(b.at - a.at), n = d / a.step;
+    return d - n * a.step >= a.width && (n + 1 >= a.rows || d - (n + 1) * a.step <= -b.width);
+}
+// What the header says of each output: hidden and out may be x or the residual, and
+// nothing else may be in two places.
+bool outputs_apart(const rocknpu_norm_args& a, int64_t size, int64_t weight_size) {
+    const Rows in[2] = {rows_of(a.x, a.rows, a.x_row, a.k, size), rows_of(a.residual, a.rows, a.residual_row, a.k, size)};
+    const Rows weight = rows_of(a.weight, 1, 0, a.k, weight_size);
+    const Rows to[4] = {rows_of(a.hidden, a.rows, a.hidden_row, a.k, size), rows_of(a.out, a.rows, a.out_row, a.k, size),
+                        rows_of(a.a8, a.rows, a.k_pad, a.k_pad, 1), rows_of(a.scales, 1, 0, a.rows, 4)};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (!apart(to[i], to[j])) return false;
+        for (const Rows& from : in)
+            if (!(i < 2 && to[i].same(from)) && !apart(to[i], from)) return false;
+        if (!apart(to[i], weight)) return false;
+    }
+    return true;
+}
+
 template <typename T, typename W, int V, int R>
 int launch(const rocknpu_norm_args& a, int nt, hipStream_t stream) {
     constexpr int64_t kRowsOnce = 1 << 21;  // a launch holds less than 2^32 threads, a row up to 1024
@@ -243,7 +280,7 @@ extern "C" int rocknpu_hip_norm_a8(const rocknpu_norm_args* args, void* stream) 
     if (a.x_row < 0 || a.residual_row < 0 || a.hidden_row < 0 || a.out_row < 0) return kStatusInvalid;
     if (a.rows > 1 && ((a.hidden && a.hidden_row < a.k) || (a.out && a.out_row < a.k))) return kStatusInvalid;
     if (a.rows == 0) return kStatusOk;
-    if (!a.x || !a.a8 || !a.scales) return kStatusInvalid;
+    if (!a.x || !a.a8 || !a.scales || !outputs_apart(a, static_cast<int64_t>(size), static_cast<int64_t>(wsize))) return kStatusInvalid;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (a.type == ROCKNPU_TYPE_F32) return route<float, float>(a, s);
     if (a.weight_type == ROCKNPU_TYPE_F32)

@@ -119,8 +119,9 @@ def norm_a8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: 
     follows: returns (A8 [m, k_pad] int8, scales [m] f32, hidden), hidden the
     sum x + residual in x's type (`hidden` if given: it may be x or residual
     itself) and None without a residual. `out`, if given, takes the normed rows
-    in x's type as well. The codes are those of the row x + residual times
-    weight, the norm's factor is in the scales alone."""
+    in x's type as well; it may be x or residual, but not hidden. Outputs that
+    overlap anything else are refused. The codes are those of the row x +
+    residual times weight, the norm's factor is in the scales alone."""
     kind, shape, at = x.dtype, x.shape, x.device
     if kind not in TYPES or len(shape) != 2:
         raise ValueError(f"x has to be float32, float16 or bfloat16 [m, k], not {kind} {tuple(shape)}")

@@ -104,6 +104,17 @@ int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args * args, void * worksp
 /* Bytes of workspace for such a call (only its sizes are read). Host code only. */
 int rocknpu_hip_moe_experts_workspace(const rocknpu_moe_experts_args * args, size_t * bytes);
 
+/* How the gate and up product (gated = 1) or the down product of such a call (only its
+ * sizes are read) is dealt out where the plan has `row_tiles` row tiles, on a GPU of
+ * `cus` compute units (cus <= 0: the current device's). tile: its tiles' rows and output
+ * columns, zeros where the call goes choice by choice. workgroups: those of the launch.
+ * places, if not NULL, holds `capacity` entries of four words, one a workgroup: its row tile (-1: it
+ * has none), its column tile, and which of how many parts of it: of one, of two (halves of the columns), of
+ * four (0 and 1: those of the upper rows, 2 and 3: of the lower). A plan's first word is its row
+ * tiles. Host code only. */
+int rocknpu_hip_moe_product_places(const rocknpu_moe_experts_args * args, int gated, int32_t row_tiles, int cus,
+                                   int32_t tile[2], int32_t * places, size_t capacity, size_t * workgroups);
+
 #ifdef __cplusplus
 }
 #endif

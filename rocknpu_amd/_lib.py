@@ -98,6 +98,7 @@ SIGNATURES = {
     "rocknpu_hip_moe_route": (_i, [_vp, _vp]),
     "rocknpu_hip_moe_experts": (_i, [_vp, _vp, _sz, _vp]),
     "rocknpu_hip_moe_experts_workspace": (_i, [_vp, _vp]),
+    "rocknpu_hip_moe_product_places": (_i, [_vp, _i, ctypes.c_int32, _i, _vp, _vp, _sz, _vp]),
     "rocknpu_hip_moe_plan_words": (_i, [_i64, ctypes.c_int32, ctypes.c_int32, _vp]),
 }
 

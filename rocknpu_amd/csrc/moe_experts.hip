@@ -101,6 +101,34 @@ extern "C" int rocknpu_hip_moe_experts_workspace(const rocknpu_moe_experts_args*
     return kStatusOk;
 }
 
+extern "C" int rocknpu_hip_moe_product_places(const rocknpu_moe_experts_args* args, int gated, int32_t row_tiles, int cus,
+                                              int32_t tile[2], int32_t* places, size_t capacity, size_t* workgroups) {
+    using namespace rk;
+    if (!tile || !workgroups || !sizes_ok(args)) return kStatusInvalid;
+    const MoePlan plan = moe_plan(args->tokens, args->experts, args->top_k, nullptr, nullptr);
+    if (row_tiles < 0 || row_tiles > plan.max_tiles) return kStatusInvalid;
+    tile[0] = tile[1] = 0;
+    *workgroups = 0;
+    if (args->tokens == 0 || moe_decodes(args->tokens, args->experts, args->top_k, args->ffn_pad)) return kStatusOk;
+    const int n = gated ? args->ffn : args->hidden, xcd_cus = moe_xcd_cus(cus > 0 ? cus : device_cu_count());
+    tile[0] = plan.tile_rows;
+    tile[1] = moe_tile_columns(plan.tile_rows, gated != 0);
+    *workgroups = static_cast<size_t>(moe_product_grid(plan, n, gated != 0, xcd_cus));
+    if (!places) return kStatusOk;
+    if (*workgroups > 0x7fffffff || capacity < *workgroups) return kStatusInvalid;
+    for (size_t b = 0; b < *workgroups; ++b) {
+        const MoeShare share = moe_share(b & 7, row_tiles, (n + tile[1] - 1) / tile[1], xcd_cus, plan.tile_rows == 256);
+        int32_t* p = places + 4 * b;
+        int i = static_cast<int>(b >> 3);
+        moe_part(share, i, p[2]);
+        p[0] = -1;
+        p[1] = 0;
+        if (i < share.mine) moe_pair(share, i, p[0], p[1]);
+        p[3] = moe_splits(share, i) ? share.parts : 1;
+    }
+    return kStatusOk;
+}
+
 extern "C" int rocknpu_hip_moe_experts(const rocknpu_moe_experts_args* args, void* workspace, size_t workspace_bytes,
                                        void* stream) {
     using namespace rk;

@@ -21,6 +21,54 @@ struct MoeProduct {
 };
 int launch_moe_product(MoeProduct p, bool gated, const MoePlan& plan, hipStream_t stream);
 
+// Output columns of such a launch's tiles, CUs of an XCD, and workgroups: a split last
+// round has up to as many as the GPU has CUs.
+constexpr int moe_tile_columns(int tile_rows, bool gated) { return (tile_rows == 256 ? 256 : 128) / (gated ? 2 : 1); }
+inline int moe_xcd_cus(int cus) { return cus >= 8 ? cus / 8 : 1; }
+inline int64_t moe_product_grid(const MoePlan& plan, int n, bool gated, int xcd_cus) {
+    const int columns = moe_tile_columns(plan.tile_rows, gated);
+    const int64_t tiles = static_cast<int64_t>(plan.max_tiles) * ((n + columns - 1) / columns);
+    return (tiles + 7) / 8 * 8 + 8 + (plan.tile_rows == 256 ? 8 * static_cast<int64_t>(xcd_cus) : 0);
+}
+
+constexpr int kMoeManyTiles = 64;
+
+// What of a launch's (row tile, column tile) pairs an XCD's workgroups take; workgroup b
+// runs on XCD b % 8, which walks its share in groups of 4 row tiles: they share W in its
+// L2 where they are one expert's, and their A over the columns. With many row tiles a share is a
+// contiguous range; with few, in which a range's full and partly filled tiles
+// would not even out, an eighth of the columns of every row tile (and a range of
+// the columns that are left over). Where tiles split, what an XCD's CUs would run in a
+// last round that is at most half full runs in two parts (halves of the columns), at
+// most a quarter full in four (of the rows, too: parts 0 and 1 the upper, 2 and 3 the lower).
+struct MoeShare {
+    int tiles_m, tiles_n, xcd, eighth, own, per, rem, mine, rest, parts;
+};
+__host__ __device__ __forceinline__ MoeShare moe_share(int xcd, int tiles_m, int tiles_n, int xcd_cus, bool splits) {
+    const int eighth = tiles_m < kMoeManyTiles ? tiles_n >> 3 : 0;  // columns of each XCD's own
+    const int own = eighth * tiles_m, shared = (tiles_n - 8 * eighth) * tiles_m;
+    const int per = shared >> 3, rem = shared & 7;
+    const int mine = own + per + (xcd < rem), rest = splits ? mine % xcd_cus : 0;
+    const int parts = 2 * rest > xcd_cus || rest == 0 ? 1 : 4 * rest > xcd_cus ? 2 : 4;
+    return {tiles_m, tiles_n, xcd, eighth, own, per, rem, mine, rest, parts};
+}
+// The XCD's i-th workgroup's: which of its pairs (none from `mine` on), and which part of it.
+__host__ __device__ __forceinline__ void moe_part(const MoeShare& s, int& i, int& part) {
+    const int whole = s.mine - s.rest, j = i - whole;
+    part = i < whole ? 0 : j % s.parts;
+    i = i < whole ? i : whole + j / s.parts;
+}
+__host__ __device__ __forceinline__ bool moe_splits(const MoeShare& s, int i) { return s.parts > 1 && i >= s.mine - s.rest; }
+__host__ __device__ __forceinline__ void moe_pair(const MoeShare& s, int i, int& row, int& column) {
+    constexpr int GM = 4;
+    const bool is_own = i < s.own;
+    const int wide = is_own ? s.eighth : s.tiles_n - 8 * s.eighth;
+    const int t = is_own ? i : s.xcd * s.per + min(s.xcd, s.rem) + i - s.own;
+    const int group = t / (GM * wide), first_m = group * GM;
+    const int gsize = min(s.tiles_m - first_m, GM);
+    row = first_m + (t % (GM * wide)) % gsize;
+    column = (t % (GM * wide)) / gsize + (is_own ? s.xcd * s.eighth : 8 * s.eighth);
+}
 
 // The whole feed-forward of a few tokens, by their ids. `values` holds SwiGLU's rows
 // [tokens * top_k][ffn_pad].

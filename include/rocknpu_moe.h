@@ -81,7 +81,7 @@ typedef struct rocknpu_moe_experts_args {
     const float * weights;      /* [tokens][top_k], its weights or others */
     const int32_t * plan;       /* the plan that came with the ids */
     void * out;                 /* [tokens][hidden] of out_type, rows out_row elements apart */
-    int64_t tokens, out_row;
+    int64_t tokens, out_row;    /* tokens * hidden_pad is below 2^32 */
     int32_t experts, top_k;
     int32_t hidden, hidden_pad; /* pads are multiples of 64, at most 133120, and what they add is zero in A8 or W8 */
     int32_t ffn, ffn_pad;

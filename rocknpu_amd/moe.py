@@ -198,9 +198,11 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
     (int8, with a_scales f32 [tokens]: hip.norm_a8 or hip.quantize_a8), weighted
     by the routing and summed: [tokens, hidden] of `dtype` (f32, f16 or bf16), or
     into `out`. Products are W8A8 as hip.gemm_w8a8's, between them SwiGLU and
-    the quantisation of its rows."""
+    the quantisation of its rows. a8 has to stay below 2^32 bytes."""
     at = weights.device
     tokens, top_k = routing.ids.shape
+    if tokens * weights.hidden_pad >> 32:
+        raise ValueError(f"{tokens} rows of {weights.hidden_pad} bytes: a8 has to stay below 2^32 bytes, split the tokens")
     if a8.dtype is not torch.int8 or a8.shape != (tokens, weights.hidden_pad) or not a8.is_contiguous() or a8.device != at:
         raise ValueError(f"a8 has to be contiguous int8 [{tokens}, {weights.hidden_pad}] on {at}")
     if a_scales.dtype is not torch.float32 or a_scales.shape != (tokens,) or not a_scales.is_contiguous() or a_scales.device != at:

@@ -27,6 +27,7 @@ MAX_TOP_K = 64
 MAX_GROUPS = 64
 MAX_ROWS = 1 << 28
 PLAN_HEADER = 16
+_F32_MAX = torch.finfo(torch.float32).max
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -108,6 +109,15 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     are the scores without the bias, divided by their sum with `normalise`,
     times `factor`. A logit of -inf is an expert that cannot be chosen: where
     less than top_k can, the last ids are -1 and their weights 0."""
+    routing, launch = _route_call(logits, top_k, score, bias, groups, top_groups, group_top, normalise, factor)
+    launch()
+    return routing
+
+
+# What a call checks, allocates and packs, apart from its launches: feed_forward does
+# all of that for its calls before the first one writes anything.
+def _route_call(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, group_top=1, normalise=True, factor=1.0):
+    """route's result, still to be filled by the call that comes with it."""
     if logits.dim() != 2 or logits.dtype not in TYPES:
         raise ValueError(f"logits have to be float32, float16 or bfloat16 [tokens, experts], not {logits.dtype} {tuple(logits.shape)}")
     tokens, experts = logits.shape
@@ -126,6 +136,8 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
                          f"most {MAX_GROUPS}, and the chosen ones have to hold top_k experts")
     if not 1 <= group_top <= min(2, experts // groups):
         raise ValueError(f"group_top {group_top} is neither 1 nor 2, or more than a group's experts")
+    if not abs(factor) <= _F32_MAX:
+        raise ValueError(f"factor {factor} is not a finite float32")
     ids = logits.new_empty((tokens, top_k), dtype=torch.int32)
     weights = logits.new_empty((tokens, top_k), dtype=torch.float32)
     plan = logits.new_empty((words,), dtype=torch.int32)
@@ -133,8 +145,11 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
                        plan.data_ptr(), tokens, logits.stride(0) if tokens > 1 else experts, TYPES[logits.dtype], experts, top_k,
                        groups, top_groups, group_top, SCORES[score], normalise, factor)
     index, stream = hip.stream_of(at)
-    hip._check(hip.call_on(index, _lib.load().rocknpu_hip_moe_route, args, stream), "moe_route")
-    return Routing(ids, weights, plan, experts)
+
+    def launch():
+        hip._check(hip.call_on(index, _lib.load().rocknpu_hip_moe_route, args, stream), "moe_route")
+
+    return Routing(ids, weights, plan, experts), launch
 
 
 def _pair(pair, shape, what, device):
@@ -144,6 +159,8 @@ def _pair(pair, shape, what, device):
         raise ValueError(f"{what} has to be contiguous int8 {shape} on {device}, not {w8.dtype} {tuple(w8.shape)} on {w8.device}")
     if scales.dtype is not torch.float32 or tuple(scales.shape) != shape[:-1] or not scales.is_contiguous() or scales.device != device:
         raise ValueError(f"{what}'s scales have to be contiguous float32 {shape[:-1]} on {device}")
+    if w8.data_ptr() % 16:
+        raise ValueError(f"{what} has to begin on 16 bytes")
     return w8, scales
 
 
@@ -199,6 +216,13 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
     by the routing and summed: [tokens, hidden] of `dtype` (f32, f16 or bf16), or
     into `out`. Products are W8A8 as hip.gemm_w8a8's, between them SwiGLU and
     the quantisation of its rows. a8 has to stay below 2^32 bytes."""
+    out, launch = _experts_call(weights, a8, a_scales, routing, dtype, out, workspace)
+    launch()
+    return out
+
+
+def _experts_call(weights, a8, a_scales, routing, dtype, out, workspace=None):
+    """experts' result, still to be filled by the call that comes with it."""
     at = weights.device
     tokens, top_k = routing.ids.shape
     if tokens * weights.hidden_pad >> 32:
@@ -220,6 +244,8 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
         out = torch.empty((tokens, weights.hidden), dtype=dtype, device=at)
     elif out.dtype not in TYPES or out.shape != (tokens, weights.hidden) or out.device != at or (out.stride(1) != 1 and weights.hidden > 1):
         raise ValueError(f"out has to be float32, float16 or bfloat16 [{tokens}, {weights.hidden}] on {at} with contiguous rows")
+    elif tokens > 1 and out.stride(0) < weights.hidden:
+        raise ValueError(f"out's rows overlap: they are {weights.hidden} wide and {out.stride(0)} apart")
     key = hip.stream_of(at)
     args = _pack_experts(
         a8.data_ptr(), a_scales.data_ptr(), *weights.pointers, ids.data_ptr(), factors.data_ptr(),
@@ -233,17 +259,22 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
         if len(weights._needs) >= 1024:
             weights._needs.clear()
         need = weights._needs[tokens, top_k] = got.value
-    if workspace is None:
+    if workspace is None and need == 0:  # no tokens
+        at_workspace, nbytes = 0, 0
+    elif workspace is None:
         workspace = _workspaces.get(key)  # the stream's own
         if workspace is None or workspace.numel() < need:
             workspace = workspace_for(at, need)
-        nbytes = workspace.numel()
+        at_workspace, nbytes = workspace.data_ptr(), workspace.numel()
     elif workspace.device != at or not workspace.is_contiguous():
         raise ValueError(f"workspace has to be a contiguous tensor on {at}")
     else:
-        nbytes = workspace.numel() * workspace.element_size()
-    hip._check(hip.call_on(key[0], lib.rocknpu_hip_moe_experts, args, workspace.data_ptr(), nbytes, key[1]), "moe_experts")
-    return out
+        at_workspace, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+    def launch():
+        hip._check(hip.call_on(key[0], lib.rocknpu_hip_moe_experts, args, at_workspace, nbytes, key[1]), "moe_experts")
+
+    return out, launch
 
 
 def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, router, weights: Experts, top_k: int, *, eps: float = 1e-5,
@@ -252,12 +283,19 @@ def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, router, weights: Ex
     (`router`: a W8 pair [experts, hidden_pad] and [experts], for an f32 router
     hip.quantize_a8 of its rows), route with `routing`'s arguments, and experts.
     Returns (out [tokens, hidden] in x's type, x + residual or None); the former
-    is the next norm's x, the latter its residual."""
+    is the next norm's x, the latter its residual. A call that is refused has
+    written nothing."""
     _pair(router, (weights.experts, weights.hidden_pad), "router", weights.device)
     if x.dim() != 2 or x.shape[1] != weights.hidden or x.device != weights.device:
         raise ValueError(f"x has to be [tokens, {weights.hidden}] on {weights.device}, not {tuple(x.shape)} on {x.device}")
-    a8, a_scales, hidden = hip.norm_a8(x, norm_weight, eps, residual, hidden=hidden, k_pad=weights.hidden_pad)
-    if x.shape[0] == 0:
-        return x.new_empty((0, weights.hidden)) if out is None else out, hidden
-    logits = hip.call_on(hip.stream_of(x.device)[0], hip.gemm_w8a8, a8, a_scales, *router)
-    return experts(weights, a8, a_scales, route(logits, top_k, **routing), dtype=x.dtype, out=out), hidden
+    tokens = x.shape[0]
+    a8, a_scales = x.new_empty((tokens, weights.hidden_pad), dtype=torch.int8), x.new_empty((tokens,), dtype=torch.float32)
+    logits = x.new_empty((tokens, weights.experts), dtype=torch.float32)
+    chosen, choose = _route_call(logits, top_k, **routing)
+    out, run = _experts_call(weights, a8, a_scales, chosen, x.dtype, out)
+    hidden = hip.norm_a8(x, norm_weight, eps, residual, hidden=hidden, k_pad=weights.hidden_pad, a8=a8, scales=a_scales)[2]
+    if tokens:
+        hip.call_on(hip.stream_of(x.device)[0], hip.gemm_w8a8, a8, a_scales, *router, logits)
+        choose()
+        run()
+    return out, hidden

@@ -57,7 +57,8 @@ typedef struct rocknpu_moe_route_args {
  * index; a group without group_top experts that can be chosen ranks lowest). ids
  * are in order of rank; weights are the chosen scores (without bias), normalised and multiplied. Where
  * less than top_k experts can be chosen the last ids are -1 and their weights 0.
- * A row that holds a NaN or +inf has its lowest experts and NaN weights.
+ * A row that holds a NaN or +inf has its lowest experts and NaN weights. Outputs
+ * overlap neither each other nor what is read.
  *
  * The plan begins with 16 words of its own, then offsets [experts + 1] and order
  * [tokens * top_k]: order[offsets[e]] .. order[offsets[e + 1] - 1] are, ascending,
@@ -96,6 +97,7 @@ typedef struct rocknpu_moe_experts_args {
  * out[t] = sum over s of weights[t][s] * d, in 64 bits in the order of s, rounded
  * to f32 and to out_type. Choices of id -1 are left out; a token without any gets zeros. A row of A8
  * whose scale is NaN gives NaN in its token's output and in no other.
+ * out, the workspace and what the call reads overlap nowhere.
  * The workspace (rocknpu_hip_moe_experts_workspace bytes, 256-byte aligned, any
  * contents) is free again when the call's kernels are done. The same call gives
  * the same bits. */

@@ -277,17 +277,35 @@ def _experts_call(weights, a8, a_scales, routing, dtype, out, workspace=None):
     return out, launch
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether no byte is in both of two matrices of contiguous rows. Rows as far apart as the
+    other's may lie between them; otherwise what counts is from where to where they reach."""
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    if not a.numel() or not b.numel():
+        return True
+    rows, wide, step = a.shape[0], a.shape[1] * a.element_size(), a.stride(0) * a.element_size()
+    d = b.data_ptr() - a.data_ptr()
+    if d >= (rows - 1) * step + wide:
+        return True
+    if rows == 1 or step != b.stride(0) * b.element_size() or step < wide:
+        return False
+    return d % step >= wide and (d // step + 1 >= rows or d % step + b.shape[1] * b.element_size() <= step)
+
+
 def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, router, weights: Experts, top_k: int, *, eps: float = 1e-5,
                  residual: torch.Tensor | None = None, hidden: torch.Tensor | None = None, out: torch.Tensor | None = None, **routing):
     """A layer's second half: hip.norm_a8 of x + residual, the router's product
     (`router`: a W8 pair [experts, hidden_pad] and [experts], for an f32 router
     hip.quantize_a8 of its rows), route with `routing`'s arguments, and experts.
     Returns (out [tokens, hidden] in x's type, x + residual or None); the former
-    is the next norm's x, the latter its residual. A call that is refused has
-    written nothing."""
+    is the next norm's x, the latter its residual. `out` may be x or the residual,
+    but not what x + residual goes to. A call that is refused has written nothing."""
     _pair(router, (weights.experts, weights.hidden_pad), "router", weights.device)
     if x.dim() != 2 or x.shape[1] != weights.hidden or x.device != weights.device:
         raise ValueError(f"x has to be [tokens, {weights.hidden}] on {weights.device}, not {tuple(x.shape)} on {x.device}")
+    if hidden is not None and out is not None and out.dim() == 2 == hidden.dim() and not _apart(hidden, out):
+        raise ValueError("out and hidden overlap: the layer's output would overwrite x + residual")
     tokens = x.shape[0]
     a8, a_scales = x.new_empty((tokens, weights.hidden_pad), dtype=torch.int8), x.new_empty((tokens,), dtype=torch.float32)
     logits = x.new_empty((tokens, weights.experts), dtype=torch.float32)

@@ -207,6 +207,18 @@ _retired: list[torch.Tensor] = []
 _growing = threading.Lock()
 
 
+# A call that makes several launches on its stream's own workspace holds the stream's
+# lock while it enqueues them. The interpreter's lock is let go in the library, so
+# two threads that call on one stream would mix their launches on the workspace.
+_enqueuing: dict[tuple[int, int], threading.Lock] = {}
+
+
+def enqueuing(key: tuple[int, int]) -> threading.Lock:
+    """The lock of a stream, by (device index, stream)."""
+    lock = _enqueuing.get(key)
+    return _enqueuing.setdefault(key, threading.Lock()) if lock is None else lock
+
+
 def _stream_workspace(table: dict, device: torch.device, nbytes: int, least: int) -> torch.Tensor | None:
     """`table`'s zeroed workspace of at least nbytes (and `least`) for the
     current stream on `device`; None when one would have to be made or grown

@@ -272,7 +272,8 @@ def _experts_call(weights, a8, a_scales, routing, dtype, out, workspace=None):
         at_workspace, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
     def launch():
-        hip._check(hip.call_on(key[0], lib.rocknpu_hip_moe_experts, args, at_workspace, nbytes, key[1]), "moe_experts")
+        with hip.enqueuing(key):
+            hip._check(hip.call_on(key[0], lib.rocknpu_hip_moe_experts, args, at_workspace, nbytes, key[1]), "moe_experts")
 
     return out, launch
 

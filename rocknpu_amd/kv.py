@@ -259,7 +259,9 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
         elif workspace.device != device or not workspace.is_contiguous():
             raise ValueError(f"workspace has to be a contiguous tensor on {device}")
         ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    hip._check(lib.rocknpu_hip_kv_attention(cache._ref, ref, ws, nbytes, _stream(device)), "kv_attention")
+    stream = _stream(device)
+    with hip.enqueuing((device.index, stream)):
+        hip._check(lib.rocknpu_hip_kv_attention(cache._ref, ref, ws, nbytes, stream), "kv_attention")
     return out
 
 

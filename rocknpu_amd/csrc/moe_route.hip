@@ -293,10 +293,12 @@ __device__ void place_block(const int32_t* ids, int first, int last, int run, co
 // expert that cannot be chosen. Ranks are
 //   - without a bias, 16-bit logits: their bits, in order: exact;
 //   - without a bias, f32 logits: 2^20 (logit - the token's largest), from -16 up;
-//   - with a bias: 2^20 (score + bias), within +-8, or of sigmoids within +-1.9 2^22.
-// The last two are truncated from f32 values that are within 0.6 of a unit (1.1 at
-// 2^22) of the 64-bit one (and a softmax's sum of up to 256 within 1.3 units of its
-// share, the same for all): keys that differ by four units or more are in the right order,
+//   - with a bias: 2^20 (score + bias), within +-7.9.
+// The last two are truncated from f32 values that are within 0.6 of a unit of the
+// 64-bit one: 0.25 for the last place of a sum with the bias (0.5 for that of a
+// logit's distance from the largest), 0.13 for the reciprocal or the exponential and 0.1
+// for the roundings around it (and a softmax's sum of up to 256 within 1.3 units of its share, the
+// same for all). Keys that differ by four units or more are in the right order,
 // and sums of two that differ by eight. Where two choices, or the last one and the best that is left,
 // differ by less, or the last open group and the best closed one, or where a
 // value does not fit, the token goes to route_token. The weights are worked out
@@ -378,7 +380,7 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
             }
         } else {
             float y[P];
-            float floor = -8.0f, unit = kUnit;
+            float floor = -8.0f;
             if (!p.bias) {
                 floor = -16.0f;
 #pragma unroll
@@ -407,7 +409,7 @@ __global__ __launch_bounds__(1024) void route_rows_kernel(const RouteParams p, c
             }
 #pragma unroll
             for (int j = 0; j < P; ++j) {
-                const int q = static_cast<int>(fmaxf(y[j], floor) * unit) - static_cast<int>(floor * unit);
+                const int q = static_cast<int>(fmaxf(y[j], floor) * kUnit) - static_cast<int>(floor * kUnit);
                 key[j] = open_mask(l[j]) & (static_cast<uint32_t>(min(max(q, 1), 0xFFFFFF)) << 8 | (255 - (e0 + j)));
             }
         }

@@ -92,7 +92,7 @@ typedef struct rocknpu_moe_experts_args {
 /* The feed-forward of every token's chosen experts: for choice s of token t, on
  * expert e, g and u are the W8A8 products of the token's row with gate[e] and
  * up[e] (f32(f32(sum) * row's scale) * column's scale, as rocknpu_hip_gemm_w8a8),
- * v = f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, v's row is
+ * v = f32(g * u / (1 + exp(-g))) with what is inside to 2^-50 of its value, v's row is
  * quantised as rocknpu_hip_quantize_a8 does, d is its product with down[e], and
  * out[t] = sum over s of weights[t][s] * d, in 64 bits in the order of s, rounded
  * to f32 and to out_type. Choices of id -1 are left out; a token without any gets zeros. A row of A8

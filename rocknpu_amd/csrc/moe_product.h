@@ -38,7 +38,11 @@ constexpr int kMoeManyTiles = 64;
 // L2 where they are one expert's, and their A over the columns. With many row tiles a share is a
 // contiguous range; with few, in which a range's full and partly filled tiles
 // would not even out, an eighth of the columns of every row tile (and a range of
-// the columns that are left over). Where tiles split, what an XCD's CUs would run in a
+// the columns that are left over). us a call by an eighth and by ranges, top 2 of 8 experts of 4096 x
+// 14336: 13 row tiles 356 and 387, 12 623 and 613, 19 985 and 992, 52 2531 and 2602, 67 3288
+// and 3375, 101 4860 and 5040; 24 of 2000 x 1000: 24 tiles 43.8 and 42.4; 64 of 2048 x 1024: 154 431
+// and 432, 292 819 and 846; 8 of 2048 x 1024: 517 1630 and 1611; 256 of 4096 x 2048: 256 1938 and
+// 1829. Beyond the limit neither is the better one throughout. Where tiles split, what an XCD's CUs would run in a
 // last round that is at most half full runs in two parts (halves of the columns), at
 // most a quarter full in four (of the rows, too: parts 0 and 1 the upper, 2 and 3 the lower).
 struct MoeShare {
@@ -89,7 +93,8 @@ struct MoeDecode {
 bool moe_decodes(int64_t tokens, int experts, int top_k, int ffn_pad);
 int launch_moe_decode(const MoeDecode& p, uint32_t out_type, void* out, int64_t out_row, hipStream_t stream);
 
-// f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, to 2^-50 of the value:
+// f32(g * u / (1 + exp(-g))) with what is inside in 64 bits, to 2^-50 of the value, so
+// that about one value in 2^25 is rounded to the neighbour of the nearest f32:
 // exp(-g) = 2^n 2^r with n = rint(-g log2(e)), |r| <= 1/2 in two parts of log2(e),
 // 2^r by the polynomial through its values at the 11 Chebyshev nodes of [-1/2, 1/2]
 // (off by 2^-51.5 at most), the division by the reciprocal's Newton step and one

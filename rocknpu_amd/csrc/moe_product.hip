@@ -19,8 +19,9 @@
 //
 // Measured, us (gate and up; down): 4096 tokens, top 8 of 64 experts of 2048 x 1024,
 // 32768 rows: 235; 142. 2048 tokens, top 2 of 8 of 4096 x 14336: 620; 310, 1.5 POP/s
-// (gemm.hip on one matrix of that size: 465 to 525 on different days' GPUs; the matrix
-// units are bound by power). 64 tokens of the latter: 187; 82, 5.0 and 5.7 TB/s of weights.
+// (gemm.hip on one matrix of gate's and up's size: 462 to 525, by 16 full row tiles; here
+// 16 to 24 are begun, 19 in that call, and SwiGLU and a tile's start are 15 us of a
+// tile's 71). 64 tokens of the latter: 187; 82, 5.0 and 5.7 TB/s of weights.
 //   - 256 x 256 tiles by eight waves of 128 x 64, two a SIMD; by four waves of 128 x 128
 //     252; 160 and 630; 319. 256 x 128 tiles, two workgroups a CU, whose epilogues overlap
 //     with each other's products: 250; 165 and 671; 376.

@@ -16,7 +16,10 @@
 // where its rounding alone is 2.0e-8), so the scale has one rounding.
 //
 // Bound by memory: a row is read once, into registers, and everything is written
-// from them. One workgroup a row. With a residual (x and r read, hidden and codes
+// from them, up to 32768 columns, 16384 where no wide loads fit. The compiler keeps a part
+// of longer rows in memory (336 to 432 bytes a lane, and 760 to 772), and they run
+// at a fraction of the rate: 1024 rows of 32768 f32 94 us, 4.7 TB/s, of 65536 400 us, 2.2;
+// bf16 46 us, 5.2, and 289, 1.6; 65535 f16 1145 us, 0.4. One workgroup a row. With a residual (x and r read, hidden and codes
 // written), in a graph: 16384 rows of 4096 f32 152 us, 5.7 TB/s, bf16 88 us, 5.4; of
 // 1024 f32 35 us, 6.3; 16384 rows of 64 f32 8 us; one row of 2048 3.3 us.
 #include "common.h"
@@ -235,7 +238,10 @@ int launch(const rocknpu_norm_args& a, int nt, hipStream_t stream) {
 }
 
 // Threads a row: two runs each (one for at most 512 rows), in whole waves, at
-// most 1024.
+// most 1024. us by one run and by two, of 64, 512, 1024 and 2048 rows: 1024 f32 3.2 and
+// 3.3, 3.7 and 3.9, 4.4 and 4.4, 5.7 and 5.6; 2048 f32 3.5 and 3.5, 4.5 and 4.4, 5.9 and 5.9, 11.6
+// and 10.5; 4096 f32 4.2 and 3.9, 6.2 and 5.9, 12.8 and 10.6, 20.2 and 17.8; 2048 bf16 3.3 and
+// 3.9, 4.0 and 4.7, 5.0 and 5.1, 6.9 and 7.4; 8192 bf16 4.4 and 4.7, 7.2 and 7.8, 14.2 and 12.9, 21.7 and 20.7.
 template <typename T, typename W>
 int route(const rocknpu_norm_args& a, hipStream_t stream) {
     constexpr int V = 16 / sizeof(T);

@@ -28,6 +28,12 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+# The current stream without its object, and the current device without a look whether
+# the GPUs are set up (tensors that are there tell): where torch offers them.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def stream_of(device: torch.device) -> tuple[int, int]:
     """(index, current stream) of a GPU."""
     if device.type != "cuda":
@@ -35,13 +41,12 @@ def stream_of(device: torch.device) -> tuple[int, int]:
     index = device.index
     if index is None:
         index = torch.cuda.current_device()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the stream without its object, where torch offers that
-    return index, torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
+    return index, torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index)
 
 
 def call_on(index: int, function, *args) -> int:
     """function(*args) with GPU `index` the current one."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         return function(*args)
     with torch.cuda.device(index):
         return function(*args)
@@ -210,13 +215,11 @@ _growing = threading.Lock()
 # A call that makes several launches on its stream's own workspace holds the stream's
 # lock while it enqueues them. The interpreter's lock is let go in the library, so
 # two threads that call on one stream would mix their launches on the workspace.
-_enqueuing: dict[tuple[int, int], threading.Lock] = {}
+enqueuing: dict[tuple[int, int], threading.Lock] = {}  # by (device index, stream)
 
 
-def enqueuing(key: tuple[int, int]) -> threading.Lock:
-    """The lock of a stream, by (device index, stream)."""
-    lock = _enqueuing.get(key)
-    return _enqueuing.setdefault(key, threading.Lock()) if lock is None else lock
+def enqueuing_on(key: tuple[int, int]) -> threading.Lock:
+    return enqueuing.setdefault(key, threading.Lock())
 
 
 def _stream_workspace(table: dict, device: torch.device, nbytes: int, least: int) -> torch.Tensor | None:

@@ -260,7 +260,8 @@ def attention(cache: Cache, q: torch.Tensor, past: torch.Tensor, cu: torch.Tenso
             raise ValueError(f"workspace has to be a contiguous tensor on {device}")
         ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     stream = _stream(device)
-    with hip.enqueuing((device.index, stream)):
+    key = (device.index, stream)
+    with hip.enqueuing.get(key) or hip.enqueuing_on(key):
         hip._check(lib.rocknpu_hip_kv_attention(cache._ref, ref, ws, nbytes, stream), "kv_attention")
     return out
 

@@ -109,15 +109,15 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     are the scores without the bias, divided by their sum with `normalise`,
     times `factor`. A logit of -inf is an expert that cannot be chosen: where
     less than top_k can, the last ids are -1 and their weights 0."""
-    routing, launch = _route_call(logits, top_k, score, bias, groups, top_groups, group_top, normalise, factor)
-    launch()
+    routing, index, stream, args = _route_call(logits, top_k, score, bias, groups, top_groups, group_top, normalise, factor)
+    hip._check(hip.call_on(index, _lib.load().rocknpu_hip_moe_route, args, stream), "moe_route")
     return routing
 
 
 # What a call checks, allocates and packs, apart from its launches: feed_forward does
 # all of that for its calls before the first one writes anything.
 def _route_call(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, group_top=1, normalise=True, factor=1.0):
-    """route's result, still to be filled by the call that comes with it."""
+    """route's result, still to be filled, and what the library's call for it takes: device, stream, arguments."""
     if logits.dim() != 2 or logits.dtype not in TYPES:
         raise ValueError(f"logits have to be float32, float16 or bfloat16 [tokens, experts], not {logits.dtype} {tuple(logits.shape)}")
     tokens, experts = logits.shape
@@ -128,7 +128,7 @@ def _route_call(logits, top_k, score="softmax", bias=None, groups=1, top_groups=
         raise ValueError(f"bias has to be contiguous float32 [{experts}] on {at}")
     if score not in SCORES:
         raise ValueError(f"score {score!r} is not one of {tuple(SCORES)}")
-    words = plan_words(tokens, experts, top_k)
+    words = _plan_words.get((tokens, experts, top_k)) or plan_words(tokens, experts, top_k)
     top_groups = groups if top_groups is None else top_groups
     if not (1 <= groups <= min(MAX_GROUPS, experts) and experts % groups == 0 and 1 <= top_groups <= groups
             and top_groups * (experts // groups) >= top_k):
@@ -144,12 +144,7 @@ def _route_call(logits, top_k, score="softmax", bias=None, groups=1, top_groups=
     args = _pack_route(logits.data_ptr(), 0 if bias is None else bias.data_ptr(), ids.data_ptr(), weights.data_ptr(),
                        plan.data_ptr(), tokens, logits.stride(0) if tokens > 1 else experts, TYPES[logits.dtype], experts, top_k,
                        groups, top_groups, group_top, SCORES[score], normalise, factor)
-    index, stream = hip.stream_of(at)
-
-    def launch():
-        hip._check(hip.call_on(index, _lib.load().rocknpu_hip_moe_route, args, stream), "moe_route")
-
-    return Routing(ids, weights, plan, experts), launch
+    return Routing(ids, weights, plan, experts), *hip.stream_of(at), args
 
 
 def _pair(pair, shape, what, device):
@@ -216,13 +211,15 @@ def experts(weights: Experts, a8: torch.Tensor, a_scales: torch.Tensor, routing:
     by the routing and summed: [tokens, hidden] of `dtype` (f32, f16 or bf16), or
     into `out`. Products are W8A8 as hip.gemm_w8a8's, between them SwiGLU and
     the quantisation of its rows. a8 has to stay below 2^32 bytes."""
-    out, launch = _experts_call(weights, a8, a_scales, routing, dtype, out, workspace)
-    launch()
+    out, key, args, space, nbytes = _experts_call(weights, a8, a_scales, routing, dtype, out, workspace)
+    with hip.enqueuing.get(key) or hip.enqueuing_on(key):
+        status = hip.call_on(key[0], _lib.load().rocknpu_hip_moe_experts, args, space, nbytes, key[1])
+    hip._check(status, "moe_experts")
     return out
 
 
 def _experts_call(weights, a8, a_scales, routing, dtype, out, workspace=None):
-    """experts' result, still to be filled by the call that comes with it."""
+    """experts' result, still to be filled, and what the library's call for it takes: device and stream, arguments, workspace."""
     at = weights.device
     tokens, top_k = routing.ids.shape
     if tokens * weights.hidden_pad >> 32:
@@ -236,7 +233,7 @@ def _experts_call(weights, a8, a_scales, routing, dtype, out, workspace=None):
     ids, factors, plan = routing.ids, routing.weights, routing.plan
     if (ids.dtype is not torch.int32 or not ids.is_contiguous() or ids.device != at or factors.dtype is not torch.float32
             or factors.shape != ids.shape or not factors.is_contiguous() or factors.device != at or plan.dtype is not torch.int32
-            or not plan.is_contiguous() or plan.numel() != plan_words(tokens, weights.experts, top_k)):
+            or not plan.is_contiguous() or plan.numel() != (_plan_words.get((tokens, weights.experts, top_k)) or plan_words(tokens, weights.experts, top_k))):
         raise ValueError(f"the routing's ids and plan have to be route's own, and its weights contiguous float32 {tuple(ids.shape)} on {at}")
     if out is None:
         if dtype not in TYPES:
@@ -251,31 +248,25 @@ def _experts_call(weights, a8, a_scales, routing, dtype, out, workspace=None):
         a8.data_ptr(), a_scales.data_ptr(), *weights.pointers, ids.data_ptr(), factors.data_ptr(),
         plan.data_ptr(), out.data_ptr(), tokens, out.stride(0) if tokens > 1 else weights.hidden, weights.experts, top_k,
         weights.hidden, weights.hidden_pad, weights.ffn, weights.ffn_pad, TYPES[out.dtype])
-    lib = _lib.load()
     need = weights._needs.get((tokens, top_k))
     if need is None:
         got = ctypes.c_size_t()
-        hip._check(lib.rocknpu_hip_moe_experts_workspace(args, ctypes.addressof(got)), "moe_experts_workspace")
+        hip._check(_lib.load().rocknpu_hip_moe_experts_workspace(args, ctypes.addressof(got)), "moe_experts_workspace")
         if len(weights._needs) >= 1024:
             weights._needs.clear()
         need = weights._needs[tokens, top_k] = got.value
     if workspace is None and need == 0:  # no tokens
-        at_workspace, nbytes = 0, 0
+        space, nbytes = 0, 0
     elif workspace is None:
         workspace = _workspaces.get(key)  # the stream's own
         if workspace is None or workspace.numel() < need:
             workspace = workspace_for(at, need)
-        at_workspace, nbytes = workspace.data_ptr(), workspace.numel()
+        space, nbytes = workspace.data_ptr(), workspace.numel()
     elif workspace.device != at or not workspace.is_contiguous():
         raise ValueError(f"workspace has to be a contiguous tensor on {at}")
     else:
-        at_workspace, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-
-    def launch():
-        with hip.enqueuing(key):
-            hip._check(hip.call_on(key[0], lib.rocknpu_hip_moe_experts, args, at_workspace, nbytes, key[1]), "moe_experts")
-
-    return out, launch
+        space, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return out, key, args, space, nbytes
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -310,11 +301,13 @@ def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, router, weights: Ex
     tokens = x.shape[0]
     a8, a_scales = x.new_empty((tokens, weights.hidden_pad), dtype=torch.int8), x.new_empty((tokens,), dtype=torch.float32)
     logits = x.new_empty((tokens, weights.experts), dtype=torch.float32)
-    chosen, choose = _route_call(logits, top_k, **routing)
-    out, run = _experts_call(weights, a8, a_scales, chosen, x.dtype, out)
+    chosen, index, stream, choose = _route_call(logits, top_k, **routing)
+    out, key, run, space, nbytes = _experts_call(weights, a8, a_scales, chosen, x.dtype, out)
     hidden = hip.norm_a8(x, norm_weight, eps, residual, hidden=hidden, k_pad=weights.hidden_pad, a8=a8, scales=a_scales)[2]
     if tokens:
-        hip.call_on(hip.stream_of(x.device)[0], hip.gemm_w8a8, a8, a_scales, *router, logits)
-        choose()
-        run()
+        hip.call_on(index, hip.gemm_w8a8, a8, a_scales, *router, logits)
+        hip._check(hip.call_on(index, _lib.load().rocknpu_hip_moe_route, choose, stream), "moe_route")
+        with hip.enqueuing.get(key) or hip.enqueuing_on(key):
+            status = hip.call_on(index, _lib.load().rocknpu_hip_moe_experts, run, space, nbytes, stream)
+        hip._check(status, "moe_experts")
     return out, hidden
